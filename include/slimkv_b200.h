@@ -619,6 +619,195 @@ SLIMKV_API int slimkv_rms_norm(const void* x, int64_t x_row_stride, const void* 
 SLIMKV_API int slimkv_silu_mul(const void* gate_up, int64_t gate_up_row_stride, void* out, int64_t out_row_stride,
                                int rows, int intermediate, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Speculative decoding and cache eviction.  No reference counterpart: the
+ * reference decodes one raw token (and its Beacon) per step and never drops a
+ * cached row.
+ *
+ * slimkv_cache names the K and V rows of one layer (or of all layers) for a
+ * batch: element strides {sequence, row, head}, last dimension contiguous.
+ * Dense: `table` null, `rows` the rows a sequence can hold (a sequence stride
+ * of 0 shares one cache).  Paged: `table` int32 block tables, sequence b's
+ * page i at table[b * table_stride + i] for i < table_pages; `rows` is the
+ * rows of a page, stride[0] the stride of a page and num_pages their number.
+ * A page number outside [0, num_pages) is reported as
+ * SLIMKV_DEVICE_BAD_LENGTH and clamped into that range (read as page 0 or the
+ * last; never written).  Rows are 16-byte aligned: pointers, and strides and
+ * dims times the element size, are multiples of 16 bytes.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    const void* k;
+    const void* v;
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int rows;
+    const int32_t* table;
+    int64_t table_stride;
+    int table_pages;
+    int num_pages;
+} slimkv_cache;
+
+/* Element types of the entry points below. */
+#define SLIMKV_BF16 0
+#define SLIMKV_FP16 1
+#define SLIMKV_FP32 2
+
+/* ------------------------------------------------------------------------
+ * Ancestor words of drafted trees: masks[b][t] holds `words` = (nodes + 31) /
+ * 32 int32 words, bit i set when node t sees node i: its ancestors and
+ * itself.  parents [batch][nodes] int32, a parent before its children; a
+ * parent outside [0, t) makes node t a root.
+ * ---------------------------------------------------------------------- */
+SLIMKV_API int slimkv_tree_masks(const int32_t* parents, int batch, int nodes, int32_t* masks, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of a tree of drafted tokens over a cache (split-KV, tcgen05):
+ *   out[b,t,h] = sum_n softmax_n(scale q[b,t,h] . k[b,n,g]) v[b,n,g],
+ * g = h / (heads / kv_heads), over the keys that node t sees: the context rows
+ * n < lengths[b], and the rows lengths[b] + i of the nodes i whose bit is set
+ * in its mask words (the nodes' K/V are in the cache behind the context).
+ * Without a mask node t sees the nodes 0..t.  nodes_len (nullable, int32
+ * [batch]) limits a sequence to its first nodes; rows past it see nothing.
+ * context_only: the cache holds no rows of the nodes; every node sees the
+ * context.  A row that sees no key gets zero output and lse -inf.  What a key
+ * or value that a row does not see holds (infinities and NaN too) does not
+ * reach that row.
+ * q [batch][nodes][heads][dim_qk], out [batch][nodes][heads][dim_v], element
+ * strides {batch, node, head}, type bf16 or fp16 like the cache; lse fp32
+ * [batch][nodes][heads] contiguous, natural log.  mask: int32, words of node t
+ * of sequence b at mask + b * mask_stride + t * ((nodes + 31) / 32)
+ * (mask_stride 0: one tree for the batch).  dims multiples of 8 up to 320;
+ * heads / kv_heads at most 128; pages of a multiple of 8 rows; batch at most
+ * 4096, nodes at most 1024.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    int batch, nodes, heads, kv_heads, dim_qk, dim_v, type;
+    const void* q;
+    int64_t q_stride[3];
+    slimkv_cache cache;
+    const int32_t* lengths;
+    const int32_t* nodes_len;
+    const int32_t* mask;
+    int64_t mask_stride;
+    int context_only;
+    float scale;
+    void* out;
+    int64_t out_stride[3];
+    float* lse;
+    uint64_t wait_limit_ns;    /* bound of every pipeline wait (0: 2 s) */
+} slimkv_tree_attention_args;
+
+SLIMKV_API size_t slimkv_tree_attention_workspace_size(const slimkv_tree_attention_args* args);
+SLIMKV_API int slimkv_tree_attention(const slimkv_tree_attention_args* args, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
+/* ------------------------------------------------------------------------
+ * Greedy acceptance of a drafted tree.  Node 0 is the last accepted token.
+ * From it, the target token is the largest logit of the node (ties: the lowest
+ * token; a NaN counts above every number), and the walk goes on at the node's
+ * first child that drafted this token, if there is one.  path [batch][nodes]
+ * int32 gets the nodes of the walk (ascending, -1 past them), count [batch]
+ * their number, next [batch] int64 the target token of the last one.
+ * logits [batch][nodes][vocab] of `type` (bf16, fp16, fp32), element strides
+ * {batch, node}; tokens int64 [batch][nodes]; parents as for
+ * slimkv_tree_masks; nodes_len as above (0 nodes: count 0, next -1).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    int batch, nodes, vocab, type;
+    const void* logits;
+    int64_t logits_stride[2];
+    const int64_t* tokens;
+    const int32_t* parents;
+    const int32_t* nodes_len;
+    int32_t* path;
+    int32_t* count;
+    int64_t* next;
+} slimkv_tree_accept_args;
+
+SLIMKV_API size_t slimkv_tree_accept_workspace_size(const slimkv_tree_accept_args* args);
+SLIMKV_API int slimkv_tree_accept(const slimkv_tree_accept_args* args, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/* ------------------------------------------------------------------------
+ * Commit of the accepted nodes: cache row lengths[b] + path[b][i] moves to
+ * lengths[b] + i for i < count[b], in place, for `layers` caches whose K / V
+ * lie layer_stride elements apart, and new_lengths[b] = lengths[b] + count[b].
+ * path ascends (a path of slimkv_tree_accept).  elem_bytes 1, 2 or 4.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    int layers, batch, nodes, kv_heads, dim_qk, dim_v, elem_bytes;
+    slimkv_cache cache;
+    int64_t k_layer_stride, v_layer_stride;
+    const int32_t* lengths;
+    const int32_t* path;
+    const int32_t* count;
+    int32_t* new_lengths;
+} slimkv_tree_commit_args;
+
+SLIMKV_API int slimkv_tree_commit(const slimkv_tree_commit_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention weight of each key, accumulated for eviction (tcgen05):
+ *   mass[b,g,n] = decay mass[b,g,n] + sum_{i < counts[b]} sum_{h of group g}
+ *                 exp(scale q[b,r_i,h] . k[b,n,g] - lse[b,r_i,h]),  r_i = rows[b][i],
+ * for n < lengths[b] (old keys) and, unless context_only, the keys
+ * lengths[b] + i of the rows themselves (chain order: row i sees the keys
+ * n <= lengths[b] + i; their old mass counts as 0).  Other entries of mass keep
+ * their values.  rows null: r_i = i; counts null: every row.  A row whose lse
+ * is infinite (it saw no key) gives nothing.
+ * q [batch][nodes][heads][dim], lse fp32 [batch][nodes][heads] contiguous,
+ * mass fp32, element strides {batch, head}, at least the used rows long.  Only
+ * cache.k is read.  Types, dims and pages as slimkv_tree_attention.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    int batch, nodes, heads, kv_heads, dim, type;
+    const void* q;
+    int64_t q_stride[3];
+    slimkv_cache cache;
+    const int32_t* lengths;
+    const int32_t* rows;       /* [batch][nodes] */
+    const int32_t* counts;
+    const float* lse;
+    float* mass;
+    int64_t mass_stride[2];
+    int mass_rows;
+    int context_only;
+    float scale, decay;
+    uint64_t wait_limit_ns;
+} slimkv_key_mass_args;
+
+SLIMKV_API int slimkv_key_mass(const slimkv_key_mass_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Eviction: each (sequence, KV head) keeps min(lengths[b], keep) rows: its
+ * first `sinks` rows, its last `recent` rows and, of the others, those of the
+ * largest mass (ties: the lowest row; a NaN counts above every number), in
+ * their order, written to rows 0.. of the output cache; the output rows from
+ * there to `keep` are zeroed.  mass / positions (int32, nullable: both or
+ * neither of in and out) move along.  new_lengths[b] = min(lengths[b], keep).
+ * sinks + recent <= keep.  The output must not overlap the input.
+ * elem_bytes 1, 2 or 4; mass strides {batch, head} elements, mass_rows long.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    int batch, kv_heads, dim_qk, dim_v, elem_bytes;
+    slimkv_cache in, out;
+    const int32_t* lengths;
+    const float* mass;
+    int64_t mass_stride[2];
+    int mass_rows;
+    const int32_t* positions;
+    int64_t positions_stride[2];
+    float* out_mass;
+    int64_t out_mass_stride[2];
+    int32_t* out_positions;
+    int64_t out_positions_stride[2];
+    int keep, sinks, recent;
+    int32_t* new_lengths;
+} slimkv_evict_args;
+
+SLIMKV_API size_t slimkv_evict_workspace_size(const slimkv_evict_args* args);
+SLIMKV_API int slimkv_evict(const slimkv_evict_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

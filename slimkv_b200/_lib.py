@@ -147,6 +147,61 @@ class PrefillAttentionArgs(ctypes.Structure):
     ]
 
 
+class Cache(ctypes.Structure):
+    """Mirror of ``slimkv_cache``."""
+    _fields_ = [
+        ('k', _P), ('v', _P), ('k_stride', _L * 3), ('v_stride', _L * 3), ('rows', _I), ('table', _P),
+        ('table_stride', _L), ('table_pages', _I), ('num_pages', _I),
+    ]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """Mirror of ``slimkv_tree_attention_args``."""
+    _fields_ = [
+        ('batch', _I), ('nodes', _I), ('heads', _I), ('kv_heads', _I), ('dim_qk', _I), ('dim_v', _I), ('type', _I),
+        ('q', _P), ('q_stride', _L * 3), ('cache', Cache), ('lengths', _P), ('nodes_len', _P), ('mask', _P),
+        ('mask_stride', _L), ('context_only', _I), ('scale', ctypes.c_float), ('out', _P), ('out_stride', _L * 3),
+        ('lse', _P), ('wait_limit_ns', ctypes.c_uint64),
+    ]
+
+
+class TreeAcceptArgs(ctypes.Structure):
+    """Mirror of ``slimkv_tree_accept_args``."""
+    _fields_ = [
+        ('batch', _I), ('nodes', _I), ('vocab', _I), ('type', _I), ('logits', _P), ('logits_stride', _L * 2),
+        ('tokens', _P), ('parents', _P), ('nodes_len', _P), ('path', _P), ('count', _P), ('next', _P),
+    ]
+
+
+class TreeCommitArgs(ctypes.Structure):
+    """Mirror of ``slimkv_tree_commit_args``."""
+    _fields_ = [
+        ('layers', _I), ('batch', _I), ('nodes', _I), ('kv_heads', _I), ('dim_qk', _I), ('dim_v', _I),
+        ('elem_bytes', _I), ('cache', Cache), ('k_layer_stride', _L), ('v_layer_stride', _L), ('lengths', _P),
+        ('path', _P), ('count', _P), ('new_lengths', _P),
+    ]
+
+
+class KeyMassArgs(ctypes.Structure):
+    """Mirror of ``slimkv_key_mass_args``."""
+    _fields_ = [
+        ('batch', _I), ('nodes', _I), ('heads', _I), ('kv_heads', _I), ('dim', _I), ('type', _I), ('q', _P),
+        ('q_stride', _L * 3), ('cache', Cache), ('lengths', _P), ('rows', _P), ('counts', _P), ('lse', _P),
+        ('mass', _P), ('mass_stride', _L * 2), ('mass_rows', _I), ('context_only', _I), ('scale', ctypes.c_float),
+        ('decay', ctypes.c_float), ('wait_limit_ns', ctypes.c_uint64),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    """Mirror of ``slimkv_evict_args``."""
+    _fields_ = [
+        ('batch', _I), ('kv_heads', _I), ('dim_qk', _I), ('dim_v', _I), ('elem_bytes', _I), ('src', Cache),
+        ('dst', Cache), ('lengths', _P), ('mass', _P), ('mass_stride', _L * 2), ('mass_rows', _I), ('positions', _P),
+        ('positions_stride', _L * 2), ('out_mass', _P), ('out_mass_stride', _L * 2), ('out_positions', _P),
+        ('out_positions_stride', _L * 2), ('keep', _I), ('sinks', _I), ('recent', _I), ('new_lengths', _P),
+    ]
+
+
 _PL = ctypes.POINTER(ctypes.c_int64)
 
 SIGNATURES = {
@@ -180,6 +235,15 @@ SIGNATURES = {
     'slimkv_reconstruct_kv_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(ReconstructArgs)]),
     'slimkv_reconstruct_kv': (_I, [ctypes.POINTER(ReconstructArgs), _P]),
     'slimkv_prefill_attention': (_I, [ctypes.POINTER(PrefillAttentionArgs), _P]),
+    'slimkv_tree_masks': (_I, [_P, _I, _I, _P, _P]),
+    'slimkv_tree_attention_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(TreeAttentionArgs)]),
+    'slimkv_tree_attention': (_I, [ctypes.POINTER(TreeAttentionArgs), _P, ctypes.c_size_t, _P]),
+    'slimkv_tree_accept_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(TreeAcceptArgs)]),
+    'slimkv_tree_accept': (_I, [ctypes.POINTER(TreeAcceptArgs), _P, ctypes.c_size_t, _P]),
+    'slimkv_tree_commit': (_I, [ctypes.POINTER(TreeCommitArgs), _P]),
+    'slimkv_key_mass': (_I, [ctypes.POINTER(KeyMassArgs), _P]),
+    'slimkv_evict_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(EvictArgs)]),
+    'slimkv_evict': (_I, [ctypes.POINTER(EvictArgs), _P, ctypes.c_size_t, _P]),
     'slimkv_rms_norm': (_I, [_P, _L, _P, _P, _L, _I, _I, ctypes.c_float, _P]),
     'slimkv_silu_mul': (_I, [_P, _L, _P, _L, _I, _I, _P]),
 }

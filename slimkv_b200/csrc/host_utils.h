@@ -56,6 +56,11 @@ struct Carver {
 // Device address of this device's status word (resolved once per device).
 unsigned int* status_word();
 
+// Pointers, strides and row widths of a cache whose rows are read or moved as
+// 16-byte units; SLIMKV_OK or an error naming `what` (text in last error).
+int check_cache(const slimkv_cache& cache, int batch, int dim_k, int dim_v, int elem_bytes, bool need_v,
+                const char* what);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace slimkv

@@ -1,0 +1,311 @@
+// The steps around the attention of a drafted tree (C ABI slimkv_tree_masks,
+// slimkv_tree_accept, slimkv_tree_commit): the ancestor words of a tree, its
+// greedy acceptance, and the move of the accepted rows next to the context.
+#include <algorithm>
+
+#include "cache_view.cuh"
+#include "host_utils.h"
+
+namespace slimkv {
+namespace {
+
+// ------------------------------------------------------------ tree masks --
+// One thread per node: walk up the parents (each below its child, so the walk
+// ends) and set their bits in the node's own row of words.
+__global__ void tree_masks_kernel(const int32_t* parents, int nodes, int words, int32_t* masks) {
+    const int t = blockIdx.x * blockDim.x + threadIdx.x, b = blockIdx.y;
+    if (t >= nodes) return;
+    const int32_t* par = parents + int64_t(b) * nodes;
+    int32_t* row = masks + (int64_t(b) * nodes + t) * words;
+    int at = t;
+    for (int w = words - 1; w >= 0; --w) {          // ancestors descend: one word after the other
+        uint32_t bits = 0;
+        while (at >= 32 * w && at >= 0) {
+            bits |= 1u << (at & 31);
+            const int p = __ldg(par + at);
+            at = p < at ? p : -1;
+        }
+        row[w] = int32_t(bits);
+    }
+}
+
+// ---------------------------------------------------------------- argmax --
+// The largest logit of a row as one 64-bit number: its order-preserving bits
+// (NaN above everything, the two zeros equal) over the complement of its
+// index, so that a maximum of them takes the lowest index of equal values.
+__device__ __forceinline__ uint64_t rank_of(float x, uint32_t index) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    const uint32_t o = x != x ? 0xffffffffu : (u >> 31 ? ~u : u | 0x80000000u);
+    return uint64_t(o) << 32 | uint32_t(~index);
+}
+__device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+template <typename T> __device__ __forceinline__ float to_float(T x);
+template <> __device__ __forceinline__ float to_float(float x) { return x; }
+template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ void scan_vector(const uint4& w, uint32_t at, uint64_t& best) {
+    constexpr int kN = 16 / int(sizeof(T));
+    const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) best = max_u64(best, rank_of(to_float(x[i]), at + i));
+}
+
+// The best of elements [lo, hi) of a row, over the threads of a block.
+template <typename T, int kThreads>
+__device__ __forceinline__ uint64_t scan_row(const T* row, int lo, int hi, uint64_t* part) {
+    constexpr int kN = 16 / int(sizeof(T));
+    uint64_t best = 0;
+    const int lead = int(((16 - (reinterpret_cast<uintptr_t>(row + lo) & 15)) & 15) / sizeof(T));
+    const int body = std::min(lo + lead, hi);
+    const int vectors = (hi - body) / kN, tail = body + vectors * kN;
+    for (int i = lo + int(threadIdx.x); i < body; i += kThreads) best = max_u64(best, rank_of(to_float(row[i]), i));
+    const uint4* v = reinterpret_cast<const uint4*>(row + body);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < vectors; i += kThreads) scan_vector<T>(__ldg(v + i), body + i * kN, best);
+    for (int i = tail + int(threadIdx.x); i < hi; i += kThreads) best = max_u64(best, rank_of(to_float(row[i]), i));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = best;
+    __syncthreads();
+    best = part[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) best = max_u64(best, part[w]);
+    return best;
+}
+
+struct AcceptArgs {
+    int nodes, vocab, splits;
+    const void* logits;
+    int64_t stride_batch, stride_node;
+    const int64_t* tokens;
+    const int32_t* parents;
+    const int32_t* nodes_len;
+    int32_t* path;
+    int32_t* count;
+    int64_t* next;
+    uint64_t* best;             // [batch][nodes][splits]
+};
+
+constexpr int kScanThreads = 256;
+
+// Every node's argmax, its vocabulary split over gridDim.x blocks.
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads) accept_scan_kernel(AcceptArgs a) {
+    __shared__ uint64_t part[kScanThreads / 32];
+    const int t = blockIdx.y, b = blockIdx.z;
+    if (a.nodes_len && t >= __ldg(a.nodes_len + b)) return;
+    const T* row = static_cast<const T*>(a.logits) + b * a.stride_batch + t * a.stride_node;
+    const int lo = int(int64_t(a.vocab) * blockIdx.x / a.splits), hi = int(int64_t(a.vocab) * (blockIdx.x + 1) / a.splits);
+    const uint64_t best = scan_row<T, kScanThreads>(row, lo, hi, part);
+    if (threadIdx.x == 0) a.best[(int64_t(b) * a.nodes + t) * a.splits + blockIdx.x] = best;
+}
+
+// The walk: one warp per sequence.
+__global__ void __launch_bounds__(32) accept_walk_kernel(AcceptArgs a) {
+    const int b = blockIdx.x, lane = threadIdx.x;
+    const int n = a.nodes_len ? min(max(__ldg(a.nodes_len + b), 0), a.nodes) : a.nodes;
+    const int64_t* tokens = a.tokens + int64_t(b) * a.nodes;
+    const int32_t* parents = a.parents + int64_t(b) * a.nodes;
+    int32_t* path = a.path + int64_t(b) * a.nodes;
+    int cur = n > 0 ? 0 : -1, len = 0;
+    int64_t next = -1;
+    while (cur >= 0) {
+        if (lane == 0) path[len] = cur;
+        ++len;
+        uint64_t best = 0;
+        for (int i = lane; i < a.splits; i += 32) best = max_u64(best, a.best[(int64_t(b) * a.nodes + cur) * a.splits + i]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, o));
+        next = int64_t(uint32_t(~uint32_t(best)));
+        int child = -1;
+        for (int c0 = cur + 1; c0 < n && child < 0; c0 += 32) {
+            const int c = c0 + lane;
+            const unsigned hit = __ballot_sync(0xffffffffu, c < n && __ldg(parents + c) == cur && __ldg(tokens + c) == next);
+            if (hit) child = c0 + __ffs(int(hit)) - 1;
+        }
+        cur = child;
+    }
+    for (int i = len + lane; i < a.nodes; i += 32) path[i] = -1;
+    if (lane == 0) {
+        a.count[b] = len;
+        a.next[b] = next;
+    }
+}
+
+int accept_splits(const slimkv_tree_accept_args* a) {
+    // Blocks of at least 4096 logits, about eight per SM over all rows.
+    const int64_t rows = int64_t(a->batch) * a->nodes;
+    const int64_t want = (int64_t(device_info().sm_count) * 8 + rows - 1) / rows;
+    return int(std::max<int64_t>(1, std::min<int64_t>(want, a->vocab / 4096)));
+}
+
+int check_accept(const slimkv_tree_accept_args* a) {
+    if (!a) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "null arguments");
+    if (a->batch < 1 || a->batch > 65535 || a->nodes < 1 || a->nodes > 1024 || a->vocab < 1)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree accept: batch in 1..65535, nodes in 1..1024, vocab >= 1");
+    if (a->type != SLIMKV_BF16 && a->type != SLIMKV_FP16 && a->type != SLIMKV_FP32)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree accept: unknown logits type %d", a->type);
+    return SLIMKV_OK;
+}
+
+// ---------------------------------------------------------------- commit --
+struct CommitArgs {
+    uint8_t *k, *v;
+    CacheView cache;            // strides in bytes
+    int64_t k_layer, v_layer;   // bytes
+    int kv_heads, k_units, v_units, lanes;      // 16-byte units of a K / V row; lanes of one layer
+    int layers, nodes;
+    const int32_t *lengths, *path, *count;
+    int32_t* new_lengths;
+    unsigned int* status;
+};
+
+constexpr int kCommitRows = 8;
+
+// One thread per 16-byte column of a (layer, K or V, head): rows move in
+// ascending order, kCommitRows loaded before they are stored.  path[i] >= i
+// ascends, so a row is read before a later one is written over it.
+__global__ void __launch_bounds__(256) tree_commit_kernel(CommitArgs a) {
+    const int b = blockIdx.y;
+    const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    const int len = __ldg(a.lengths + b), want = __ldg(a.count + b);
+    const int count = min(max(want, 0), a.nodes);
+    if (at == 0) {
+        a.new_lengths[b] = len + count;
+        if (want != count || len < 0) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
+    }
+    if (at >= int64_t(a.layers) * a.lanes || len < 0) return;
+    const int layer = int(at / a.lanes);
+    int lane = int(at - int64_t(layer) * a.lanes);
+    const bool is_v = lane >= a.kv_heads * a.k_units;
+    if (is_v) lane -= a.kv_heads * a.k_units;
+    const int units = is_v ? a.v_units : a.k_units, head = lane / units;
+    const int64_t* st = is_v ? a.cache.v_stride : a.cache.k_stride;
+    uint8_t* base = (is_v ? a.v + layer * a.v_layer : a.k + layer * a.k_layer) + head * st[2] + int64_t(lane - head * units) * 16;
+    const int64_t cap = cache_capacity(a.cache);
+    const int32_t* path = a.path + int64_t(b) * a.nodes;
+    for (int i0 = 0; i0 < count; i0 += kCommitRows) {
+        uint4 row[kCommitRows];
+        bool move[kCommitRows];
+#pragma unroll
+        for (int j = 0; j < kCommitRows; ++j) {
+            const int i = i0 + j;
+            const int p = i < count ? __ldg(path + i) : i;
+            int64_t page;
+            int r;
+            move[j] = p != i;
+            if (!move[j]) continue;
+            if (p < i || p >= a.nodes || int64_t(len) + p >= cap || !cache_row(a.cache, b, len + p, page, r)) {
+                report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
+                move[j] = false;
+                continue;
+            }
+            row[j] = *reinterpret_cast<const uint4*>(base + page * st[0] + r * st[1]);
+        }
+#pragma unroll
+        for (int j = 0; j < kCommitRows; ++j) {
+            int64_t page;
+            int r;
+            if (move[j] && cache_row(a.cache, b, len + i0 + j, page, r))
+                *reinterpret_cast<uint4*>(base + page * st[0] + r * st[1]) = row[j];
+        }
+    }
+}
+
+}  // namespace
+
+// Checks of a cache whose rows are moved as 16-byte units; see host_utils.h.
+int check_cache(const slimkv_cache& c, int batch, int dim_k, int dim_v, int elem_bytes, bool need_v, const char* what) {
+    if (!c.k || (need_v && !c.v)) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "%s: null cache", what);
+    if (c.rows < 1) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "%s: the cache needs rows", what);
+    if (c.table && (c.table_pages < 1 || c.num_pages < 1 || (batch > 1 && c.table_stride < c.table_pages && c.table_stride != 0) ||
+                    int64_t(c.rows) * c.table_pages > 0x7fffffffLL))
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "%s: block tables need pages, their stride and fewer than 2^31 rows", what);
+    if (dim_k < 1 || (need_v && dim_v < 1)) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "%s: dims must be positive", what);
+    bool ok = aligned16(c.k) && int64_t(dim_k) * elem_bytes % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && c.k_stride[i] * elem_bytes % 16 == 0 && c.k_stride[i] >= 0;
+    if (need_v) {
+        ok = ok && aligned16(c.v) && int64_t(dim_v) * elem_bytes % 16 == 0;
+        for (int i = 0; i < 3; ++i) ok = ok && c.v_stride[i] * elem_bytes % 16 == 0 && c.v_stride[i] >= 0;
+    }
+    return ok ? SLIMKV_OK : fail(SLIMKV_ERR_ALIGNMENT, "%s: cache pointers, strides and rows must be multiples of 16 bytes", what);
+}
+
+}  // namespace slimkv
+
+using namespace slimkv;
+
+extern "C" int slimkv_tree_masks(const int32_t* parents, int batch, int nodes, int32_t* masks, void* stream) {
+    if (!parents || !masks) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree masks: null pointer");
+    if (batch < 1 || batch > 65535 || nodes < 1 || nodes > 1024)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree masks: batch in 1..65535, nodes in 1..1024");
+    const int threads = std::min(256, (nodes + 31) / 32 * 32);
+    tree_masks_kernel<<<dim3((nodes + threads - 1) / threads, batch), threads, 0, static_cast<cudaStream_t>(stream)>>>(
+        parents, nodes, (nodes + 31) / 32, masks);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "tree masks launch failed: %s", cudaGetErrorString(e));
+}
+
+extern "C" size_t slimkv_tree_accept_workspace_size(const slimkv_tree_accept_args* a) {
+    if (check_accept(a) != SLIMKV_OK) return 0;
+    return size_t(a->batch) * a->nodes * accept_splits(a) * sizeof(uint64_t);
+}
+
+extern "C" int slimkv_tree_accept(const slimkv_tree_accept_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_accept(a)) return rc;
+    if (!a->logits || !a->tokens || !a->parents || !a->path || !a->count || !a->next)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree accept: null pointer");
+    if (a->logits_stride[0] < 0 || a->logits_stride[1] < 0)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree accept: negative strides");
+    AcceptArgs k{a->nodes, a->vocab, accept_splits(a), a->logits, a->logits_stride[0], a->logits_stride[1], a->tokens,
+                 a->parents, a->nodes_len, a->path, a->count, a->next, static_cast<uint64_t*>(workspace)};
+    if (!workspace || workspace_bytes < slimkv_tree_accept_workspace_size(a) || reinterpret_cast<uintptr_t>(workspace) % 8)
+        return fail(SLIMKV_ERR_WORKSPACE, "tree accept: workspace too small or misaligned");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const dim3 grid(k.splits, a->nodes, a->batch);
+    if (a->type == SLIMKV_BF16) accept_scan_kernel<__nv_bfloat16><<<grid, kScanThreads, 0, st>>>(k);
+    else if (a->type == SLIMKV_FP16) accept_scan_kernel<__half><<<grid, kScanThreads, 0, st>>>(k);
+    else accept_scan_kernel<float><<<grid, kScanThreads, 0, st>>>(k);
+    accept_walk_kernel<<<a->batch, 32, 0, st>>>(k);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "tree accept launch failed: %s", cudaGetErrorString(e));
+}
+
+extern "C" int slimkv_tree_commit(const slimkv_tree_commit_args* a, void* stream) {
+    if (!a || !a->lengths || !a->path || !a->count || !a->new_lengths)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree commit: null pointer");
+    if (a->layers < 1 || a->batch < 1 || a->batch > 65535 || a->nodes < 1 || a->nodes > 1024 || a->kv_heads < 1)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree commit: layers, heads >= 1, batch in 1..65535, nodes in 1..1024");
+    if (a->elem_bytes != 1 && a->elem_bytes != 2 && a->elem_bytes != 4)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree commit: elements of 1, 2 or 4 bytes");
+    if (int rc = check_cache(a->cache, a->batch, a->dim_qk, a->dim_v, a->elem_bytes, true, "tree commit")) return rc;
+    const int e = a->elem_bytes;
+    if (a->k_layer_stride * e % 16 || a->v_layer_stride * e % 16)
+        return fail(SLIMKV_ERR_ALIGNMENT, "tree commit: layer strides must be multiples of 16 bytes");
+    CommitArgs k{};
+    k.k = static_cast<uint8_t*>(const_cast<void*>(a->cache.k));
+    k.v = static_cast<uint8_t*>(const_cast<void*>(a->cache.v));
+    k.cache = cache_view(a->cache);
+    for (int i = 0; i < 3; ++i) { k.cache.k_stride[i] *= e; k.cache.v_stride[i] *= e; }
+    k.k_layer = a->k_layer_stride * e;
+    k.v_layer = a->v_layer_stride * e;
+    k.kv_heads = a->kv_heads;
+    k.k_units = a->dim_qk * e / 16;
+    k.v_units = a->dim_v * e / 16;
+    k.lanes = a->kv_heads * (k.k_units + k.v_units);
+    k.layers = a->layers;
+    k.nodes = a->nodes;
+    k.lengths = a->lengths;
+    k.path = a->path;
+    k.count = a->count;
+    k.new_lengths = a->new_lengths;
+    k.status = status_word();
+    const int64_t blocks = (int64_t(a->layers) * k.lanes + 255) / 256;
+    if (blocks > 0x7fffffff) return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "tree commit: too many rows in one call");
+    tree_commit_kernel<<<dim3(unsigned(blocks), a->batch), 256, 0, static_cast<cudaStream_t>(stream)>>>(k);
+    const cudaError_t err = cudaGetLastError();
+    return err == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "tree commit launch failed: %s", cudaGetErrorString(err));
+}

@@ -1,0 +1,213 @@
+"""Accumulated attention weight and eviction (``slimkv_b200.eviction``)
+against plain 64-bit forms."""
+import math
+import random
+
+import pytest
+import torch
+
+import tree_oracle as oracle
+from slimkv_b200 import _lib, eviction, tree
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(7)
+
+
+def make(B, T, H, G, D, lengths, dtype=BF16, page=0, seed=0, spare=9):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    cap = max(lengths) + T + spare
+    rand = lambda *s: torch.randn(*s, generator=gen, device='cuda', dtype=dtype)
+    tables = None
+    if page:
+        per = -(-cap // page)
+        k = rand(B * per, page, 2, G, D)[:, :, 0]
+        tables = torch.randperm(B * per, generator=gen, device='cuda').view(B, per).to(torch.int32)
+    else:
+        k = rand(B, G, cap, D).transpose(1, 2)
+    q = rand(B, T, H, D)
+    mass = torch.rand(B, G, cap, generator=gen, device='cuda')
+    return q, k, mass, torch.tensor(lengths, dtype=torch.int32, device='cuda'), tables
+
+
+def check_mass(q, k, lse, mass, lens, scale, **kw):
+    old = mass.clone()
+    got = eviction.key_mass(q, k, lse, mass, lens, scale, **kw)
+    torch.cuda.synchronize()
+    assert got is mass and _lib.device_status() == 0
+    tables = kw.pop('block_tables', None)
+    rows, counts = kw.pop('rows', None), kw.pop('counts', None)
+    want, tol = oracle.mass(q, k, lse, old, lens.tolist(), scale, None if rows is None else rows.tolist() and rows.cpu(),
+                            None if counts is None else counts.tolist(), tables=tables, **kw)
+    off = (mass.double().cpu() - want).abs() - 1.05 * tol
+    # Entries past a sequence's rows have a bound of 0: they keep their bits.
+    assert off.max() <= 0, f'off its bound by {off.max():.3e}'
+
+
+@pytest.mark.parametrize('B,T,H,G,D,lengths,dtype,page', [
+    (1, 1, 32, 8, 128, [1028], BF16, 0), (2, 3, 8, 2, 128, [0, 300], BF16, 16), (3, 8, 8, 8, 64, [127, 1, 128], FP16, 48),
+    (2, 5, 6, 2, 96, [500, 77], BF16, 24), (1, 20, 16, 1, 64, [260], BF16, 0), (2, 70, 8, 1, 128, [129, 40], FP16, 0),
+    (1, 2, 3, 1, 8, [50], BF16, 0)])
+@pytest.mark.parametrize('decay', [1.0, 0.9])
+def test_accepted_rows(B, T, H, G, D, lengths, dtype, page, decay):
+    q, k, mass, lens, tables = make(B, T, H, G, D, lengths, dtype, page, seed=T)
+    rng = random.Random(T)
+    counts = [rng.randint(1, T) for _ in range(B)]
+    rows = torch.tensor([sorted(rng.sample(range(T), c)) + [-1] * (T - c) for c in counts], dtype=torch.int32, device='cuda')
+    counts = torch.tensor(counts, dtype=torch.int32, device='cuda')
+    lse = 3 + torch.rand(B, T, H, device='cuda') * 4
+    scale = D ** -0.5
+    check_mass(q, k, lse, mass, lens, scale, rows=rows, counts=counts, decay=decay, block_tables=tables)
+    check_mass(q, k, lse, mass, lens, scale, decay=decay, block_tables=tables)      # every row
+
+
+@pytest.mark.parametrize('T,rank,lengths', [(1, 320, [700, 0]), (8, 320, [1000, 129]), (12, 160, [33, 500])])
+def test_latents(T, rank, lengths):
+    lat = torch.randn(2, 2, max(lengths) + 2, rank, device='cuda').to(BF16)
+    for b, n in enumerate(lengths):
+        lat[b, :, n:] = math.nan
+    k = lat[:, 0].unsqueeze(2)
+    q = torch.randn(2, T, 32, rank, device='cuda').to(BF16)
+    lens = torch.tensor(lengths, dtype=torch.int32, device='cuda')
+    mass = torch.rand(2, 1, k.shape[1], device='cuda')
+    lse = 5 + torch.rand(2, T, 32, device='cuda')
+    counts = torch.tensor([T, 0], dtype=torch.int32, device='cuda')
+    check_mass(q, k, lse, mass, lens, rank ** -0.5, context_only=True, decay=0.5)
+    check_mass(q, k, lse, mass, lens, rank ** -0.5, context_only=True, counts=counts)
+
+
+def test_masses_of_a_row_sum_to_its_heads():
+    """With the lse that tree_attention returned, each accepted row gives G * group = H in all."""
+    q, k, mass, lens, _ = make(2, 4, 8, 2, 64, [300, 5])
+    _, lse = tree.tree_attention(q, k, k, lens, 0.125)
+    eviction.key_mass(q, k, lse, mass.zero_(), lens, 0.125)
+    assert torch.allclose(mass.sum((1, 2)), torch.full((2,), 32.0, device='cuda'), atol=1e-3)
+
+
+def test_empty_rows_and_unseen_keys():
+    """Rows without a key (infinite lse) give nothing; NaN keys past the end stay out."""
+    q, k, mass, lens, _ = make(2, 3, 4, 2, 64, [100, 128])
+    k[0, 103:], k[1, 131:] = math.nan, math.inf
+    mass[:, :, 131:] = math.nan
+    keep = mass.clone()
+    lse = torch.full((2, 3, 4), 4.0, device='cuda')
+    lse[0, 1], lse[1, 2, 0] = -math.inf, math.inf
+    eviction.key_mass(q, k, lse, mass, lens, 0.125)
+    want, tol = oracle.mass(q, k, lse, keep, [100, 128], 0.125)
+    live = tol > 0
+    assert ((mass.double().cpu() - want).abs() <= 1.05 * tol)[live].all()
+    assert torch.equal(mass.cpu()[~live].isnan(), keep.cpu()[~live].isnan())
+
+
+def test_mass_refusals():
+    q, k, mass, lens, _ = make(2, 3, 4, 2, 64, [100, 128])
+    lse = torch.zeros(2, 3, 4, device='cuda')
+    for args in ((q.float(), k, lse, mass, lens, 0.1), (q, k, lse.half(), mass, lens, 0.1), (q, k, lse, mass.double(), lens, 0.1),
+                 (q, k, lse, mass, lens.long(), 0.1), (q, k, lse, mass[:, :1], lens, 0.1), (q, k, lse, mass, lens, math.inf),
+                 (q, k, lse, mass, lens[:1], 0.1)):
+        with pytest.raises(RuntimeError):
+            eviction.key_mass(*args)
+
+
+def test_mass_rows_out_of_the_tree_are_reported():
+    q, k, mass, lens, _ = make(1, 3, 4, 2, 64, [100])
+    _lib.device_status(clear=True)
+    eviction.key_mass(q, k, torch.zeros(1, 3, 4, device='cuda'), mass, lens, 0.1,
+                      rows=torch.tensor([[0, 7, -1]], dtype=torch.int32, device='cuda'))
+    assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH
+
+
+# ------------------------------------------------------------------ evict --
+def same(got, want):
+    k, v, mass, positions, lengths = got
+    for x, y in ((k, want[0]), (v, want[1])):
+        assert torch.equal(x.cpu().double(), y)
+    m = mass.cpu().double()
+    assert torch.equal(m.nan_to_num(nan=-5.0), want[2].nan_to_num(nan=-5.0))
+    if positions is not None:
+        assert torch.equal(positions.cpu(), want[3])
+    assert torch.equal(lengths.cpu(), want[4])
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize('B,G,D,Dv,lengths,keep,sinks,recent,dtype,page', [
+    (1, 1, 8, 8, [1], 1, 0, 0, BF16, 0), (2, 8, 128, 128, [300, 255], 200, 4, 32, BF16, 0), (3, 2, 64, 128, [0, 1000, 513], 512, 4, 0, FP16, 0),
+    (2, 1, 320, 320, [3000, 2999], 700, 0, 257, BF16, 0), (1, 4, 16, 4, [70000], 50, 3, 40, torch.float32, 0),
+    (2, 2, 64, 64, [400, 33], 256, 2, 2, BF16, 16), (2, 3, 32, 16, [90, 260], 300, 4, 4, torch.uint8, 5), (1, 2, 64, 64, [1025], 1, 0, 1, BF16, 0)])
+@pytest.mark.parametrize('kind', ['spread', 'ties', 'odd'])
+def test_evict(B, G, D, Dv, lengths, keep, sinks, recent, dtype, page, kind):
+    gen = torch.Generator(device='cuda').manual_seed(keep)
+    cap = max(lengths) + 3
+    per = -(-cap // page) if page else 0
+    shape = (B * per, page, G) if page else (B, cap, G)
+    k, v = (torch.randint(0, 200, shape + (d,), generator=gen, device='cuda').to(dtype) for d in (D, Dv))
+    tables = torch.randperm(B * per, generator=gen, device='cuda').view(B, per).to(torch.int32) if page else None
+    mass = torch.randn(B, G, cap, generator=gen, device='cuda').mul_(2).exp_()
+    if kind == 'ties':
+        mass = (mass > 1).float() * 2
+    elif kind == 'odd':
+        pick = torch.randint(0, 8, mass.shape, generator=gen, device='cuda')
+        for i, x in enumerate((math.nan, math.inf, -math.inf, 0.0, -0.0, -1.0)):
+            mass[pick == i] = x
+    positions = torch.randint(0, 1 << 30, mass.shape, generator=gen, device='cuda', dtype=torch.int32)
+    lens = torch.tensor(lengths, dtype=torch.int32, device='cuda')
+    want = oracle.evict(k, v, mass, positions, lengths, keep, sinks, recent, tables)
+    same(eviction.evict(k, v, mass, positions, lens, keep, sinks, recent, block_tables=tables), want)
+    same(eviction.evict(k, v, mass, None, lens, keep, sinks, recent, block_tables=tables), want)
+
+
+def test_evict_into_given_buffers():
+    k = torch.randn(2, 500, 2, 64, device='cuda').to(BF16)
+    mass = torch.rand(2, 2, 500, device='cuda')
+    lens = torch.tensor([500, 90], dtype=torch.int32, device='cuda')
+    ok, ov = torch.full((2, 140, 2, 72), 7.0, device='cuda', dtype=BF16), torch.full((2, 2, 140, 64), 7.0, device='cuda', dtype=BF16)
+    om = torch.full((2, 2, 140), 7.0, device='cuda')
+    got = eviction.evict(k, k, mass, None, lens, 128, sinks=4, recent=16, out=(ok[..., :64], ov.transpose(1, 2), om, None))
+    want = oracle.evict(k, k, mass, None, [500, 90], 128, 4, 16)
+    same((got[0][:, :128], got[1][:, :128], got[2][..., :128], None, got[4]), want)
+    assert (ok[:, 128:] == 7).all() and (ok[..., 64:] == 7).all() and (ov[:, :, 128:] == 7).all() and (om[..., 128:] == 7).all()
+
+
+def test_evict_refusals():
+    k = torch.randn(2, 50, 2, 64, device='cuda').to(BF16)
+    mass = torch.rand(2, 2, 50, device='cuda')
+    lens = torch.tensor([50, 9], dtype=torch.int32, device='cuda')
+    for kw in (dict(keep=0), dict(keep=10, sinks=6, recent=5), dict(keep=10, sinks=-1)):
+        with pytest.raises(RuntimeError):
+            eviction.evict(k, k, mass, None, lens, **kw)
+    with pytest.raises(RuntimeError):
+        eviction.evict(k, k, mass.double(), None, lens, 10)
+    with pytest.raises(RuntimeError):
+        eviction.evict(k, k, mass, mass, lens, 10)
+    with pytest.raises(RuntimeError):                    # onto itself
+        eviction.evict(k, k.clone(), mass, None, lens, 10, out=(k, k.clone(), mass.clone(), None))
+    with pytest.raises(RuntimeError):                    # too small
+        eviction.evict(k, k, mass, None, lens, 40, out=(k[:, :20].clone(), k[:, :20].clone(), mass.clone(), None))
+    with pytest.raises(RuntimeError):                    # 12-byte rows
+        eviction.evict(k[..., :6], k[..., :6], mass, None, lens, 10)
+
+
+def test_a_bounded_cache_step():
+    """Attention, acceptance, commit, mass and eviction, as a serving loop calls them."""
+    B, T, H, G, D, V = 2, 6, 8, 2, 64, 97
+    rng = random.Random(3)
+    lengths = [60, 41]
+    q, k, mass, lens, _ = make(B, T, H, G, D, lengths, spare=30)
+    v = torch.randn_like(k)
+    parents = torch.tensor([[-1, 0, 0, 1, 1, 3], [-1, 0, 1, 2, 0, 4]], dtype=torch.int32, device='cuda')
+    _, lse = tree.tree_attention(q, k, v, lens, 0.125, mask=tree.tree_masks(parents))
+    logits = torch.randn(B, T, V, device='cuda')
+    tokens = torch.arange(B * T, device='cuda').view(B, T)      # all different
+    logits[0, 0, tokens[0, 1]] = logits[0, 1, tokens[0, 4]] = 9.0
+    path, count, _ = tree.tree_accept(logits, tokens, parents)
+    assert path[0].tolist() == [0, 1, 4, -1, -1, -1]
+    new = tree.tree_commit(k, v, lens, path, count)
+    eviction.key_mass(q, k, lse, mass, lens, 0.125, rows=path, counts=count, decay=0.9)
+    positions = torch.arange(k.shape[1], device='cuda', dtype=torch.int32).expand(B, G, -1).contiguous()
+    got = eviction.evict(k, v, mass, positions, new, 40, sinks=4, recent=8)
+    same(got, oracle.evict(k, v, mass, positions, new.tolist(), 40, 4, 8))
+    assert got[4].tolist() == [40, 40] and (got[3][0, :, -8:].cpu() == torch.arange(55, 63)).all()
