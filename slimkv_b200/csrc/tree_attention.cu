@@ -14,8 +14,8 @@
 // before that rounding, so lse keeps fp32 accuracy).
 //
 // Work: a unit is one 128-key tile of one (sequence, KV head, group of NQ row
-// tiles) segment: the context rows, then (a tile of their own) the nodes' own
-// rows, where each row sees what its ancestor words say.  The units of all
+// tiles) segment: the context rows, then the nodes' own rows, of which each
+// row sees what its ancestor words say.  The units of all
 // segments in a row are cut into one equal share per CTA; a share's part of a
 // segment is a piece.  A piece that holds a whole segment writes the output;
 // the others (at most two per CTA: its first and its last) leave normalised
@@ -25,9 +25,9 @@
 // Bound: with few rows per KV head HBM (each K / V row read once); with 128
 // rows or more the tensor cores and the exponentials.
 //
-// One CTA per SM, warps: 0 = Q and K loads (TMA), 3 = V loads, 1 = MMA issue,
-// 2 = TMEM owner, 4-7 (and 8-11) = softmax of row tile 0 (1), a thread per
-// row.  Every wait is bounded.
+// One CTA per SM, warps: 0 = Q and K loads (TMA), 3 = V loads, 1 = MMA issue
+// (one thread), 2 = TMEM owner, 4-7 (and 8-11) = softmax of row tile 0 (1), a
+// thread per row.  Every wait is bounded.
 #include <algorithm>
 
 #include "cache_view.cuh"
@@ -46,16 +46,16 @@ constexpr int kMaxChunks = 5;                    // dims <= 320
 constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a row's maximum grows by more than 2^8
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
-constexpr int kCombineRows = 16;
 
 struct Bars {
-    uint64_t kfull[kMaxRing], kempty[kMaxRing], vfull[kMaxRing], vempty[kMaxRing];
+    uint64_t kfull[kMaxRing], kempty[kMaxRing];                 // per 64-column chunk
+    uint64_t vfull[kMaxRing], vempty[kMaxRing];                 // per tile
     uint64_t qfull, qempty;
     // [row tile][buffer]
     uint64_t sfull[2][2], sempty[2][2], pfull[2][2], odone[2][2], oempty[2], final_mma;
     uint32_t tmem_base;
     int abort;
-    int bad_values;          // 1 + the piece whose node values hold infinities or NaN
+    int bad_values[2];           // 1 + a piece whose node values hold infinities or NaN
     Share share;
 };
 constexpr uint32_t kSmemBytes = 1024 + kTileArea + uint32_t(sizeof(Bars));
@@ -66,7 +66,8 @@ struct Job {
     int tpt, tile_rows;         // nodes of a row tile and its rows (tpt * group <= 128)
     int row_groups;             // groups of NQ row tiles
     int kc, vc, dim_v;          // 64-column chunks of a K / V row
-    int kring, vring;
+    int kring;                  // K chunks in shared memory
+    int vstages;                // V tiles in shared memory
     int context_only, paged, shared_cache;
     int box;                    // rows of one TMA box
     CacheView cache;
@@ -79,7 +80,7 @@ struct Job {
     void* out;
     int64_t o_sb, o_st, o_sh;
     float* lse;
-    float* part_o;              // [2 ctas][NQ * tile_rows][dim_v]
+    float* part_o;              // [2 ctas][dim_v / 4][NQ * tile_rows][4]
     float* part_lse;            // [2 ctas][NQ * tile_rows]
     int ctas;
     unsigned int* status;
@@ -87,18 +88,15 @@ struct Job {
 };
 
 // ------------------------------------------------------------- schedule --
-// What one sequence asks for.
+// What one sequence asks for: its keys are the cache rows [0, end), the context
+// and then the nodes' own rows.
 struct Seq {
-    int len, nodes;             // context rows, nodes
-    int ctx_tiles, tiles;       // key tiles of the context, and with the nodes' own rows
-    int tree_row;               // cache row at which the first node tile starts
+    int len, nodes, end;
+    int tiles;                  // key tiles
     int groups;                 // groups of row tiles with live rows
-    // First cache row of a key tile and its keys [lo, hi) that any row sees.
-    __device__ __forceinline__ int row0(int tile) const {
-        return tile < ctx_tiles ? tile * kKeys : tree_row + (tile - ctx_tiles) * kKeys;
-    }
-    __device__ __forceinline__ int lo(int tile) const { return tile < ctx_tiles ? 0 : min(max(len - row0(tile), 0), kKeys); }
-    __device__ __forceinline__ int hi(int tile) const { return min(kKeys, (tile < ctx_tiles ? len : len + nodes) - row0(tile)); }
+    // Keys of a tile that any row sees, and whether some of them are nodes.
+    __device__ __forceinline__ int hi(int tile) const { return min(kKeys, end - tile * kKeys); }
+    __device__ __forceinline__ bool has_nodes(int tile) const { return (tile + 1) * kKeys > len && end > len; }
 };
 template <int NQ>
 struct Plan {
@@ -107,19 +105,13 @@ struct Plan {
     __device__ __forceinline__ explicit Plan(const Job& j) : J(j), batch(j.batch), kv_heads(j.kv_heads), ctas(j.ctas) {}
     __device__ __forceinline__ Seq sequence(int b) const {
         Seq s;
-        const int nodes = J.nodes_len ? min(max(__ldg(J.nodes_len + b), 0), J.nodes) : J.nodes;
-        const int64_t room = J.capacity - (J.context_only ? 0 : nodes);
-        s.len = int(min(int64_t(max(__ldg(J.lengths + b), 0)), max(room, int64_t(0))));
-        s.nodes = nodes;
-        s.ctx_tiles = (s.len + kKeys - 1) / kKeys;
-        s.tree_row = s.len;
-        int tree = 0;
-        if (!J.context_only && nodes > 0 && room >= 0) {
-            if (J.paged) s.tree_row = s.len / J.box * J.box;     // boxes do not cross pages
-            tree = (s.len - s.tree_row + nodes + kKeys - 1) / kKeys;
-        }
-        s.tiles = s.ctx_tiles + tree;
-        s.groups = (nodes + NQ * J.tpt - 1) / (NQ * J.tpt);
+        s.nodes = J.nodes_len ? min(max(__ldg(J.nodes_len + b), 0), J.nodes) : J.nodes;
+        // A sequence that its cache cannot hold is cut to what fits (and reported).
+        const int64_t own = J.context_only ? 0 : min(int64_t(s.nodes), J.capacity);
+        s.len = int(min(int64_t(max(__ldg(J.lengths + b), 0)), J.capacity - own));
+        s.end = s.len + int(own);
+        s.tiles = (s.end + kKeys - 1) / kKeys;
+        s.groups = (s.nodes + NQ * J.tpt - 1) / (NQ * J.tpt);
         return s;
     }
 };
@@ -154,9 +146,16 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
         : "memory");
 }
 
+// A wait that is over costs one test; one that is not looks for an abort of
+// another warp and for its limit.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
-    if (*const_cast<volatile int*>(&bs->abort)) return false;
-    if (mbar_wait(bar, parity, J.wait_ns)) return true;
+    if (mbar_test(bar, parity)) return true;
+    for (uint64_t waited = 0; waited < J.wait_ns;) {
+        const uint64_t step = min(J.wait_ns - waited, uint64_t(100000));
+        if (mbar_wait(bar, parity, step)) return true;
+        if (*const_cast<volatile int*>(&bs->abort)) return false;
+        waited += step;
+    }
     bs->abort = 1;
     report(J.status, SLIMKV_DEVICE_TIMEOUT);
     return false;
@@ -177,12 +176,14 @@ struct Columns {
     __device__ static constexpr uint32_t p(int q, int buf) { return NQ == 2 ? s(q, 0) : kWide ? 448u : 384u + 64u * buf; }
 };
 
-// Which of 32 nodes from `first` (may be negative) node t sees.
 __device__ __forceinline__ uint32_t mask_word(const int32_t* row, int words, int w) {
     return w >= 0 && w < words ? uint32_t(__ldg(row + w)) : 0u;
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-__device__ __forceinline__ uint32_t seen_nodes(const int32_t* row, int words, int t, int nodes, int first) {
+// Which of the 32 keys from node `first` on (below 0: context) node t sees:
+// the context, and the nodes of its words (without words: up to itself).
+__device__ __forceinline__ uint32_t seen_keys(const int32_t* row, int words, int t, int nodes, int first) {
+    const uint32_t context = low_bits(-first);
     uint32_t bits;
     if (row) {
         const int w = first >> 5;               // floor
@@ -190,7 +191,51 @@ __device__ __forceinline__ uint32_t seen_nodes(const int32_t* row, int words, in
     } else {
         bits = low_bits(t + 1 - first);
     }
-    return bits & low_bits(nodes - first) & ~low_bits(-first);
+    return context | (bits & low_bits(nodes - first));
+}
+
+// The box of a key tile that this lane loads: its page (dense: its sequence)
+// and row.  Boxes past the last used row repeat that row's (they are masked).
+template <class W>
+__device__ __forceinline__ int box_of(const Job& J, const W& w, int tile, int lane, int& row) {
+    row = tile * kKeys + lane * J.box;
+    if (!J.paged) return J.shared_cache ? 0 : w.b;
+    int64_t page = 0;
+    if (lane < kKeys / J.box) {
+        const int last = tile * kKeys + w.s.hi(tile) - 1;
+        if (!cache_row(J.cache, w.b, min(row, last / J.box * J.box), page, row)) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+    }
+    return int(page);
+}
+// Whether a V tile holds rows that nobody sees, or the nodes' own.
+__device__ __forceinline__ bool needs_fix(const Seq& s, int tile) { return s.has_nodes(tile) || s.hi(tile) < kKeys; }
+
+// Row r of a V tile in shared memory: zeroed when nobody sees it (its P is 0,
+// and 0 x NaN is not 0); of a node's row, infinities and NaN become 0 (the
+// epilogue adds them to the rows that see them).  True when there were any.
+template <bool kHalf>
+__device__ __forceinline__ bool fix_values(uint8_t* tile, int chunks, int r, bool seen, bool node) {
+    constexpr uint32_t kExp = kHalf ? 0x7c00u : 0x7f80u;
+    if (seen && !node) return false;
+    bool bad = false;
+#pragma unroll 1
+    for (int j = 0; j < chunks * 8; ++j) {
+        uint4* at = reinterpret_cast<uint4*>(tile + (j >> 3) * kChunk + r * 128) + ((j ^ r) & 7);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        bool write = !seen;
+        if (seen) {
+            v = *at;
+            uint32_t* x = &v.x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if ((x[e] & kExp) == kExp) { x[e] &= 0xffff0000u; write = true; }
+                if ((x[e] >> 16 & kExp) == kExp) { x[e] &= 0xffffu; write = true; }
+            }
+            bad |= write;
+        }
+        if (write) *at = v;
+    }
+    return bad;
 }
 
 // ----------------------------------------------------------------- kernel --
@@ -227,7 +272,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         }
         mbar_init(&bs->final_mma, 1);
         bs->abort = 0;
-        bs->bad_values = 0;
+        bs->bad_values[0] = bs->bad_values[1] = 0;
         fence_barrier_init();
     }
     if (warp == 2) {
@@ -243,14 +288,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     const uint32_t sbase = smem_u32(smem);
     const bool any = int(blockIdx.x) < bs->share.ctas;
 
-    if (any && (warp == 0 || warp == 3)) {
-        // ---- producers: warp 0 each piece's Q and K chunks, warp 3 the V chunks ----
-        const bool keys = warp == 0;
-        const int chunks = keys ? J.kc : J.vc, ring = keys ? J.kring : J.vring;
-        uint64_t* full = keys ? bs->kfull : bs->vfull;
-        uint64_t* empty = keys ? bs->kempty : bs->vempty;
-        const CUtensorMap* map = keys ? &kmap : &vmap;
-        uint8_t* dst = smem + (keys ? off_k : off_v);
+    if (any && warp == 0) {
+        // ---- each piece's Q, and the K chunks ----
         const int boxes = kKeys / J.box;
         int slot = 0;
         uint32_t lap = 0;
@@ -258,168 +297,133 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         Walk<Plan<NQ>> w;
         w.start(plan, &bs->share);
         while (ok && w.next(plan)) {
-            if (keys) {
-                if (w.piece > 0) ok = warp_wait(&bs->qempty, (w.piece - 1) & 1, bs, J);
-                if (!ok) break;
-                if (lane == 0) {
-                    mbar_expect_tx(&bs->qfull, uint32_t(NQ * J.kc) * uint32_t(J.tile_rows) * 128u);
-                    for (int q = 0; q < NQ; ++q)
-                        for (int c = 0; c < J.kc; ++c)
-                            tma_load_4d(smem + (q * J.kc + c) * kChunk, &qmap, &bs->qfull, c * 64, w.g * J.group,
-                                        (w.group * NQ + q) * J.tpt, w.b);
-                }
-                __syncwarp();
+            if (w.piece > 0 && !(ok = warp_wait(&bs->qempty, (w.piece - 1) & 1, bs, J))) break;
+            if (lane == 0) {
+                mbar_expect_tx(&bs->qfull, uint32_t(NQ * J.kc) * uint32_t(J.tile_rows) * 128u);
+                for (int q = 0; q < NQ; ++q)
+                    for (int c = 0; c < J.kc; ++c)
+                        tma_load_4d(smem + (q * J.kc + c) * kChunk, &qmap, &bs->qfull, c * 64, w.g * J.group,
+                                    (w.group * NQ + q) * J.tpt, w.b);
             }
+            __syncwarp();
             for (int tile = w.t0; tile < w.t1 && ok; ++tile) {
-                // This lane's box: rows past the last used one repeat its box (they are masked).
-                int64_t page = J.shared_cache ? 0 : w.b;
-                int row = w.s.row0(tile) + lane * J.box;
-                if (J.paged && lane < boxes) {
-                    const int last = w.s.row0(tile) + w.s.hi(tile) - 1;
-                    if (!cache_row(J.cache, w.b, min(row, last / J.box * J.box), page, row) && keys)
-                        report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
-                }
-                for (int c = 0; c < chunks; ++c) {
-                    if (lap && !(ok = warp_wait(&empty[slot], (lap - 1) & 1, bs, J))) break;
-                    if (lane == 0) mbar_expect_tx(&full[slot], kChunk);
+                int row;
+                const int page = box_of(J, w, tile, lane, row);
+                for (int c = 0; c < J.kc; ++c) {
+                    if (lap && !(ok = warp_wait(&bs->kempty[slot], (lap - 1) & 1, bs, J))) break;
+                    if (lane == 0) mbar_expect_tx(&bs->kfull[slot], kChunk);
                     __syncwarp();
                     if (lane < boxes)
-                        tma_load_4d(dst + slot * kChunk + lane * J.box * 128, map, &full[slot], c * 64, w.g, row, int(page));
-                    if (++slot == ring) { slot = 0; ++lap; }
+                        tma_load_4d(smem + off_k + slot * kChunk + lane * J.box * 128, &kmap, &bs->kfull[slot], c * 64, w.g, row, page);
+                    if (++slot == J.kring) { slot = 0; ++lap; }
                 }
+            }
+        }
+    } else if (any && warp == 3) {
+        // ---- the V tiles ----
+        const int boxes = kKeys / J.box;
+        int stage = 0;
+        uint32_t lap = 0;
+        bool ok = true;
+        Walk<Plan<NQ>> w;
+        w.start(plan, &bs->share);
+        while (ok && w.next(plan)) {
+            for (int tile = w.t0; tile < w.t1; ++tile) {
+                int row;
+                const int page = box_of(J, w, tile, lane, row);
+                if (lap && !(ok = warp_wait(&bs->vempty[stage], (lap - 1) & 1, bs, J))) break;
+                if (lane == 0) mbar_expect_tx(&bs->vfull[stage], uint32_t(J.vc) * kChunk);
+                __syncwarp();
+                if (lane < boxes)
+                    for (int c = 0; c < J.vc; ++c)
+                        tma_load_4d(smem + off_v + (stage * J.vc + c) * kChunk + lane * J.box * 128, &vmap, &bs->vfull[stage], c * 64,
+                                    w.g, row, page);
+                if (++stage == J.vstages) { stage = 0; ++lap; }
             }
         }
     } else if (any && warp == 1) {
-        // ---- MMA issuer ----
-        const bool leader = lane == 0;
-        const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0);
-        const uint32_t idesc_o = idesc<kHalf>(128, 64, 0, 1);
-        int kslot = 0, vslot = 0;
-        uint32_t klap = 0, vlap = 0;
-        bool ok = true;
-        Walk<Plan<NQ>> ws, wp;                     // S runs one tile ahead of P.V
-        ws.start(plan, &bs->share);
-        wp.start(plan, &bs->share);
-        int s_tile = 0, p_tile = 0;          // next tile of the piece each is in
-        int s_count = 0;                     // S tiles begun before
-        bool s_more = ws.next(plan);
-        s_tile = ws.t0;
-        // The K chunks of S tile `s_count` are awaited by its first row tile and released by its last.
-        auto issue_s = [&](int q) {
-            if (q == 0) {
-                if (s_tile == ws.t0) ok = warp_wait(&bs->qfull, ws.piece & 1, bs, J);
-                const int sb = s_count % kBufs;
-                if (NQ == 1 && ok && s_count >= kBufs) ok = warp_wait(&bs->sempty[0][sb], ((s_count / kBufs) - 1) & 1, bs, J);
-                if (!ok) return;
-            }
-            tc_fence_after();
-            for (int c = 0; c < J.kc && ok; ++c) {
-                int slot = kslot + c;
-                uint32_t lap = klap;
-                while (slot >= J.kring) { slot -= J.kring; ++lap; }
+        if (elect_one()) {
+            // ---- MMA issue: S runs one tile ahead of P.V ----
+            const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0);
+            // Matrix descriptors (K-major Q and K; MN-major V): the low word moves with the address.
+            const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024), k_desc = umma_desc_sw128(sbase + off_k, 16, 1024);
+            const uint64_t v_desc = umma_desc_sw128(sbase + off_v, kChunk, 1024);
+            constexpr uint64_t kChunkStep = kChunk >> 4;
+            int kslot = 0, stage = 0, s_tile, p_tile = 0, s_count = 0;
+            uint32_t klap = 0, vlap = 0;
+            bool ok = true;
+            Walk<Plan<NQ>> ws, wp;
+            ws.start(plan, &bs->share);
+            wp = ws;
+            bool s_more = ws.next(plan);
+            s_tile = ws.t0;
+            // The K chunks of a tile are awaited for its first row tile and released by its last.
+            auto issue_s = [&](int q) {
+                const int buf = kBufs == 2 ? s_count & 1 : 0;
                 if (q == 0) {
-                    ok = warp_wait(&bs->kfull[slot], lap & 1, bs, J);
+                    if (s_tile == ws.t0) ok = wait_bar(&bs->qfull, ws.piece & 1, bs, J);
+                    if (NQ == 1 && ok && s_count >= kBufs) ok = wait_bar(&bs->sempty[0][buf], ((s_count / kBufs) - 1) & 1, bs, J);
                     if (!ok) return;
                     tc_fence_after();
                 }
-                if (leader) {
-                    const uint32_t ka = sbase + off_k + slot * kChunk;
+                const uint32_t d = tbase + Col::s(q, buf);
+                for (int c = 0; c < J.kc; ++c) {
+                    int slot = kslot + c;
+                    uint32_t lap = klap;
+                    while (slot >= J.kring) { slot -= J.kring; ++lap; }
+                    if (q == 0 && !(ok = wait_bar(&bs->kfull[slot], lap & 1, bs, J))) return;
+                    const uint64_t a = q_desc + uint32_t(q * J.kc + c) * kChunkStep, b = k_desc + uint32_t(slot) * kChunkStep;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        umma_bf16(tbase + Col::s(q, s_count % kBufs),
-                                  umma_desc_sw128(sbase + (q * J.kc + c) * kChunk + kk * 32, 16, 1024),
-                                  umma_desc_sw128(ka + kk * 32, 16, 1024), idesc_s, (c | kk) != 0);
+                    for (int kk = 0; kk < 4; ++kk) umma_bf16(d, a + 2 * kk, b + 2 * kk, idesc_s, (c | kk) != 0);
                     if (q == NQ - 1) umma_commit(&bs->kempty[slot]);
                 }
-                __syncwarp();
-            }
-            if (leader) umma_commit(&bs->sfull[q][s_count % kBufs]);
-            if (q == NQ - 1) {
-                if (leader && s_tile == ws.t1 - 1) umma_commit(&bs->qempty);
-                kslot += J.kc;
-                while (kslot >= J.kring) { kslot -= J.kring; ++klap; }
-                ++s_count;
-                if (++s_tile == ws.t1) {
-                    s_more = ws.next(plan);
-                    s_tile = ws.t0;
-                }
-            }
-            __syncwarp();
-        };
-        for (int q = 0; q < NQ && ok; ++q) issue_s(q);
-        for (int i = 0; ok; ++i) {
-            if (i == 0 || p_tile == wp.t1) {
-                if (!wp.next(plan)) break;
-                p_tile = wp.t0;
-            }
-            if (NQ == 1 && s_more) issue_s(0);
-            const bool first = p_tile == wp.t0;
-            const int lo = wp.s.lo(p_tile), hi = wp.s.hi(p_tile);
-            const bool own_rows = p_tile >= wp.s.ctx_tiles;
-            const bool s_next = s_more;      // NQ == 2: the S tile issued behind this tile's P.V
-            // Every row tile's previous piece has left its O (and bad_values).
-            for (int q = 0; q < NQ && ok && first && wp.piece > 0; ++q) ok = warp_wait(&bs->oempty[q], (wp.piece - 1) & 1, bs, J);
-            for (int q = 0; q < NQ && ok; ++q) {
-                ok = warp_wait(&bs->pfull[q][i & 1], (i >> 1) & 1, bs, J);
-                if (!ok) break;
-                tc_fence_after();
-                for (int c = 0; c < J.vc && ok; ++c) {
-                    int slot = vslot + c;
-                    uint32_t lap = vlap;
-                    while (slot >= J.vring) { slot -= J.vring; ++lap; }
-                    if (q == 0) {
-                        ok = warp_wait(&bs->vfull[slot], lap & 1, bs, J);
-                        if (!ok) break;
-                        if (lo > 0 || hi < kKeys || own_rows) {
-                            // Rows nobody sees are zeroed (their P is 0, and 0 x NaN is not), and so are
-                            // infinities and NaN among the nodes' values: the epilogue adds those to the
-                            // rows that see them.
-                            uint4* rows = reinterpret_cast<uint4*>(smem + off_v + slot * kChunk);
-                            bool bad = false;
-                            for (int j = lane; j < kKeys * 8; j += 32) {
-                                const int r = j >> 3;
-                                if (r < lo || r >= hi) {
-                                    rows[j] = make_uint4(0, 0, 0, 0);
-                                } else if (own_rows) {
-                                    constexpr uint32_t kExp = kHalf ? 0x7c00u : 0x7f80u;
-                                    uint4 v = rows[j];
-                                    uint32_t* x = &v.x;
-                                    bool hit = false;
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        if ((x[e] & kExp) == kExp) { x[e] &= 0xffff0000u; hit = true; }
-                                        if ((x[e] >> 16 & kExp) == kExp) { x[e] &= 0xffffu; hit = true; }
-                                    }
-                                    if (hit) { rows[j] = v; bad = true; }
-                                }
-                            }
-                            if (__any_sync(0xffffffffu, bad) && leader)
-                                *const_cast<volatile int*>(&bs->bad_values) = wp.piece + 1;
-                            __threadfence_block();
-                            fence_async_shared();
-                            __syncwarp();
-                        }
-                        tc_fence_after();
+                umma_commit(&bs->sfull[q][buf]);
+                if (q == NQ - 1) {
+                    if (s_tile == ws.t1 - 1) umma_commit(&bs->qempty);
+                    kslot += J.kc;
+                    while (kslot >= J.kring) { kslot -= J.kring; ++klap; }
+                    ++s_count;
+                    if (++s_tile == ws.t1) {
+                        s_more = ws.next(plan);
+                        s_tile = ws.t0;
                     }
-                    if (leader) {
-                        const uint32_t va = sbase + off_v + slot * kChunk;
+                }
+            };
+            for (int q = 0; q < NQ && ok; ++q) issue_s(q);
+            for (int i = 0; ok; ++i) {
+                if (i == 0 || p_tile == wp.t1) {
+                    if (!wp.next(plan)) break;
+                    p_tile = wp.t0;
+                }
+                if (NQ == 1 && s_more) issue_s(0);
+                const bool first = p_tile == wp.t0;
+                const bool s_next = s_more;      // NQ == 2: the S tile issued behind this tile's P.V
+                // Every row tile's previous piece has left its O.
+                for (int q = 0; q < NQ && ok && first && wp.piece > 0; ++q) ok = wait_bar(&bs->oempty[q], (wp.piece - 1) & 1, bs, J);
+                if (ok) ok = wait_bar(&bs->vfull[stage], vlap & 1, bs, J);
+                const uint64_t vb = v_desc + uint32_t(stage * J.vc) * kChunkStep;
+                for (int q = 0; q < NQ && ok; ++q) {
+                    if (!(ok = wait_bar(&bs->pfull[q][i & 1], (i >> 1) & 1, bs, J))) break;
+                    tc_fence_after();
+                    const uint32_t a = tbase + Col::p(q, kBufs == 2 ? i & 1 : 0);
+                    // A V tile's chunks lie side by side: up to four are one MMA of N = 256.
+                    for (int c = 0; c < J.vc; c += 4) {
+                        const uint32_t d = tbase + Col::o(q) + 64u * c, id = idesc<kHalf>(128, 64 * min(4, J.vc - c), 0, 1);
+                        const uint64_t b = vb + uint32_t(c) * kChunkStep;
 #pragma unroll
                         for (int ks = 0; ks < kKeys / 16; ++ks)
-                            umma_ts(tbase + Col::o(q) + 64u * c, tbase + Col::p(q, i % kBufs) + 8u * ks,
-                                    umma_desc_sw128(va + ks * 2048, kChunk, 1024), idesc_o, (!first || ks > 0) ? 1u : 0u);
-                        if (q == NQ - 1) umma_commit(&bs->vempty[slot]);
+                            umma_ts(d, a + 8u * ks, b + 128 * ks, id, (!first || ks > 0) ? 1u : 0u);
                     }
-                    __syncwarp();
+                    if (q == NQ - 1) umma_commit(&bs->vempty[stage]);
+                    umma_commit(&bs->odone[q][i & 1]);
+                    if (NQ == 2 && s_next) issue_s(q);
                 }
-                if (ok && leader) umma_commit(&bs->odone[q][i & 1]);
-                __syncwarp();
-                if (NQ == 2 && ok && s_next) issue_s(q);
+                if (++stage == J.vstages) { stage = 0; ++vlap; }
+                ++p_tile;
             }
-            vslot += J.vc;
-            while (vslot >= J.vring) { vslot -= J.vring; ++vlap; }
-            ++p_tile;
+            umma_commit(&bs->final_mma);
         }
-        if (leader) umma_commit(&bs->final_mma);
+        __syncwarp();
     } else if (any && warp >= 4) {
         // ---- softmax and epilogue of row tile qt: thread <-> row (TMEM lane) ----
         const int qt = (warp - 4) >> 2, quarter = warp & 3;
@@ -428,7 +432,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         const uint32_t o_base = tbase + lane_addr + Col::o(qt);
         const int jh = r % J.group;
         bool failed = false;
-        int i = 0;                                              // tiles done
+        int i = 0, stage = 0;                                   // tiles done, V stage
+        uint32_t vlap = 0;
         Walk<Plan<NQ>> w;
         w.start(plan, &bs->share);
         while (!failed && w.next(plan)) {
@@ -438,54 +443,55 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             const int32_t* words = J.mask ? J.mask + w.b * J.mask_stride + int64_t(min(t, J.nodes - 1)) * J.words : nullptr;
             float m_run = -INFINITY, l_run = 0.f;
             for (int tile = w.t0; tile < w.t1; ++tile, ++i) {
-                const int sb = i % kBufs;
+                const int sb = kBufs == 2 ? i & 1 : 0;
+                const bool masked = needs_fix(w.s, tile);
+                // Which keys the row sees, 32 to a word.
+                uint32_t seen[kKeys / 32];
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < kKeys / 32; ++c)
+                        seen[c] = w.s.has_nodes(tile) ? seen_keys(words, J.words, t, w.s.end - w.s.len, tile * kKeys + 32 * c - w.s.len)
+                                                      : low_bits(w.s.hi(tile) - 32 * c);
+                }
                 if (!warp_wait(&bs->sfull[qt][sb], (i / kBufs) & 1, bs, J)) { failed = true; break; }
                 tc_fence_after();
                 const uint32_t s_addr = tbase + lane_addr + Col::s(qt, sb);
                 const uint32_t p_addr = tbase + lane_addr + Col::p(qt, sb);
-                const int row0 = w.s.row0(tile), hi = w.s.hi(tile);
-                const bool own_rows = tile >= w.s.ctx_tiles;
-                auto seen = [&](int c) -> uint32_t {            // of the keys 32c .. 32c + 31
-                    return own_rows ? seen_nodes(words, J.words, t, w.s.nodes, row0 + 32 * c - w.s.len) : low_bits(hi - 32 * c);
-                };
-                const bool masked = own_rows || hi < kKeys;
-                float v[NQ == 1 ? kKeys : 32];
-                float mx = -INFINITY;
-                if (warp_live) {
+                // kStep scores at a time, twice over them: the row maximum, then the probabilities
+                // (loops, not one straight run: the code of a tile has to come through the
+                // instruction cache once per launch).  Wide rows have one S buffer and hold all
+                // of a tile's scores, so that the next S may start.
+                constexpr int kStep = kWide ? kKeys : 64;
+                float v[kStep];
+                auto load = [&](int c) {
 #pragma unroll
-                    for (int c = 0; c < kKeys / 32; ++c) {
-                        float* x = NQ == 1 ? v + 32 * c : v;
-                        tmem_ld32(s_addr + 32u * c, x);
-                        if (NQ != 1 || c == kKeys / 32 - 1) tmem_wait_ld();
-                        if constexpr (NQ != 1) {
-                            if (masked) {
-                                const uint32_t bits = seen(c);
+                    for (int e = 0; e < kStep; e += 32) tmem_ld32(s_addr + uint32_t(c + e), v + e);
+                    tmem_wait_ld();
+                    if (masked) {
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, bits >> e & 1 ? x[e] : -INFINITY);
-                            } else {
+                        for (int e = 0; e < kStep; e += 32) {
+                            const uint32_t bits = kWide ? seen[e / 32] : e == 0 ? (c ? seen[2] : seen[0]) : (c ? seen[3] : seen[1]);
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, x[e]);
-                            }
+                            for (int k = 0; k < 32; ++k)
+                                if (!(bits >> k & 1)) v[e + k] = -INFINITY;
                         }
                     }
+                };
+                float mx = -INFINITY;
+                if (warp_live) {
+#pragma unroll 1
+                    for (int c = 0; c < kKeys; c += kStep) {
+                        load(c);
+                        float m2 = -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < kStep; e += 2) { mx = fmaxf(mx, v[e]); m2 = fmaxf(m2, v[e + 1]); }
+                        mx = fmaxf(mx, m2);
+                    }
                 }
-                if constexpr (NQ == 1) {
+                if constexpr (kWide) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bs->sempty[0][sb]);
-                    if (warp_live) {
-                        if (masked) {
-#pragma unroll
-                            for (int c = 0; c < kKeys / 32; ++c) {
-                                const uint32_t bits = seen(c);
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (!(bits >> e & 1)) v[(NQ == 1 ? 32 * c : 0) + e] = -INFINITY;
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < (NQ == 1 ? kKeys : 32); ++e) mx = fmaxf(mx, v[e]);
-                    }
                 }
                 mx *= J.scale_log2;                             // scale > 0
                 float alpha = 1.f;
@@ -496,12 +502,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 }
                 // P(i) takes the buffer of P(i - kBufs); a rescale of O needs P.V(i - 1) done.
                 const bool rescale = tile > w.t0 && __any_sync(0xffffffffu, alpha != 1.f);
-                const int back = rescale ? 1 : kBufs;
+                const bool fix = qt == 0 && masked;
+                const int back = rescale || fix ? 1 : kBufs;
                 if (i >= back) {
                     if (!warp_wait(&bs->odone[qt][(i - back) & 1], ((i - back) >> 1) & 1, bs, J)) { failed = true; break; }
                     tc_fence_after();
                 }
                 if (rescale) {
+#pragma unroll 1
                     for (int c = 0; c < 2 * J.vc; ++c) {
                         float o[32];
                         tmem_ld32(o_base + 32u * c, o);
@@ -514,33 +522,41 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 }
                 if (warp_live) {
                     const float shift = m_run == -INFINITY ? 0.f : m_run;
-                    float sum = 0.f;
+                    float sum = 0.f, sum2 = 0.f;
+#pragma unroll 1
+                    for (int c = 0; c < kKeys; c += kStep) {
+                        if constexpr (!kWide) load(c);
 #pragma unroll
-                    for (int c = 0; c < kKeys / 32; ++c) {
-                        float* x = NQ == 1 ? v + 32 * c : v;
-                        if constexpr (NQ != 1) {
-                            tmem_ld32(s_addr + 32u * c, x);
-                            tmem_wait_ld();
-                            if (masked) {
-                                const uint32_t bits = seen(c);
+                        for (int e = 0; e < kStep; e += 32) {
+                            float packed[16];
 #pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (!(bits >> e & 1)) x[e] = -INFINITY;
+                            for (int k = 0; k < 16; ++k) {
+                                const float p0 = sfu_exp2(fmaf(v[e + 2 * k], J.scale_log2, -shift));
+                                const float p1 = sfu_exp2(fmaf(v[e + 2 * k + 1], J.scale_log2, -shift));
+                                sum += p0;
+                                sum2 += p1;
+                                packed[k] = __uint_as_float(pack2<kHalf>(p0, p1));
                             }
+                            tmem_st16(p_addr + uint32_t(c + e) / 2, packed);
                         }
-                        float packed[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float p0 = sfu_exp2(fmaf(x[2 * e], J.scale_log2, -shift));
-                            const float p1 = sfu_exp2(fmaf(x[2 * e + 1], J.scale_log2, -shift));
-                            sum += p0 + p1;
-                            packed[e] = __uint_as_float(pack2<kHalf>(p0, p1));
-                        }
-                        tmem_st16(p_addr + 16u * c, packed);
                     }
-                    l_run += sum;
+                    l_run += sum + sum2;
                     tmem_wait_st();
                 }
+                if constexpr (NQ == 1 && !kWide) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bs->sempty[0][sb]);
+                }
+                if (fix) {
+                    // P.V(i - 1) is done, so this tile is the next that lands in its stage.
+                    if (!warp_wait(&bs->vfull[stage], vlap & 1, bs, J)) { failed = true; break; }
+                    const bool bad = fix_values<kHalf>(smem + off_v + uint32_t(stage * J.vc) * kChunk, J.vc, r, r < w.s.hi(tile),
+                                                       tile * kKeys + r >= w.s.len);
+                    if (bad) *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) = w.piece + 1;
+                    fence_async_shared();
+                }
+                if (++stage == J.vstages) { stage = 0; ++vlap; }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bs->pfull[qt][i & 1]);
@@ -550,11 +566,13 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             if (!warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J)) { failed = true; break; }
             tc_fence_after();
             const bool whole = w.whole();
-            const bool bad = *const_cast<volatile int*>(&bs->bad_values) == w.piece + 1;
+            const bool bad = *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) == w.piece + 1;
             const float inv = l_run != 0.f ? 1.f / l_run : 0.f;      // a NaN sum stays NaN
             const float lse2 = l_run != 0.f ? m_run + log2f(l_run) : -INFINITY;
             const int h = w.g * J.group + jh;
-            const int64_t slot_row = int64_t(2 * blockIdx.x + (w.piece > 0)) * (NQ * J.tile_rows) + qt * J.tile_rows + r;
+            const int rows = NQ * J.tile_rows, slot = 2 * blockIdx.x + (w.piece > 0), row = qt * J.tile_rows + r;
+            float4* part = reinterpret_cast<float4*>(J.part_o) + int64_t(slot) * (J.dim_v / 4) * rows + row;
+#pragma unroll 1
             for (int c = 0; c < 2 * J.vc; ++c) {
                 float o[32];
                 if (warp_live) {
@@ -564,16 +582,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 if (live) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] *= inv;
-                    if (bad && w.t1 > w.s.ctx_tiles) {
+                    if (bad) {
                         // Infinities and NaN of the nodes' values, for the rows that see them.
                         for (int n0 = 0; n0 < w.s.nodes; n0 += 32) {
-                            uint32_t bits = seen_nodes(words, J.words, t, w.s.nodes, n0);
+                            uint32_t bits = seen_keys(words, J.words, t, w.s.nodes, n0);
                             for (; bits; bits &= bits - 1) {
-                                const int row = w.s.len + n0 + __ffs(int(bits)) - 1;
-                                if (row < w.s.row0(max(w.t0, w.s.ctx_tiles)) || row >= w.s.row0(w.t1 - 1) + kKeys) continue;
+                                int at = w.s.len + n0 + __ffs(int(bits)) - 1;
+                                if (at < w.t0 * kKeys || at >= w.t1 * kKeys) continue;
                                 int64_t page = J.shared_cache ? 0 : w.b;
-                                int at = row;
-                                if (J.paged) cache_row(J.cache, w.b, row, page, at);
+                                if (J.paged) cache_row(J.cache, w.b, at, page, at);
                                 const int64_t base = page * J.cache.v_stride[0] + at * J.cache.v_stride[1] + w.g * J.cache.v_stride[2];
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) {
@@ -597,19 +614,18 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                                                pack2<kHalf>(o[8 * u + 4], o[8 * u + 5]), pack2<kHalf>(o[8 * u + 6], o[8 * u + 7]));
                         }
                     } else {
-                        float* dst = J.part_o + slot_row * J.dim_v;
+                        // [slot][4 dims][row]: the rows of a warp side by side.
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const int d = 32 * c + 4 * u;
-                            if (d < J.dim_v) *reinterpret_cast<float4*>(dst + d) = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
-                        }
+                        for (int u = 0; u < 8; ++u)
+                            if (32 * c + 4 * u < J.dim_v)
+                                part[int64_t(8 * c + u) * rows] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
                     }
                 }
                 __syncwarp();
             }
             if (live) {
                 if (whole) J.lse[(int64_t(w.b) * J.nodes + t) * J.heads + h] = lse2 * kLn2;
-                else J.part_lse[slot_row] = lse2;
+                else J.part_lse[slot * rows + row] = lse2;
             }
             tc_fence_before();
             __syncwarp();
@@ -628,7 +644,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 mbar_wait(&bs->kfull[s], 0, 100000000ull);
                 mbar_wait(&bs->kfull[s], 1, 100000000ull);
             }
-            for (int s = 0; s < J.vring; ++s) {
+            for (int s = 0; s < J.vstages; ++s) {
                 mbar_wait(&bs->vfull[s], 0, 100000000ull);
                 mbar_wait(&bs->vfull[s], 1, 100000000ull);
             }
@@ -644,74 +660,73 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
 }
 
 // Merges the pieces of a segment's rows, and writes the rows that see nothing:
-// kCombineRows rows of a (sequence, KV head, row group) per block, a warp per
-// row at a time.
+// 32 rows (a lane each) and 64 dims (16 to a warp) of a (sequence, KV head,
+// row group) per block.
 template <int NQ, bool kHalf>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Job J) {
     __shared__ long long scan[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = blockIdx.x;
-    const int group = s % J.row_groups;
-    s /= J.row_groups;
-    const int g = s % J.kv_heads, b = s / J.kv_heads;
+    int at = blockIdx.x;
+    const int group = at % J.row_groups;
+    at /= J.row_groups;
+    const int g = at % J.kv_heads, b = at / J.kv_heads;
     const Plan<NQ> plan(J);
     long long total, before;
     sum_units<128>(plan, b, total, before, scan);
-    const Seq q = plan.sequence(b);
+    const Seq s = plan.sequence(b);
     int c0 = 0, c1 = 0, slot0 = 0;
-    const bool some = group < q.groups && q.tiles > 0;
+    const bool some = group < s.groups && s.tiles > 0;
     if (some) {
-        const long long u0 = before + ((long long)g * q.groups + group) * q.tiles;
+        const long long u0 = before + ((long long)g * s.groups + group) * s.tiles;
         const int ctas = share_count(total, J.ctas);
         c0 = share_of(total, u0, ctas);
-        c1 = share_of(total, u0 + q.tiles - 1, ctas);
+        c1 = share_of(total, u0 + s.tiles - 1, ctas);
         slot0 = 2 * c0 + (share_begin(total, c0, ctas) != u0 ? 1 : 0);
     }
-    if (threadIdx.x == 0 && g == 0 && group == 0 && blockIdx.y == 0) {
+    if (threadIdx.x == 0 && g == 0 && group == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
         const int len = __ldg(J.lengths + b), nodes = J.nodes_len ? __ldg(J.nodes_len + b) : J.nodes;
-        if (len != q.len || nodes != q.nodes) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+        if (len != s.len || nodes != s.nodes || (!J.context_only && s.end != s.len + s.nodes)) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
     }
+    const int rows = NQ * J.tile_rows, r = blockIdx.y * 32 + lane, d0 = blockIdx.z * 64 + 16 * warp;
+    const int t = group * NQ * J.tpt + r / J.group, h = g * J.group + r % J.group;
+    const bool live = some && t < s.nodes;
     grid_dependency_wait();
-    const int rows = NQ * J.tile_rows;
-    for (int k = warp; k < kCombineRows; k += 4) {
-        const int r = blockIdx.y * kCombineRows + k;
-        if (r >= rows) break;
-        const int t = group * NQ * J.tpt + r / J.group, h = g * J.group + r % J.group;
-        if (t >= J.nodes) break;
-        const bool live = some && t < q.nodes;
-        if (live && c0 == c1) continue;
-        uint16_t* dst = static_cast<uint16_t*>(J.out) + b * J.o_sb + t * J.o_st + h * J.o_sh;
-        float* lse = J.lse + (int64_t(b) * J.nodes + t) * J.heads + h;
-        if (!live) {
-            for (int d = 8 * lane; d < J.dim_v; d += 256) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
-            if (lane == 0) *lse = -INFINITY;
-            continue;
-        }
-        auto row_of = [&](int c) { return int64_t(c == c0 ? slot0 : 2 * c) * rows + r; };
-        float m = -INFINITY;
-        for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, J.part_lse[row_of(c)]);
+    if (r >= rows || t >= J.nodes || d0 >= J.dim_v || (live && c0 == c1)) return;
+    auto slot_of = [&](int c) { return int64_t(c == c0 ? slot0 : 2 * c); };
+    float m = -INFINITY, sum = 0.f, shift = 0.f;
+    float4 acc[4];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float shift = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
-        for (int c = c0 + lane; c <= c1; c += 32) sum += exp2f(J.part_lse[row_of(c)] - shift);
+    for (int u = 0; u < 4; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+#pragma unroll 4
+        for (int c = c0; c <= c1; ++c) m = fmaxf(m, J.part_lse[slot_of(c) * rows + r]);
+        shift = m == -INFINITY ? 0.f : m;
+#pragma unroll 2
+        for (int c = c0; c <= c1; ++c) {
+            const int64_t slot = slot_of(c);
+            const float w = exp2f(J.part_lse[slot * rows + r] - shift);
+            const float4* part = reinterpret_cast<const float4*>(J.part_o) + (slot * (J.dim_v / 4) + d0 / 4) * rows + r;
+            float4 x[4];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = sum != 0.f ? 1.f / sum : 0.f;
-        if (lane == 0) *lse = sum != 0.f ? (shift + log2f(sum)) * kLn2 : -INFINITY;
-        for (int d = 4 * lane; d < J.dim_v; d += 128) {
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c = c0; c <= c1; ++c) {
-                const int64_t row = row_of(c);
-                const float w = exp2f(J.part_lse[row] - shift);
-                if (w == 0.f) continue;
-                const float4 x = *reinterpret_cast<const float4*>(J.part_o + row * J.dim_v + d);
-                acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y);
-                acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
-            }
-            *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack2<kHalf>(acc.x * inv, acc.y * inv), pack2<kHalf>(acc.z * inv, acc.w * inv));
+            for (int u = 0; u < 4; ++u) x[u] = d0 + 4 * u < J.dim_v ? part[int64_t(u) * rows] : make_float4(0.f, 0.f, 0.f, 0.f);
+            sum += w;
+            if (w != 0.f)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    acc[u].x = fmaf(w, x[u].x, acc[u].x); acc[u].y = fmaf(w, x[u].y, acc[u].y);
+                    acc[u].z = fmaf(w, x[u].z, acc[u].z); acc[u].w = fmaf(w, x[u].w, acc[u].w);
+                }
         }
     }
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    uint16_t* dst = static_cast<uint16_t*>(J.out) + b * J.o_sb + t * J.o_st + h * J.o_sh + d0;
+#pragma unroll
+    for (int u = 0; u < 4; u += 2)
+        if (d0 + 4 * u < J.dim_v)
+            *reinterpret_cast<uint4*>(dst + 4 * u) =
+                make_uint4(pack2<kHalf>(acc[u].x * inv, acc[u].y * inv), pack2<kHalf>(acc[u].z * inv, acc[u].w * inv),
+                           pack2<kHalf>(acc[u + 1].x * inv, acc[u + 1].y * inv), pack2<kHalf>(acc[u + 1].z * inv, acc[u + 1].w * inv));
+    if (d0 == 0) J.lse[(int64_t(b) * J.nodes + t) * J.heads + h] = sum != 0.f ? (shift + log2f(sum)) * kLn2 : -INFINITY;
 }
 
 // ------------------------------------------------------------------- host --
@@ -758,7 +773,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
     }
     kernel<<<J.ctas, 128 + 128 * NQ, kSmemBytes, stream>>>(qm, km, vm, J);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(J.batch * J.kv_heads * J.row_groups, (NQ * J.tile_rows + kCombineRows - 1) / kCombineRows);
+    cfg.gridDim = dim3(J.batch * J.kv_heads * J.row_groups, (NQ * J.tile_rows + 31) / 32, (J.dim_v + 63) / 64);
     cfg.blockDim = dim3(128);
     cfg.stream = stream;
     cudaLaunchAttribute dependent{};
@@ -836,8 +851,8 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.vc = (a->dim_v + 63) / 64;
     J.dim_v = a->dim_v;
     const int slots = int(kTileArea / kChunk) - nq * J.kc;
-    J.kring = std::min(kMaxRing, slots / 2);
-    J.vring = std::min(kMaxRing, slots - J.kring);
+    J.vstages = std::max(1, slots / 2 / J.vc);
+    J.kring = std::min(kMaxRing, slots - J.vstages * J.vc);
     J.context_only = a->context_only;
     J.paged = paged;
     J.cache = cache_view(cache);
