@@ -86,14 +86,14 @@ __device__ __forceinline__ void find_share(const Plan& P, Share* share) {
 // A CTA's pieces in order (CTAs with a share only).
 template <class Plan>
 struct Walk {
-    long long u, end;           // next unit, end of the share
+    int left;                   // units of the share still to come
     int b, g, group;            // the piece's segment
     decltype(((const Plan*)nullptr)->sequence(0)) s;
     int t0, t1;                 // its key tiles
     int piece;                  // pieces begun before this one
     __device__ __forceinline__ void start(const Plan& P, const Share* share) {
-        u = share_begin(share->total, blockIdx.x, share->ctas);
-        end = share_begin(share->total, blockIdx.x + 1, share->ctas);
+        const long long u = share_begin(share->total, blockIdx.x, share->ctas);
+        left = int(share_begin(share->total, blockIdx.x + 1, share->ctas) - u);
         piece = -1;
         b = share->first_b;
         s = P.sequence(b);
@@ -105,7 +105,7 @@ struct Walk {
     }
     // Moves to the next piece; false when the share is done.
     __device__ __forceinline__ bool next(const Plan& P) {
-        if (u >= end) return false;
+        if (left == 0) return false;
         if (t1 >= s.tiles) {
             t1 = 0;
             if (++group >= s.groups) {
@@ -118,8 +118,8 @@ struct Walk {
             }
         }
         t0 = t1;
-        t1 = int(min((long long)s.tiles, t0 + (end - u)));
-        u += t1 - t0;
+        t1 = min(s.tiles, t0 + left);
+        left -= t1 - t0;
         ++piece;
         return true;
     }

@@ -5,15 +5,15 @@
 //   s_n = scale q . k_n,   lse = log sum_n e^{s_n},   out = sum_n e^{s_n - lse} v_n.
 // The G = heads / kv_heads query heads of a KV head share its keys, so the
 // rows of a KV head are (node, head of the group) pairs: 128 of them (whole
-// nodes) fill one M = 128 tile of the tensor core, and a 128-key tile of K and
-// V serves them all:
-//   S [128 rows x 128 keys] = Q . K^T,   O [128 rows x dim_v] += P . V
+// nodes) fill one M = 128 tile of the tensor core, and a 64-key tile of K and V
+// serves one or two such row tiles:
+//   S [128 rows x 64 keys] = Q . K^T,   O [128 rows x dim_v] += P . V
 // with tcgen05 (fp32 accumulators in TMEM; P = 2^(s - m) written back to TMEM
 // in the inputs' 16-bit type as the A operand of the second product, which
 // costs about what rounding the output costs; the row sums stay in fp32
 // before that rounding, so lse keeps fp32 accuracy).
 //
-// Work: a unit is one 128-key tile of one (sequence, KV head, group of NQ row
+// Work: a unit is one 64-key tile of one (sequence, KV head, group of NQ row
 // tiles) segment: the context rows, then the nodes' own rows, of which each
 // row sees what its ancestor words say.  The units of all
 // segments in a row are cut into one equal share per CTA; a share's part of a
@@ -25,9 +25,16 @@
 // Bound: with few rows per KV head HBM (each K / V row read once); with 128
 // rows or more the tensor cores and the exponentials.
 //
+// Why 64 keys: S and P of a tile fit 64 tensor-memory columns, so two tiles are
+// in flight for each row tile next to O (320 + 2 x 64, or 2 x (128 + 2 x 64)
+// columns): the S of tile n + 1 is there when the softmax of tile n ends, and
+// the softmax never waits for a product.  (With 128-key tiles and one S per row
+// tile, softmax and products took turns: 4,870 cycles for two row tiles and 128
+// keys, 2,700 of them the softmax.)
+//
 // One CTA per SM, warps: 0 = Q and K loads (TMA), 3 = V loads, 1 = MMA issue
-// (one thread), 2 = TMEM owner, 4-7 (and 8-11) = softmax of row tile 0 (1), a
-// thread per row.  Every wait is bounded.
+// of row tile 0, 2 = TMEM owner and MMA issue of row tile 1, 4-7 (and 8-11) =
+// softmax of row tile 0 (1), a thread per row.  Every wait is bounded.
 #include <algorithm>
 
 #include "cache_view.cuh"
@@ -38,21 +45,21 @@ namespace slimkv {
 namespace {
 
 constexpr int kRows = 128;
-constexpr int kKeys = 128;
-constexpr uint32_t kChunk = 128 * 128;           // [128 x 64] 16-bit elements
+constexpr int kKeys = 64;                        // keys of a tile
+constexpr uint32_t kQChunk = 128 * 128;          // [128 rows x 64] 16-bit elements
+constexpr uint32_t kChunk = kKeys * 128;         // [64 keys x 64]
 constexpr uint32_t kTileArea = 224 * 1024;
-constexpr int kMaxRing = 8;
+constexpr int kMaxRing = 10;
 constexpr int kMaxChunks = 5;                    // dims <= 320
 constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a row's maximum grows by more than 2^8
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 struct Bars {
-    uint64_t kfull[kMaxRing], kempty[kMaxRing];                 // per 64-column chunk
-    uint64_t vfull[kMaxRing], vempty[kMaxRing];                 // per tile
+    uint64_t kfull[kMaxRing], kempty[kMaxRing], vfull[kMaxRing], vempty[kMaxRing], vfixed[kMaxRing];
     uint64_t qfull, qempty;
-    // [row tile][buffer]
-    uint64_t sfull[2][2], sempty[2][2], pfull[2][2], odone[2][2], oempty[2], final_mma;
+    // [row tile][tile parity]
+    uint64_t sfull[2][2], pfull[2][2], odone[2][2], oempty[2], final_mma;
     uint32_t tmem_base;
     int abort;
     int bad_values[2];           // 1 + a piece whose node values hold infinities or NaN
@@ -66,8 +73,7 @@ struct Job {
     int tpt, tile_rows;         // nodes of a row tile and its rows (tpt * group <= 128)
     int row_groups;             // groups of NQ row tiles
     int kc, vc, dim_v;          // 64-column chunks of a K / V row
-    int kring;                  // K chunks in shared memory
-    int vstages;                // V tiles in shared memory
+    int kring, vring;           // ring slots: of a whole row, or (dims above 128) of one chunk
     int context_only, paged, shared_cache;
     int box;                    // rows of one TMA box
     CacheView cache;
@@ -137,6 +143,21 @@ template <bool kHalf>
 __device__ __forceinline__ constexpr uint32_t idesc(int m, int n, int a_mn, int b_mn) {
     return umma_idesc_bf16(m, n, a_mn, b_mn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
 }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t bits2(float2 x) { return uint64_t(__float_as_uint(x.y)) << 32 | __float_as_uint(x.x); }
+__device__ __forceinline__ float2 float2_of(uint64_t x) {
+    return make_float2(__uint_as_float(uint32_t(x)), __uint_as_float(uint32_t(x >> 32)));
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+    return float2_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return float2_of(d);
+}
 // A from tensor memory (two 16-bit K elements per column), B from shared memory.
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc_, uint32_t accumulate) {
     asm volatile(
@@ -160,20 +181,20 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* b
     report(J.status, SLIMKV_DEVICE_TIMEOUT);
     return false;
 }
+__device__ __forceinline__ bool all_lanes(bool x) { return __all_sync(0xffffffffu, x); }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
     return __all_sync(0xffffffffu, wait_bar(bar, parity, bs, J));
 }
 
-// Tensor memory columns.  One row tile, dims <= 128: O, two S, two P.  One row
-// tile, wider: O (up to 320), S, P.  Two row tiles: O and S of each, P in its
-// S (a tile's scores are in registers before its P is written, and the next
-// S is issued behind the P.V that reads that P).
-template <int NQ, bool kWide>
+// Tensor memory columns: O of each row tile, then two S tiles of each; a tile's
+// P goes over its S, which is in registers by then (and the next S there is
+// issued behind the P.V that reads that P).
+template <int NQ, int C>
 struct Columns {
-    static constexpr int kBufs = NQ == 1 && !kWide ? 2 : 1;
     __device__ static constexpr uint32_t o(int q) { return uint32_t(q * 128); }
-    __device__ static constexpr uint32_t s(int q, int buf) { return NQ == 2 ? 256u + 128u * q : kWide ? 320u : 128u + 128u * buf; }
-    __device__ static constexpr uint32_t p(int q, int buf) { return NQ == 2 ? s(q, 0) : kWide ? 448u : 384u + 64u * buf; }
+    __device__ static constexpr uint32_t s(int q, int buf) {
+        return (C == 0 ? 320u : 128u * NQ) + uint32_t((2 * q + buf) * kKeys);
+    }
 };
 
 __device__ __forceinline__ uint32_t mask_word(const int32_t* row, int words, int w) {
@@ -207,20 +228,26 @@ __device__ __forceinline__ int box_of(const Job& J, const W& w, int tile, int la
     }
     return int(page);
 }
+// Slot and lap of a tile's first ring entry, `per` entries to a tile.
+__device__ __forceinline__ void ring_at(int tile, int per, int ring, int& slot, uint32_t& lap) {
+    const int n = tile * per;
+    lap = uint32_t(n / ring);
+    slot = n - int(lap) * ring;
+}
 // Whether a V tile holds rows that nobody sees, or the nodes' own.
 __device__ __forceinline__ bool needs_fix(const Seq& s, int tile) { return s.has_nodes(tile) || s.hi(tile) < kKeys; }
 
-// Row r of a V tile in shared memory: zeroed when nobody sees it (its P is 0,
+// Row r of a V chunk in shared memory (every second 16 bytes): zeroed when nobody sees it (its P is 0,
 // and 0 x NaN is not 0); of a node's row, infinities and NaN become 0 (the
 // epilogue adds them to the rows that see them).  True when there were any.
 template <bool kHalf>
-__device__ __forceinline__ bool fix_values(uint8_t* tile, int chunks, int r, bool seen, bool node) {
+__device__ __forceinline__ bool fix_values(uint8_t* chunk, int r, int u0, bool seen, bool node) {
     constexpr uint32_t kExp = kHalf ? 0x7c00u : 0x7f80u;
     if (seen && !node) return false;
     bool bad = false;
 #pragma unroll 1
-    for (int j = 0; j < chunks * 8; ++j) {
-        uint4* at = reinterpret_cast<uint4*>(tile + (j >> 3) * kChunk + r * 128) + ((j ^ r) & 7);
+    for (int u = u0; u < 8; u += 2) {
+        uint4* at = reinterpret_cast<uint4*>(chunk + r * 128) + ((u ^ r) & 7);
         uint4 v = make_uint4(0, 0, 0, 0);
         bool write = !seen;
         if (seen) {
@@ -238,39 +265,53 @@ __device__ __forceinline__ bool fix_values(uint8_t* tile, int chunks, int r, boo
     return bad;
 }
 
+// Ring geometry.  Rows of up to 128 dims: a slot is a whole row of C chunks
+// (shorter rows are filled up with zeros), all of it constants; wider rows: a
+// slot is one chunk of the job's (a tile's five take too much for two tiles).
+template <int NQ, int C>
+struct Rings {
+    static constexpr int kGroup = C == 0 ? 1 : C;
+    static constexpr int kFree = C == 0 ? 0 : int((kTileArea - uint32_t(NQ * C) * kQChunk) / kChunk);
+    static constexpr int kSlots = kFree / 2 / kGroup < kMaxRing ? kFree / 2 / kGroup : kMaxRing;
+    __host__ __device__ static int kc(const Job& J) { return C == 0 ? J.kc : C; }
+    __host__ __device__ static int vc(const Job& J) { return C == 0 ? J.vc : C; }
+    __host__ __device__ static int kring(const Job& J) { return C == 0 ? J.kring : kSlots; }
+    __host__ __device__ static int vring(const Job& J) { return C == 0 ? J.vring : kSlots; }
+};
+
 // ----------------------------------------------------------------- kernel --
-template <int NQ, bool kWide, bool kHalf>
+template <int NQ, int C, bool kHalf>
 __global__ void __launch_bounds__(128 + 128 * NQ, 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Job J) {
     constexpr int kThreads = 128 + 128 * NQ;
-    using Col = Columns<NQ, kWide>;
-    constexpr int kBufs = Col::kBufs;
+    using Col = Columns<NQ, C>;
+    using R = Rings<NQ, C>;
+    const int kc = R::kc(J), vc = R::vc(J), kring = R::kring(J), vring = R::vring(J);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Bars* bs = reinterpret_cast<Bars*>(smem + kTileArea);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // Layout: Q (NQ x kc chunks) | K ring | V ring.
-    const uint32_t off_k = uint32_t(NQ * J.kc) * kChunk;
-    const uint32_t off_v = off_k + uint32_t(J.kring) * kChunk;
+    const uint32_t off_k = uint32_t(NQ * kc) * kQChunk;
+    const uint32_t off_v = off_k + uint32_t(kring * R::kGroup) * kChunk;
 
     if (tid == 0) {
         for (int s = 0; s < kMaxRing; ++s) {
-            mbar_init(&bs->kfull[s], 1); mbar_init(&bs->kempty[s], 1);
-            mbar_init(&bs->vfull[s], 1); mbar_init(&bs->vempty[s], 1);
+            mbar_init(&bs->kfull[s], 1); mbar_init(&bs->kempty[s], NQ);
+            mbar_init(&bs->vfull[s], 1); mbar_init(&bs->vempty[s], NQ); mbar_init(&bs->vfixed[s], 4);
         }
         mbar_init(&bs->qfull, 1);
-        mbar_init(&bs->qempty, 1);
+        mbar_init(&bs->qempty, NQ);
         for (int q = 0; q < 2; ++q) {
             mbar_init(&bs->oempty[q], 4);
             for (int s = 0; s < 2; ++s) {
                 mbar_init(&bs->sfull[q][s], 1);
-                mbar_init(&bs->sempty[q][s], 4);
                 mbar_init(&bs->pfull[q][s], 4);
                 mbar_init(&bs->odone[q][s], 1);
             }
         }
-        mbar_init(&bs->final_mma, 1);
+        mbar_init(&bs->final_mma, NQ);
         bs->abort = 0;
         bs->bad_values[0] = bs->bad_values[1] = 0;
         fence_barrier_init();
@@ -284,12 +325,18 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tbase = bs->tmem_base;
+    const uint32_t tbase = 0;               // all 512 columns are this CTA's: they begin at column 0
     const uint32_t sbase = smem_u32(smem);
     const bool any = int(blockIdx.x) < bs->share.ctas;
 
-    if (any && warp == 0) {
-        // ---- each piece's Q, and the K chunks ----
+    if (any && (warp == 0 || warp == 3)) {
+        // ---- loads: warp 0 each piece's Q and the K chunks, warp 3 the V chunks ----
+        const bool keys = warp == 0;
+        const int chunks = keys ? kc : vc, per = R::kGroup, ring = keys ? kring : vring;
+        uint64_t* full = keys ? bs->kfull : bs->vfull;
+        uint64_t* empty = keys ? bs->kempty : bs->vempty;
+        const CUtensorMap* map = keys ? &kmap : &vmap;
+        uint8_t* dst = smem + (keys ? off_k : off_v);
         const int boxes = kKeys / J.box;
         int slot = 0;
         uint32_t lap = 0;
@@ -297,132 +344,140 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         Walk<Plan<NQ>> w;
         w.start(plan, &bs->share);
         while (ok && w.next(plan)) {
-            if (w.piece > 0 && !(ok = warp_wait(&bs->qempty, (w.piece - 1) & 1, bs, J))) break;
-            if (lane == 0) {
-                mbar_expect_tx(&bs->qfull, uint32_t(NQ * J.kc) * uint32_t(J.tile_rows) * 128u);
-                for (int q = 0; q < NQ; ++q)
-                    for (int c = 0; c < J.kc; ++c)
-                        tma_load_4d(smem + (q * J.kc + c) * kChunk, &qmap, &bs->qfull, c * 64, w.g * J.group,
-                                    (w.group * NQ + q) * J.tpt, w.b);
+            if (keys) {
+                if (w.piece > 0 && !(ok = warp_wait(&bs->qempty, (w.piece - 1) & 1, bs, J))) break;
+                if (lane == 0) {
+                    mbar_expect_tx(&bs->qfull, uint32_t(NQ * kc) * uint32_t(J.tile_rows) * 128u);
+                    for (int q = 0; q < NQ; ++q)
+                        for (int c = 0; c < kc; ++c)
+                            tma_load_4d(smem + (q * kc + c) * kQChunk, &qmap, &bs->qfull, c * 64, w.g * J.group,
+                                        (w.group * NQ + q) * J.tpt, w.b);
+                }
+                __syncwarp();
             }
-            __syncwarp();
             for (int tile = w.t0; tile < w.t1 && ok; ++tile) {
                 int row;
                 const int page = box_of(J, w, tile, lane, row);
-                for (int c = 0; c < J.kc; ++c) {
-                    if (lap && !(ok = warp_wait(&bs->kempty[slot], (lap - 1) & 1, bs, J))) break;
-                    if (lane == 0) mbar_expect_tx(&bs->kfull[slot], kChunk);
+                for (int c = 0; c < chunks; c += per) {
+                    if (lap && !(ok = warp_wait(&empty[slot], (lap - 1) & 1, bs, J))) break;
+                    if (lane == 0) mbar_expect_tx(&full[slot], uint32_t(per) * kChunk);
                     __syncwarp();
                     if (lane < boxes)
-                        tma_load_4d(smem + off_k + slot * kChunk + lane * J.box * 128, &kmap, &bs->kfull[slot], c * 64, w.g, row, page);
-                    if (++slot == J.kring) { slot = 0; ++lap; }
+                        for (int k = 0; k < per; ++k)
+                            tma_load_4d(dst + (slot * per + k) * kChunk + lane * J.box * 128, map, &full[slot], (c + k) * 64, w.g, row, page);
+                    if (++slot == ring) { slot = 0; ++lap; }
                 }
             }
         }
-    } else if (any && warp == 3) {
-        // ---- the V tiles ----
-        const int boxes = kKeys / J.box;
-        int stage = 0;
-        uint32_t lap = 0;
-        bool ok = true;
-        Walk<Plan<NQ>> w;
-        w.start(plan, &bs->share);
-        while (ok && w.next(plan)) {
-            for (int tile = w.t0; tile < w.t1; ++tile) {
-                int row;
-                const int page = box_of(J, w, tile, lane, row);
-                if (lap && !(ok = warp_wait(&bs->vempty[stage], (lap - 1) & 1, bs, J))) break;
-                if (lane == 0) mbar_expect_tx(&bs->vfull[stage], uint32_t(J.vc) * kChunk);
-                __syncwarp();
-                if (lane < boxes)
-                    for (int c = 0; c < J.vc; ++c)
-                        tma_load_4d(smem + off_v + (stage * J.vc + c) * kChunk + lane * J.box * 128, &vmap, &bs->vfull[stage], c * 64,
-                                    w.g, row, page);
-                if (++stage == J.vstages) { stage = 0; ++lap; }
+    } else if (any && warp <= NQ) {
+        // ---- MMA issue, a warp for each row tile: S two tiles ahead of P.V.  The tensor
+        // core queues only a few MMAs, so what the warp does between them is time lost,
+        // unless another warp's MMAs fill it (one warp for both row tiles: 8,100 cycles for
+        // 128 keys, two: XXXX).  The warp stays converged, its branches go by votes, and one
+        // elected thread has the instructions alone, so that operands are uniform registers. ----
+        const int q = NQ == 2 ? warp - 1 : 0;
+        const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0), idesc_o = idesc<kHalf>(128, 64 * R::kGroup, 0, 1);
+        // Matrix descriptors (K-major Q and K; MN-major V): the low word moves with the address.
+        constexpr uint64_t kQStep = kQChunk >> 4, kStep = kChunk >> 4;
+        const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024) + uint32_t(q * kc) * kQStep;
+        const uint64_t k_desc = umma_desc_sw128(sbase + off_k, 16, 1024), v_desc = umma_desc_sw128(sbase + off_v, kChunk, 1024);
+        int kslot = 0, vslot = 0;
+        uint32_t klap = 0, vlap = 0, s_buf = 0, q_lap = 0, fixes = 0;    // fixes: each slot's parity of vfixed
+        bool ok = true;                          // of this lane; votes at the branches
+        Walk<Plan<NQ>> ws, wp;
+        ws.start(plan, &bs->share);
+        wp = ws;
+        bool s_more = all_lanes(ws.next(plan));
+        int s_tile = ws.t0;
+        auto issue_s = [&] {
+            if (all_lanes(s_tile == ws.t0)) {
+                ok = ok && wait_bar(&bs->qfull, q_lap, bs, J);
+                q_lap ^= 1;
             }
-        }
-    } else if (any && warp == 1) {
-        if (elect_one()) {
-            // ---- MMA issue: S runs one tile ahead of P.V ----
-            const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0);
-            // Matrix descriptors (K-major Q and K; MN-major V): the low word moves with the address.
-            const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024), k_desc = umma_desc_sw128(sbase + off_k, 16, 1024);
-            const uint64_t v_desc = umma_desc_sw128(sbase + off_v, kChunk, 1024);
-            constexpr uint64_t kChunkStep = kChunk >> 4;
-            int kslot = 0, stage = 0, s_tile, p_tile = 0, s_count = 0;
-            uint32_t klap = 0, vlap = 0;
-            bool ok = true;
-            Walk<Plan<NQ>> ws, wp;
-            ws.start(plan, &bs->share);
-            wp = ws;
-            bool s_more = ws.next(plan);
-            s_tile = ws.t0;
-            // The K chunks of a tile are awaited for its first row tile and released by its last.
-            auto issue_s = [&](int q) {
-                const int buf = kBufs == 2 ? s_count & 1 : 0;
-                if (q == 0) {
-                    if (s_tile == ws.t0) ok = wait_bar(&bs->qfull, ws.piece & 1, bs, J);
-                    if (NQ == 1 && ok && s_count >= kBufs) ok = wait_bar(&bs->sempty[0][buf], ((s_count / kBufs) - 1) & 1, bs, J);
-                    if (!ok) return;
-                    tc_fence_after();
-                }
-                const uint32_t d = tbase + Col::s(q, buf);
-                for (int c = 0; c < J.kc; ++c) {
-                    int slot = kslot + c;
-                    uint32_t lap = klap;
-                    while (slot >= J.kring) { slot -= J.kring; ++lap; }
-                    if (q == 0 && !(ok = wait_bar(&bs->kfull[slot], lap & 1, bs, J))) return;
-                    const uint64_t a = q_desc + uint32_t(q * J.kc + c) * kChunkStep, b = k_desc + uint32_t(slot) * kChunkStep;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) umma_bf16(d, a + 2 * kk, b + 2 * kk, idesc_s, (c | kk) != 0);
-                    if (q == NQ - 1) umma_commit(&bs->kempty[slot]);
-                }
-                umma_commit(&bs->sfull[q][buf]);
-                if (q == NQ - 1) {
-                    if (s_tile == ws.t1 - 1) umma_commit(&bs->qempty);
-                    kslot += J.kc;
-                    while (kslot >= J.kring) { kslot -= J.kring; ++klap; }
-                    ++s_count;
-                    if (++s_tile == ws.t1) {
-                        s_more = ws.next(plan);
-                        s_tile = ws.t0;
+            for (int c = 0, slot = kslot, lap = klap; c < kc; c += R::kGroup) {
+                ok = ok && wait_bar(&bs->kfull[slot], lap, bs, J);
+                if (++slot == kring) { slot = 0; lap ^= 1; }
+            }
+            const bool last = all_lanes(s_tile == ws.t1 - 1);
+            if (!all_lanes(ok)) return;
+            if (elect_one()) {
+                const uint32_t d = Col::s(q, s_buf);
+#pragma unroll
+                for (int c = 0, slot = kslot; c < kc; c += R::kGroup) {
+#pragma unroll
+                    for (int k = 0; k < R::kGroup; ++k) {
+                        const uint64_t a = q_desc + uint32_t(c + k) * kQStep, b = k_desc + uint32_t(slot * R::kGroup + k) * kStep;
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) umma_bf16(d, a + 2 * kk, b + 2 * kk, idesc_s, (c | k | kk) != 0);
                     }
+                    umma_commit(&bs->kempty[slot]);
+                    if (++slot == kring) slot = 0;
                 }
-            };
-            for (int q = 0; q < NQ && ok; ++q) issue_s(q);
-            for (int i = 0; ok; ++i) {
-                if (i == 0 || p_tile == wp.t1) {
-                    if (!wp.next(plan)) break;
-                    p_tile = wp.t0;
+                umma_commit(&bs->sfull[q][s_buf]);
+                if (last) umma_commit(&bs->qempty);
+            }
+            __syncwarp();
+            kslot += kc / R::kGroup;
+            if (kslot >= kring) { kslot -= kring; klap ^= 1; }
+            s_buf ^= 1;
+            ++s_tile;
+            if (last) {
+                s_more = all_lanes(ws.next(plan));
+                s_tile = ws.t0;
+            }
+        };
+        issue_s();
+        if (s_more) issue_s();
+        uint32_t p_buf = 0, p_lap = 0, o_lap = 0;
+        bool again = false;                      // a piece came before
+        while (all_lanes(ok && wp.next(plan))) {
+            int tile = wp.t0;
+            bool first = true;
+            do {
+                if (first && again) {            // the previous piece has left its O
+                    ok = ok && wait_bar(&bs->oempty[q], o_lap, bs, J);
+                    o_lap ^= 1;
                 }
-                if (NQ == 1 && s_more) issue_s(0);
-                const bool first = p_tile == wp.t0;
-                const bool s_next = s_more;      // NQ == 2: the S tile issued behind this tile's P.V
-                // Every row tile's previous piece has left its O.
-                for (int q = 0; q < NQ && ok && first && wp.piece > 0; ++q) ok = wait_bar(&bs->oempty[q], (wp.piece - 1) & 1, bs, J);
-                if (ok) ok = wait_bar(&bs->vfull[stage], vlap & 1, bs, J);
-                const uint64_t vb = v_desc + uint32_t(stage * J.vc) * kChunkStep;
-                for (int q = 0; q < NQ && ok; ++q) {
-                    if (!(ok = wait_bar(&bs->pfull[q][i & 1], (i >> 1) & 1, bs, J))) break;
-                    tc_fence_after();
-                    const uint32_t a = tbase + Col::p(q, kBufs == 2 ? i & 1 : 0);
-                    // A V tile's chunks lie side by side: up to four are one MMA of N = 256.
-                    for (int c = 0; c < J.vc; c += 4) {
-                        const uint32_t d = tbase + Col::o(q) + 64u * c, id = idesc<kHalf>(128, 64 * min(4, J.vc - c), 0, 1);
-                        const uint64_t b = vb + uint32_t(c) * kChunkStep;
+#pragma unroll
+                for (int c = 0, slot = vslot, lap = vlap; c < vc; c += R::kGroup) {
+                    ok = ok && wait_bar(&bs->vfull[slot], lap, bs, J);
+                    if (++slot == vring) { slot = 0; lap ^= 1; }
+                }
+                // Row tile 0 looks after the V rows (fix_values), row tile 1 waits for it.
+                if (NQ == 2 && q == 1 && all_lanes(needs_fix(wp.s, tile))) {
+                    ok = ok && wait_bar(&bs->vfixed[vslot], fixes >> vslot & 1, bs, J);
+                    fixes ^= 1u << vslot;
+                }
+                ok = ok && wait_bar(&bs->pfull[q][p_buf], p_lap, bs, J);
+                if (!all_lanes(ok)) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a = Col::s(q, p_buf);
+#pragma unroll
+                    for (int c = 0, slot = vslot; c < vc; c += R::kGroup) {
+                        const uint32_t d = Col::o(q) + 64u * c;
+                        const uint64_t b = v_desc + uint32_t(slot * R::kGroup) * kStep;
 #pragma unroll
                         for (int ks = 0; ks < kKeys / 16; ++ks)
-                            umma_ts(d, a + 8u * ks, b + 128 * ks, id, (!first || ks > 0) ? 1u : 0u);
+                            umma_ts(d, a + 8u * ks, b + 128 * ks, idesc_o, (!first || ks > 0) ? 1u : 0u);
+                        umma_commit(&bs->vempty[slot]);
+                        if (++slot == vring) slot = 0;
                     }
-                    if (q == NQ - 1) umma_commit(&bs->vempty[stage]);
-                    umma_commit(&bs->odone[q][i & 1]);
-                    if (NQ == 2 && s_next) issue_s(q);
+                    umma_commit(&bs->odone[q][p_buf]);
                 }
-                if (++stage == J.vstages) { stage = 0; ++vlap; }
-                ++p_tile;
-            }
-            umma_commit(&bs->final_mma);
+                __syncwarp();
+                vslot += vc / R::kGroup;
+                if (vslot >= vring) { vslot -= vring; vlap ^= 1; }
+                if (p_buf) p_lap ^= 1;
+                p_buf ^= 1;
+                first = false;
+                ++tile;
+                if (s_more) issue_s();
+            } while (all_lanes(ok && tile < wp.t1));
+            again = true;
         }
+        if (elect_one()) umma_commit(&bs->final_mma);
         __syncwarp();
     } else if (any && warp >= 4) {
         // ---- softmax and epilogue of row tile qt: thread <-> row (TMEM lane) ----
@@ -432,8 +487,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         const uint32_t o_base = tbase + lane_addr + Col::o(qt);
         const int jh = r % J.group;
         bool failed = false;
-        int i = 0, stage = 0;                                   // tiles done, V stage
-        uint32_t vlap = 0;
+        int i = 0;                                              // tiles done
         Walk<Plan<NQ>> w;
         w.start(plan, &bs->share);
         while (!failed && w.next(plan)) {
@@ -443,55 +497,35 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             const int32_t* words = J.mask ? J.mask + w.b * J.mask_stride + int64_t(min(t, J.nodes - 1)) * J.words : nullptr;
             float m_run = -INFINITY, l_run = 0.f;
             for (int tile = w.t0; tile < w.t1; ++tile, ++i) {
-                const int sb = kBufs == 2 ? i & 1 : 0;
                 const bool masked = needs_fix(w.s, tile);
                 // Which keys the row sees, 32 to a word.
-                uint32_t seen[kKeys / 32];
+                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
                 if (masked) {
 #pragma unroll
-                    for (int c = 0; c < kKeys / 32; ++c)
+                    for (int c = 0; c < 2; ++c)
                         seen[c] = w.s.has_nodes(tile) ? seen_keys(words, J.words, t, w.s.end - w.s.len, tile * kKeys + 32 * c - w.s.len)
                                                       : low_bits(w.s.hi(tile) - 32 * c);
                 }
-                if (!warp_wait(&bs->sfull[qt][sb], (i / kBufs) & 1, bs, J)) { failed = true; break; }
+                if (!warp_wait(&bs->sfull[qt][i & 1], (i >> 1) & 1, bs, J)) { failed = true; break; }
                 tc_fence_after();
-                const uint32_t s_addr = tbase + lane_addr + Col::s(qt, sb);
-                const uint32_t p_addr = tbase + lane_addr + Col::p(qt, sb);
-                // kStep scores at a time, twice over them: the row maximum, then the probabilities
-                // (loops, not one straight run: the code of a tile has to come through the
-                // instruction cache once per launch).  Wide rows have one S buffer and hold all
-                // of a tile's scores, so that the next S may start.
-                constexpr int kStep = kWide ? kKeys : 64;
-                float v[kStep];
-                auto load = [&](int c) {
-#pragma unroll
-                    for (int e = 0; e < kStep; e += 32) tmem_ld32(s_addr + uint32_t(c + e), v + e);
+                const uint32_t s_addr = tbase + lane_addr + Col::s(qt, i & 1);
+                float v[kKeys];
+                float mx = -INFINITY;
+                if (warp_live) {
+                    tmem_ld32(s_addr, v);
+                    tmem_ld32(s_addr + 32u, v + 32);
                     tmem_wait_ld();
                     if (masked) {
 #pragma unroll
-                        for (int e = 0; e < kStep; e += 32) {
-                            const uint32_t bits = kWide ? seen[e / 32] : e == 0 ? (c ? seen[2] : seen[0]) : (c ? seen[3] : seen[1]);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (!(bits >> k & 1)) v[e + k] = -INFINITY;
-                        }
+                        for (int e = 0; e < kKeys; ++e)
+                            if (!(seen[e / 32] >> (e % 32) & 1)) v[e] = -INFINITY;
                     }
-                };
-                float mx = -INFINITY;
-                if (warp_live) {
-#pragma unroll 1
-                    for (int c = 0; c < kKeys; c += kStep) {
-                        load(c);
-                        float m2 = -INFINITY;
+                    float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                        for (int e = 0; e < kStep; e += 2) { mx = fmaxf(mx, v[e]); m2 = fmaxf(m2, v[e + 1]); }
-                        mx = fmaxf(mx, m2);
-                    }
-                }
-                if constexpr (kWide) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bs->sempty[0][sb]);
+                    for (int e = 4; e < kKeys; e += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], v[e + k]), v[(e + 4 + k) % kKeys]);
+                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
                 mx *= J.scale_log2;                             // scale > 0
                 float alpha = 1.f;
@@ -500,17 +534,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     m_run = fmaxf(m_run, mx);
                     l_run *= alpha;
                 }
-                // P(i) takes the buffer of P(i - kBufs); a rescale of O needs P.V(i - 1) done.
                 const bool rescale = tile > w.t0 && __any_sync(0xffffffffu, alpha != 1.f);
                 const bool fix = qt == 0 && masked;
-                const int back = rescale || fix ? 1 : kBufs;
-                if (i >= back) {
-                    if (!warp_wait(&bs->odone[qt][(i - back) & 1], ((i - back) >> 1) & 1, bs, J)) { failed = true; break; }
+                if ((rescale || fix) && i > 0) {
+                    if (!warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J)) { failed = true; break; }
                     tc_fence_after();
                 }
                 if (rescale) {
 #pragma unroll 1
-                    for (int c = 0; c < 2 * J.vc; ++c) {
+                    for (int c = 0; c < 2 * vc; ++c) {
                         float o[32];
                         tmem_ld32(o_base + 32u * c, o);
                         tmem_wait_ld();
@@ -522,41 +554,45 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 }
                 if (warp_live) {
                     const float shift = m_run == -INFINITY ? 0.f : m_run;
-                    float sum = 0.f, sum2 = 0.f;
-#pragma unroll 1
-                    for (int c = 0; c < kKeys; c += kStep) {
-                        if constexpr (!kWide) load(c);
+                    const float2 scale2 = make_float2(J.scale_log2, J.scale_log2), shift2 = make_float2(-shift, -shift);
+                    float2 sum = make_float2(0.f, 0.f), sum2 = sum;
 #pragma unroll
-                        for (int e = 0; e < kStep; e += 32) {
-                            float packed[16];
+                    for (int e = 0; e < kKeys; e += 32) {
+                        float packed[16];
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                const float p0 = sfu_exp2(fmaf(v[e + 2 * k], J.scale_log2, -shift));
-                                const float p1 = sfu_exp2(fmaf(v[e + 2 * k + 1], J.scale_log2, -shift));
-                                sum += p0;
-                                sum2 += p1;
-                                packed[k] = __uint_as_float(pack2<kHalf>(p0, p1));
-                            }
-                            tmem_st16(p_addr + uint32_t(c + e) / 2, packed);
+                        for (int k = 0; k < 16; ++k) {
+                            const float2 x = fma2(make_float2(v[e + 2 * k], v[e + 2 * k + 1]), scale2, shift2);
+                            const float2 p = make_float2(sfu_exp2(x.x), sfu_exp2(x.y));
+                            if (k & 1) sum2 = add2(sum2, p);
+                            else sum = add2(sum, p);
+                            packed[k] = __uint_as_float(pack2<kHalf>(p.x, p.y));
                         }
+                        tmem_st16(s_addr + uint32_t(e) / 2, packed);
                     }
-                    l_run += sum + sum2;
+                    l_run += (sum.x + sum.y) + (sum2.x + sum2.y);
                     tmem_wait_st();
                 }
-                if constexpr (NQ == 1 && !kWide) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bs->sempty[0][sb]);
-                }
                 if (fix) {
-                    // P.V(i - 1) is done, so this tile is the next that lands in its stage.
-                    if (!warp_wait(&bs->vfull[stage], vlap & 1, bs, J)) { failed = true; break; }
-                    const bool bad = fix_values<kHalf>(smem + off_v + uint32_t(stage * J.vc) * kChunk, J.vc, r, r < w.s.hi(tile),
-                                                       tile * kKeys + r >= w.s.len);
+                    // P.V(i - 1) is done, so this tile's chunks are the next that land in their slots.
+                    int slot = 0;
+                    uint32_t lap = 0;
+                    ring_at(i, vc / R::kGroup, vring, slot, lap);
+                    bool bad = false, ok = true;
+                    for (int c = 0; c < vc && ok; c += R::kGroup) {
+                        if (!(ok = warp_wait(&bs->vfull[slot], lap & 1, bs, J))) break;
+                        for (int k = 0; k < R::kGroup; ++k)
+                            bad |= fix_values<kHalf>(smem + off_v + uint32_t(slot * R::kGroup + k) * kChunk, r & 63, r >> 6,
+                                                     (r & 63) < w.s.hi(tile), tile * kKeys + (r & 63) >= w.s.len);
+                        if (++slot == vring) { slot = 0; ++lap; }
+                    }
+                    if (!ok) { failed = true; break; }
                     if (bad) *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) = w.piece + 1;
                     fence_async_shared();
+                    if constexpr (NQ == 2) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bs->vfixed[(i * (vc / R::kGroup)) % vring]);
+                    }
                 }
-                if (++stage == J.vstages) { stage = 0; ++vlap; }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bs->pfull[qt][i & 1]);
@@ -573,7 +609,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             const int rows = NQ * J.tile_rows, slot = 2 * blockIdx.x + (w.piece > 0), row = qt * J.tile_rows + r;
             float4* part = reinterpret_cast<float4*>(J.part_o) + int64_t(slot) * (J.dim_v / 4) * rows + row;
 #pragma unroll 1
-            for (int c = 0; c < 2 * J.vc; ++c) {
+            for (int c = 0; c < 2 * vc; ++c) {
                 float o[32];
                 if (warp_live) {
                     tmem_ld32(o_base + 32u * c, o);
@@ -640,11 +676,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         // that ran out the copies that were not.
         if (tid == 64) mbar_wait(&bs->final_mma, 0, 2000000000ull);
         if (bs->abort && tid == 0) {
-            for (int s = 0; s < J.kring; ++s) {
+            for (int s = 0; s < kring; ++s) {
                 mbar_wait(&bs->kfull[s], 0, 100000000ull);
                 mbar_wait(&bs->kfull[s], 1, 100000000ull);
             }
-            for (int s = 0; s < J.vstages; ++s) {
+            for (int s = 0; s < vring; ++s) {
                 mbar_wait(&bs->vfull[s], 0, 100000000ull);
                 mbar_wait(&bs->vfull[s], 1, 100000000ull);
             }
@@ -655,7 +691,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     __syncthreads();
     if (warp == 2) {
         tc_fence_after();
-        tmem_dealloc(tbase, 512);
+        tmem_dealloc(bs->tmem_base, 512);
     }
 }
 
@@ -761,9 +797,9 @@ void carve(Carver& c, const slimkv_tree_attention_args* a, Job& J) {
     J.part_lse = c.take<float>(rows);
 }
 
-template <int NQ, bool kWide, bool kHalf>
+template <int NQ, int C, bool kHalf>
 int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Job& J, cudaStream_t stream) {
-    auto kernel = tree_attention_kernel<NQ, kWide, kHalf>;
+    auto kernel = tree_attention_kernel<NQ, C, kHalf>;
     static bool configured[64] = {};
     const int dev = device_info().device;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
@@ -850,9 +886,10 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.kc = (a->dim_qk + 63) / 64;
     J.vc = (a->dim_v + 63) / 64;
     J.dim_v = a->dim_v;
-    const int slots = int(kTileArea / kChunk) - nq * J.kc;
-    J.vstages = std::max(1, slots / 2 / J.vc);
-    J.kring = std::min(kMaxRing, slots - J.vstages * J.vc);
+    const bool wide = J.kc > 2 || J.vc > 2;
+    const int chunks = int((kTileArea - uint32_t(J.kc) * kQChunk) / kChunk);      // wide rows: one row tile
+    J.vring = std::min(kMaxRing, chunks / 2);
+    J.kring = std::min(kMaxRing, chunks - J.vring);
     J.context_only = a->context_only;
     J.paged = paged;
     J.cache = cache_view(cache);
@@ -870,8 +907,11 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.status = status_word();
     J.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool wide = J.kc > 2 || J.vc > 2, half = a->type == SLIMKV_FP16;
-    if (nq == 2) return half ? launch<2, false, true>(qm, km, vm, J, st) : launch<2, false, false>(qm, km, vm, J, st);
-    if (wide) return half ? launch<1, true, true>(qm, km, vm, J, st) : launch<1, true, false>(qm, km, vm, J, st);
-    return half ? launch<1, false, true>(qm, km, vm, J, st) : launch<1, false, false>(qm, km, vm, J, st);
+    const bool half = a->type == SLIMKV_FP16;
+    const int width = wide ? 0 : std::max(J.kc, J.vc);
+    auto pick = [&](auto one, auto two, auto any, auto one2, auto two2) {
+        return (nq == 2 ? (width == 1 ? one2 : two2) : width == 1 ? one : width == 2 ? two : any)(qm, km, vm, J, st);
+    };
+    return half ? pick(launch<1, 1, true>, launch<1, 2, true>, launch<1, 0, true>, launch<2, 1, true>, launch<2, 2, true>)
+                : pick(launch<1, 1, false>, launch<1, 2, false>, launch<1, 0, false>, launch<2, 1, false>, launch<2, 2, false>);
 }
