@@ -52,7 +52,7 @@ struct Share {
     long long first_u;          // units before sequence first_b
     int first_b;
     int ctas;                   // CTAs with a share
-    long long scan[24];
+    long long scan[40];         // two words for each of up to 20 warps
 };
 
 // Fills `share` (all threads; the caller synchronises before reading it).

@@ -33,8 +33,8 @@
 // keys, 2,700 of them the softmax.)
 //
 // One CTA per SM, warps: 0 = Q and K loads (TMA), 3 = V loads, 1 = MMA issue
-// of row tile 0, 2 = TMEM owner and MMA issue of row tile 1, 4-7 (and 8-11) =
-// softmax of row tile 0 (1), a thread per row.  Every wait is bounded.
+// of row tile 0, 2 = TMEM owner and MMA issue of row tile 1, the
+// others from 4 on = softmax.  Every wait is bounded.
 #include <algorithm>
 
 #include "cache_view.cuh"
@@ -55,6 +55,13 @@ constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a row's m
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
+// Threads that share a row's softmax: two with one row tile, where the row's
+// latency counts; one with two row tiles, which keep the units busy by turns.
+template <int NQ>
+constexpr int kHalvesOf = NQ == 1 ? 2 : 1;
+template <int NQ>
+constexpr int kSoftmaxThreads = 128 * NQ * kHalvesOf<NQ>;
+
 struct Bars {
     uint64_t kfull[kMaxRing], kempty[kMaxRing], vfull[kMaxRing], vempty[kMaxRing], vfixed[kMaxRing];
     uint64_t qfull, qempty;
@@ -63,6 +70,7 @@ struct Bars {
     uint32_t tmem_base;
     int abort;
     int bad_values[2];           // 1 + a piece whose node values hold infinities or NaN
+    float exchange[2][kRows];    // [row tile]: between a row's two threads
     Share share;
 };
 constexpr uint32_t kSmemBytes = 1024 + kTileArea + uint32_t(sizeof(Bars));
@@ -143,21 +151,6 @@ template <bool kHalf>
 __device__ __forceinline__ constexpr uint32_t idesc(int m, int n, int a_mn, int b_mn) {
     return umma_idesc_bf16(m, n, a_mn, b_mn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
 }
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ uint64_t bits2(float2 x) { return uint64_t(__float_as_uint(x.y)) << 32 | __float_as_uint(x.x); }
-__device__ __forceinline__ float2 float2_of(uint64_t x) {
-    return make_float2(__uint_as_float(uint32_t(x)), __uint_as_float(uint32_t(x >> 32)));
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
-    return float2_of(d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
-    return float2_of(d);
-}
 // A from tensor memory (two 16-bit K elements per column), B from shared memory.
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc_, uint32_t accumulate) {
     asm volatile(
@@ -180,6 +173,17 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* b
     bs->abort = 1;
     report(J.status, SLIMKV_DEVICE_TIMEOUT);
     return false;
+}
+// Whether `x` holds for any of the 256 softmax threads of a row tile (their
+// barrier `id`).
+__device__ __forceinline__ bool any_of_row_tile(int id, bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(any)
+        : "r"(uint32_t(x)), "r"(id)
+        : "memory");
+    return any != 0;
 }
 __device__ __forceinline__ bool all_lanes(bool x) { return __all_sync(0xffffffffu, x); }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
@@ -237,16 +241,16 @@ __device__ __forceinline__ void ring_at(int tile, int per, int ring, int& slot, 
 // Whether a V tile holds rows that nobody sees, or the nodes' own.
 __device__ __forceinline__ bool needs_fix(const Seq& s, int tile) { return s.has_nodes(tile) || s.hi(tile) < kKeys; }
 
-// Row r of a V chunk in shared memory (every second 16 bytes): zeroed when nobody sees it (its P is 0,
+// Row r of a V chunk in shared memory (every kStep-th 16 bytes): zeroed when nobody sees it (its P is 0,
 // and 0 x NaN is not 0); of a node's row, infinities and NaN become 0 (the
 // epilogue adds them to the rows that see them).  True when there were any.
-template <bool kHalf>
+template <bool kHalf, int kStep>
 __device__ __forceinline__ bool fix_values(uint8_t* chunk, int r, int u0, bool seen, bool node) {
     constexpr uint32_t kExp = kHalf ? 0x7c00u : 0x7f80u;
     if (seen && !node) return false;
     bool bad = false;
 #pragma unroll 1
-    for (int u = u0; u < 8; u += 2) {
+    for (int u = u0; u < 8; u += kStep) {
         uint4* at = reinterpret_cast<uint4*>(chunk + r * 128) + ((u ^ r) & 7);
         uint4 v = make_uint4(0, 0, 0, 0);
         bool write = !seen;
@@ -281,10 +285,11 @@ struct Rings {
 
 // ----------------------------------------------------------------- kernel --
 template <int NQ, int C, bool kHalf>
-__global__ void __launch_bounds__(128 + 128 * NQ, 1)
+__global__ void __launch_bounds__(128 + kSoftmaxThreads<NQ>, 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Job J) {
-    constexpr int kThreads = 128 + 128 * NQ;
+    constexpr int kThreads = 128 + kSoftmaxThreads<NQ>;
+    constexpr int kHalves = kHalvesOf<NQ>, kWarps = 4 * kHalves, kCols = kKeys / kHalves;
     using Col = Columns<NQ, C>;
     using R = Rings<NQ, C>;
     const int kc = R::kc(J), vc = R::vc(J), kring = R::kring(J), vring = R::vring(J);
@@ -299,15 +304,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     if (tid == 0) {
         for (int s = 0; s < kMaxRing; ++s) {
             mbar_init(&bs->kfull[s], 1); mbar_init(&bs->kempty[s], NQ);
-            mbar_init(&bs->vfull[s], 1); mbar_init(&bs->vempty[s], NQ); mbar_init(&bs->vfixed[s], 4);
+            mbar_init(&bs->vfull[s], 1); mbar_init(&bs->vempty[s], NQ); mbar_init(&bs->vfixed[s], kWarps);
         }
         mbar_init(&bs->qfull, 1);
         mbar_init(&bs->qempty, NQ);
         for (int q = 0; q < 2; ++q) {
-            mbar_init(&bs->oempty[q], 4);
+            mbar_init(&bs->oempty[q], kWarps);
             for (int s = 0; s < 2; ++s) {
                 mbar_init(&bs->sfull[q][s], 1);
-                mbar_init(&bs->pfull[q][s], 4);
+                mbar_init(&bs->pfull[q][s], kWarps);
                 mbar_init(&bs->odone[q][s], 1);
             }
         }
@@ -325,7 +330,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tbase = 0;               // all 512 columns are this CTA's: they begin at column 0
+    // All 512 tensor memory columns are this CTA's: addresses begin at column 0.
     const uint32_t sbase = smem_u32(smem);
     const bool any = int(blockIdx.x) < bs->share.ctas;
 
@@ -373,7 +378,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         // ---- MMA issue, a warp for each row tile: S two tiles ahead of P.V.  The tensor
         // core queues only a few MMAs, so what the warp does between them is time lost,
         // unless another warp's MMAs fill it (one warp for both row tiles: 8,100 cycles for
-        // 128 keys, two: XXXX).  The warp stays converged, its branches go by votes, and one
+        // 128 keys, two: 4,600).  The warp stays converged, its branches go by votes, and one
         // elected thread has the instructions alone, so that operands are uniform registers. ----
         const int q = NQ == 2 ? warp - 1 : 0;
         const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0), idesc_o = idesc<kHalf>(128, 64 * R::kGroup, 0, 1);
@@ -480,17 +485,31 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         if (elect_one()) umma_commit(&bs->final_mma);
         __syncwarp();
     } else if (any && warp >= 4) {
-        // ---- softmax and epilogue of row tile qt: thread <-> row (TMEM lane) ----
-        const int qt = (warp - 4) >> 2, quarter = warp & 3;
+        // ---- softmax and epilogue of row tile qt: kHalves threads for a row (TMEM lane), each
+        // with kCols of a tile's keys.  Two threads share the row's running maximum: a barrier
+        // of the row tile's threads asks whether any row outgrew it by 2^8, and only then do
+        // they exchange maxima.  After a wait that ran out every thread still meets at every
+        // barrier, without work. ----
+        const int qt = (warp - 4) / kWarps, half = kHalves == 2 ? (warp >> 2) & 1 : 0, quarter = warp & 3;
         const int r = 32 * quarter + lane;
         const uint32_t lane_addr = uint32_t(32 * quarter) << 16;
-        const uint32_t o_base = tbase + lane_addr + Col::o(qt);
+        const uint32_t o_base = lane_addr + Col::o(qt);
         const int jh = r % J.group;
-        bool failed = false;
+        // All threads of a row get op over their x.
+        auto over_row = [&](float x, auto op) {
+            if constexpr (kHalves == 1) return x;
+            float* at = &bs->exchange[qt][r];
+            if (half) *at = x;
+            named_bar(1 + qt, 256);
+            if (!half) *at = x = op(x, *at);
+            named_bar(1 + qt, 256);
+            return half ? *at : x;
+        };
+        bool ok = true;
         int i = 0;                                              // tiles done
         Walk<Plan<NQ>> w;
         w.start(plan, &bs->share);
-        while (!failed && w.next(plan)) {
+        while (w.next(plan)) {
             const int t = (w.group * NQ + qt) * J.tpt + r / J.group;
             const bool live = r < J.tile_rows && t < w.s.nodes;
             const bool warp_live = __any_sync(0xffffffffu, live);
@@ -498,108 +517,120 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             float m_run = -INFINITY, l_run = 0.f;
             for (int tile = w.t0; tile < w.t1; ++tile, ++i) {
                 const bool masked = needs_fix(w.s, tile);
-                // Which keys the row sees, 32 to a word.
-                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+                uint32_t seen[kCols / 32];                      // which of its keys the row sees
                 if (masked) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        seen[c] = w.s.has_nodes(tile) ? seen_keys(words, J.words, t, w.s.end - w.s.len, tile * kKeys + 32 * c - w.s.len)
-                                                      : low_bits(w.s.hi(tile) - 32 * c);
+                    for (int c = 0; c < kCols / 32; ++c) {
+                        const int k = kCols * half + 32 * c;
+                        seen[c] = w.s.has_nodes(tile) ? seen_keys(words, J.words, t, w.s.end - w.s.len, tile * kKeys + k - w.s.len)
+                                                      : low_bits(w.s.hi(tile) - k);
+                    }
                 }
-                if (!warp_wait(&bs->sfull[qt][i & 1], (i >> 1) & 1, bs, J)) { failed = true; break; }
+                ok = ok && warp_wait(&bs->sfull[qt][i & 1], (i >> 1) & 1, bs, J);
                 tc_fence_after();
-                const uint32_t s_addr = tbase + lane_addr + Col::s(qt, i & 1);
-                float v[kKeys];
+                const uint32_t s_addr = lane_addr + Col::s(qt, i & 1);
+                float v[kCols];
                 float mx = -INFINITY;
                 if (warp_live) {
-                    tmem_ld32(s_addr, v);
-                    tmem_ld32(s_addr + 32u, v + 32);
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 32) tmem_ld32(s_addr + uint32_t(kCols * half + c), v + c);
                     tmem_wait_ld();
                     if (masked) {
 #pragma unroll
-                        for (int e = 0; e < kKeys; ++e)
+                        for (int e = 0; e < kCols; ++e)
                             if (!(seen[e / 32] >> (e % 32) & 1)) v[e] = -INFINITY;
                     }
                     float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int e = 4; e < kKeys; e += 8)
+                    for (int e = 4; e < kCols - 4; e += 8)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], v[e + k]), v[(e + 4 + k) % kKeys]);
+                        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(fmaxf(m4[k], v[e + k]), v[e + 4 + k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], v[kCols - 4 + k]);
                     mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
                 mx *= J.scale_log2;                             // scale > 0
-                float alpha = 1.f;
-                if (mx > m_run + kLazyLog2 || m_run == -INFINITY) {
-                    alpha = mx == -INFINITY || m_run == -INFINITY ? 1.f : exp2f(m_run - mx);
-                    m_run = fmaxf(m_run, mx);
-                    l_run *= alpha;
-                }
-                const bool rescale = tile > w.t0 && __any_sync(0xffffffffu, alpha != 1.f);
+                // Two threads of a row: all have read this tile's S when they pass here, so P may
+                // go over it.
+                const bool more = live && mx > m_run + kLazyLog2;
+                const bool grown = kHalves == 2 ? any_of_row_tile(1 + qt, more) : __any_sync(0xffffffffu, more);
                 const bool fix = qt == 0 && masked;
-                if ((rescale || fix) && i > 0) {
-                    if (!warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J)) { failed = true; break; }
+                if (((grown && tile > w.t0) || fix) && i > 0) {
+                    ok = ok && warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J);
                     tc_fence_after();
                 }
-                if (rescale) {
-#pragma unroll 1
-                    for (int c = 0; c < 2 * vc; ++c) {
-                        float o[32];
-                        tmem_ld32(o_base + 32u * c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= alpha;
-                        tmem_st32(o_base + 32u * c, o);
+                if (grown) {
+                    mx = over_row(mx, [](float a, float b) { return fmaxf(a, b); });
+                    float alpha = 1.f;
+                    if (mx > m_run + kLazyLog2) {
+                        alpha = m_run == -INFINITY ? 1.f : exp2f(m_run - mx);
+                        m_run = mx;
+                        l_run *= alpha;
                     }
-                    tmem_wait_st();
+                    if (ok && tile > w.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+                        for (int c = half; c < 4 * vc; c += kHalves) {
+                            float o[16];
+                            tmem_ld16(o_base + 16u * c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                            tmem_st16(o_base + 16u * c, o);
+                        }
+                        tmem_wait_st();
+                    }
                 }
                 if (warp_live) {
                     const float shift = m_run == -INFINITY ? 0.f : m_run;
-                    const float2 scale2 = make_float2(J.scale_log2, J.scale_log2), shift2 = make_float2(-shift, -shift);
-                    float2 sum = make_float2(0.f, 0.f), sum2 = sum;
+                    // Plain scalar arithmetic: packed pairs of fp32 (f32x2) took twice the time next
+                    // to the exponentials, 1,138 against 497 cycles for 64 keys of a warp.
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < kKeys; e += 32) {
+                    for (int c = 0; c < kCols; c += 32) {
                         float packed[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            const float2 x = fma2(make_float2(v[e + 2 * k], v[e + 2 * k + 1]), scale2, shift2);
-                            const float2 p = make_float2(sfu_exp2(x.x), sfu_exp2(x.y));
-                            if (k & 1) sum2 = add2(sum2, p);
-                            else sum = add2(sum, p);
-                            packed[k] = __uint_as_float(pack2<kHalf>(p.x, p.y));
+                            const float p0 = sfu_exp2(fmaf(v[c + 2 * k], J.scale_log2, -shift));
+                            const float p1 = sfu_exp2(fmaf(v[c + 2 * k + 1], J.scale_log2, -shift));
+                            sum[2 * k & 3] += p0;
+                            sum[(2 * k + 1) & 3] += p1;
+                            packed[k] = __uint_as_float(pack2<kHalf>(p0, p1));
                         }
-                        tmem_st16(s_addr + uint32_t(e) / 2, packed);
+                        tmem_st16(s_addr + uint32_t(kCols * half + c) / 2, packed);
                     }
-                    l_run += (sum.x + sum.y) + (sum2.x + sum2.y);
+                    l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tmem_wait_st();
                 }
-                if (fix) {
+                if (fix && ok) {
                     // P.V(i - 1) is done, so this tile's chunks are the next that land in their slots.
                     int slot = 0;
                     uint32_t lap = 0;
                     ring_at(i, vc / R::kGroup, vring, slot, lap);
-                    bool bad = false, ok = true;
+                    const int first = slot;
+                    bool bad = false;
                     for (int c = 0; c < vc && ok; c += R::kGroup) {
-                        if (!(ok = warp_wait(&bs->vfull[slot], lap & 1, bs, J))) break;
-                        for (int k = 0; k < R::kGroup; ++k)
-                            bad |= fix_values<kHalf>(smem + off_v + uint32_t(slot * R::kGroup + k) * kChunk, r & 63, r >> 6,
-                                                     (r & 63) < w.s.hi(tile), tile * kKeys + (r & 63) >= w.s.len);
+                        ok = warp_wait(&bs->vfull[slot], lap & 1, bs, J);
+                        for (int k = 0; k < R::kGroup && ok; ++k)
+                            bad |= fix_values<kHalf, 2 * kHalves>(smem + off_v + uint32_t(slot * R::kGroup + k) * kChunk, r & 63,
+                                                                  2 * half + (r >> 6), (r & 63) < w.s.hi(tile),
+                                                                  tile * kKeys + (r & 63) >= w.s.len);
                         if (++slot == vring) { slot = 0; ++lap; }
                     }
-                    if (!ok) { failed = true; break; }
                     if (bad) *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) = w.piece + 1;
                     fence_async_shared();
                     if constexpr (NQ == 2) {
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&bs->vfixed[(i * (vc / R::kGroup)) % vring]);
+                        if (lane == 0) mbar_arrive(&bs->vfixed[first]);
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bs->pfull[qt][i & 1]);
             }
-            if (failed) break;
-            // ---- the piece's rows ----
-            if (!warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J)) { failed = true; break; }
+            // ---- the piece's rows: the sums of all threads of a row, then each its columns ----
+            l_run = over_row(l_run, [](float a, float b) { return a + b; });
+            ok = ok && warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J);
+            if (!ok) continue;
             tc_fence_after();
             const bool whole = w.whole();
             const bool bad = *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) == w.piece + 1;
@@ -609,15 +640,15 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             const int rows = NQ * J.tile_rows, slot = 2 * blockIdx.x + (w.piece > 0), row = qt * J.tile_rows + r;
             float4* part = reinterpret_cast<float4*>(J.part_o) + int64_t(slot) * (J.dim_v / 4) * rows + row;
 #pragma unroll 1
-            for (int c = 0; c < 2 * vc; ++c) {
-                float o[32];
+            for (int c = half; c < 4 * vc; c += kHalves) {
+                float o[16];
                 if (warp_live) {
-                    tmem_ld32(o_base + 32u * c, o);
+                    tmem_ld16(o_base + 16u * c, o);
                     tmem_wait_ld();
                 }
                 if (live) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] *= inv;
+                    for (int e = 0; e < 16; ++e) o[e] *= inv;
                     if (bad) {
                         // Infinities and NaN of the nodes' values, for the rows that see them.
                         for (int n0 = 0; n0 < w.s.nodes; n0 += 32) {
@@ -629,8 +660,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                                 if (J.paged) cache_row(J.cache, w.b, at, page, at);
                                 const int64_t base = page * J.cache.v_stride[0] + at * J.cache.v_stride[1] + w.g * J.cache.v_stride[2];
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) {
-                                    const int d = 32 * c + e;
+                                for (int e = 0; e < 16; ++e) {
+                                    const int d = 16 * c + e;
                                     if (d < J.dim_v) {
                                         const float x = value_at<kHalf>(J.v, base + d);
                                         if (!isfinite(x)) o[e] += x;
@@ -642,8 +673,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     if (whole) {
                         uint16_t* dst = static_cast<uint16_t*>(J.out) + w.b * J.o_sb + t * J.o_st + h * J.o_sh;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int d = 32 * c + 8 * u;
+                        for (int u = 0; u < 2; ++u) {
+                            const int d = 16 * c + 8 * u;
                             if (d < J.dim_v)
                                 *reinterpret_cast<uint4*>(dst + d) =
                                     make_uint4(pack2<kHalf>(o[8 * u], o[8 * u + 1]), pack2<kHalf>(o[8 * u + 2], o[8 * u + 3]),
@@ -652,14 +683,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     } else {
                         // [slot][4 dims][row]: the rows of a warp side by side.
 #pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            if (32 * c + 4 * u < J.dim_v)
-                                part[int64_t(8 * c + u) * rows] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                        for (int u = 0; u < 4; ++u)
+                            if (16 * c + 4 * u < J.dim_v)
+                                part[int64_t(4 * c + u) * rows] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
                     }
                 }
                 __syncwarp();
             }
-            if (live) {
+            if (live && half == 0) {
                 if (whole) J.lse[(int64_t(w.b) * J.nodes + t) * J.heads + h] = lse2 * kLn2;
                 else J.part_lse[slot * rows + row] = lse2;
             }
@@ -807,7 +838,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
             return fail(SLIMKV_ERR_CUDA, "cudaFuncSetAttribute (tree attention) failed");
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    kernel<<<J.ctas, 128 + 128 * NQ, kSmemBytes, stream>>>(qm, km, vm, J);
+    kernel<<<J.ctas, 128 + kSoftmaxThreads<NQ>, kSmemBytes, stream>>>(qm, km, vm, J);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(J.batch * J.kv_heads * J.row_groups, (NQ * J.tile_rows + 31) / 32, (J.dim_v + 63) / 64);
     cfg.blockDim = dim3(128);
