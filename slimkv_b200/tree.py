@@ -18,40 +18,78 @@ that decode.  Torch wrappers over ``include/slimkv_b200.h``: checks, current
 stream, workspaces from PyTorch's allocator (calls can be captured in CUDA
 graphs).  There is no CPU path.
 """
-import ctypes
+from ctypes import byref
 
 import torch
 
 from . import _lib
-from .kernels import _ptr, _require, _stream
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
+# A decode step makes these calls once per layer, outside a graph with the
+# launch itself as their only other cost: the checks build no text unless they
+# fail, and the device is only switched to when it is another one.
+def _refuse(msg, *args):
+    raise RuntimeError(msg % args)
+
+
 def _i32(t, shape, what):
-    _require(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous() and t.shape == shape,
-             f'{what} must be contiguous int32 {list(shape)} on CUDA')
+    if not (t.is_cuda and t.dtype == torch.int32 and t.shape == shape and t.is_contiguous()):
+        _refuse('%s must be contiguous int32 %s on CUDA', what, list(shape))
     return t.data_ptr()
 
 
-def fill_cache(c, k, v, block_tables, batch):
-    """``slimkv_cache`` of k / v ``[B or 1, rows, Hkv, D]`` (dense; 1: shared by
-    the batch) or ``[pages, page, Hkv, D]`` with int32 ``block_tables [B, n]``."""
-    for x, stride in ((k, c.k_stride), (v, c.v_stride)):
-        _require(x.is_cuda and x.dim() == 4 and x.stride(3) == 1 and x.dtype == k.dtype,
-                 'caches must be [B, rows, Hkv, D] (or pages) on CUDA with a contiguous last dimension')
-        stride[:] = x.stride()[:3]
-    _require(k.shape[:3] == v.shape[:3] and k.device == v.device, 'K and V must agree in all but their last dimension')
-    c.k, c.v, c.rows = k.data_ptr(), v.data_ptr(), k.shape[1]
-    if block_tables is None:
-        _require(k.shape[0] in (1, batch), 'one cache for each sequence, or one for all')
-        if k.shape[0] == 1:
-            c.k_stride[0] = c.v_stride[0] = 0
+def _run(device, call, *args):
+    """``call(*args, stream)`` on ``device`` and its current stream; raises its error."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        _require(block_tables.is_cuda and block_tables.dtype == torch.int32 and block_tables.dim() == 2 and
-                 block_tables.shape[0] == batch and block_tables.stride(1) == 1, 'block tables must be int32 [B, n] on CUDA')
+        with torch.cuda.device(index):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _workspace(device, size_of, a):
+    """A new workspace of ``size_of(a)`` bytes (0: the call itself refuses its arguments)."""
+    if device.index == torch.cuda.current_device():
+        size = size_of(byref(a))
+    else:
+        with torch.cuda.device(device):
+            size = size_of(byref(a))
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _check_rows(k, v, dims):
+    if not (k.is_cuda and v.is_cuda and k.dim() == v.dim() == dims and k.dtype == v.dtype and k.device == v.device):
+        _refuse('caches must be CUDA tensors [B, rows, Hkv, D] (or pages) of one type on one device')
+
+
+def fill_cache(c, k, v, block_tables, batch, first=0):
+    """``slimkv_cache`` of k / v ``[B or 1, rows, Hkv, D]`` (dense; 1: shared by
+    the batch) or ``[pages, page, Hkv, D]`` with int32 ``block_tables [B, n]``;
+    ``first`` dimensions in front are the caller's."""
+    ks, vs, shape, v_shape = k.stride(), v.stride(), k.shape, v.shape
+    if ks[-1] != 1 or vs[-1] != 1 or shape[:-1] != v_shape[:-1]:
+        _refuse('caches need a contiguous last dimension, and K and V must agree in all others')
+    c.k, c.v, c.rows = k.data_ptr(), v.data_ptr(), shape[first + 1]
+    sequences = shape[first]
+    x, y = c.k_stride, c.v_stride
+    x[0], x[1], x[2] = ks[first:first + 3]
+    y[0], y[1], y[2] = vs[first:first + 3]
+    if block_tables is None:
+        if sequences != batch:
+            if sequences != 1:
+                _refuse('one cache for each sequence, or one for all')
+            x[0] = y[0] = 0
+    else:
+        if not (block_tables.is_cuda and block_tables.dtype == torch.int32 and block_tables.dim() == 2 and
+                block_tables.shape[0] == batch and block_tables.stride(1) == 1):
+            _refuse('block tables must be int32 [B, n] on CUDA')
         c.table, c.table_stride = block_tables.data_ptr(), block_tables.stride(0)
-        c.table_pages, c.num_pages = block_tables.shape[1], k.shape[0]
+        c.table_pages, c.num_pages = block_tables.shape[1], sequences
 
 
 def tree_masks(parents):
@@ -59,12 +97,12 @@ def tree_masks(parents):
     T]`` int32 (a parent before its children; -1: a root) -> int32 ``[B, T,
     (T + 31) // 32]``, bit i of node t set when t sees i (its ancestors and
     itself)."""
-    _require(parents.dim() == 2, 'parents must be [B, T]')
+    if parents.dim() != 2:
+        _refuse('parents must be [B, T]')
     p = _i32(parents, parents.shape, 'parents')
     batch, nodes = parents.shape
     out = torch.empty((batch, nodes, (nodes + 31) // 32), dtype=torch.int32, device=parents.device)
-    with torch.cuda.device(parents.device):
-        _lib.check(_lib.load().slimkv_tree_masks(p, batch, nodes, _ptr(out), _stream()))
+    _run(parents.device, _lib.load().slimkv_tree_masks, p, batch, nodes, out.data_ptr())
     return out
 
 
@@ -84,39 +122,45 @@ def tree_attention(q, k, v, lengths, scale, mask=None, nodes=None, block_tables=
     Returns ``(out [B, T, H, Dv], lse [B, T, H] fp32 natural log)``; a row that
     sees nothing gets zeros and -inf.  Dims: multiples of 8 up to 320.
     """
-    _require(q.is_cuda and q.dim() == 4 and q.stride(3) == 1 and q.dtype in (torch.bfloat16, torch.float16),
-             'q must be bf16 or fp16 [B, T, H, D] on CUDA with a contiguous last dimension')
-    _require(k.dtype == q.dtype and k.shape[-1] == q.shape[3] and k.device == q.device, 'caches of q\'s type, dim and device')
+    kind = q.dtype
+    if not (q.is_cuda and q.dim() == 4 and kind in (torch.bfloat16, torch.float16)):
+        _refuse('q must be bf16 or fp16 [B, T, H, D] on CUDA')
     batch, t, heads, dim = q.shape
+    qs, dev = q.stride(), q.device
+    _check_rows(k, v, 4)
+    if qs[3] != 1 or k.dtype != kind or k.shape[3] != dim or k.device != dev:
+        _refuse('q needs a contiguous last dimension, and caches of its type, dim and device')
     a = _lib.TreeAttentionArgs()
     fill_cache(a.cache, k, v, block_tables, batch)
     dim_v = v.shape[3]
     if out is None:
-        out = torch.empty((batch, t, heads, dim_v), dtype=q.dtype, device=q.device)
+        out = torch.empty((batch, t, heads, dim_v), dtype=kind, device=dev)
+    elif not (out.shape == (batch, t, heads, dim_v) and out.dtype == kind and out.device == dev and out.stride(3) == 1):
+        _refuse('out must be [B, T, H, Dv] of q\'s type')
     if lse is None:
-        lse = torch.empty((batch, t, heads), dtype=torch.float32, device=q.device)
-    _require(out.shape == (batch, t, heads, dim_v) and out.dtype == q.dtype and out.is_cuda and out.stride(3) == 1,
-             'out must be [B, T, H, Dv] of q\'s type')
-    _require(lse.shape == (batch, t, heads) and lse.dtype == torch.float32 and lse.is_cuda and lse.is_contiguous(),
-             'lse must be contiguous fp32 [B, T, H]')
-    a.batch, a.nodes, a.heads, a.kv_heads, a.dim_qk, a.dim_v, a.type = (batch, t, heads, k.shape[2], dim, dim_v,
-                                                                        _TYPES[q.dtype])
+        lse = torch.empty((batch, t, heads), dtype=torch.float32, device=dev)
+    elif not (lse.shape == (batch, t, heads) and lse.dtype == torch.float32 and lse.device == dev and lse.is_contiguous()):
+        _refuse('lse must be contiguous fp32 [B, T, H]')
+    a.batch, a.nodes, a.heads, a.kv_heads = batch, t, heads, k.shape[2]
+    a.dim_qk, a.dim_v, a.type = dim, dim_v, _TYPES[kind]
     a.q, a.out, a.lse, a.lengths = q.data_ptr(), out.data_ptr(), lse.data_ptr(), _i32(lengths, (batch,), 'lengths')
-    a.q_stride[:] = q.stride()[:3]
-    a.out_stride[:] = out.stride()[:3]
+    x, y = a.q_stride, a.out_stride
+    x[0], x[1], x[2] = qs[:3]
+    y[0], y[1], y[2] = out.stride()[:3]
     if nodes is not None:
         a.nodes_len = _i32(nodes, (batch,), 'nodes')
     if mask is not None:
-        _require(not context_only, 'the nodes\' own rows are not in a context_only cache: no mask')
-        _require(mask.dim() == 3 and mask.shape[0] in (1, batch), 'mask must be [B or 1, T, words]')
-        a.mask = _i32(mask, (mask.shape[0], t, (t + 31) // 32), 'mask')
-        a.mask_stride = mask.stride(0) if mask.shape[0] > 1 else 0
-    a.context_only, a.scale, a.wait_limit_ns = int(bool(context_only)), float(scale), int(wait_limit_ns)
+        if context_only:
+            _refuse('the nodes\' own rows are not in a context_only cache: no mask')
+        many = mask.shape[0] if mask.dim() == 3 else 0
+        if many not in (1, batch):
+            _refuse('mask must be [B or 1, T, words]')
+        a.mask = _i32(mask, (many, t, (t + 31) // 32), 'mask')
+        a.mask_stride = mask.stride(0) if many > 1 else 0
+    a.context_only, a.scale, a.wait_limit_ns = bool(context_only), scale, wait_limit_ns
     lib = _lib.load()
-    with torch.cuda.device(q.device):
-        size = lib.slimkv_tree_attention_workspace_size(ctypes.byref(a))
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _lib.check(lib.slimkv_tree_attention(ctypes.byref(a), _ptr(ws), size, _stream()))
+    ws = _workspace(dev, lib.slimkv_tree_attention_workspace_size, a)
+    _run(dev, lib.slimkv_tree_attention, byref(a), ws.data_ptr(), ws.numel())
     return out, lse
 
 
@@ -131,27 +175,25 @@ def tree_accept(logits, tokens, parents, nodes=None):
     Ties of the largest logit go to the lowest token; a NaN counts above every
     number.
     """
-    _require(logits.is_cuda and logits.dim() == 3 and logits.stride(2) == 1 and logits.dtype in _TYPES,
-             'logits must be bf16, fp16 or fp32 [B, T, V] on CUDA with a contiguous last dimension')
+    if not (logits.is_cuda and logits.dim() == 3 and logits.dtype in _TYPES and logits.stride(2) == 1):
+        _refuse('logits must be bf16, fp16 or fp32 [B, T, V] on CUDA with a contiguous last dimension')
     batch, t, vocab = logits.shape
-    _require(tokens.is_cuda and tokens.dtype == torch.int64 and tokens.shape == (batch, t) and tokens.is_contiguous(),
-             'tokens must be contiguous int64 [B, T] on CUDA')
+    dev = logits.device
+    if not (tokens.dtype == torch.int64 and tokens.shape == (batch, t) and tokens.device == dev and tokens.is_contiguous()):
+        _refuse('tokens must be contiguous int64 [B, T] on the logits\' device')
     a = _lib.TreeAcceptArgs()
     a.batch, a.nodes, a.vocab, a.type = batch, t, vocab, _TYPES[logits.dtype]
     a.logits, a.tokens, a.parents = logits.data_ptr(), tokens.data_ptr(), _i32(parents, (batch, t), 'parents')
-    a.logits_stride[:] = logits.stride()[:2]
+    a.logits_stride[0], a.logits_stride[1] = logits.stride()[:2]
     if nodes is not None:
         a.nodes_len = _i32(nodes, (batch,), 'nodes')
-    dev = logits.device
     path = torch.empty((batch, t), dtype=torch.int32, device=dev)
     count = torch.empty(batch, dtype=torch.int32, device=dev)
     following = torch.empty(batch, dtype=torch.int64, device=dev)
     a.path, a.count, a.next = path.data_ptr(), count.data_ptr(), following.data_ptr()
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        size = lib.slimkv_tree_accept_workspace_size(ctypes.byref(a))
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        _lib.check(lib.slimkv_tree_accept(ctypes.byref(a), _ptr(ws), size, _stream()))
+    ws = _workspace(dev, lib.slimkv_tree_accept_workspace_size, a)
+    _run(dev, lib.slimkv_tree_accept, byref(a), ws.data_ptr(), ws.numel())
     return path, count, following
 
 
@@ -165,22 +207,23 @@ def tree_commit(k, v, lengths, path, count, block_tables=None):
     any 1-, 2- or 4-byte type.  ``path`` / ``count`` as :func:`tree_accept`
     returns them.  Returns the new lengths (int32 ``[B]``).
     """
-    _require(k.dim() == v.dim() and k.dim() in (4, 5) and k.dtype == v.dtype, 'k and v must be [(layers,) B, rows, Hkv, D]')
-    if k.dim() == 4:
-        k, v = k.unsqueeze(0), v.unsqueeze(0)
-    _require(k.shape[0] == v.shape[0] and k.shape[0] > 0 and path.dim() == 2, 'K and V of the same layers; path [B, T]')
+    first = k.dim() - 4
+    if first not in (0, 1) or path.dim() != 2:
+        _refuse('k and v must be [(layers,) B, rows, Hkv, D], path [B, T]')
+    _check_rows(k, v, 4 + first)
     batch, t = path.shape
-    _require(block_tables is not None or k.shape[1] == batch, 'one cache for each sequence')
+    shape, v_dim, dev = k.shape, v.shape[-1], k.device
+    if block_tables is None and shape[first] != batch:
+        _refuse('one cache for each sequence')
     a = _lib.TreeCommitArgs()
-    fill_cache(a.cache, k[0], v[0], block_tables, batch)
-    a.cache.k_stride[0], a.cache.v_stride[0] = k.stride(1), v.stride(1)
-    a.layers, a.batch, a.nodes, a.kv_heads = k.shape[0], batch, t, k.shape[3]
-    a.dim_qk, a.dim_v, a.elem_bytes = k.shape[4], v.shape[4], k.element_size()
-    a.k_layer_stride, a.v_layer_stride = k.stride(0), v.stride(0)
-    new_lengths = torch.empty(batch, dtype=torch.int32, device=k.device)
+    fill_cache(a.cache, k, v, block_tables, batch, first)
+    a.layers, a.batch, a.nodes, a.kv_heads = shape[0] if first else 1, batch, t, shape[-2]
+    a.dim_qk, a.dim_v, a.elem_bytes = shape[-1], v_dim, k.element_size()
+    if first:
+        a.k_layer_stride, a.v_layer_stride = k.stride(0), v.stride(0)
+    new_lengths = torch.empty(batch, dtype=torch.int32, device=dev)
     a.lengths, a.path, a.count = (_i32(lengths, (batch,), 'lengths'), _i32(path, (batch, t), 'path'),
                                   _i32(count, (batch,), 'count'))
     a.new_lengths = new_lengths.data_ptr()
-    with torch.cuda.device(k.device):
-        _lib.check(_lib.load().slimkv_tree_commit(ctypes.byref(a), _stream()))
+    _run(dev, _lib.load().slimkv_tree_commit, byref(a))
     return new_lengths
