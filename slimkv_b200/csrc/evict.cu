@@ -4,13 +4,13 @@
 // `recent` rows and the rows of the largest mass up to `keep`, in order.  Two
 // launches:
 //   evict_select_kernel  one cluster of CTAs per segment: the keep-th largest
-//     of its masses (order-preserving 32-bit keys, radix selection with digits
-//     of 11, 11 and 10 bits, whose counts the CTAs add up over distributed
-//     shared memory), how many rows equal to it still fit, and for every run
-//     of kRun rows how many rows above it and equal to it come before the run;
+//     of its masses (order-preserving 32-bit keys, radix selection with four
+//     8-bit digits, whose counts the CTAs add up over distributed shared
+//     memory), how many rows equal to it still fit, and for every run of kRun
+//     rows how many rows above it and equal to it come before the run;
 //   evict_gather_kernel  one block per run, a dependent launch: which of its
-//     rows stay and where they go, then their K, V, mass and position moved, a
-//     warp to a row, 16 bytes a lane.
+//     rows stay and where they go, then their K, V, mass and position moved, 16
+//     bytes a lane, eight of them under way at a time.
 // Bound: HBM, the masses once (later readings come from L2) and each kept row
 // read and written.
 #include <algorithm>
@@ -23,9 +23,10 @@ namespace {
 
 constexpr int kRun = 128;                 // rows of one gather block
 constexpr int kGatherThreads = 256;
-constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
 constexpr int kSelectThreads = 1024;
+constexpr int kBins = 256, kKeys = 4;      // digit values; keys of a thread in registers
+constexpr int kTile = kKeys * kSelectThreads, kChunks = kTile / 32;   // rows of a CTA's tile, 32 to a chunk
 constexpr uint32_t kAlways = 0xffffffffu; // key of a protected row
 
 struct EvictArgs {
@@ -66,10 +67,11 @@ __device__ __forceinline__ int segment_length(const EvictArgs& a, int b) {
 }
 
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs a) {
-    __shared__ uint32_t hist[3][kBins];       // one per digit: no pass clears what another still reads
-    __shared__ uint32_t warp_sum[32];
+    __shared__ uint32_t hist[4][kBins];       // one per digit: no pass clears what another still reads
+    __shared__ uint32_t warp_sum[8];
     __shared__ uint32_t pick[2];              // the chosen digit, rows above it
     __shared__ uint32_t counts[2];            // this CTA's rows above and equal to the threshold
+    __shared__ uint2 chunk[kChunks];
     const uint32_t ranks = cluster_size(), rank = cluster_rank();
     const int segment = blockIdx.x / ranks, g = segment % a.kv_heads, b = segment / a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -81,57 +83,72 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
         if (given != len) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
     }
     grid_launch_dependents();
-    // This CTA's rows: whole runs.
+    // This CTA's rows: whole runs, in tiles of kTile; key j of a thread is row
+    // 32 (32 j + warp) + lane of the tile.
     const int runs_each = (a.runs + int(ranks) - 1) / int(ranks);
     const int run0 = min(int(rank) * runs_each, a.runs), run1 = min(run0 + runs_each, a.runs);
     const int n0 = min(run0 * kRun, len), n1 = min(run1 * kRun, len);
+    const int tiles = (n1 - n0 + kTile - 1) / kTile;
+    uint32_t keys[kKeys];
+    auto load = [&](int tile) {
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+            const int n = n0 + tile * kTile + 32 * (32 * j + warp) + lane;
+            keys[j] = n < n1 ? key_of(__ldg(mass + n), n, len, a.sinks, a.recent) : 0u;   // 0: below every row's key
+        }
+    };
+    for (int i = tid; i < 4 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+    if (tiles == 1) load(0);
     uint32_t prefix = 0, want = uint32_t(min(a.keep, len));
     const bool all = len <= a.keep;
     if (!all) {
-        for (int i = tid; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
         __syncthreads();
         // `want` of the rows that match `prefix` so far are still to be found.
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above_bits = pass == 0 ? 32 : shift + 11 - (pass == 2);
-            const uint32_t bins = pass == 2 ? 1024u : 2048u;
-            for (int n = n0 + tid; n < n1; n += kSelectThreads) {
-                const uint32_t key = key_of(__ldg(mass + n), n, len, a.sinks, a.recent);
-                if (pass == 0 || (key >> above_bits) == (prefix >> above_bits)) atomicAdd(&hist[pass][key >> shift & (bins - 1)], 1u);
+#pragma unroll 1
+        for (int pass = 0; pass < 4; ++pass) {
+            const int shift = 24 - 8 * pass;
+            for (int tile = 0; tile < tiles; ++tile) {
+                if (tiles > 1) load(tile);
+#pragma unroll
+                for (int j = 0; j < kKeys; ++j) {
+                    // Masses share few exponents: lanes with the same digit count once.
+                    const bool in = keys[j] && (pass == 0 || (keys[j] ^ prefix) >> (shift + 8) == 0);
+                    const uint32_t digit = in ? keys[j] >> shift & 255 : 256u;
+                    const unsigned same = __match_any_sync(0xffffffffu, digit);
+                    if (in && lane == __ffs(int(same)) - 1) atomicAdd(&hist[pass][digit], uint32_t(__popc(same)));
+                }
             }
             __syncthreads();
-            cluster_sync();
-            // Bins of all CTAs from the top: thread t has bins 2047 - 2t and 2046 - 2t.
-            uint32_t c[2];
+            if (ranks > 1) cluster_sync();
+            // Thread t < 256 has bin 255 - t, of all CTAs: rows above it, from the top.
+            uint32_t c = 0, above = 0;
+            if (tid < kBins) {
+                const uint32_t* bin = &hist[pass][kBins - 1 - tid];
+                if (ranks == 1) {
+                    c = *bin;
+                } else {
+                    uint32_t of[kMaxCluster];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t* bin = &hist[pass][kBins - 1 - 2 * tid - i];
-                c[i] = 0;
-                for (uint32_t r = 0; r < ranks; ++r) c[i] += cluster_load(bin, r);
-            }
-            const uint32_t sum = c[0] + c[1];
-            uint32_t above = sum;
+                    for (uint32_t r = 0; r < kMaxCluster; ++r) of[r] = r < ranks ? cluster_load(bin, r) : 0u;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, above, o);
-                if (lane >= o) above += up;
+                    for (uint32_t r = 0; r < kMaxCluster; ++r) c += of[r];
+                }
+                above = c;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t up = __shfl_up_sync(0xffffffffu, above, o);
+                    if (lane >= o) above += up;
+                }
+                if (lane == 31) warp_sum[warp] = above;
             }
-            if (lane == 31) warp_sum[warp] = above;
             __syncthreads();
-            uint32_t before = warp_sum[lane];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
-                if (lane >= o) before += up;
-            }
-            before = __shfl_sync(0xffffffffu, before, warp ? warp - 1 : 0);
-            above += (warp ? before : 0u) - sum;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (above < want && above + c[i] >= want) {
-                    pick[0] = uint32_t(kBins - 1 - 2 * tid - i);
+            if (tid < kBins) {
+                above -= c;
+                for (int w = 0; w < warp; ++w) above += warp_sum[w];
+                if (above < want && above + c >= want) {
+                    pick[0] = uint32_t(kBins - 1 - tid);
                     pick[1] = above;
                 }
-                above += c[i];
             }
             __syncthreads();
             prefix |= pick[0] << shift;
@@ -142,36 +159,40 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
         a.threshold[segment] = prefix;        // all: 0, below every row's key
         a.ties[segment] = all ? 0u : want;
     }
-    // Rows above and equal to the threshold before each run: a warp takes a run
-    // at a time, 32 of them are scanned together, first within the CTA.
+    // Rows above and equal to the threshold before each run, first within the CTA.
     uint2* before = a.before + int64_t(segment) * a.runs;
-    uint32_t* gt_of = hist[0];                // (every CTA of the cluster is past pass 0)
-    uint32_t* tie_of = hist[0] + 32;
     uint32_t base_gt = 0, base_tie = 0;
-    for (int r0 = run0; r0 < run1; r0 += 32) {
-        uint32_t gt = 0, tie = 0;
-        if (r0 + warp < run1) {
-            for (int i = 0; i < kRun; i += 32) {
-                const int n = (r0 + warp) * kRun + i + lane;
-                const uint32_t key = n < len ? key_of(__ldg(mass + n), n, len, a.sinks, a.recent) : 0u;
-                gt += __popc(__ballot_sync(0xffffffffu, n < len && key > prefix));
-                tie += __popc(__ballot_sync(0xffffffffu, n < len && key == prefix));
-            }
+    for (int tile = 0; tile < tiles; ++tile) {
+        if (tiles > 1) load(tile);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+            const uint32_t gt = __popc(__ballot_sync(0xffffffffu, keys[j] > prefix));
+            const uint32_t tie = __popc(__ballot_sync(0xffffffffu, keys[j] && keys[j] == prefix));
+            if (lane == 0) chunk[32 * j + warp] = make_uint2(gt, tie);
         }
         __syncthreads();
-        if (lane == 0) { gt_of[warp] = gt; tie_of[warp] = tie; }
-        __syncthreads();
-        uint32_t g_in = gt_of[lane], t_in = tie_of[lane];
-        const uint32_t g_own = g_in, t_own = t_in;
+        // Every warp scans the tile's chunks, four to a lane.
+        uint2 own[4], sum = make_uint2(0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            own[i] = chunk[4 * lane + i];
+            sum.x += own[i].x;
+            sum.y += own[i].y;
+        }
+        uint2 incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t gu = __shfl_up_sync(0xffffffffu, g_in, o), tu = __shfl_up_sync(0xffffffffu, t_in, o);
-            if (lane >= o) { g_in += gu; t_in += tu; }
+            const uint32_t gu = __shfl_up_sync(0xffffffffu, incl.x, o), tu = __shfl_up_sync(0xffffffffu, incl.y, o);
+            if (lane >= o) { incl.x += gu; incl.y += tu; }
         }
-        if (warp == 0 && r0 + lane < run1) before[r0 + lane] = make_uint2(base_gt + g_in - g_own, base_tie + t_in - t_own);
-        base_gt += __shfl_sync(0xffffffffu, g_in, 31);
-        base_tie += __shfl_sync(0xffffffffu, t_in, 31);
+        const int run = run0 + tile * (kTile / kRun) + lane;      // (a run is four chunks)
+        if (warp == 0 && run < run1) before[run] = make_uint2(base_gt + incl.x - sum.x, base_tie + incl.y - sum.y);
+        base_gt += __shfl_sync(0xffffffffu, incl.x, 31);
+        base_tie += __shfl_sync(0xffffffffu, incl.y, 31);
     }
+    // Runs of this CTA past its rows (all of them in a segment shorter than the budget).
+    for (int run = run0 + tiles * (kTile / kRun) + tid; run < run1; run += kSelectThreads) before[run] = make_uint2(base_gt, base_tie);
     if (ranks == 1) return;
     // Then what the CTAs before this one hold.
     if (tid == 0) { counts[0] = base_gt; counts[1] = base_tie; }
@@ -190,9 +211,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
     }
     cluster_sync();                           // no CTA leaves while another reads its counts
 }
+static_assert(kRun == 128 && kChunks == 128, "a run is four chunks, a tile 32 runs");
 
 __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs a) {
-    __shared__ uint8_t src[kRun];
+    __shared__ int64_t from[2][kRun], to[2][kRun];      // byte offsets of the kept rows: K, V (-1: no such page)
     __shared__ uint32_t warp_tie[kRun / 32], warp_keep[kRun / 32];
     const int run = blockIdx.x, g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int segment = b * a.kv_heads + g;
@@ -225,64 +247,65 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
         total += warp_keep[w];
     }
     const int first = int(before.x + min(before.y, ties));
+    bool bad = false;
     if (stays) {
-        src[local] = uint8_t(tid);
         const int d = first + local;
+        int64_t ip, op;
+        int ir, orow;
+        const bool in = cache_row(a.in, b, n, ip, ir), out = cache_row(a.out, b, d, op, orow);
+        bad = !in || !out;
+        from[0][local] = bad ? -1 : ip * a.in.k_stride[0] + ir * a.in.k_stride[1] + g * a.in.k_stride[2];
+        from[1][local] = bad ? -1 : ip * a.in.v_stride[0] + ir * a.in.v_stride[1] + g * a.in.v_stride[2];
+        to[0][local] = op * a.out.k_stride[0] + orow * a.out.k_stride[1] + g * a.out.k_stride[2];
+        to[1][local] = op * a.out.v_stride[0] + orow * a.out.v_stride[1] + g * a.out.v_stride[2];
         if (a.out_mass) a.out_mass[b * a.out_mass_stride[0] + g * a.out_mass_stride[1] + d] = x;
         if (a.out_positions)
             a.out_positions[b * a.out_positions_stride[0] + g * a.out_positions_stride[1] + d] =
                 __ldg(a.positions + b * a.positions_stride[0] + g * a.positions_stride[1] + n);
     }
     __syncthreads();
-    // The kept rows, kRows of a warp at a time so that their loads overlap; then the zeroed
-    // rows [kept, keep) of this run.
-    constexpr int kWarps = kGatherThreads / 32, kRows = 4;
-    bool bad = false;
-    auto row_of = [&](const CacheView& c, int m, const int64_t* st) -> int64_t {
-        int64_t page;
-        int row;
-        if (!cache_row(c, b, m, page, row)) { bad = true; return -1; }
-        return page * st[0] + row * st[1] + g * st[2];
-    };
-    auto move = [&](const uint8_t* from, uint8_t* to, const int64_t* in, const int64_t* out, int units) {
-        for (int r0 = warp; r0 < total; r0 += kWarps * kRows) {
-            const uint4* p[kRows];
-            uint4* q[kRows];
+    // The kept rows: pieces of 32 lanes x 16 bytes of a row's K and V, kPieces of a warp
+    // under way at a time; then the zeroed rows [kept, keep) of this run.
+    constexpr int kWarps = kGatherThreads / 32, kPieces = 8;
+    const int units = a.k_units + a.v_units, per_row = (units + 31) / 32, pieces = total * per_row;
+    // p / per_row by multiplication: exact while p per_row < 2^20 (p < 128 per_row, per_row <= 64).
+    const uint32_t inverse = (1u << 20) / uint32_t(per_row) + 1u;
+    const bool small = per_row <= 64;
+    for (int p0 = warp; p0 < pieces; p0 += kWarps * kPieces) {
+        uint4 w[kPieces];
+        uint4* dst[kPieces];
 #pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                const int r = r0 + k * kWarps;
-                p[k] = nullptr;
-                if (r < total) {
-                    const int64_t i = row_of(a.in, n0 + src[r], in), o = row_of(a.out, first + r, out);
-                    if (i >= 0 && o >= 0) {
-                        p[k] = reinterpret_cast<const uint4*>(from + i);
-                        q[k] = reinterpret_cast<uint4*>(to + o);
-                    }
-                }
-            }
-            for (int u = lane; u < units; u += 32) {
-                uint4 w[kRows];
-#pragma unroll
-                for (int k = 0; k < kRows; ++k)
-                    if (p[k]) w[k] = __ldcs(p[k] + u);
-#pragma unroll
-                for (int k = 0; k < kRows; ++k)
-                    if (p[k]) __stcs(q[k] + u, w[k]);
-            }
+        for (int k = 0; k < kPieces; ++k) {
+            const int p = p0 + k * kWarps;
+            dst[k] = nullptr;
+            if (p >= pieces) continue;
+            const int r = small ? int(uint32_t(p) * inverse >> 20) : p / per_row;
+            int u = (p - r * per_row) * 32 + lane;
+            if (u >= units) continue;
+            const int is_v = u >= a.k_units;
+            if (is_v) u -= a.k_units;
+            const int64_t i = from[is_v][r];
+            if (i < 0) continue;
+            dst[k] = reinterpret_cast<uint4*>((is_v ? a.out_v : a.out_k) + to[is_v][r]) + u;
+            w[k] = __ldcs(reinterpret_cast<const uint4*>((is_v ? a.v : a.k) + i) + u);
         }
-    };
-    move(a.k, a.out_k, a.in.k_stride, a.out.k_stride, a.k_units);
-    move(a.v, a.out_v, a.in.v_stride, a.out.v_stride, a.v_units);
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k)
+            if (dst[k]) __stcs(dst[k], w[k]);
+    }
     const int z0 = max(n0, kept), z1 = min(n0 + kRun, a.keep);
     for (int d = z0 + tid; d < z1; d += kGatherThreads) {
         if (a.out_mass) a.out_mass[b * a.out_mass_stride[0] + g * a.out_mass_stride[1] + d] = 0.f;
         if (a.out_positions) a.out_positions[b * a.out_positions_stride[0] + g * a.out_positions_stride[1] + d] = 0;
     }
     for (int d = z0 + warp; d < z1; d += kWarps) {
-        const int64_t ok = row_of(a.out, d, a.out.k_stride), ov = row_of(a.out, d, a.out.v_stride);
-        if (ok < 0 || ov < 0) continue;
-        for (int u = lane; u < a.k_units; u += 32) reinterpret_cast<uint4*>(a.out_k + ok)[u] = make_uint4(0, 0, 0, 0);
-        for (int u = lane; u < a.v_units; u += 32) reinterpret_cast<uint4*>(a.out_v + ov)[u] = make_uint4(0, 0, 0, 0);
+        int64_t page;
+        int row;
+        if (!cache_row(a.out, b, d, page, row)) { bad = true; continue; }
+        uint4* ok = reinterpret_cast<uint4*>(a.out_k + page * a.out.k_stride[0] + row * a.out.k_stride[1] + g * a.out.k_stride[2]);
+        uint4* ov = reinterpret_cast<uint4*>(a.out_v + page * a.out.v_stride[0] + row * a.out.v_stride[1] + g * a.out.v_stride[2]);
+        for (int u = lane; u < a.k_units; u += 32) ok[u] = make_uint4(0, 0, 0, 0);
+        for (int u = lane; u < a.v_units; u += 32) ov[u] = make_uint4(0, 0, 0, 0);
     }
     if (bad) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
 }
@@ -374,9 +397,9 @@ extern "C" int slimkv_evict(const slimkv_evict_args* a, void* workspace, size_t 
     if (!workspace || !c.fits() || reinterpret_cast<uintptr_t>(workspace) % 8)
         return fail(SLIMKV_ERR_WORKSPACE, "evict: workspace of %zu bytes needed", c.used);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // A CTA of a cluster takes at least four rows a thread: up to 8 CTAs (32768 rows and more).
+    // CTAs of a cluster as many (up to 8) as keep their keys in registers.
     int ranks = 1;
-    while (ranks < kMaxCluster && int64_t(k.rows) > int64_t(ranks) * 4 * kSelectThreads) ranks *= 2;
+    while (ranks < kMaxCluster && int64_t(k.rows) > int64_t(ranks) * kTile) ranks *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(a->kv_heads) * unsigned(a->batch) * unsigned(ranks));
     cfg.blockDim = dim3(kSelectThreads);

@@ -16,8 +16,9 @@
 // Bound: HBM (each K row read once) up to about 170 rows of 128, then the
 // exponentials.
 //
-// Warps: 0 = K loads (TMA), 1 = MMA issue, 2 = TMEM owner, 4-7 = Q rows
-// gathered into shared memory, then the sums.  Every wait is bounded.
+// Warps: 0 = K loads (TMA), 1 = MMA issue, 2 = TMEM owner, 4-11 = Q rows
+// gathered into shared memory, then the sums, 4-7 of a CTA's even tiles and
+// 8-11 of its odd ones.  Every wait is bounded.
 #include <algorithm>
 
 #include "cache_view.cuh"
@@ -32,7 +33,7 @@ constexpr int kMaxCols = 256;
 constexpr uint32_t kChunk = 128 * 128;
 constexpr uint32_t kTileArea = 224 * 1024;
 constexpr int kMaxRing = 12;
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Bars {
@@ -48,7 +49,7 @@ static_assert(kSmemBytes <= 232448, "shared memory budget");
 
 struct Job {
     int batch, nodes, heads, kv_heads, group, ctas;
-    int dim, kc, kring, cols;   // 64-column chunks of a K row, ring slots, columns of a row block
+    int dim, kring, cols;       // ring slots (64-column chunks of 128 keys), columns of a row block
     int context_only, paged, shared_cache, box;
     CacheView cache;
     int64_t capacity;           // rows a sequence may hold (cache and mass)
@@ -83,13 +84,21 @@ struct Plan {
     }
 };
 
+// A wait that is over costs one test; one that is not looks for an abort of
+// another warp and for its limit.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
-    if (*const_cast<volatile int*>(&bs->abort)) return false;
-    if (mbar_wait(bar, parity, J.wait_ns)) return true;
+    if (mbar_test(bar, parity)) return true;
+    for (uint64_t waited = 0; waited < J.wait_ns;) {
+        const uint64_t step = min(J.wait_ns - waited, uint64_t(100000));
+        if (mbar_wait(bar, parity, step)) return true;
+        if (*const_cast<volatile int*>(&bs->abort)) return false;
+        waited += step;
+    }
     bs->abort = 1;
     report(J.status, SLIMKV_DEVICE_TIMEOUT);
     return false;
 }
+__device__ __forceinline__ bool all_lanes(bool x) { return __all_sync(0xffffffffu, x); }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
     return __all_sync(0xffffffffu, wait_bar(bar, parity, bs, J));
 }
@@ -98,7 +107,8 @@ __device__ __forceinline__ void copy16(void* dst, const void* src, bool some) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(some ? 16 : 0) : "memory");
 }
 
-template <bool kHalf>
+// kc: 64-column chunks of a K row.
+template <int kc, bool kHalf>
 __global__ void __launch_bounds__(kThreads, 1)
 key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ Job J) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -107,11 +117,11 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // Layout: Q (kc chunks of cols x 64) | K ring.
     const uint32_t q_chunk = uint32_t(J.cols) * 128u;
-    const uint32_t off_k = (uint32_t(J.kc) * q_chunk + 1023u) & ~1023u;
+    const uint32_t off_k = (uint32_t(kc) * q_chunk + 1023u) & ~1023u;
 
     if (tid == 0) {
         for (int s = 0; s < kMaxRing; ++s) { mbar_init(&bs->kfull[s], 1); mbar_init(&bs->kempty[s], 1); }
-        mbar_init(&bs->qfull, 4);
+        mbar_init(&bs->qfull, 8);
         for (int s = 0; s < 2; ++s) { mbar_init(&bs->sfull[s], 1); mbar_init(&bs->sempty[s], 4); }
         mbar_init(&bs->final_mma, 1);
         bs->abort = 0;
@@ -126,7 +136,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tbase = bs->tmem_base;
+    // All 512 tensor memory columns are this CTA's: addresses begin at column 0.
     const uint32_t sbase = smem_u32(smem);
     const bool any = int(blockIdx.x) < bs->share.ctas;
     auto blocks_of = [&](const Seq& s) { return max(1, (s.count * J.group + J.cols - 1) / J.cols); };
@@ -151,7 +161,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                         if (!cache_row(J.cache, w.b, min(row, last / J.box * J.box), page, row))
                             report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
                     }
-                    for (int c = 0; c < J.kc; ++c) {
+                    for (int c = 0; c < kc; ++c) {
                         if (lap && !(ok = warp_wait(&bs->kempty[slot], (lap - 1) & 1, bs, J))) break;
                         if (lane == 0) mbar_expect_tx(&bs->kfull[slot], kChunk);
                         __syncwarp();
@@ -163,122 +173,126 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 }
         }
     } else if (any && warp == 1) {
-        // ---- MMA issuer ----
-        const bool leader = lane == 0;
-        int slot = 0, i = 0, q_blocks = 0;
-        uint32_t lap = 0;
-        bool ok = true;
+        // ---- MMA issue: the warp stays converged and one elected thread has the
+        // instructions, so that their operands are uniform registers ----
+        const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024), k_desc = umma_desc_sw128(sbase + off_k, 16, 1024);
+        const uint32_t q_step = q_chunk >> 4;
+        int slot = 0;
+        uint32_t lap = 0, buf = 0, s_lap = 0, q_lap = 0;
+        bool again = false, ok = true;                      // again: both S buffers have been used
         Walk<Plan> w;
         w.start(plan, &bs->share);
-        while (ok && w.next(plan)) {
+        while (all_lanes(ok && w.next(plan))) {
             const int blocks = blocks_of(w.s);
-            for (int block = 0; block < blocks && ok; ++block, ++q_blocks) {
+            for (int block = 0; all_lanes(ok && block < blocks); ++block) {
                 const int n = max(16, (cols_of(w.s, block) + 15) & ~15);
                 // fp16: both operand formats (bits [7,10) and [10,13)) are 0.
                 const uint32_t idesc = umma_idesc_bf16(128, n, 0, 0) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
-                ok = warp_wait(&bs->qfull, q_blocks & 1, bs, J);
-                for (int tile = w.t0; tile < w.t1 && ok; ++tile, ++i) {
-                    const int sb = i & 1;
-                    if (i >= 2) ok = warp_wait(&bs->sempty[sb], ((i >> 1) - 1) & 1, bs, J);
-                    for (int c = 0; c < J.kc && ok; ++c) {
-                        ok = warp_wait(&bs->kfull[slot], lap & 1, bs, J);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (leader) {
-                            const uint32_t ka = sbase + off_k + slot * kChunk, qa = sbase + c * q_chunk;
+                ok = ok && wait_bar(&bs->qfull, q_lap, bs, J);
+                q_lap ^= 1;
+                for (int tile = w.t0; all_lanes(ok && tile < w.t1); ++tile) {
+                    if (again) ok = ok && wait_bar(&bs->sempty[buf], s_lap ^ 1, bs, J);
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
-                                umma_bf16(tbase + sb * kMaxCols, umma_desc_sw128(ka + kk * 32, 16, 1024),
-                                          umma_desc_sw128(qa + kk * 32, 16, 1024), idesc, (c | kk) != 0);
+                    for (int c = 0; c < kc; ++c) {
+                        ok = ok && wait_bar(&bs->kfull[slot], lap, bs, J);
+                        if (!all_lanes(ok)) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint64_t a = k_desc + uint32_t(slot) * (kChunk >> 4), b = q_desc + uint32_t(c) * q_step;
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) umma_bf16(buf * kMaxCols, a + 2 * kk, b + 2 * kk, idesc, (c | kk) != 0);
                             umma_commit(&bs->kempty[slot]);
+                            if (c == kc - 1) umma_commit(&bs->sfull[buf]);
                         }
                         __syncwarp();
-                        if (++slot == J.kring) { slot = 0; ++lap; }
+                        if (++slot == J.kring) { slot = 0; lap ^= 1; }
                     }
-                    if (ok && leader) umma_commit(&bs->sfull[sb]);
-                    __syncwarp();
+                    if (buf) { s_lap ^= 1; again = true; }
+                    buf ^= 1;
                 }
             }
         }
-        if (leader) umma_commit(&bs->final_mma);
+        if (elect_one()) umma_commit(&bs->final_mma);
+        __syncwarp();
     } else if (any && warp >= 4) {
         // ---- Q rows into shared memory, then a key per thread ----
-        const int quarter = warp & 3, st = tid - 128;
+        const int quarter = warp & 3, turn = (warp >> 2) - 1;
         const uint32_t lane_addr = uint32_t(32 * quarter) << 16;
-        int i = 0;
-        bool failed = false;
+        int i = 0;                                          // tiles begun before
+        bool ok = true;
         Walk<Plan> w;
         w.start(plan, &bs->share);
-        // After a wait that ran out the four warps still meet at every barrier, without work.
+        // After a wait that ran out the eight warps still meet at every barrier, without work.
         while (w.next(plan)) {
             const int blocks = blocks_of(w.s);
             float* mass = J.mass + w.b * J.m_sb + w.g * J.m_sh;
             for (int block = 0; block < blocks; ++block) {
-                // The products of the block before are done (their S was awaited by every thread of the four warps).
-                named_bar(1, 128);
+                // The products of the block before are done: each S was awaited by its warps.
+                named_bar(1, 256);
                 const int cols = cols_of(w.s, block), padded = max(16, (cols + 15) & ~15);
-                const int units = J.kc * 8;
-                for (int k = st; k < padded * units; k += 128) {
-                    const int col = k / units, u = k - col * units;
+                // A warp per row: its node, then 16 bytes a lane; rows past the block's are zeros.
+                for (int col = warp - 4; col < padded; col += 8) {
                     const int at = block * J.cols + col, row = at / J.group;
                     int r = row;
                     if (J.rows && col < cols) r = __ldg(J.rows + int64_t(w.b) * J.nodes + row);
-                    const bool some = col < cols && r >= 0 && r < J.nodes && u * 8 < J.dim;
-                    const uint16_t* src = some ? J.q + w.b * J.q_sb + r * J.q_st + (w.g * J.group + at % J.group) * J.q_sh + u * 8 : J.q;
-                    copy16(smem + (u >> 3) * q_chunk + col * 128 + (((u & 7) ^ (col & 7)) << 4), src, some);
-                }
-                for (int col = st; col < padded; col += 128) {
-                    const int at = block * J.cols + col, row = at / J.group;
-                    float off = INFINITY;
-                    if (col < cols) {
-                        const int r = J.rows ? __ldg(J.rows + int64_t(w.b) * J.nodes + row) : row;
-                        if (r >= 0 && r < J.nodes) {
-                            const float x = __ldg(J.lse + (int64_t(w.b) * J.nodes + r) * J.heads + w.g * J.group + at % J.group);
+                    const bool some = col < cols && r >= 0 && r < J.nodes;
+                    const int h = w.g * J.group + at - row * J.group;
+                    const uint16_t* src = J.q + (some ? w.b * J.q_sb + r * J.q_st + h * J.q_sh : 0);
+                    for (int u = lane; u < kc * 8; u += 32)
+                        copy16(smem + (u >> 3) * q_chunk + col * 128 + (((u & 7) ^ (col & 7)) << 4), some && u * 8 < J.dim ? src + u * 8 : J.q,
+                               some && u * 8 < J.dim);
+                    if (lane == 0) {
+                        float off = INFINITY;
+                        if (some) {
+                            const float x = __ldg(J.lse + (int64_t(w.b) * J.nodes + r) * J.heads + h);
                             if (x != -INFINITY) off = x * kLog2e;
-                        } else {
+                        } else if (col < cols) {
                             report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
                         }
+                        bs->lse[col] = off;
                     }
-                    bs->lse[col] = off;
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_async_shared();
-                named_bar(1, 128);
+                named_bar(1, 256);
                 if (lane == 0) mbar_arrive(&bs->qfull);
-                for (int tile = w.t0; tile < w.t1 && !failed; ++tile, ++i) {
-                    const int sb = i & 1;
+                for (int tile = w.t0; tile < w.t1; ++tile, ++i) {
+                    if ((i & 1) != turn || !ok) continue;
                     const int n = tile * kKeys + 32 * quarter + lane;
                     const bool live = n < w.s.end;
                     const float old = !live ? 0.f : block ? mass[n] : n < w.s.len ? J.decay * mass[n] : 0.f;
-                    if (!warp_wait(&bs->sfull[sb], (i >> 1) & 1, bs, J)) { failed = true; break; }
+                    if (!(ok = warp_wait(&bs->sfull[turn], (i >> 1) & 1, bs, J))) continue;
                     tc_fence_after();
                     // The columns of rows that see key n: all for an old key, those of its own
                     // row and the rows behind it for an accepted one.
                     const int first = n < w.s.len ? 0 : (n - w.s.len) * J.group - block * J.cols;
+                    const bool whole = __all_sync(0xffffffffu, first <= 0);
                     float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
                     for (int c = 0; c < cols; c += 32) {
                         float v[32];
-                        tmem_ld32(tbase + lane_addr + uint32_t(sb * kMaxCols + c), v);
+                        tmem_ld32(lane_addr + uint32_t(turn * kMaxCols + c), v);
                         tmem_wait_ld();
-                        const bool full = __all_sync(0xffffffffu, first <= c) && c + 32 <= cols;
+                        if (whole && c + 32 <= cols) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 off = *reinterpret_cast<const float4*>(&bs->lse[c + e]);
-                            float p0 = sfu_exp2(fmaf(v[e], J.scale_log2, -off.x)), p1 = sfu_exp2(fmaf(v[e + 1], J.scale_log2, -off.y));
-                            float p2 = sfu_exp2(fmaf(v[e + 2], J.scale_log2, -off.z)), p3 = sfu_exp2(fmaf(v[e + 3], J.scale_log2, -off.w));
-                            if (!full) {
-                                const int k = c + e;
-                                p0 = k >= first && k < cols ? p0 : 0.f;
-                                p1 = k + 1 >= first && k + 1 < cols ? p1 : 0.f;
-                                p2 = k + 2 >= first && k + 2 < cols ? p2 : 0.f;
-                                p3 = k + 3 >= first && k + 3 < cols ? p3 : 0.f;
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 off = *reinterpret_cast<const float4*>(&bs->lse[c + e]);
+                                acc[0] += sfu_exp2(fmaf(v[e], J.scale_log2, -off.x));
+                                acc[1] += sfu_exp2(fmaf(v[e + 1], J.scale_log2, -off.y));
+                                acc[2] += sfu_exp2(fmaf(v[e + 2], J.scale_log2, -off.z));
+                                acc[3] += sfu_exp2(fmaf(v[e + 3], J.scale_log2, -off.w));
                             }
-                            acc[0] += p0; acc[1] += p1; acc[2] += p2; acc[3] += p3;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float p = sfu_exp2(fmaf(v[e], J.scale_log2, -bs->lse[c + e]));
+                                acc[e & 3] += c + e >= first && c + e < cols ? p : 0.f;
+                            }
                         }
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&bs->sempty[sb]);
+                    if (lane == 0) mbar_arrive(&bs->sempty[turn]);
                     if (live) mass[n] = old + ((acc[0] + acc[1]) + (acc[2] + acc[3]));
                 }
             }
@@ -301,13 +315,13 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
     __syncthreads();
     if (warp == 2) {
         tc_fence_after();
-        tmem_dealloc(tbase, 512);
+        tmem_dealloc(bs->tmem_base, 512);
     }
 }
 
-template <bool kHalf>
+template <int kc, bool kHalf>
 int launch(const CUtensorMap& km, const Job& J, cudaStream_t stream) {
-    auto kernel = key_mass_kernel<kHalf>;
+    auto kernel = key_mass_kernel<kc, kHalf>;
     static bool configured[64] = {};
     const int dev = device_info().device;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
@@ -359,9 +373,9 @@ extern "C" int slimkv_key_mass(const slimkv_key_mass_args* a, void* stream) {
     J.group = a->heads / a->kv_heads;
     J.ctas = device_info().sm_count;
     J.dim = a->dim;
-    J.kc = (a->dim + 63) / 64;
+    const int kc = (a->dim + 63) / 64;
     J.cols = std::min(kMaxCols, (a->nodes * J.group + 15) / 16 * 16);
-    J.kring = std::min<int>(kMaxRing, (kTileArea - ((uint32_t(J.kc) * J.cols * 128u + 1023u) & ~1023u)) / kChunk);
+    J.kring = std::min<int>(kMaxRing, (kTileArea - ((uint32_t(kc) * J.cols * 128u + 1023u) & ~1023u)) / kChunk);
     J.context_only = a->context_only;
     J.paged = paged;
     J.cache = cache_view(cache);
@@ -379,5 +393,12 @@ extern "C" int slimkv_key_mass(const slimkv_key_mass_args* a, void* stream) {
     J.status = status_word();
     J.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return a->type == SLIMKV_FP16 ? launch<true>(km, J, st) : launch<false>(km, J, st);
+    const bool half = a->type == SLIMKV_FP16;
+    switch (kc) {
+        case 1: return half ? launch<1, true>(km, J, st) : launch<1, false>(km, J, st);
+        case 2: return half ? launch<2, true>(km, J, st) : launch<2, false>(km, J, st);
+        case 3: return half ? launch<3, true>(km, J, st) : launch<3, false>(km, J, st);
+        case 4: return half ? launch<4, true>(km, J, st) : launch<4, false>(km, J, st);
+        default: return half ? launch<5, true>(km, J, st) : launch<5, false>(km, J, st);
+    }
 }
