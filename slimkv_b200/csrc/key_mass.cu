@@ -127,12 +127,13 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
         bs->abort = 0;
         fence_barrier_init();
     }
+    if (tid == 32) tma_prefetch_desc(&kmap);
     if (warp == 2) {
         tmem_alloc(&bs->tmem_base, 512);
         tmem_relinquish();
     }
     const Plan plan(J);
-    find_share<kThreads>(plan, &bs->share);
+    if (warp == 3) find_share(plan, &bs->share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -230,26 +231,36 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                 // The products of the block before are done: each S was awaited by its warps.
                 named_bar(1, 256);
                 const int cols = cols_of(w.s, block), padded = max(16, (cols + 15) & ~15);
-                // A warp per row: its node, then 16 bytes a lane; rows past the block's are zeros.
-                for (int col = warp - 4; col < padded; col += 8) {
-                    const int at = block * J.cols + col, row = at / J.group;
+                // Warp w takes the columns w, w + 8, ...: first a lane for each (row and
+                // log-sum-exp, one latency for all), then all lanes for one after the other, 16
+                // bytes a lane; zeros past the block's rows.
+                {
+                    const int col = warp - 4 + 8 * lane, at = block * J.cols + col, row = at / J.group;
                     int r = row;
                     if (J.rows && col < cols) r = __ldg(J.rows + int64_t(w.b) * J.nodes + row);
                     const bool some = col < cols && r >= 0 && r < J.nodes;
                     const int h = w.g * J.group + at - row * J.group;
-                    const uint16_t* src = J.q + (some ? w.b * J.q_sb + r * J.q_st + h * J.q_sh : 0);
-                    for (int u = lane; u < kc * 8; u += 32)
-                        copy16(smem + (u >> 3) * q_chunk + col * 128 + (((u & 7) ^ (col & 7)) << 4), some && u * 8 < J.dim ? src + u * 8 : J.q,
-                               some && u * 8 < J.dim);
-                    if (lane == 0) {
-                        float off = INFINITY;
-                        if (some) {
-                            const float x = __ldg(J.lse + (int64_t(w.b) * J.nodes + r) * J.heads + h);
-                            if (x != -INFINITY) off = x * kLog2e;
-                        } else if (col < cols) {
-                            report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+                    float off = INFINITY;
+                    if (some) {
+                        const float x = __ldg(J.lse + (int64_t(w.b) * J.nodes + r) * J.heads + h);
+                        if (x != -INFINITY) off = x * kLog2e;
+                    } else if (col < cols) {
+                        report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+                    }
+                    if (col < padded) bs->lse[col] = off;
+                    const int64_t mine = some ? w.b * J.q_sb + r * J.q_st + h * J.q_sh : -1;
+#pragma unroll 4
+                    for (int l = 0; l < 32; ++l) {
+                        const int64_t from = __shfl_sync(0xffffffffu, mine, l);
+                        const int c = warp - 4 + 8 * l;
+                        if (c >= padded) break;
+#pragma unroll
+                        for (int u0 = 0; u0 < kc * 8; u0 += 32) {
+                            const int u = u0 + lane;
+                            const bool live = from >= 0 && u * 8 < J.dim;
+                            if (u < kc * 8)
+                                copy16(smem + (u >> 3) * q_chunk + c * 128 + (((u & 7) ^ (c & 7)) << 4), J.q + (live ? from + u * 8 : 0), live);
                         }
-                        bs->lse[col] = off;
                     }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
@@ -380,6 +391,8 @@ extern "C" int slimkv_key_mass(const slimkv_key_mass_args* a, void* stream) {
     J.paged = paged;
     J.cache = cache_view(cache);
     J.capacity = std::min<int64_t>(cache_capacity(J.cache), a->mass_rows);
+    if (double(J.batch) * J.kv_heads * double(J.capacity / kKeys + 1) >= 2147483648.0)
+        return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "key mass: too many rows in one call");
     J.q = static_cast<const uint16_t*>(a->q);
     J.q_sb = a->q_stride[0]; J.q_st = a->q_stride[1]; J.q_sh = a->q_stride[2];
     J.lengths = a->lengths;

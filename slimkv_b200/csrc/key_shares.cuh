@@ -12,69 +12,81 @@
 
 namespace slimkv {
 
+// Callers make sure that a call has fewer than 2^31 units.
 template <class Plan>
-__device__ __forceinline__ long long units_of(const Plan& P, int b) {
+__device__ __forceinline__ uint32_t units_of(const Plan& P, int b) {
     const auto s = P.sequence(b);
-    return (long long)P.kv_heads * s.groups * s.tiles;
+    return uint32_t(P.kv_heads) * uint32_t(s.groups) * uint32_t(s.tiles);
 }
 // CTAs with a share: every share holds at least one unit.
-__device__ __forceinline__ int share_count(long long total, int ctas) { return int(min(total, (long long)ctas)); }
-__device__ __forceinline__ long long share_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
-// The CTA whose share holds unit u.
-__device__ __forceinline__ int share_of(long long total, long long u, int ctas) { return int(((u + 1) * ctas - 1) / total); }
+__device__ __forceinline__ uint32_t share_count(uint32_t total, int ctas) { return min(total, uint32_t(ctas)); }
+// floor(total cta / ctas) in 32 bits.
+__device__ __forceinline__ uint32_t share_begin(uint32_t total, uint32_t cta, uint32_t ctas) {
+    const uint32_t q = total / ctas;
+    return q * cta + (total - q * ctas) * cta / ctas;
+}
+// The CTA whose share holds unit u: an estimate, put right.
+__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t u, uint32_t ctas) {
+    uint32_t c = min(uint32_t(float(u) * float(ctas) / float(total)), ctas - 1);
+    while (share_begin(total, c, ctas) > u) --c;
+    while (c + 1 < ctas && share_begin(total, c + 1, ctas) <= u) ++c;
+    return c;
+}
 
 // Units of all sequences, and of those before sequence `upto`, over the block
 // (`scan`: two words per warp).
 template <int kThreads, class Plan>
-__device__ __forceinline__ void sum_units(const Plan& P, int upto, long long& total, long long& before, long long* scan) {
+__device__ __forceinline__ void sum_units(const Plan& P, int upto, uint32_t& total, uint32_t& before, uint32_t* scan) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    long long all = 0, head = 0;
+    uint32_t all = 0, head = 0;
     for (int b = tid; b < P.batch; b += kThreads) {
-        const long long u = units_of(P, b);
+        const uint32_t u = units_of(P, b);
         all += u;
         if (b < upto) head += u;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        all += __shfl_xor_sync(0xffffffffu, all, o);
-        head += __shfl_xor_sync(0xffffffffu, head, o);
-    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    head = __reduce_add_sync(0xffffffffu, head);
     if (lane == 0) { scan[2 * warp] = all; scan[2 * warp + 1] = head; }
     __syncthreads();
     total = before = 0;
+#pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) { total += scan[2 * w]; before += scan[2 * w + 1]; }
     __syncthreads();
 }
 
 // Where a CTA's share begins, in shared memory.
 struct Share {
-    long long total;            // units of all sequences
-    long long first_u;          // units before sequence first_b
+    uint32_t total;             // units of all sequences
+    uint32_t first_u;           // units before sequence first_b
     int first_b;
     int ctas;                   // CTAs with a share
-    long long scan[40];         // two words for each of up to 20 warps
 };
 
-// Fills `share` (all threads; the caller synchronises before reading it).
-template <int kThreads, class Plan>
+// Fills `share`, by one warp (the caller synchronises before reading it).
+template <class Plan>
 __device__ __forceinline__ void find_share(const Plan& P, Share* share) {
     const int lane = threadIdx.x & 31;
-    long long total, before;
-    sum_units<kThreads>(P, 0, total, before, share->scan);
-    const int ctas = share_count(total, P.ctas);
-    if (threadIdx.x == 0) { share->total = total; share->ctas = ctas; }
-    if (threadIdx.x >= 32 || int(blockIdx.x) >= ctas) return;
-    const long long u0 = share_begin(total, blockIdx.x, ctas);
-    long long base = 0;
+    uint32_t total = 0, first = 0;              // units of the first 32 sequences stay in registers
+    for (int b = lane; b < P.batch; b += 32) {
+        const uint32_t u = units_of(P, b);
+        if (b == lane) first = u;
+        total += u;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    const uint32_t ctas = share_count(total, P.ctas);
+    if (lane == 0) { share->total = total; share->ctas = int(ctas); }
+    if (blockIdx.x >= ctas) return;
+    const uint32_t u0 = share_begin(total, blockIdx.x, ctas);
+    uint32_t base = 0;
     for (int b0 = 0; b0 < P.batch && base <= u0; b0 += 32) {
-        const long long own = b0 + lane < P.batch ? units_of(P, b0 + lane) : 0;
-        long long incl = own;
+        const uint32_t own = b0 == 0 ? first : b0 + lane < P.batch ? units_of(P, b0 + lane) : 0;
+        uint32_t incl = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += up;
         }
-        const long long ex = base + incl - own;
+        const uint32_t ex = base + incl - own;
         if (own && u0 >= ex && u0 < ex + own) {
             share->first_b = b0 + lane;
             share->first_u = ex;
@@ -92,16 +104,15 @@ struct Walk {
     int t0, t1;                 // its key tiles
     int piece;                  // pieces begun before this one
     __device__ __forceinline__ void start(const Plan& P, const Share* share) {
-        const long long u = share_begin(share->total, blockIdx.x, share->ctas);
+        const uint32_t u = share_begin(share->total, blockIdx.x, share->ctas);
         left = int(share_begin(share->total, blockIdx.x + 1, share->ctas) - u);
         piece = -1;
         b = share->first_b;
         s = P.sequence(b);
-        const long long off = u - share->first_u;
-        const int seg = int(off / s.tiles);
-        g = seg / s.groups;
-        group = seg - g * s.groups;
-        t1 = int(off - (long long)seg * s.tiles);       // as if a piece had ended here
+        const uint32_t off = u - share->first_u, seg = off / uint32_t(s.tiles);
+        g = int(seg / uint32_t(s.groups));
+        group = int(seg) - g * s.groups;
+        t1 = int(off - seg * uint32_t(s.tiles));        // as if a piece had ended here
     }
     // Moves to the next piece; false when the share is done.
     __device__ __forceinline__ bool next(const Plan& P) {

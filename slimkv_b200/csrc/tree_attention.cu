@@ -321,12 +321,17 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         bs->bad_values[0] = bs->bad_values[1] = 0;
         fence_barrier_init();
     }
+    if (tid == 32) {
+        tma_prefetch_desc(&qmap);
+        tma_prefetch_desc(&kmap);
+        tma_prefetch_desc(&vmap);
+    }
     if (warp == 2) {
         tmem_alloc(&bs->tmem_base, 512);
         tmem_relinquish();
     }
     const Plan<NQ> plan(J);
-    find_share<kThreads>(plan, &bs->share);
+    if (warp == 3) find_share(plan, &bs->share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -731,23 +736,23 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
 // row group) per block.
 template <int NQ, bool kHalf>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Job J) {
-    __shared__ long long scan[8];
+    __shared__ uint32_t scan[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int at = blockIdx.x;
     const int group = at % J.row_groups;
     at /= J.row_groups;
     const int g = at % J.kv_heads, b = at / J.kv_heads;
     const Plan<NQ> plan(J);
-    long long total, before;
+    uint32_t total, before;
     sum_units<128>(plan, b, total, before, scan);
     const Seq s = plan.sequence(b);
     int c0 = 0, c1 = 0, slot0 = 0;
     const bool some = group < s.groups && s.tiles > 0;
     if (some) {
-        const long long u0 = before + ((long long)g * s.groups + group) * s.tiles;
-        const int ctas = share_count(total, J.ctas);
-        c0 = share_of(total, u0, ctas);
-        c1 = share_of(total, u0 + s.tiles - 1, ctas);
+        const uint32_t u0 = before + uint32_t(g * s.groups + group) * uint32_t(s.tiles);
+        const uint32_t ctas = share_count(total, J.ctas);
+        c0 = int(share_of(total, u0, ctas));
+        c1 = int(share_of(total, u0 + s.tiles - 1, ctas));
         slot0 = 2 * c0 + (share_begin(total, c0, ctas) != u0 ? 1 : 0);
     }
     if (threadIdx.x == 0 && g == 0 && group == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
@@ -912,8 +917,6 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.heads = a->heads;
     J.kv_heads = a->kv_heads;
     J.row_groups = (a->nodes + nq * J.tpt - 1) / (nq * J.tpt);
-    if (int64_t(J.batch) * J.kv_heads * J.row_groups > 0x7fffffffLL)
-        return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "tree attention: too many rows in one call");
     J.kc = (a->dim_qk + 63) / 64;
     J.vc = (a->dim_v + 63) / 64;
     J.dim_v = a->dim_v;
@@ -925,6 +928,8 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.paged = paged;
     J.cache = cache_view(cache);
     J.capacity = cache_capacity(J.cache);
+    if (double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / kKeys + 1) >= 2147483648.0)
+        return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "tree attention: too many rows in one call");
     J.lengths = a->lengths;
     J.nodes_len = a->nodes_len;
     J.mask = a->context_only ? nullptr : a->mask;
