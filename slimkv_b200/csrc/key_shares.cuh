@@ -33,25 +33,17 @@ __device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t u, uint32_
     return c;
 }
 
-// Units of all sequences, and of those before sequence `upto`, over the block
-// (`scan`: two words per warp).
-template <int kThreads, class Plan>
-__device__ __forceinline__ void sum_units(const Plan& P, int upto, uint32_t& total, uint32_t& before, uint32_t* scan) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t all = 0, head = 0;
-    for (int b = tid; b < P.batch; b += kThreads) {
-        const uint32_t u = units_of(P, b);
-        all += u;
-        if (b < upto) head += u;
-    }
-    all = __reduce_add_sync(0xffffffffu, all);
-    head = __reduce_add_sync(0xffffffffu, head);
-    if (lane == 0) { scan[2 * warp] = all; scan[2 * warp + 1] = head; }
-    __syncthreads();
+// Units of all sequences, and of those before sequence `upto`, by one warp.
+template <class Plan>
+__device__ __forceinline__ void sum_units(const Plan& P, int upto, uint32_t& total, uint32_t& before) {
     total = before = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) { total += scan[2 * w]; before += scan[2 * w + 1]; }
-    __syncthreads();
+    for (int b = threadIdx.x & 31; b < P.batch; b += 32) {
+        const uint32_t u = units_of(P, b);
+        total += u;
+        if (b < upto) before += u;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    before = __reduce_add_sync(0xffffffffu, before);
 }
 
 // Where a CTA's share begins, in shared memory.

@@ -731,74 +731,112 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     }
 }
 
+constexpr int kCombineThreads = 256;
+
 // Merges the pieces of a segment's rows, and writes the rows that see nothing:
-// 32 rows (a lane each) and 64 dims (16 to a warp) of a (sequence, KV head,
-// row group) per block.
+// 32 rows (a lane each) and 64 dims (8 to a warp) of a (sequence, KV head, row
+// group) per block, four pieces' loads under way at a time.  Segments have two
+// or three pieces when there are many, tens when there are few: fewer dims to a
+// warp cost the first case instructions (4: 34 us for 128 segments of 256
+// rows), more the second latency (16: 23 us for 8 segments of 128 rows in 19
+// pieces).
 template <int NQ, bool kHalf>
-__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Job J) {
-    __shared__ uint32_t scan[8];
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Job J) {
+    __shared__ int range[3];                // first and last CTA of the segment's pieces, slot of the first
+    __shared__ uint2 tile[32][17];          // the merged rows, 4 dims to an entry (17: no bank twice)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int at = blockIdx.x;
     const int group = at % J.row_groups;
     at /= J.row_groups;
     const int g = at % J.kv_heads, b = at / J.kv_heads;
     const Plan<NQ> plan(J);
-    uint32_t total, before;
-    sum_units<128>(plan, b, total, before, scan);
     const Seq s = plan.sequence(b);
-    int c0 = 0, c1 = 0, slot0 = 0;
     const bool some = group < s.groups && s.tiles > 0;
-    if (some) {
-        const uint32_t u0 = before + uint32_t(g * s.groups + group) * uint32_t(s.tiles);
-        const uint32_t ctas = share_count(total, J.ctas);
-        c0 = int(share_of(total, u0, ctas));
-        c1 = int(share_of(total, u0 + s.tiles - 1, ctas));
-        slot0 = 2 * c0 + (share_begin(total, c0, ctas) != u0 ? 1 : 0);
+    if (some && warp == 0) {
+        uint32_t total, before;
+        sum_units(plan, b, total, before);
+        if (lane == 0) {
+            const uint32_t u0 = before + uint32_t(g * s.groups + group) * uint32_t(s.tiles);
+            const uint32_t ctas = share_count(total, J.ctas), c0 = share_of(total, u0, ctas);
+            range[0] = int(c0);
+            range[1] = int(share_of(total, u0 + s.tiles - 1, ctas));
+            range[2] = 2 * int(c0) + (share_begin(total, c0, ctas) != u0 ? 1 : 0);
+        }
     }
-    if (threadIdx.x == 0 && g == 0 && group == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
+    if (threadIdx.x == 32 && g == 0 && group == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
         const int len = __ldg(J.lengths + b), nodes = J.nodes_len ? __ldg(J.nodes_len + b) : J.nodes;
         if (len != s.len || nodes != s.nodes || (!J.context_only && s.end != s.len + s.nodes)) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
     }
-    const int rows = NQ * J.tile_rows, r = blockIdx.y * 32 + lane, d0 = blockIdx.z * 64 + 16 * warp;
-    const int t = group * NQ * J.tpt + r / J.group, h = g * J.group + r % J.group;
-    const bool live = some && t < s.nodes;
-    grid_dependency_wait();
-    if (r >= rows || t >= J.nodes || d0 >= J.dim_v || (live && c0 == c1)) return;
+    __syncthreads();
+    const int c0 = some ? range[0] : 0, c1 = some ? range[1] : 0, slot0 = some ? range[2] : 0;
+    // A segment in one piece whose rows are all live is written already.
+    if (some && c0 == c1 && (group + 1) * NQ * J.tpt <= s.nodes) return;
+    const int rows = NQ * J.tile_rows, r0 = blockIdx.y * 32, r = r0 + lane, d0 = blockIdx.z * 64 + 8 * warp;
+    // Whether row r (of node t) is this kernel's to write, and whether it has pieces.
+    const bool split = c0 != c1;
+    auto node_of = [&](int row) { return group * NQ * J.tpt + row / J.group; };
+    auto mine = [&](int row) {
+        const int t = node_of(row);
+        return row < rows && t < J.nodes && (split || !some || t >= s.nodes);
+    };
+    const bool live = some && node_of(r) < s.nodes && mine(r) && d0 < J.dim_v;
     auto slot_of = [&](int c) { return int64_t(c == c0 ? slot0 : 2 * c); };
+    grid_dependency_wait();
     float m = -INFINITY, sum = 0.f, shift = 0.f;
-    float4 acc[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     if (live) {
-#pragma unroll 4
-        for (int c = c0; c <= c1; ++c) m = fmaxf(m, J.part_lse[slot_of(c) * rows + r]);
+        constexpr int kAhead = 4;
+        for (int c = c0; c <= c1; c += kAhead) {
+            float l[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) l[k] = c + k <= c1 ? J.part_lse[slot_of(c + k) * rows + r] : -INFINITY;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) m = fmaxf(m, l[k]);
+        }
         shift = m == -INFINITY ? 0.f : m;
-#pragma unroll 2
-        for (int c = c0; c <= c1; ++c) {
-            const int64_t slot = slot_of(c);
-            const float w = exp2f(J.part_lse[slot * rows + r] - shift);
-            const float4* part = reinterpret_cast<const float4*>(J.part_o) + (slot * (J.dim_v / 4) + d0 / 4) * rows + r;
-            float4 x[4];
+        const float4* part = reinterpret_cast<const float4*>(J.part_o) + int64_t(d0 / 4) * rows + r;
+        const int64_t step = int64_t(J.dim_v / 4) * rows;
+        for (int c = c0; c <= c1; c += kAhead) {
+            float w[kAhead];
+            float4 x[kAhead][2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] = d0 + 4 * u < J.dim_v ? part[int64_t(u) * rows] : make_float4(0.f, 0.f, 0.f, 0.f);
-            sum += w;
-            if (w != 0.f)
+            for (int k = 0; k < kAhead; ++k) {
+                w[k] = -INFINITY;
+                if (c + k > c1) continue;
+                const int64_t slot = slot_of(c + k);
+                w[k] = J.part_lse[slot * rows + r];
+                x[k][0] = part[slot * step];
+                x[k][1] = part[slot * step + rows];
+            }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    acc[u].x = fmaf(w, x[u].x, acc[u].x); acc[u].y = fmaf(w, x[u].y, acc[u].y);
-                    acc[u].z = fmaf(w, x[u].z, acc[u].z); acc[u].w = fmaf(w, x[u].w, acc[u].w);
+            for (int k = 0; k < kAhead; ++k) {
+                const float f = sfu_exp2(w[k] - shift);
+                sum += f;
+                if (f == 0.f) continue;             // (an empty piece's rows are not read into the sum)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    acc[u].x = fmaf(f, x[k][u].x, acc[u].x); acc[u].y = fmaf(f, x[k][u].y, acc[u].y);
+                    acc[u].z = fmaf(f, x[k][u].z, acc[u].z); acc[u].w = fmaf(f, x[k][u].w, acc[u].w);
                 }
+            }
         }
     }
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    uint16_t* dst = static_cast<uint16_t*>(J.out) + b * J.o_sb + t * J.o_st + h * J.o_sh + d0;
 #pragma unroll
-    for (int u = 0; u < 4; u += 2)
-        if (d0 + 4 * u < J.dim_v)
-            *reinterpret_cast<uint4*>(dst + 4 * u) =
-                make_uint4(pack2<kHalf>(acc[u].x * inv, acc[u].y * inv), pack2<kHalf>(acc[u].z * inv, acc[u].w * inv),
-                           pack2<kHalf>(acc[u + 1].x * inv, acc[u + 1].y * inv), pack2<kHalf>(acc[u + 1].z * inv, acc[u + 1].w * inv));
-    if (d0 == 0) J.lse[(int64_t(b) * J.nodes + t) * J.heads + h] = sum != 0.f ? (shift + log2f(sum)) * kLn2 : -INFINITY;
+    for (int u = 0; u < 2; ++u)
+        tile[lane][2 * warp + u] = make_uint2(pack2<kHalf>(acc[u].x * inv, acc[u].y * inv), pack2<kHalf>(acc[u].z * inv, acc[u].w * inv));
+    auto head_of = [&](int row) { return g * J.group + row % J.group; };
+    if (d0 == 0 && mine(r))
+        J.lse[(int64_t(b) * J.nodes + node_of(r)) * J.heads + head_of(r)] = sum != 0.f ? (shift + log2f(sum)) * kLn2 : -INFINITY;
+    __syncthreads();
+    // Out by rows: 16 lanes hold 64 dims, 128 bytes, of a row.
+    const int u = threadIdx.x & 15, d = blockIdx.z * 64 + 4 * u;
+#pragma unroll
+    for (int k = threadIdx.x >> 4; k < 32; k += kCombineThreads / 16)
+        if (mine(r0 + k) && d < J.dim_v) {
+            uint16_t* dst = static_cast<uint16_t*>(J.out) + b * J.o_sb + node_of(r0 + k) * J.o_st + head_of(r0 + k) * J.o_sh + d;
+            *reinterpret_cast<uint2*>(dst) = tile[k][u];
+        }
 }
 
 // ------------------------------------------------------------------- host --
@@ -846,7 +884,7 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
     kernel<<<J.ctas, 128 + kSoftmaxThreads<NQ>, kSmemBytes, stream>>>(qm, km, vm, J);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(J.batch * J.kv_heads * J.row_groups, (NQ * J.tile_rows + 31) / 32, (J.dim_v + 63) / 64);
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = stream;
     cudaLaunchAttribute dependent{};
     dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
