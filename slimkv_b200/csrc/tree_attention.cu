@@ -36,6 +36,7 @@
 // of row tile 0, 2 = TMEM owner and MMA issue of row tile 1, the
 // others from 4 on = softmax.  Every wait is bounded.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_view.cuh"
 #include "host_utils.h"
@@ -49,7 +50,7 @@ constexpr int kKeys = 64;                        // keys of a tile
 constexpr uint32_t kQChunk = 128 * 128;          // [128 rows x 64] 16-bit elements
 constexpr uint32_t kChunk = kKeys * 128;         // [64 keys x 64]
 constexpr uint32_t kTileArea = 224 * 1024;
-constexpr int kMaxRing = 10;
+constexpr int kMaxRing = 12;
 constexpr int kMaxChunks = 5;                    // dims <= 320
 constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a row's maximum grows by more than 2^8
 constexpr float kLog2e = 1.4426950408889634f;
@@ -70,7 +71,7 @@ struct Bars {
     uint32_t tmem_base;
     int abort;
     int bad_values[2];           // 1 + a piece whose node values hold infinities or NaN
-    float exchange[2][kRows];    // [row tile]: between a row's two threads
+    float exchange[kRows];       // between a row's two threads
     Share share;
 };
 constexpr uint32_t kSmemBytes = 1024 + kTileArea + uint32_t(sizeof(Bars));
@@ -80,8 +81,7 @@ struct Job {
     int batch, nodes, heads, kv_heads, group;
     int tpt, tile_rows;         // nodes of a row tile and its rows (tpt * group <= 128)
     int row_groups;             // groups of NQ row tiles
-    int kc, vc, dim_v;          // 64-column chunks of a K / V row
-    int kring, vring;           // ring slots: of a whole row, or (dims above 128) of one chunk
+    int dim_v;
     int context_only, paged, shared_cache;
     int box;                    // rows of one TMA box
     CacheView cache;
@@ -197,7 +197,7 @@ template <int NQ, int C>
 struct Columns {
     __device__ static constexpr uint32_t o(int q) { return uint32_t(q * 128); }
     __device__ static constexpr uint32_t s(int q, int buf) {
-        return (C == 0 ? 320u : 128u * NQ) + uint32_t((2 * q + buf) * kKeys);
+        return (C > 2 ? 64u * C : 128u * NQ) + uint32_t((2 * q + buf) * kKeys);
     }
 };
 
@@ -232,12 +232,6 @@ __device__ __forceinline__ int box_of(const Job& J, const W& w, int tile, int la
     }
     return int(page);
 }
-// Slot and lap of a tile's first ring entry, `per` entries to a tile.
-__device__ __forceinline__ void ring_at(int tile, int per, int ring, int& slot, uint32_t& lap) {
-    const int n = tile * per;
-    lap = uint32_t(n / ring);
-    slot = n - int(lap) * ring;
-}
 // Whether a V tile holds rows that nobody sees, or the nodes' own.
 __device__ __forceinline__ bool needs_fix(const Seq& s, int tile) { return s.has_nodes(tile) || s.hi(tile) < kKeys; }
 
@@ -269,18 +263,19 @@ __device__ __forceinline__ bool fix_values(uint8_t* chunk, int r, int u0, bool s
     return bad;
 }
 
-// Ring geometry.  Rows of up to 128 dims: a slot is a whole row of C chunks
-// (shorter rows are filled up with zeros), all of it constants; wider rows: a
-// slot is one chunk of the job's (a tile's five take too much for two tiles).
+// Ring geometry for rows of C 64-column chunks (shorter ones are filled up with
+// zeros).  A V slot is a whole row, a K slot too up to 128 dims, and one chunk
+// above, where whole rows would leave no second tile.  All of it constant: with
+// loops of run-time length the MMA operands are no uniform registers, and the
+// wide rows' MMAs took 100 cycles each.
 template <int NQ, int C>
 struct Rings {
-    static constexpr int kGroup = C == 0 ? 1 : C;
-    static constexpr int kFree = C == 0 ? 0 : int((kTileArea - uint32_t(NQ * C) * kQChunk) / kChunk);
-    static constexpr int kSlots = kFree / 2 / kGroup < kMaxRing ? kFree / 2 / kGroup : kMaxRing;
-    __host__ __device__ static int kc(const Job& J) { return C == 0 ? J.kc : C; }
-    __host__ __device__ static int vc(const Job& J) { return C == 0 ? J.vc : C; }
-    __host__ __device__ static int kring(const Job& J) { return C == 0 ? J.kring : kSlots; }
-    __host__ __device__ static int vring(const Job& J) { return C == 0 ? J.vring : kSlots; }
+    static constexpr int kFree = int((kTileArea - uint32_t(NQ * C) * kQChunk) / kChunk);
+    static constexpr int kGroup = C > 2 ? 1 : C;             // chunks of a K slot
+    static constexpr int kPer = C / kGroup;                  // K slots of a tile
+    static constexpr int kV = kFree / 2 / C < 2 ? 2 : kFree / 2 / C < kMaxRing ? kFree / 2 / C : kMaxRing;
+    static constexpr int kK = (kFree - kV * C) / kGroup < kMaxRing ? (kFree - kV * C) / kGroup : kMaxRing;
+    static_assert(kK >= kPer + 1 && kV >= 2, "two tiles under way");
 };
 
 // ----------------------------------------------------------------- kernel --
@@ -292,35 +287,31 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     constexpr int kHalves = kHalvesOf<NQ>, kWarps = 4 * kHalves, kCols = kKeys / kHalves;
     using Col = Columns<NQ, C>;
     using R = Rings<NQ, C>;
-    const int kc = R::kc(J), vc = R::vc(J), kring = R::kring(J), vring = R::vring(J);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Bars* bs = reinterpret_cast<Bars*>(smem + kTileArea);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // Layout: Q (NQ x kc chunks) | K ring | V ring.
-    const uint32_t off_k = uint32_t(NQ * kc) * kQChunk;
-    const uint32_t off_v = off_k + uint32_t(kring * R::kGroup) * kChunk;
+    // Layout: Q (NQ x C chunks) | K ring | V ring.
+    const uint32_t off_k = uint32_t(NQ * C) * kQChunk;
+    const uint32_t off_v = off_k + uint32_t(R::kK * R::kGroup) * kChunk;
 
-    if (tid == 0) {
-        for (int s = 0; s < kMaxRing; ++s) {
-            mbar_init(&bs->kfull[s], 1); mbar_init(&bs->kempty[s], NQ);
-            mbar_init(&bs->vfull[s], 1); mbar_init(&bs->vempty[s], NQ); mbar_init(&bs->vfixed[s], kWarps);
-        }
+    if (tid < kMaxRing) {
+        mbar_init(&bs->kfull[tid], 1); mbar_init(&bs->kempty[tid], NQ);
+        mbar_init(&bs->vfull[tid], 1); mbar_init(&bs->vempty[tid], NQ); mbar_init(&bs->vfixed[tid], kWarps);
+    } else if (tid < kMaxRing + 4) {
+        const int q = (tid - kMaxRing) & 1, s = (tid - kMaxRing) >> 1;
+        mbar_init(&bs->sfull[q][s], 1);
+        mbar_init(&bs->pfull[q][s], kWarps);
+        mbar_init(&bs->odone[q][s], 1);
+        if (s == 0) mbar_init(&bs->oempty[q], kWarps);
+    } else if (tid == kMaxRing + 4) {
         mbar_init(&bs->qfull, 1);
         mbar_init(&bs->qempty, NQ);
-        for (int q = 0; q < 2; ++q) {
-            mbar_init(&bs->oempty[q], kWarps);
-            for (int s = 0; s < 2; ++s) {
-                mbar_init(&bs->sfull[q][s], 1);
-                mbar_init(&bs->pfull[q][s], kWarps);
-                mbar_init(&bs->odone[q][s], 1);
-            }
-        }
         mbar_init(&bs->final_mma, NQ);
         bs->abort = 0;
         bs->bad_values[0] = bs->bad_values[1] = 0;
-        fence_barrier_init();
     }
+    if (tid < 32) fence_barrier_init();
     if (tid == 32) {
         tma_prefetch_desc(&qmap);
         tma_prefetch_desc(&kmap);
@@ -342,7 +333,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     if (any && (warp == 0 || warp == 3)) {
         // ---- loads: warp 0 each piece's Q and the K chunks, warp 3 the V chunks ----
         const bool keys = warp == 0;
-        const int chunks = keys ? kc : vc, per = R::kGroup, ring = keys ? kring : vring;
+        const int per = keys ? R::kGroup : C, ring = keys ? R::kK : R::kV;
         uint64_t* full = keys ? bs->kfull : bs->vfull;
         uint64_t* empty = keys ? bs->kempty : bs->vempty;
         const CUtensorMap* map = keys ? &kmap : &vmap;
@@ -357,10 +348,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             if (keys) {
                 if (w.piece > 0 && !(ok = warp_wait(&bs->qempty, (w.piece - 1) & 1, bs, J))) break;
                 if (lane == 0) {
-                    mbar_expect_tx(&bs->qfull, uint32_t(NQ * kc) * uint32_t(J.tile_rows) * 128u);
+                    mbar_expect_tx(&bs->qfull, uint32_t(NQ * C) * uint32_t(J.tile_rows) * 128u);
                     for (int q = 0; q < NQ; ++q)
-                        for (int c = 0; c < kc; ++c)
-                            tma_load_4d(smem + (q * kc + c) * kQChunk, &qmap, &bs->qfull, c * 64, w.g * J.group,
+                        for (int c = 0; c < C; ++c)
+                            tma_load_4d(smem + (q * C + c) * kQChunk, &qmap, &bs->qfull, c * 64, w.g * J.group,
                                         (w.group * NQ + q) * J.tpt, w.b);
                 }
                 __syncwarp();
@@ -368,7 +359,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             for (int tile = w.t0; tile < w.t1 && ok; ++tile) {
                 int row;
                 const int page = box_of(J, w, tile, lane, row);
-                for (int c = 0; c < chunks; c += per) {
+                for (int c = 0; c < C; c += per) {
                     if (lap && !(ok = warp_wait(&empty[slot], (lap - 1) & 1, bs, J))) break;
                     if (lane == 0) mbar_expect_tx(&full[slot], uint32_t(per) * kChunk);
                     __syncwarp();
@@ -386,10 +377,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         // 128 keys, two: 4,600).  The warp stays converged, its branches go by votes, and one
         // elected thread has the instructions alone, so that operands are uniform registers. ----
         const int q = NQ == 2 ? warp - 1 : 0;
-        const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0), idesc_o = idesc<kHalf>(128, 64 * R::kGroup, 0, 1);
+        const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0), idesc_o = idesc<kHalf>(128, 64 * (C < 4 ? C : 4), 0, 1), idesc_o1 = idesc<kHalf>(128, 64, 0, 1);
         // Matrix descriptors (K-major Q and K; MN-major V): the low word moves with the address.
         constexpr uint64_t kQStep = kQChunk >> 4, kStep = kChunk >> 4;
-        const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024) + uint32_t(q * kc) * kQStep;
+        const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024) + uint32_t(q * C) * kQStep;
         const uint64_t k_desc = umma_desc_sw128(sbase + off_k, 16, 1024), v_desc = umma_desc_sw128(sbase + off_v, kChunk, 1024);
         int kslot = 0, vslot = 0;
         uint32_t klap = 0, vlap = 0, s_buf = 0, q_lap = 0, fixes = 0;    // fixes: each slot's parity of vfixed
@@ -405,16 +396,16 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 q_lap ^= 1;
             }
 #pragma unroll
-            for (int c = 0, slot = kslot, lap = klap; c < kc; c += R::kGroup) {
+            for (int c = 0, slot = kslot, lap = klap; c < C; c += R::kGroup) {
                 ok = ok && wait_bar(&bs->kfull[slot], lap, bs, J);
-                if (++slot == kring) { slot = 0; lap ^= 1; }
+                if (++slot == R::kK) { slot = 0; lap ^= 1; }
             }
             const bool last = all_lanes(s_tile == ws.t1 - 1);
             if (!all_lanes(ok)) return;
             if (elect_one()) {
                 const uint32_t d = Col::s(q, s_buf);
 #pragma unroll
-                for (int c = 0, slot = kslot; c < kc; c += R::kGroup) {
+                for (int c = 0, slot = kslot; c < C; c += R::kGroup) {
 #pragma unroll
                     for (int k = 0; k < R::kGroup; ++k) {
                         const uint64_t a = q_desc + uint32_t(c + k) * kQStep, b = k_desc + uint32_t(slot * R::kGroup + k) * kStep;
@@ -422,14 +413,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                         for (int kk = 0; kk < 4; ++kk) umma_bf16(d, a + 2 * kk, b + 2 * kk, idesc_s, (c | k | kk) != 0);
                     }
                     umma_commit(&bs->kempty[slot]);
-                    if (++slot == kring) slot = 0;
+                    if (++slot == R::kK) slot = 0;
                 }
                 umma_commit(&bs->sfull[q][s_buf]);
                 if (last) umma_commit(&bs->qempty);
             }
             __syncwarp();
-            kslot += kc / R::kGroup;
-            if (kslot >= kring) { kslot -= kring; klap ^= 1; }
+            kslot += R::kPer;
+            if (kslot >= R::kK) { kslot -= R::kK; klap ^= 1; }
             s_buf ^= 1;
             ++s_tile;
             if (last) {
@@ -449,11 +440,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     ok = ok && wait_bar(&bs->oempty[q], o_lap, bs, J);
                     o_lap ^= 1;
                 }
-#pragma unroll
-                for (int c = 0, slot = vslot, lap = vlap; c < vc; c += R::kGroup) {
-                    ok = ok && wait_bar(&bs->vfull[slot], lap, bs, J);
-                    if (++slot == vring) { slot = 0; lap ^= 1; }
-                }
+                ok = ok && wait_bar(&bs->vfull[vslot], vlap, bs, J);
                 // Row tile 0 looks after the V rows (fix_values), row tile 1 waits for it.
                 if (NQ == 2 && q == 1 && all_lanes(needs_fix(wp.s, tile))) {
                     ok = ok && wait_bar(&bs->vfixed[vslot], fixes >> vslot & 1, bs, J);
@@ -464,21 +451,19 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 tc_fence_after();
                 if (elect_one()) {
                     const uint32_t a = Col::s(q, p_buf);
+                    const uint64_t b = v_desc + uint32_t(vslot * C) * kStep;
+                    // The row's chunks lie side by side: up to four are one MMA of N = 256.
 #pragma unroll
-                    for (int c = 0, slot = vslot; c < vc; c += R::kGroup) {
-                        const uint32_t d = Col::o(q) + 64u * c;
-                        const uint64_t b = v_desc + uint32_t(slot * R::kGroup) * kStep;
-#pragma unroll
-                        for (int ks = 0; ks < kKeys / 16; ++ks)
-                            umma_ts(d, a + 8u * ks, b + 128 * ks, idesc_o, (!first || ks > 0) ? 1u : 0u);
-                        umma_commit(&bs->vempty[slot]);
-                        if (++slot == vring) slot = 0;
+                    for (int ks = 0; ks < kKeys / 16; ++ks) {
+                        umma_ts(Col::o(q), a + 8u * ks, b + 128 * ks, idesc_o, (!first || ks > 0) ? 1u : 0u);
+                        if constexpr (C == 5)
+                            umma_ts(Col::o(q) + 256u, a + 8u * ks, b + 4 * kStep + 128 * ks, idesc_o1, (!first || ks > 0) ? 1u : 0u);
                     }
+                    umma_commit(&bs->vempty[vslot]);
                     umma_commit(&bs->odone[q][p_buf]);
                 }
                 __syncwarp();
-                vslot += vc / R::kGroup;
-                if (vslot >= vring) { vslot -= vring; vlap ^= 1; }
+                if (++vslot == R::kV) { vslot = 0; vlap ^= 1; }
                 if (p_buf) p_lap ^= 1;
                 p_buf ^= 1;
                 first = false;
@@ -503,7 +488,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         // All threads of a row get op over their x.
         auto over_row = [&](float x, auto op) {
             if constexpr (kHalves == 1) return x;
-            float* at = &bs->exchange[qt][r];
+            float* at = &bs->exchange[r];
             if (half) *at = x;
             named_bar(1 + qt, 256);
             if (!half) *at = x = op(x, *at);
@@ -574,7 +559,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     }
                     if (ok && tile > w.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
-                        for (int c = half; c < 4 * vc; c += kHalves) {
+                        for (int c = half; c < 4 * C; c += kHalves) {
                             float o[16];
                             tmem_ld16(o_base + 16u * c, o);
                             tmem_wait_ld();
@@ -607,25 +592,18 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     tmem_wait_st();
                 }
                 if (fix && ok) {
-                    // P.V(i - 1) is done, so this tile's chunks are the next that land in their slots.
-                    int slot = 0;
-                    uint32_t lap = 0;
-                    ring_at(i, vc / R::kGroup, vring, slot, lap);
-                    const int first = slot;
+                    // P.V(i - 1) is done, so this tile is the next that lands in its slot.
+                    const int slot = i % R::kV;
                     bool bad = false;
-                    for (int c = 0; c < vc && ok; c += R::kGroup) {
-                        ok = warp_wait(&bs->vfull[slot], lap & 1, bs, J);
-                        for (int k = 0; k < R::kGroup && ok; ++k)
-                            bad |= fix_values<kHalf, 2 * kHalves>(smem + off_v + uint32_t(slot * R::kGroup + k) * kChunk, r & 63,
-                                                                  2 * half + (r >> 6), (r & 63) < w.s.hi(tile),
-                                                                  tile * kKeys + (r & 63) >= w.s.len);
-                        if (++slot == vring) { slot = 0; ++lap; }
-                    }
+                    ok = warp_wait(&bs->vfull[slot], (i / R::kV) & 1, bs, J);
+                    for (int c = 0; c < C && ok; ++c)
+                        bad |= fix_values<kHalf, 2 * kHalves>(smem + off_v + uint32_t(slot * C + c) * kChunk, r & 63, 2 * half + (r >> 6),
+                                                              (r & 63) < w.s.hi(tile), tile * kKeys + (r & 63) >= w.s.len);
                     if (bad) *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) = w.piece + 1;
                     fence_async_shared();
                     if constexpr (NQ == 2) {
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&bs->vfixed[first]);
+                        if (lane == 0) mbar_arrive(&bs->vfixed[slot]);
                     }
                 }
                 tc_fence_before();
@@ -645,7 +623,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             const int rows = NQ * J.tile_rows, slot = 2 * blockIdx.x + (w.piece > 0), row = qt * J.tile_rows + r;
             float4* part = reinterpret_cast<float4*>(J.part_o) + int64_t(slot) * (J.dim_v / 4) * rows + row;
 #pragma unroll 1
-            for (int c = half; c < 4 * vc; c += kHalves) {
+            for (int c = half; c < 4 * C; c += kHalves) {
                 float o[16];
                 if (warp_live) {
                     tmem_ld16(o_base + 16u * c, o);
@@ -712,11 +690,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         // that ran out the copies that were not.
         if (tid == 64) mbar_wait(&bs->final_mma, 0, 2000000000ull);
         if (bs->abort && tid == 0) {
-            for (int s = 0; s < kring; ++s) {
+            for (int s = 0; s < R::kK; ++s) {
                 mbar_wait(&bs->kfull[s], 0, 100000000ull);
                 mbar_wait(&bs->kfull[s], 1, 100000000ull);
             }
-            for (int s = 0; s < vring; ++s) {
+            for (int s = 0; s < R::kV; ++s) {
                 mbar_wait(&bs->vfull[s], 0, 100000000ull);
                 mbar_wait(&bs->vfull[s], 1, 100000000ull);
             }
@@ -955,13 +933,7 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.heads = a->heads;
     J.kv_heads = a->kv_heads;
     J.row_groups = (a->nodes + nq * J.tpt - 1) / (nq * J.tpt);
-    J.kc = (a->dim_qk + 63) / 64;
-    J.vc = (a->dim_v + 63) / 64;
     J.dim_v = a->dim_v;
-    const bool wide = J.kc > 2 || J.vc > 2;
-    const int chunks = int((kTileArea - uint32_t(J.kc) * kQChunk) / kChunk);      // wide rows: one row tile
-    J.vring = std::min(kMaxRing, chunks / 2);
-    J.kring = std::min(kMaxRing, chunks - J.vring);
     J.context_only = a->context_only;
     J.paged = paged;
     J.cache = cache_view(cache);
@@ -982,10 +954,18 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool half = a->type == SLIMKV_FP16;
-    const int width = wide ? 0 : std::max(J.kc, J.vc);
-    auto pick = [&](auto one, auto two, auto any, auto one2, auto two2) {
-        return (nq == 2 ? (width == 1 ? one2 : two2) : width == 1 ? one : width == 2 ? two : any)(qm, km, vm, J, st);
+    auto run = [&](auto rows, auto chunks) {
+        return half ? launch<decltype(rows)::value, decltype(chunks)::value, true>(qm, km, vm, J, st)
+                    : launch<decltype(rows)::value, decltype(chunks)::value, false>(qm, km, vm, J, st);
     };
-    return half ? pick(launch<1, 1, true>, launch<1, 2, true>, launch<1, 0, true>, launch<2, 1, true>, launch<2, 2, true>)
-                : pick(launch<1, 1, false>, launch<1, 2, false>, launch<1, 0, false>, launch<2, 1, false>, launch<2, 2, false>);
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    switch ((std::max(a->dim_qk, a->dim_v) + 63) / 64) {
+        case 1: return nq == 2 ? run(two, one) : run(one, one);
+        case 2: return nq == 2 ? run(two, two) : run(one, two);
+        case 3: return run(one, integral_constant<int, 3>());
+        case 4: return run(one, integral_constant<int, 4>());
+        default: return run(one, integral_constant<int, 5>());
+    }
 }
