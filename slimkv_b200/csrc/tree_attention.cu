@@ -25,15 +25,15 @@
 // Bound: with few rows per KV head HBM (each K / V row read once); with 128
 // rows or more the tensor cores and the exponentials.
 //
-// Why 64 keys: S and P of a tile fit 64 tensor-memory columns, so two tiles are
-// in flight for each row tile next to O (320 + 2 x 64, or 2 x (128 + 2 x 64)
-// columns): the S of tile n + 1 is there when the softmax of tile n ends, and
-// the softmax never waits for a product.  (With 128-key tiles and one S per row
+// Why 64 keys: S and P of a tile fit 64 tensor-memory columns, so two to four
+// tiles are under way for each row tile next to O (320 + 3 x 64, or 2 x (128 +
+// 2 x 64) columns): the S of tile n + 1 is there when the softmax of tile n
+// ends, and the softmax never waits for a product.  (With 128-key tiles and one S per row
 // tile, softmax and products took turns: 4,870 cycles for two row tiles and 128
 // keys, 2,700 of them the softmax.)
 //
-// One CTA per SM, warps: 0 = Q and K loads (TMA), 3 = V loads, 1 = MMA issue
-// of row tile 0, 2 = TMEM owner and MMA issue of row tile 1, the
+// One CTA per SM, warps: 0 = Q and K loads (TMA), 3 = V loads, 1 and 2 = MMA
+// issue (2 owns the TMEM), the
 // others from 4 on = softmax.  Every wait is bounded.
 #include <algorithm>
 #include <type_traits>
@@ -66,8 +66,8 @@ constexpr int kSoftmaxThreads = 128 * NQ * kHalvesOf<NQ>;
 struct Bars {
     uint64_t kfull[kMaxRing], kempty[kMaxRing], vfull[kMaxRing], vempty[kMaxRing], vfixed[kMaxRing];
     uint64_t qfull, qempty;
-    // [row tile][tile parity]
-    uint64_t sfull[2][2], pfull[2][2], odone[2][2], oempty[2], final_mma;
+    // [row tile][S/P buffer]
+    uint64_t sfull[2][4], pfull[2][4], odone[2][4], oempty[2], final_mma;
     uint32_t tmem_base;
     int abort;
     int bad_values[2];           // 1 + a piece whose node values hold infinities or NaN
@@ -190,15 +190,15 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Bars* 
     return __all_sync(0xffffffffu, wait_bar(bar, parity, bs, J));
 }
 
-// Tensor memory columns: O of each row tile, then two S tiles of each; a tile's
-// P goes over its S, which is in registers by then (and the next S there is
-// issued behind the P.V that reads that P).
+// Tensor memory columns: O of each row tile, then its S buffers, as many as
+// fit; a tile's P goes over its S, which is in registers by then.
 template <int NQ, int C>
 struct Columns {
-    __device__ static constexpr uint32_t o(int q) { return uint32_t(q * 128); }
-    __device__ static constexpr uint32_t s(int q, int buf) {
-        return (C > 2 ? 64u * C : 128u * NQ) + uint32_t((2 * q + buf) * kKeys);
-    }
+    static constexpr int kO = NQ == 1 ? 64 * C : 128;
+    static constexpr int kBufs = NQ == 2 ? 2 : (512 - kO) / kKeys < 4 ? (512 - kO) / kKeys : 4;
+    __device__ static constexpr uint32_t o(int q) { return uint32_t(q * kO); }
+    __device__ static constexpr uint32_t s(int q, int buf) { return uint32_t(NQ * kO + (kBufs * q + buf) * kKeys); }
+    static_assert(NQ * (kO + kBufs * kKeys) <= 512 && kBufs >= 2, "tensor memory");
 };
 
 __device__ __forceinline__ uint32_t mask_word(const int32_t* row, int words, int w) {
@@ -298,16 +298,16 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     if (tid < kMaxRing) {
         mbar_init(&bs->kfull[tid], 1); mbar_init(&bs->kempty[tid], NQ);
         mbar_init(&bs->vfull[tid], 1); mbar_init(&bs->vempty[tid], NQ); mbar_init(&bs->vfixed[tid], kWarps);
-    } else if (tid < kMaxRing + 4) {
+    } else if (tid < kMaxRing + 8) {
         const int q = (tid - kMaxRing) & 1, s = (tid - kMaxRing) >> 1;
         mbar_init(&bs->sfull[q][s], 1);
         mbar_init(&bs->pfull[q][s], kWarps);
         mbar_init(&bs->odone[q][s], 1);
         if (s == 0) mbar_init(&bs->oempty[q], kWarps);
-    } else if (tid == kMaxRing + 4) {
+    } else if (tid == kMaxRing + 8) {
         mbar_init(&bs->qfull, 1);
         mbar_init(&bs->qempty, NQ);
-        mbar_init(&bs->final_mma, NQ);
+        mbar_init(&bs->final_mma, 2);
         bs->abort = 0;
         bs->bad_values[0] = bs->bad_values[1] = 0;
     }
@@ -370,42 +370,54 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 }
             }
         }
-    } else if (any && warp <= NQ) {
-        // ---- MMA issue, a warp for each row tile: S two tiles ahead of P.V.  The tensor
-        // core queues only a few MMAs, so what the warp does between them is time lost,
-        // unless another warp's MMAs fill it (one warp for both row tiles: 8,100 cycles for
-        // 128 keys, two: 4,600).  The warp stays converged, its branches go by votes, and one
-        // elected thread has the instructions alone, so that operands are uniform registers. ----
+    } else if (any && warp <= 2) {
+        // ---- MMA issue by two warps: with one row tile, warp 1 the S and warp 2 the P.V;
+        // with two, warp 1 + q both products of row tile q, S two tiles ahead.  The tensor
+        // core queues only a few MMAs, so what a warp does between them is time lost unless
+        // another warp's MMAs fill it (two row tiles, 128 keys: 8,100 cycles with one warp,
+        // 4,600 with two; 320 dims, 64 keys: 3,450 and XXXX).  A warp stays converged, its
+        // branches go by votes, and one elected thread has the instructions alone, so that
+        // operands are uniform registers. ----
+        constexpr int kBufs = Col::kBufs;
         const int q = NQ == 2 ? warp - 1 : 0;
-        const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0), idesc_o = idesc<kHalf>(128, 64 * (C < 4 ? C : 4), 0, 1), idesc_o1 = idesc<kHalf>(128, 64, 0, 1);
+        const uint32_t idesc_s = idesc<kHalf>(128, kKeys, 0, 0);
+        const uint32_t idesc_o = idesc<kHalf>(128, 64 * (C < 4 ? C : 4), 0, 1), idesc_o1 = idesc<kHalf>(128, 64, 0, 1);
         // Matrix descriptors (K-major Q and K; MN-major V): the low word moves with the address.
         constexpr uint64_t kQStep = kQChunk >> 4, kStep = kChunk >> 4;
         const uint64_t q_desc = umma_desc_sw128(sbase, 16, 1024) + uint32_t(q * C) * kQStep;
         const uint64_t k_desc = umma_desc_sw128(sbase + off_k, 16, 1024), v_desc = umma_desc_sw128(sbase + off_v, kChunk, 1024);
-        int kslot = 0, vslot = 0;
-        uint32_t klap = 0, vlap = 0, s_buf = 0, q_lap = 0, fixes = 0;    // fixes: each slot's parity of vfixed
         bool ok = true;                          // of this lane; votes at the branches
-        Walk<Plan<NQ>> ws, wp;
-        ws.start(plan, &bs->share);
-        wp = ws;
-        bool s_more = all_lanes(ws.next(plan));
-        int s_tile = ws.t0;
+        // S of the share's tiles in order.
+        struct {
+            int slot, tile;
+            uint32_t lap, buf, round, q_lap;     // round: of the S buffers
+            bool more;
+        } f{};
+        Walk<Plan<NQ>> ws;
+        auto begin_s = [&] {
+            ws.start(plan, &bs->share);
+            f.more = all_lanes(ws.next(plan));
+            f.tile = ws.t0;
+        };
         auto issue_s = [&] {
-            if (all_lanes(s_tile == ws.t0)) {
-                ok = ok && wait_bar(&bs->qfull, q_lap, bs, J);
-                q_lap ^= 1;
+            if (all_lanes(f.tile == ws.t0)) {
+                ok = ok && wait_bar(&bs->qfull, f.q_lap, bs, J);
+                f.q_lap ^= 1;
             }
+            // The buffer's last P has been read (two row tiles: this warp issued that P.V before).
+            if (NQ == 1 && f.round) ok = ok && wait_bar(&bs->odone[0][f.buf], (f.round - 1) & 1, bs, J);
 #pragma unroll
-            for (int c = 0, slot = kslot, lap = klap; c < C; c += R::kGroup) {
+            for (int c = 0, slot = f.slot, lap = f.lap; c < C; c += R::kGroup) {
                 ok = ok && wait_bar(&bs->kfull[slot], lap, bs, J);
                 if (++slot == R::kK) { slot = 0; lap ^= 1; }
             }
-            const bool last = all_lanes(s_tile == ws.t1 - 1);
+            const bool last = all_lanes(f.tile == ws.t1 - 1);
             if (!all_lanes(ok)) return;
+            tc_fence_after();
             if (elect_one()) {
-                const uint32_t d = Col::s(q, s_buf);
+                const uint32_t d = Col::s(q, f.buf);
 #pragma unroll
-                for (int c = 0, slot = kslot; c < C; c += R::kGroup) {
+                for (int c = 0, slot = f.slot; c < C; c += R::kGroup) {
 #pragma unroll
                     for (int k = 0; k < R::kGroup; ++k) {
                         const uint64_t a = q_desc + uint32_t(c + k) * kQStep, b = k_desc + uint32_t(slot * R::kGroup + k) * kStep;
@@ -415,62 +427,71 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     umma_commit(&bs->kempty[slot]);
                     if (++slot == R::kK) slot = 0;
                 }
-                umma_commit(&bs->sfull[q][s_buf]);
+                umma_commit(&bs->sfull[q][f.buf]);
                 if (last) umma_commit(&bs->qempty);
             }
             __syncwarp();
-            kslot += R::kPer;
-            if (kslot >= R::kK) { kslot -= R::kK; klap ^= 1; }
-            s_buf ^= 1;
-            ++s_tile;
+            f.slot += R::kPer;
+            if (f.slot >= R::kK) { f.slot -= R::kK; f.lap ^= 1; }
+            if (++f.buf == kBufs) { f.buf = 0; ++f.round; }
+            ++f.tile;
             if (last) {
-                s_more = all_lanes(ws.next(plan));
-                s_tile = ws.t0;
+                f.more = all_lanes(ws.next(plan));
+                f.tile = ws.t0;
             }
         };
-        issue_s();
-        if (s_more) issue_s();
-        uint32_t p_buf = 0, p_lap = 0, o_lap = 0;
-        bool again = false;                      // a piece came before
-        while (all_lanes(ok && wp.next(plan))) {
-            int tile = wp.t0;
-            bool first = true;
-            do {
-                if (first && again) {            // the previous piece has left its O
-                    ok = ok && wait_bar(&bs->oempty[q], o_lap, bs, J);
-                    o_lap ^= 1;
-                }
-                ok = ok && wait_bar(&bs->vfull[vslot], vlap, bs, J);
-                // Row tile 0 looks after the V rows (fix_values), row tile 1 waits for it.
-                if (NQ == 2 && q == 1 && all_lanes(needs_fix(wp.s, tile))) {
-                    ok = ok && wait_bar(&bs->vfixed[vslot], fixes >> vslot & 1, bs, J);
-                    fixes ^= 1u << vslot;
-                }
-                ok = ok && wait_bar(&bs->pfull[q][p_buf], p_lap, bs, J);
-                if (!all_lanes(ok)) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t a = Col::s(q, p_buf);
-                    const uint64_t b = v_desc + uint32_t(vslot * C) * kStep;
-                    // The row's chunks lie side by side: up to four are one MMA of N = 256.
-#pragma unroll
-                    for (int ks = 0; ks < kKeys / 16; ++ks) {
-                        umma_ts(Col::o(q), a + 8u * ks, b + 128 * ks, idesc_o, (!first || ks > 0) ? 1u : 0u);
-                        if constexpr (C == 5)
-                            umma_ts(Col::o(q) + 256u, a + 8u * ks, b + 4 * kStep + 128 * ks, idesc_o1, (!first || ks > 0) ? 1u : 0u);
+        if (NQ == 2 || warp == 1) begin_s();
+        if (NQ == 1 && warp == 1) {
+            while (all_lanes(ok && f.more)) issue_s();
+        } else {
+            if constexpr (NQ == 2) {
+                issue_s();
+                if (f.more) issue_s();
+            }
+            int slot = 0;
+            uint32_t lap = 0, buf = 0, round = 0, o_lap = 0, fixes = 0;     // fixes: each slot's parity of vfixed
+            bool again = false;                  // a piece came before
+            Walk<Plan<NQ>> wp;
+            wp.start(plan, &bs->share);
+            while (all_lanes(ok && wp.next(plan))) {
+                int tile = wp.t0;
+                bool first = true;
+                do {
+                    if (first && again) {        // the previous piece has left its O
+                        ok = ok && wait_bar(&bs->oempty[q], o_lap, bs, J);
+                        o_lap ^= 1;
                     }
-                    umma_commit(&bs->vempty[vslot]);
-                    umma_commit(&bs->odone[q][p_buf]);
-                }
-                __syncwarp();
-                if (++vslot == R::kV) { vslot = 0; vlap ^= 1; }
-                if (p_buf) p_lap ^= 1;
-                p_buf ^= 1;
-                first = false;
-                ++tile;
-                if (s_more) issue_s();
-            } while (all_lanes(ok && tile < wp.t1));
-            again = true;
+                    ok = ok && wait_bar(&bs->vfull[slot], lap, bs, J);
+                    // Row tile 0 looks after the V rows (fix_values), row tile 1 waits for it.
+                    if (NQ == 2 && q == 1 && all_lanes(needs_fix(wp.s, tile))) {
+                        ok = ok && wait_bar(&bs->vfixed[slot], fixes >> slot & 1, bs, J);
+                        fixes ^= 1u << slot;
+                    }
+                    ok = ok && wait_bar(&bs->pfull[q][buf], round & 1, bs, J);
+                    if (!all_lanes(ok)) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t a = Col::s(q, buf);
+                        const uint64_t b = v_desc + uint32_t(slot * C) * kStep;
+                        // The row's chunks lie side by side: up to four are one MMA of N = 256.
+#pragma unroll
+                        for (int ks = 0; ks < kKeys / 16; ++ks) {
+                            umma_ts(Col::o(q), a + 8u * ks, b + 128 * ks, idesc_o, (!first || ks > 0) ? 1u : 0u);
+                            if constexpr (C == 5)
+                                umma_ts(Col::o(q) + 256u, a + 8u * ks, b + 4 * kStep + 128 * ks, idesc_o1, (!first || ks > 0) ? 1u : 0u);
+                        }
+                        umma_commit(&bs->vempty[slot]);
+                        umma_commit(&bs->odone[q][buf]);
+                    }
+                    __syncwarp();
+                    if (++slot == R::kV) { slot = 0; lap ^= 1; }
+                    if (++buf == kBufs) { buf = 0; ++round; }
+                    first = false;
+                    ++tile;
+                    if (NQ == 2 && f.more) issue_s();
+                } while (all_lanes(ok && tile < wp.t1));
+                again = true;
+            }
         }
         if (elect_one()) umma_commit(&bs->final_mma);
         __syncwarp();
@@ -495,6 +516,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             named_bar(1 + qt, 256);
             return half ? *at : x;
         };
+        constexpr int kBufs = Col::kBufs;
         bool ok = true;
         int i = 0;                                              // tiles done
         Walk<Plan<NQ>> w;
@@ -516,9 +538,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                                                       : low_bits(w.s.hi(tile) - k);
                     }
                 }
-                ok = ok && warp_wait(&bs->sfull[qt][i & 1], (i >> 1) & 1, bs, J);
+                const int buf = i % kBufs;
+                ok = ok && warp_wait(&bs->sfull[qt][buf], (i / kBufs) & 1, bs, J);
                 tc_fence_after();
-                const uint32_t s_addr = lane_addr + Col::s(qt, i & 1);
+                const uint32_t s_addr = lane_addr + Col::s(qt, buf);
                 float v[kCols];
                 float mx = -INFINITY;
                 if (warp_live) {
@@ -546,7 +569,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 const bool grown = kHalves == 2 ? any_of_row_tile(1 + qt, more) : __any_sync(0xffffffffu, more);
                 const bool fix = qt == 0 && masked;
                 if (((grown && tile > w.t0) || fix) && i > 0) {
-                    ok = ok && warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J);
+                    ok = ok && warp_wait(&bs->odone[qt][(i - 1) % kBufs], ((i - 1) / kBufs) & 1, bs, J);
                     tc_fence_after();
                 }
                 if (grown) {
@@ -608,11 +631,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bs->pfull[qt][i & 1]);
+                if (lane == 0) mbar_arrive(&bs->pfull[qt][buf]);
             }
             // ---- the piece's rows: the sums of all threads of a row, then each its columns ----
             l_run = over_row(l_run, [](float a, float b) { return a + b; });
-            ok = ok && warp_wait(&bs->odone[qt][(i - 1) & 1], ((i - 1) >> 1) & 1, bs, J);
+            ok = ok && warp_wait(&bs->odone[qt][(i - 1) % kBufs], ((i - 1) / kBufs) & 1, bs, J);
             if (!ok) continue;
             tc_fence_after();
             const bool whole = w.whole();
