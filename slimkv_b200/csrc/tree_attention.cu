@@ -375,7 +375,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         // with two, warp 1 + q both products of row tile q, S two tiles ahead.  The tensor
         // core queues only a few MMAs, so what a warp does between them is time lost unless
         // another warp's MMAs fill it (two row tiles, 128 keys: 8,100 cycles with one warp,
-        // 4,600 with two; 320 dims, 64 keys: 3,450 and XXXX).  A warp stays converged, its
+        // 4,600 with two; 320 dims, 64 keys: 3,450 and 1,900).  A warp stays converged, its
         // branches go by votes, and one elected thread has the instructions alone, so that
         // operands are uniform registers. ----
         constexpr int kBufs = Col::kBufs;
@@ -568,7 +568,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 const bool more = live && mx > m_run + kLazyLog2;
                 const bool grown = kHalves == 2 ? any_of_row_tile(1 + qt, more) : __any_sync(0xffffffffu, more);
                 const bool fix = qt == 0 && masked;
-                if (((grown && tile > w.t0) || fix) && i > 0) {
+                // (A ring of more V slots than S buffers: the slot's last tile is over, S(i) came after it.)
+                if (((grown && tile > w.t0) || (fix && R::kV <= kBufs)) && i > 0) {
                     ok = ok && warp_wait(&bs->odone[qt][(i - 1) % kBufs], ((i - 1) / kBufs) & 1, bs, J);
                     tc_fence_after();
                 }
@@ -615,7 +616,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     tmem_wait_st();
                 }
                 if (fix && ok) {
-                    // P.V(i - 1) is done, so this tile is the next that lands in its slot.
+                    // The slot's tile before this one is over, so this is the next that lands there.
                     const int slot = i % R::kV;
                     bool bad = false;
                     ok = warp_wait(&bs->vfull[slot], (i / R::kV) & 1, bs, J);
@@ -734,13 +735,14 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
 
 constexpr int kCombineThreads = 256;
 
-// Merges the pieces of a segment's rows, and writes the rows that see nothing:
-// 32 rows (a lane each) and 64 dims (8 to a warp) of a (sequence, KV head, row
-// group) per block, four pieces' loads under way at a time.  Segments have two
-// or three pieces when there are many, tens when there are few: fewer dims to a
-// warp cost the first case instructions (4: 34 us for 128 segments of 256
-// rows), more the second latency (16: 23 us for 8 segments of 128 rows in 19
-// pieces).
+// Merges the pieces of a segment's rows, and writes the rows that see nothing.
+// A (sequence, KV head, row group) has gridDim.y blocks, which take its parts
+// of 32 rows (a lane each) and 64 dims (8 to a warp) by turns, four pieces'
+// loads under way at a time.  Segments have two or three pieces when there are
+// many, tens when there are few: fewer dims to a warp cost the first case
+// instructions (4: 34 us for 128 segments of 256 rows), more the second latency
+// (16: 23 us for 8 segments of 128 rows in 19 pieces); and many blocks to a
+// segment cost many short segments more than the merge.
 template <int NQ, bool kHalf>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Job J) {
     __shared__ int range[3];                // first and last CTA of the segment's pieces, slot of the first
@@ -764,80 +766,83 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
             range[2] = 2 * int(c0) + (share_begin(total, c0, ctas) != u0 ? 1 : 0);
         }
     }
-    if (threadIdx.x == 32 && g == 0 && group == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
+    if (threadIdx.x == 32 && g == 0 && group == 0 && blockIdx.y == 0) {
         const int len = __ldg(J.lengths + b), nodes = J.nodes_len ? __ldg(J.nodes_len + b) : J.nodes;
         if (len != s.len || nodes != s.nodes || (!J.context_only && s.end != s.len + s.nodes)) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
     }
     __syncthreads();
     const int c0 = some ? range[0] : 0, c1 = some ? range[1] : 0, slot0 = some ? range[2] : 0;
     // A segment in one piece whose rows are all live is written already.
-    if (some && c0 == c1 && (group + 1) * NQ * J.tpt <= s.nodes) return;
-    const int rows = NQ * J.tile_rows, r0 = blockIdx.y * 32, r = r0 + lane, d0 = blockIdx.z * 64 + 8 * warp;
-    // Whether row r (of node t) is this kernel's to write, and whether it has pieces.
+    if (some && c0 == c1 && min((group + 1) * NQ * J.tpt, J.nodes) <= s.nodes) return;
+    const int rows = NQ * J.tile_rows, first_node = group * NQ * J.tpt;
+    const int used = min(rows, (J.nodes - first_node) * J.group);       // the group's rows that are nodes
+    const int dim_parts = (J.dim_v + 63) / 64, parts = (used + 31) / 32 * dim_parts;
     const bool split = c0 != c1;
-    auto node_of = [&](int row) { return group * NQ * J.tpt + row / J.group; };
-    auto mine = [&](int row) {
-        const int t = node_of(row);
-        return row < rows && t < J.nodes && (split || !some || t >= s.nodes);
-    };
-    const bool live = some && node_of(r) < s.nodes && mine(r) && d0 < J.dim_v;
     auto slot_of = [&](int c) { return int64_t(c == c0 ? slot0 : 2 * c); };
+    auto node_of = [&](int row) { return first_node + row / J.group; };
+    auto head_of = [&](int row) { return g * J.group + row % J.group; };
+    // Whether a row is this kernel's to write.
+    auto mine = [&](int row) { return row < used && (split || !some || node_of(row) >= s.nodes); };
     grid_dependency_wait();
-    float m = -INFINITY, sum = 0.f, shift = 0.f;
-    float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-    if (live) {
-        constexpr int kAhead = 4;
-        for (int c = c0; c <= c1; c += kAhead) {
-            float l[kAhead];
+    for (int part = blockIdx.y; part < parts; part += gridDim.y) {
+        const int r0 = part / dim_parts * 32, r = r0 + lane, dim0 = part % dim_parts * 64, d0 = dim0 + 8 * warp;
+        const bool live = some && mine(r) && node_of(r) < s.nodes && d0 < J.dim_v;
+        float m = -INFINITY, sum = 0.f, shift = 0.f;
+        float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        if (live) {
+            constexpr int kAhead = 4;
+            for (int c = c0; c <= c1; c += kAhead) {
+                float l[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) l[k] = c + k <= c1 ? J.part_lse[slot_of(c + k) * rows + r] : -INFINITY;
+                for (int k = 0; k < kAhead; ++k) l[k] = c + k <= c1 ? J.part_lse[slot_of(c + k) * rows + r] : -INFINITY;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) m = fmaxf(m, l[k]);
-        }
-        shift = m == -INFINITY ? 0.f : m;
-        const float4* part = reinterpret_cast<const float4*>(J.part_o) + int64_t(d0 / 4) * rows + r;
-        const int64_t step = int64_t(J.dim_v / 4) * rows;
-        for (int c = c0; c <= c1; c += kAhead) {
-            float w[kAhead];
-            float4 x[kAhead][2];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                w[k] = -INFINITY;
-                if (c + k > c1) continue;
-                const int64_t slot = slot_of(c + k);
-                w[k] = J.part_lse[slot * rows + r];
-                x[k][0] = part[slot * step];
-                x[k][1] = part[slot * step + rows];
+                for (int k = 0; k < kAhead; ++k) m = fmaxf(m, l[k]);
             }
+            shift = m == -INFINITY ? 0.f : m;
+            const float4* part = reinterpret_cast<const float4*>(J.part_o) + int64_t(d0 / 4) * rows + r;
+            const int64_t step = int64_t(J.dim_v / 4) * rows;
+            for (int c = c0; c <= c1; c += kAhead) {
+                float w[kAhead];
+                float4 x[kAhead][2];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const float f = sfu_exp2(w[k] - shift);
-                sum += f;
-                if (f == 0.f) continue;             // (an empty piece's rows are not read into the sum)
+                for (int k = 0; k < kAhead; ++k) {
+                    w[k] = -INFINITY;
+                    if (c + k > c1) continue;
+                    const int64_t slot = slot_of(c + k);
+                    w[k] = J.part_lse[slot * rows + r];
+                    x[k][0] = part[slot * step];
+                    x[k][1] = part[slot * step + rows];
+                }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    acc[u].x = fmaf(f, x[k][u].x, acc[u].x); acc[u].y = fmaf(f, x[k][u].y, acc[u].y);
-                    acc[u].z = fmaf(f, x[k][u].z, acc[u].z); acc[u].w = fmaf(f, x[k][u].w, acc[u].w);
+                for (int k = 0; k < kAhead; ++k) {
+                    const float f = sfu_exp2(w[k] - shift);
+                    sum += f;
+                    if (f == 0.f) continue;             // (an empty piece's rows are not read into the sum)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        acc[u].x = fmaf(f, x[k][u].x, acc[u].x); acc[u].y = fmaf(f, x[k][u].y, acc[u].y);
+                        acc[u].z = fmaf(f, x[k][u].z, acc[u].z); acc[u].w = fmaf(f, x[k][u].w, acc[u].w);
+                    }
                 }
             }
         }
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            tile[lane][2 * warp + u] = make_uint2(pack2<kHalf>(acc[u].x * inv, acc[u].y * inv), pack2<kHalf>(acc[u].z * inv, acc[u].w * inv));
+        if (d0 == 0 && mine(r))
+            J.lse[(int64_t(b) * J.nodes + node_of(r)) * J.heads + head_of(r)] = sum != 0.f ? (shift + log2f(sum)) * kLn2 : -INFINITY;
+        __syncthreads();
+        // Out by rows: 16 lanes hold 64 dims, 128 bytes, of a row.
+        const int u = threadIdx.x & 15, d = dim0 + 4 * u;
+#pragma unroll
+        for (int k = threadIdx.x >> 4; k < 32; k += kCombineThreads / 16)
+            if (mine(r0 + k) && d < J.dim_v) {
+                uint16_t* dst = static_cast<uint16_t*>(J.out) + b * J.o_sb + node_of(r0 + k) * J.o_st + head_of(r0 + k) * J.o_sh + d;
+                *reinterpret_cast<uint2*>(dst) = tile[k][u];
+            }
+        __syncthreads();                        // the next part's rows go into the same tile
     }
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-        tile[lane][2 * warp + u] = make_uint2(pack2<kHalf>(acc[u].x * inv, acc[u].y * inv), pack2<kHalf>(acc[u].z * inv, acc[u].w * inv));
-    auto head_of = [&](int row) { return g * J.group + row % J.group; };
-    if (d0 == 0 && mine(r))
-        J.lse[(int64_t(b) * J.nodes + node_of(r)) * J.heads + head_of(r)] = sum != 0.f ? (shift + log2f(sum)) * kLn2 : -INFINITY;
-    __syncthreads();
-    // Out by rows: 16 lanes hold 64 dims, 128 bytes, of a row.
-    const int u = threadIdx.x & 15, d = blockIdx.z * 64 + 4 * u;
-#pragma unroll
-    for (int k = threadIdx.x >> 4; k < 32; k += kCombineThreads / 16)
-        if (mine(r0 + k) && d < J.dim_v) {
-            uint16_t* dst = static_cast<uint16_t*>(J.out) + b * J.o_sb + node_of(r0 + k) * J.o_st + head_of(r0 + k) * J.o_sh + d;
-            *reinterpret_cast<uint2*>(dst) = tile[k][u];
-        }
 }
 
 // ------------------------------------------------------------------- host --
@@ -884,7 +889,9 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
     }
     kernel<<<J.ctas, 128 + kSoftmaxThreads<NQ>, kSmemBytes, stream>>>(qm, km, vm, J);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(J.batch * J.kv_heads * J.row_groups, (NQ * J.tile_rows + 31) / 32, (J.dim_v + 63) / 64);
+    const int segments = J.batch * J.kv_heads * J.row_groups;
+    const int parts = (std::min(NQ * J.tile_rows, J.nodes * J.group) + 31) / 32 * ((J.dim_v + 63) / 64);
+    cfg.gridDim = dim3(segments, std::max(1, std::min(parts, 8 * J.ctas / segments)));
     cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = stream;
     cudaLaunchAttribute dependent{};
