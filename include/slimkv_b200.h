@@ -783,8 +783,9 @@ SLIMKV_API int slimkv_key_mass(const slimkv_key_mass_args* args, void* stream);
  * first `sinks` rows, its last `recent` rows and, of the others, those of the
  * largest mass (ties: the lowest row; a NaN counts above every number), in
  * their order, written to rows 0.. of the output cache; the output rows from
- * there to `keep` are zeroed.  mass / positions (int32, nullable: both or
- * neither of in and out) move along.  new_lengths[b] = min(lengths[b], keep).
+ * there to `keep` are zeroed.  The masses move along into out_mass (nullable),
+ * positions (int32) into out_positions (both or neither).  new_lengths[b] =
+ * min(lengths[b], keep).
  * sinks + recent <= keep.  The output must not overlap the input.
  * elem_bytes 1, 2 or 4; mass strides {batch, head} elements, mass_rows long.
  * ---------------------------------------------------------------------- */
