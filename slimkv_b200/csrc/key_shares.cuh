@@ -1,6 +1,6 @@
 // Equal shares of a batch's key tiles, cut on the device from its lengths.
 //
-// A unit is one 128-key tile of one segment (sequence, KV head, row group);
+// A unit is one key tile of one segment (sequence, KV head, row group);
 // the units of all segments in a row are cut into one equal share per CTA, and
 // the part of a segment inside a share is a piece.  Plan names the work:
 //   int batch, kv_heads, ctas;

@@ -28,13 +28,12 @@
 // Why 64 keys: S and P of a tile fit 64 tensor-memory columns, so two to four
 // tiles are under way for each row tile next to O (320 + 3 x 64, or 2 x (128 +
 // 2 x 64) columns): the S of tile n + 1 is there when the softmax of tile n
-// ends, and the softmax never waits for a product.  (With 128-key tiles and one S per row
-// tile, softmax and products took turns: 4,870 cycles for two row tiles and 128
-// keys, 2,700 of them the softmax.)
+// ends, and the softmax never waits for a product.  (With 128-key tiles and one
+// S per row tile, softmax and products took turns: 4,870 cycles for two row
+// tiles and 128 keys, 2,700 of them the softmax.)
 //
 // One CTA per SM, warps: 0 = Q and K loads (TMA), 3 = V loads, 1 and 2 = MMA
-// issue (2 owns the TMEM), the
-// others from 4 on = softmax.  Every wait is bounded.
+// issue (2 owns the TMEM), the others from 4 on = softmax.  Every wait is bounded.
 #include <algorithm>
 #include <type_traits>
 
@@ -70,7 +69,7 @@ struct Bars {
     uint64_t sfull[2][4], pfull[2][4], odone[2][4], oempty[2], final_mma;
     uint32_t tmem_base;
     int abort;
-    int bad_values[2];           // 1 + a piece whose node values hold infinities or NaN
+    int bad_values[4];           // 1 + a piece whose node values hold infinities or NaN, by piece % 4
     float exchange[kRows];       // between a row's two threads
     Share share;
 };
@@ -309,7 +308,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         mbar_init(&bs->qempty, NQ);
         mbar_init(&bs->final_mma, 2);
         bs->abort = 0;
-        bs->bad_values[0] = bs->bad_values[1] = 0;
+        for (int& x : bs->bad_values) x = 0;
     }
     if (tid < 32) fence_barrier_init();
     if (tid == 32) {
@@ -623,7 +622,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                     for (int c = 0; c < C && ok; ++c)
                         bad |= fix_values<kHalf, 2 * kHalves>(smem + off_v + uint32_t(slot * C + c) * kChunk, r & 63, 2 * half + (r >> 6),
                                                               (r & 63) < w.s.hi(tile), tile * kKeys + (r & 63) >= w.s.len);
-                    if (bad) *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) = w.piece + 1;
+                    // (Row tile 0 is up to three pieces ahead of row tile 1: a Q goes when both have
+                    // issued its products, and a row tile issues S up to two tiles ahead.)
+                    if (bad) *const_cast<volatile int*>(&bs->bad_values[w.piece & 3]) = w.piece + 1;
                     fence_async_shared();
                     if constexpr (NQ == 2) {
                         __syncwarp();
@@ -640,7 +641,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             if (!ok) continue;
             tc_fence_after();
             const bool whole = w.whole();
-            const bool bad = *const_cast<volatile int*>(&bs->bad_values[w.piece & 1]) == w.piece + 1;
+            const bool bad = *const_cast<volatile int*>(&bs->bad_values[w.piece & 3]) == w.piece + 1;
             const float inv = l_run != 0.f ? 1.f / l_run : 0.f;      // a NaN sum stays NaN
             const float lse2 = l_run != 0.f ? m_run + log2f(l_run) : -INFINITY;
             const int h = w.g * J.group + jh;
@@ -772,6 +773,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
     }
     __syncthreads();
     const int c0 = some ? range[0] : 0, c1 = some ? range[1] : 0, slot0 = some ? range[2] : 0;
+    grid_dependency_wait();                 // every block: what follows this grid counts on the one before it too
     // A segment in one piece whose rows are all live is written already.
     if (some && c0 == c1 && min((group + 1) * NQ * J.tpt, J.nodes) <= s.nodes) return;
     const int rows = NQ * J.tile_rows, first_node = group * NQ * J.tpt;
@@ -783,7 +785,6 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
     auto head_of = [&](int row) { return g * J.group + row % J.group; };
     // Whether a row is this kernel's to write.
     auto mine = [&](int row) { return row < used && (split || !some || node_of(row) >= s.nodes); };
-    grid_dependency_wait();
     for (int part = blockIdx.y; part < parts; part += gridDim.y) {
         const int r0 = part / dim_parts * 32, r = r0 + lane, dim0 = part % dim_parts * 64, d0 = dim0 + 8 * warp;
         const bool live = some && mine(r) && node_of(r) < s.nodes && d0 < J.dim_v;

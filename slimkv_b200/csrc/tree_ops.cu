@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
     __shared__ uint64_t of_rank[2][kPathCtas];          // by the step's parity
     __shared__ int child[2];
     const uint32_t rank = cluster_rank();
+    cluster_arrive();                                   // the others run, before anything is stored to them
     const int b = blockIdx.x / kPathCtas, tid = threadIdx.x;
     const int n = a.nodes_len ? min(max(__ldg(a.nodes_len + b), 0), a.nodes) : a.nodes;
     for (int i = tid; i < n; i += kPathThreads) {
@@ -188,6 +189,7 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
     int32_t* path = a.path + int64_t(b) * a.nodes;
     int cur = n > 0 ? 0 : -1, len = 0;
     int64_t next = -1;
+    cluster_wait();
     while (cur >= 0) {
         const int parity = len & 1;
         if (rank == 0 && tid == 0) path[len] = cur;

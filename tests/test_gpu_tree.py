@@ -154,6 +154,26 @@ def test_unseen_infinities_do_not_spread(T, page):
     assert got[0][:, 0].isfinite().all() and got[0][:, 5:].isfinite().all()
 
 
+@pytest.mark.parametrize('T,D', [(64, 64), (64, 128), (5, 64)])
+def test_seen_infinities_in_many_short_pieces(T, D):
+    """Shares of many segments of one or two key tiles, some of whose nodes hold
+    infinities: they reach the rows that see them in every segment."""
+    B, G = 40, 8
+    lengths = [(7 * b) % 30 for b in range(B)]
+    q, k, v, lens, _ = make(B, T, 32, G, D, lengths, seed=7)
+    seen = trees(B, T, 8)
+    for b, n in enumerate(lengths):
+        v[b, n + (3 if b % 3 else T - 1), b % G, b % D] = math.inf
+    want = torch.zeros(B, T, 32, D, dtype=torch.bool)
+    for b in range(B):
+        node = 3 if b % 3 else T - 1
+        want[b, :, 4 * (b % G):4 * (b % G) + 4, b % D] = seen[b, :, node, None]
+    for _ in range(20):
+        out, _ = tree.tree_attention(q, k, v, lens, D ** -0.5, mask=oracle.words_of(seen).cuda())
+        assert torch.equal(out.cpu() == math.inf, want) and not out.isnan().any()
+    assert _lib.device_status(clear=True) == 0
+
+
 @pytest.mark.parametrize('scale', [2.0, 0.5])
 def test_peaked_scores(scale):
     """Scores up to the hundreds: maxima that keep growing along the keys."""
