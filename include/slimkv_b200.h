@@ -732,7 +732,8 @@ SLIMKV_API int slimkv_tree_accept(const slimkv_tree_accept_args* args, void* wor
  * Commit of the accepted nodes: cache row lengths[b] + path[b][i] moves to
  * lengths[b] + i for i < count[b], in place, for `layers` caches whose K / V
  * lie layer_stride elements apart, and new_lengths[b] = lengths[b] + count[b].
- * path ascends (a path of slimkv_tree_accept).  elem_bytes 1, 2 or 4.
+ * path ascends (a path of slimkv_tree_accept).  elem_bytes 1, 2 or 4;
+ * new_lengths must not be lengths.
  * ---------------------------------------------------------------------- */
 typedef struct {
     int layers, batch, nodes, kv_heads, dim_qk, dim_v, elem_bytes;
@@ -786,7 +787,8 @@ SLIMKV_API int slimkv_key_mass(const slimkv_key_mass_args* args, void* stream);
  * there to `keep` are zeroed.  The masses move along into out_mass (nullable),
  * positions (int32) into out_positions (both or neither).  new_lengths[b] =
  * min(lengths[b], keep).
- * sinks + recent <= keep.  The output must not overlap the input.
+ * sinks + recent <= keep.  The output must not overlap the input, nor
+ * new_lengths be lengths.
  * elem_bytes 1, 2 or 4; mass strides {batch, head} elements, mass_rows long.
  * ---------------------------------------------------------------------- */
 typedef struct {

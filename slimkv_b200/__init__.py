@@ -16,6 +16,8 @@ thin torch bindings that mirror the reference's Python entry points:
 * ``slimkv_b200.reconstruct``— the reconstruct decode backend
 * ``slimkv_b200.parallel``   — sequence split across GPUs, max-over-ranks timing
 * ``slimkv_b200.tensor_parallel`` — decode split by KV head and by sequence across GPUs
+* ``slimkv_b200.tree``       — verification of drafted token trees: attention, acceptance, commit
+* ``slimkv_b200.eviction``   — a cache kept within a budget by the attention its keys receive
 * ``slimkv_b200.rope``       — RoPE tables built exactly like the reference
 """
 __version__ = '0.2.0'

@@ -14,7 +14,7 @@ from ctypes import byref
 import torch
 
 from . import _lib
-from .tree import _TYPES, _check_rows, _i32, _refuse, _run, _workspace, fill_cache
+from .tree import _TYPES, _check_rows, _i32, _refuse, _run, _run_in_workspace, fill_cache
 
 
 def _plane(t, dtype, batch, heads, rows, strides, what):
@@ -97,8 +97,9 @@ def evict(k, v, mass, positions, lengths, keep, sinks=0, recent=0, block_tables=
         out_k = torch.empty_strided((batch, keep, heads, dim), (heads * keep * dim, dim, keep * dim, 1), dtype=k.dtype, device=dev)
         out_v = torch.empty_strided((batch, keep, heads, dim_v), (heads * keep * dim_v, dim_v, keep * dim_v, 1), dtype=k.dtype,
                                     device=dev)
-        out_mass = torch.empty((batch, heads, keep), dtype=torch.float32, device=dev)
-        out_positions = None if positions is None else torch.empty((batch, heads, keep), dtype=torch.int32, device=dev)
+        plane = (batch, heads, keep), (heads * keep, keep, 1)
+        out_mass = torch.empty_strided(*plane, dtype=torch.float32, device=dev)
+        out_positions = None if positions is None else torch.empty_strided(*plane, dtype=torch.int32, device=dev)
     else:
         out_k, out_v, out_mass, out_positions = out
         _check_rows(out_k, out_v, 4)
@@ -114,10 +115,9 @@ def evict(k, v, mass, positions, lengths, keep, sinks=0, recent=0, block_tables=
     if positions is not None:
         a.positions = _plane(positions, torch.int32, batch, heads, mass.shape[2], a.positions_stride, 'positions')
         a.out_positions = _plane(out_positions, torch.int32, batch, heads, keep, a.out_positions_stride, 'out positions')
-    new_lengths = torch.empty(batch, dtype=torch.int32, device=dev)
+    new_lengths = torch.empty_strided((batch,), (1,), dtype=torch.int32, device=dev)
     a.lengths, a.new_lengths = _i32(lengths, (batch,), 'lengths'), new_lengths.data_ptr()
     a.keep, a.sinks, a.recent = keep, sinks, recent
     lib = _lib.load()
-    ws = _workspace(dev, lib.slimkv_evict_workspace_size, a)
-    _run(dev, lib.slimkv_evict, byref(a), ws.data_ptr(), ws.numel())
+    _run_in_workspace(dev, lib.slimkv_evict_workspace_size, lib.slimkv_evict, a)
     return out_k, out_v, out_mass, out_positions, new_lengths
