@@ -5,12 +5,11 @@
 // launches:
 //   evict_select_kernel  one cluster of CTAs per segment: the keep-th largest
 //     of its masses (order-preserving 32-bit keys, radix selection with four
-//     8-bit digits, whose counts the CTAs add up over distributed shared
-//     memory), how many rows equal to it still fit, and for every run of kRun
-//     rows how many rows above it and equal to it come before the run;
-//   evict_gather_kernel  one block per run, a dependent launch: which of its
-//     rows stay and where they go, then their K, V, mass and position moved, 16
-//     bytes a lane, eight of them under way at a time.
+//     8-bit digits, whose counts the CTAs add up over distributed shared memory;
+//     the same counts say what the CTAs before this one keep), then the kept
+//     rows in order, into a list;
+//   evict_gather_kernel  a dependent launch, one block per 32 rows of the output:
+//     K, V, mass and position of the listed rows moved, 16 bytes a lane.
 // Bound: HBM, the masses once (later readings come from L2) and each kept row
 // read and written.
 #include <algorithm>
@@ -21,12 +20,16 @@
 namespace slimkv {
 namespace {
 
-constexpr int kRun = 128;                 // rows of one gather block
+constexpr int kRows = 32;                 // output rows of one gather block
 constexpr int kGatherThreads = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kSelectThreads = 1024;
-constexpr int kBins = 256, kKeys = 4;      // digit values; keys of a thread in registers
+// Four digits of 8 bits: with three of 11, 11 and 10 each CTA of a cluster of 8 reads
+// 128 KB of the others' counts for a digit, and 16 segments of 32k rows took 42 us.
+constexpr int kPasses = 4, kBins = 256;
+constexpr int kKeys = 4;                  // keys of a thread in registers
 constexpr int kTile = kKeys * kSelectThreads, kChunks = kTile / 32;   // rows of a CTA's tile, 32 to a chunk
+static_assert(kChunks == 128, "four chunks to a lane");
 constexpr uint32_t kAlways = 0xffffffffu; // key of a protected row
 
 struct EvictArgs {
@@ -44,14 +47,11 @@ struct EvictArgs {
     int32_t* out_positions;
     int64_t out_positions_stride[2];
     int rows;                                 // rows a segment can hold
-    int keep, sinks, recent, runs;
+    int keep, sinks, recent;
     int32_t* new_lengths;
     unsigned int* status;
-    // Workspace, one entry per segment: the threshold key, the rows equal to
-    // it that stay, and [runs] pairs of counts before each run.
-    uint32_t* threshold;
-    uint32_t* ties;
-    uint2* before;
+    int32_t* kept;                            // workspace: each segment's kept rows, list_rows to a segment
+    int list_rows;
 };
 
 // Order-preserving key of row n's mass; kAlways for a protected row.  A NaN
@@ -66,11 +66,13 @@ __device__ __forceinline__ int segment_length(const EvictArgs& a, int b) {
     return min(max(__ldg(a.lengths + b), 0), a.rows);
 }
 
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs a) {
-    __shared__ uint32_t hist[4][kBins];       // one per digit: no pass clears what another still reads
-    __shared__ uint32_t warp_sum[8];
-    __shared__ uint32_t pick[2];              // the chosen digit, rows above it
-    __shared__ uint32_t counts[2];            // this CTA's rows above and equal to the threshold
+// (Two CTAs on an SM: a cluster stays in one part of the chip, where 16 clusters of 8
+// else came one after the other, 31 us against 23.)
+__global__ void __launch_bounds__(kSelectThreads, 2) evict_select_kernel(EvictArgs a) {
+    __shared__ uint32_t hist[kPasses][kBins];      // one per digit: no pass clears what another still reads
+    __shared__ uint32_t warp_sum[kBins / 32];
+    __shared__ uint32_t pick[3];              // the chosen digit, rows above it, rows with it
+    __shared__ uint32_t earlier[2];           // rows above and equal to the threshold of the CTAs before this one
     __shared__ uint2 chunk[kChunks];
     const uint32_t ranks = cluster_size(), rank = cluster_rank();
     const int segment = blockIdx.x / ranks, g = segment % a.kv_heads, b = segment / a.kv_heads;
@@ -83,11 +85,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
         if (given != len) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
     }
     grid_launch_dependents();
-    // This CTA's rows: whole runs, in tiles of kTile; key j of a thread is row
-    // 32 (32 j + warp) + lane of the tile.
-    const int runs_each = (a.runs + int(ranks) - 1) / int(ranks);
-    const int run0 = min(int(rank) * runs_each, a.runs), run1 = min(run0 + runs_each, a.runs);
-    const int n0 = min(run0 * kRun, len), n1 = min(run1 * kRun, len);
+    // This CTA's rows, in tiles of kTile; key j of a thread is row 32 (32 j + warp) + lane of the tile.
+    const int each = ((len + int(ranks) - 1) / int(ranks) + 31) / 32 * 32;      // whole lines, at most a tile's where one does
+    const int n0 = min(int(rank) * each, len), n1 = min(n0 + each, len);
     const int tiles = (n1 - n0 + kTile - 1) / kTile;
     uint32_t keys[kKeys];
     auto load = [&](int tile) {
@@ -97,15 +97,19 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
             keys[j] = n < n1 ? key_of(__ldg(mass + n), n, len, a.sinks, a.recent) : 0u;   // 0: below every row's key
         }
     };
-    for (int i = tid; i < 4 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+    for (int i = tid; i < kPasses * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+    if (tid < 2) earlier[tid] = 0;
     if (tiles == 1) load(0);
-    uint32_t prefix = 0, want = uint32_t(min(a.keep, len));
+    // Nothing to choose: every key is above threshold 0.
     const bool all = len <= a.keep;
+    uint32_t prefix = 0, want = uint32_t(min(a.keep, len));
+    uint32_t base_gt = all ? uint32_t(n0) : 0, base_tie = 0;
     if (!all) {
+        uint32_t gt = 0, tie = 0;             // of the CTAs before this one, in this thread's bins
         __syncthreads();
         // `want` of the rows that match `prefix` so far are still to be found.
 #pragma unroll 1
-        for (int pass = 0; pass < 4; ++pass) {
+        for (int pass = 0; pass < kPasses; ++pass) {
             const int shift = 24 - 8 * pass;
             for (int tile = 0; tile < tiles; ++tile) {
                 if (tiles > 1) load(tile);
@@ -113,7 +117,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
                 for (int j = 0; j < kKeys; ++j) {
                     // Masses share few exponents: lanes with the same digit count once.
                     const bool in = keys[j] && (pass == 0 || (keys[j] ^ prefix) >> (shift + 8) == 0);
-                    const uint32_t digit = in ? keys[j] >> shift & 255 : 256u;
+                    const uint32_t digit = in ? keys[j] >> shift & (kBins - 1) : uint32_t(kBins);
                     const unsigned same = __match_any_sync(0xffffffffu, digit);
                     if (in && lane == __ffs(int(same)) - 1) atomicAdd(&hist[pass][digit], uint32_t(__popc(same)));
                 }
@@ -121,17 +125,20 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
             __syncthreads();
             if (ranks > 1) cluster_sync();
             // Thread t < 256 has bin 255 - t, of all CTAs: rows above it, from the top.
-            uint32_t c = 0, above = 0;
+            const uint32_t bin = uint32_t(kBins - 1 - tid);
+            uint32_t c = 0, less = 0, above = 0;
             if (tid < kBins) {
-                const uint32_t* bin = &hist[pass][kBins - 1 - tid];
                 if (ranks == 1) {
-                    c = *bin;
+                    c = hist[pass][bin];
                 } else {
                     uint32_t of[kMaxCluster];
 #pragma unroll
-                    for (uint32_t r = 0; r < kMaxCluster; ++r) of[r] = r < ranks ? cluster_load(bin, r) : 0u;
+                    for (uint32_t r = 0; r < kMaxCluster; ++r) of[r] = r < ranks ? cluster_load(&hist[pass][bin], r) : 0u;
 #pragma unroll
-                    for (uint32_t r = 0; r < kMaxCluster; ++r) c += of[r];
+                    for (uint32_t r = 0; r < kMaxCluster; ++r) {
+                        c += of[r];
+                        if (r < rank) less += of[r];
+                    }
                 }
                 above = c;
 #pragma unroll
@@ -143,42 +150,63 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
             }
             __syncthreads();
             if (tid < kBins) {
-                above -= c;
-                for (int w = 0; w < warp; ++w) above += warp_sum[w];
+                above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0u) - c;
                 if (above < want && above + c >= want) {
-                    pick[0] = uint32_t(kBins - 1 - tid);
+                    pick[0] = bin;
                     pick[1] = above;
+                    pick[2] = c;
                 }
             }
             __syncthreads();
-            prefix |= pick[0] << shift;
+            const uint32_t digit = pick[0];
+            prefix |= digit << shift;
             want -= pick[1];
+            // When all rows with these digits stay, the rest of their digits does not matter
+            // (most often known after three of them).
+            const bool done = pick[2] == want;
+            if (tid < kBins) {
+                if (bin > digit || (done && bin == digit)) gt += less;
+                else if (pass == kPasses - 1 && bin == digit) tie = less;
+            }
+            if (done) {
+                prefix -= 1;                  // every key from the prefix on is above the threshold (no key begins with 0, 0)
+                want = 0;
+                break;
+            }
+        }
+        if (ranks > 1) {
+            cluster_arrive();                 // this CTA has read the others' counts
+            gt = __reduce_add_sync(0xffffffffu, gt);
+            if (lane == 0 && gt) atomicAdd(&earlier[0], gt);
+            if (tie) atomicAdd(&earlier[1], tie);
+            __syncthreads();
+            base_gt = earlier[0];
+            base_tie = earlier[1];
         }
     }
-    if (rank == 0 && tid == 0) {
-        a.threshold[segment] = prefix;        // all: 0, below every row's key
-        a.ties[segment] = all ? 0u : want;
-    }
-    // Rows above and equal to the threshold before each run, first within the CTA.
-    uint2* before = a.before + int64_t(segment) * a.runs;
-    uint32_t base_gt = 0, base_tie = 0;
+    // The kept rows in order: those above the threshold and the first `want` equal to it.
+    const uint32_t ties = all ? 0u : want;
+    int32_t* list = a.kept + int64_t(segment) * a.list_rows;
     for (int tile = 0; tile < tiles; ++tile) {
         if (tiles > 1) load(tile);
         __syncthreads();
+        unsigned gt[kKeys], tie[kKeys];       // lanes
 #pragma unroll
         for (int j = 0; j < kKeys; ++j) {
-            const uint32_t gt = __popc(__ballot_sync(0xffffffffu, keys[j] > prefix));
-            const uint32_t tie = __popc(__ballot_sync(0xffffffffu, keys[j] && keys[j] == prefix));
-            if (lane == 0) chunk[32 * j + warp] = make_uint2(gt, tie);
+            gt[j] = __ballot_sync(0xffffffffu, keys[j] > prefix);
+            tie[j] = __ballot_sync(0xffffffffu, keys[j] && keys[j] == prefix);
+            if (lane == 0) chunk[32 * j + warp] = make_uint2(__popc(gt[j]), __popc(tie[j]));
         }
         __syncthreads();
-        // Every warp scans the tile's chunks, four to a lane.
-        uint2 own[4], sum = make_uint2(0, 0);
+        // Every warp scans the tile's chunks, four to a lane; its own chunk 32 j + warp is number
+        // warp % 4 of lane 8 j + warp / 4.
+        uint2 sum = make_uint2(0, 0), at = make_uint2(0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            own[i] = chunk[4 * lane + i];
-            sum.x += own[i].x;
-            sum.y += own[i].y;
+            if (i == warp % 4) at = sum;
+            const uint2 x = chunk[4 * lane + i];
+            sum.x += x.x;
+            sum.y += x.y;
         }
         uint2 incl = sum;
 #pragma unroll
@@ -186,128 +214,76 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(EvictArgs 
             const uint32_t gu = __shfl_up_sync(0xffffffffu, incl.x, o), tu = __shfl_up_sync(0xffffffffu, incl.y, o);
             if (lane >= o) { incl.x += gu; incl.y += tu; }
         }
-        const int run = run0 + tile * (kTile / kRun) + lane;      // (a run is four chunks)
-        if (warp == 0 && run < run1) before[run] = make_uint2(base_gt + incl.x - sum.x, base_tie + incl.y - sum.y);
+        at.x += incl.x - sum.x;
+        at.y += incl.y - sum.y;
+        const unsigned below = (1u << lane) - 1u;
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+            const int from = 8 * j + warp / 4;
+            const uint32_t g0 = base_gt + __shfl_sync(0xffffffffu, at.x, from) + __popc(gt[j] & below);
+            const uint32_t t0 = base_tie + __shfl_sync(0xffffffffu, at.y, from) + __popc(tie[j] & below);
+            const bool above = gt[j] >> lane & 1, equal = tie[j] >> lane & 1;
+            if (above || (equal && t0 < ties)) list[g0 + min(t0, ties)] = n0 + tile * kTile + 32 * (32 * j + warp) + lane;
+        }
         base_gt += __shfl_sync(0xffffffffu, incl.x, 31);
         base_tie += __shfl_sync(0xffffffffu, incl.y, 31);
     }
-    // Runs of this CTA past its rows (all of them in a segment shorter than the budget).
-    for (int run = run0 + tiles * (kTile / kRun) + tid; run < run1; run += kSelectThreads) before[run] = make_uint2(base_gt, base_tie);
-    if (ranks == 1) return;
-    // Then what the CTAs before this one hold.
-    if (tid == 0) { counts[0] = base_gt; counts[1] = base_tie; }
-    __syncthreads();
-    cluster_sync();
-    uint32_t add_gt = 0, add_tie = 0;
-    for (uint32_t r = 0; r < rank; ++r) {
-        add_gt += cluster_load(&counts[0], r);
-        add_tie += cluster_load(&counts[1], r);
-    }
-    for (int r = run0 + tid; r < run1; r += kSelectThreads) {
-        uint2 x = before[r];
-        x.x += add_gt;
-        x.y += add_tie;
-        before[r] = x;
-    }
-    cluster_sync();                           // no CTA leaves while another reads its counts
+    if (ranks > 1 && !all) cluster_wait();    // no CTA leaves while another reads its counts
 }
-static_assert(kRun == 128 && kChunks == 128, "a run is four chunks, a tile 32 runs");
 
 __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs a) {
-    __shared__ int64_t from[2][kRun], to[2][kRun];      // byte offsets of the kept rows: K, V (-1: no such page)
-    __shared__ uint32_t warp_tie[kRun / 32], warp_keep[kRun / 32];
-    const int run = blockIdx.x, g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int segment = b * a.kv_heads + g;
-    const int len = segment_length(a, b);
-    const int kept = min(len, a.keep);
-    const int n0 = run * kRun, n = n0 + tid;
-    const unsigned below = (1u << lane) - 1u;
-    float x = 0.f;
-    if (tid < kRun && n < len) x = __ldg(a.mass + b * a.mass_stride[0] + g * a.mass_stride[1] + n);
+    // Byte offsets of the rows: K, V (from -1: zeros, to -1: nothing).
+    __shared__ int64_t from[2][kRows], to[2][kRows];
+    const int d0 = blockIdx.x * kRows, g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const int kept = min(segment_length(a, b), a.keep), rows = min(kRows, a.keep - d0);
     grid_dependency_wait();
-    const uint32_t threshold = a.threshold[segment], ties = a.ties[segment];
-    const uint2 before = a.before[int64_t(segment) * a.runs + run];
-    // Which rows stay: those above the threshold and the first `ties` equal to it.
-    const uint32_t key = key_of(x, n, len, a.sinks, a.recent);
-    const bool own = tid < kRun && n < len;
-    const bool gt = own && key > threshold, tie = own && key == threshold;
-    const unsigned tie_lanes = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0 && warp < kRun / 32) warp_tie[warp] = __popc(tie_lanes);
-    __syncthreads();
-    uint32_t at = before.y + __popc(tie_lanes & below);
-    for (int w = 0; w < min(warp, kRun / 32); ++w) at += warp_tie[w];
-    const bool stays = gt || (tie && at < ties);
-    const unsigned keep_lanes = __ballot_sync(0xffffffffu, stays);
-    if (lane == 0 && warp < kRun / 32) warp_keep[warp] = __popc(keep_lanes);
-    __syncthreads();
-    int local = __popc(keep_lanes & below), total = 0;
-#pragma unroll
-    for (int w = 0; w < kRun / 32; ++w) {
-        if (w < warp) local += warp_keep[w];
-        total += warp_keep[w];
-    }
-    const int first = int(before.x + min(before.y, ties));
-    bool bad = false;
-    if (stays) {
-        const int d = first + local;
-        int64_t ip, op;
-        int ir, orow;
-        const bool in = cache_row(a.in, b, n, ip, ir), out = cache_row(a.out, b, d, op, orow);
-        bad = !in || !out;
-        from[0][local] = bad ? -1 : ip * a.in.k_stride[0] + ir * a.in.k_stride[1] + g * a.in.k_stride[2];
-        from[1][local] = bad ? -1 : ip * a.in.v_stride[0] + ir * a.in.v_stride[1] + g * a.in.v_stride[2];
-        to[0][local] = op * a.out.k_stride[0] + orow * a.out.k_stride[1] + g * a.out.k_stride[2];
-        to[1][local] = op * a.out.v_stride[0] + orow * a.out.v_stride[1] + g * a.out.v_stride[2];
-        if (a.out_mass) a.out_mass[b * a.out_mass_stride[0] + g * a.out_mass_stride[1] + d] = x;
+    if (tid < rows) {
+        const int d = d0 + tid;
+        const bool some = d < kept;
+        const int n = some ? a.kept[int64_t(b * a.kv_heads + g) * a.list_rows + d] : 0;
+        int64_t ip = 0, op;
+        int ir = 0, orow;
+        const bool in = !some || cache_row(a.in, b, n, ip, ir), out = cache_row(a.out, b, d, op, orow);
+        from[0][tid] = some ? ip * a.in.k_stride[0] + ir * a.in.k_stride[1] + g * a.in.k_stride[2] : -1;
+        from[1][tid] = some ? ip * a.in.v_stride[0] + ir * a.in.v_stride[1] + g * a.in.v_stride[2] : -1;
+        to[0][tid] = in && out ? op * a.out.k_stride[0] + orow * a.out.k_stride[1] + g * a.out.k_stride[2] : -1;
+        to[1][tid] = in && out ? op * a.out.v_stride[0] + orow * a.out.v_stride[1] + g * a.out.v_stride[2] : -1;
+        if (!in || !out) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
+        if (a.out_mass)
+            a.out_mass[b * a.out_mass_stride[0] + g * a.out_mass_stride[1] + d] =
+                some ? __ldg(a.mass + b * a.mass_stride[0] + g * a.mass_stride[1] + n) : 0.f;
         if (a.out_positions)
             a.out_positions[b * a.out_positions_stride[0] + g * a.out_positions_stride[1] + d] =
-                __ldg(a.positions + b * a.positions_stride[0] + g * a.positions_stride[1] + n);
+                some ? __ldg(a.positions + b * a.positions_stride[0] + g * a.positions_stride[1] + n) : 0;
     }
     __syncthreads();
-    // The kept rows: pieces of 32 lanes x 16 bytes of a row's K and V, kPieces of a warp
-    // under way at a time; then the zeroed rows [kept, keep) of this run.
-    constexpr int kWarps = kGatherThreads / 32, kPieces = 8;
-    const int units = a.k_units + a.v_units, per_row = (units + 31) / 32, pieces = total * per_row;
-    // p / per_row by multiplication: exact while p per_row < 2^20 (p < 128 per_row, per_row <= 64).
-    const uint32_t inverse = (1u << 20) / uint32_t(per_row) + 1u;
-    const bool small = per_row <= 64;
-    for (int p0 = warp; p0 < pieces; p0 += kWarps * kPieces) {
-        uint4 w[kPieces];
-        uint4* dst[kPieces];
+    // 16-byte units of the rows' K and V, kUnits of a thread under way at a time.
+    constexpr int kUnits = 8;
+    const int units = a.k_units + a.v_units, total = rows * units;
+    // p / units by multiplication: exact while p units < 2^20 (p < kRows units, units <= 181).
+    const uint32_t inverse = (1u << 20) / uint32_t(units) + 1u;
+    const bool small = units <= 181;
+    for (int p0 = tid; p0 < total; p0 += kGatherThreads * kUnits) {
+        uint4 w[kUnits];
+        uint4* dst[kUnits];
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-            const int p = p0 + k * kWarps;
+        for (int k = 0; k < kUnits; ++k) {
+            const int p = p0 + k * kGatherThreads;
             dst[k] = nullptr;
-            if (p >= pieces) continue;
-            const int r = small ? int(uint32_t(p) * inverse >> 20) : p / per_row;
-            int u = (p - r * per_row) * 32 + lane;
-            if (u >= units) continue;
+            if (p >= total) continue;
+            const int r = small ? int(uint32_t(p) * inverse >> 20) : p / units;
+            int u = p - r * units;
             const int is_v = u >= a.k_units;
             if (is_v) u -= a.k_units;
-            const int64_t i = from[is_v][r];
-            if (i < 0) continue;
-            dst[k] = reinterpret_cast<uint4*>((is_v ? a.out_v : a.out_k) + to[is_v][r]) + u;
-            w[k] = __ldcs(reinterpret_cast<const uint4*>((is_v ? a.v : a.k) + i) + u);
+            const int64_t i = from[is_v][r], o = to[is_v][r];
+            if (o >= 0) dst[k] = reinterpret_cast<uint4*>((is_v ? a.out_v : a.out_k) + o) + u;
+            w[k] = make_uint4(0, 0, 0, 0);
+            if (i >= 0 && o >= 0) w[k] = __ldcs(reinterpret_cast<const uint4*>((is_v ? a.v : a.k) + i) + u);
         }
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k)
+        for (int k = 0; k < kUnits; ++k)
             if (dst[k]) __stcs(dst[k], w[k]);
     }
-    const int z0 = max(n0, kept), z1 = min(n0 + kRun, a.keep);
-    for (int d = z0 + tid; d < z1; d += kGatherThreads) {
-        if (a.out_mass) a.out_mass[b * a.out_mass_stride[0] + g * a.out_mass_stride[1] + d] = 0.f;
-        if (a.out_positions) a.out_positions[b * a.out_positions_stride[0] + g * a.out_positions_stride[1] + d] = 0;
-    }
-    for (int d = z0 + warp; d < z1; d += kWarps) {
-        int64_t page;
-        int row;
-        if (!cache_row(a.out, b, d, page, row)) { bad = true; continue; }
-        uint4* ok = reinterpret_cast<uint4*>(a.out_k + page * a.out.k_stride[0] + row * a.out.k_stride[1] + g * a.out.k_stride[2]);
-        uint4* ov = reinterpret_cast<uint4*>(a.out_v + page * a.out.v_stride[0] + row * a.out.v_stride[1] + g * a.out.v_stride[2]);
-        for (int u = lane; u < a.k_units; u += 32) ok[u] = make_uint4(0, 0, 0, 0);
-        for (int u = lane; u < a.v_units; u += 32) ov[u] = make_uint4(0, 0, 0, 0);
-    }
-    if (bad) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
 }
 
 int evict_rows(const slimkv_evict_args* a) {
@@ -325,13 +301,9 @@ int check_evict(const slimkv_evict_args* a) {
     return SLIMKV_OK;
 }
 
-int evict_runs(const slimkv_evict_args* a) { return int((std::max<int64_t>(evict_rows(a), a->keep) + kRun - 1) / kRun); }
-
 void carve(Carver& c, const slimkv_evict_args* a, EvictArgs& k) {
-    const size_t segments = size_t(a->batch) * a->kv_heads;
-    k.threshold = c.take<uint32_t>(segments);
-    k.ties = c.take<uint32_t>(segments);
-    k.before = c.take<uint2>(segments * k.runs);
+    k.list_rows = std::min(evict_rows(a), a->keep);
+    k.kept = c.take<int32_t>(size_t(a->batch) * a->kv_heads * k.list_rows);
 }
 
 }  // namespace
@@ -342,7 +314,6 @@ using namespace slimkv;
 extern "C" size_t slimkv_evict_workspace_size(const slimkv_evict_args* a) {
     if (check_evict(a) != SLIMKV_OK) return 0;
     EvictArgs k{};
-    k.runs = evict_runs(a);
     Carver c(nullptr, 0);
     carve(c, a, k);
     return c.used;
@@ -389,7 +360,6 @@ extern "C" int slimkv_evict(const slimkv_evict_args* a, void* workspace, size_t 
     k.keep = a->keep;
     k.sinks = a->sinks;
     k.recent = a->recent;
-    k.runs = evict_runs(a);
     k.new_lengths = a->new_lengths;
     k.status = status_word();
     Carver c(workspace, workspace_bytes);
@@ -413,7 +383,7 @@ extern "C" int slimkv_evict(const slimkv_evict_args* a, void* workspace, size_t 
     cudaError_t err = cudaLaunchKernelEx(&cfg, evict_select_kernel, k);
     dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     dependent.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(k.runs, a->kv_heads, a->batch);
+    cfg.gridDim = dim3((a->keep - 1) / kRows + 1, a->kv_heads, a->batch);
     cfg.blockDim = dim3(kGatherThreads);
     cfg.attrs = &dependent;
     if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, evict_gather_kernel, k);

@@ -160,6 +160,20 @@ def test_evict(B, G, D, Dv, lengths, keep, sinks, recent, dtype, page, kind):
     same(eviction.evict(k, v, mass, None, lens, keep, sinks, recent, block_tables=tables), want)
 
 
+@pytest.mark.parametrize('shift', [0, 8, 16, 23])
+@pytest.mark.parametrize('n,keep', [(300, 57), (20000, 12345), (40000, 1)])
+def test_evict_masses_that_differ_in_one_digit(shift, n, keep):
+    """One, two or many equal rows per value; a threshold between values and within one."""
+    for each in (1, 2, 300):
+        values = (torch.randperm(n, device='cuda') // each) % (256 if shift < 23 else 200)
+        mass = ((values.int() << shift) + (0x3f000000 if shift < 23 else 0x00800000)).view(torch.float32)
+        mass = torch.stack([mass, -mass]).view(1, 2, n)
+        k = torch.randint(0, 200, (1, n, 2, 16), device='cuda').to(BF16)
+        lens = torch.tensor([n], dtype=torch.int32, device='cuda')
+        same(eviction.evict(k, k, mass, None, lens, keep, 1 if keep > 1 else 0, 3 if keep > 4 else 0),
+             oracle.evict(k, k, mass, None, [n], keep, 1 if keep > 1 else 0, 3 if keep > 4 else 0))
+
+
 def test_evict_into_given_buffers():
     k = torch.randn(2, 500, 2, 64, device='cuda').to(BF16)
     mass = torch.rand(2, 2, 500, device='cuda')
