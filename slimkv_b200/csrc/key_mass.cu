@@ -69,6 +69,8 @@ struct Seq {
     int tiles, groups;
 };
 struct Plan {
+    // (None: 33.9 us for 64 sequences of 100..900 rows; one: 28.3; two: 26.3.)
+    static constexpr int kPieceUnits = 2;
     const Job& J;
     int batch, kv_heads, ctas;
     __device__ __forceinline__ explicit Plan(const Job& j) : J(j), batch(j.batch), kv_heads(j.kv_heads), ctas(j.ctas) {}
@@ -391,7 +393,7 @@ extern "C" int slimkv_key_mass(const slimkv_key_mass_args* a, void* stream) {
     J.paged = paged;
     J.cache = cache_view(cache);
     J.capacity = std::min<int64_t>(cache_capacity(J.cache), a->mass_rows);
-    if (double(J.batch) * J.kv_heads * double(J.capacity / kKeys + 1) >= 2147483648.0)
+    if (double(J.batch) * J.kv_heads * double(J.capacity / kKeys + 1 + Plan::kPieceUnits) >= 2147483648.0)
         return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "key mass: too many rows in one call");
     J.q = static_cast<const uint16_t*>(a->q);
     J.q_sb = a->q_stride[0]; J.q_st = a->q_stride[1]; J.q_sh = a->q_stride[2];

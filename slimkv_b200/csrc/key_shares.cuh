@@ -2,7 +2,11 @@
 //
 // A unit is one key tile of one segment (sequence, KV head, row group);
 // the units of all segments in a row are cut into one equal share per CTA, and
-// the part of a segment inside a share is a piece.  Plan names the work:
+// the part of a segment inside a share is a piece.  In front of its tiles a
+// segment has kPieceUnits units without work: what a further piece costs a CTA
+// (every CTA has one), so that shares with several short pieces take no longer
+// than those within one segment.  Plan names the work:
+//   static constexpr int kPieceUnits;
 //   int batch, kv_heads, ctas;
 //   Seq sequence(int b) const;     // with int tiles, groups: a sequence's key
 //                                  // tiles and row groups (0: nothing to do)
@@ -13,10 +17,14 @@
 namespace slimkv {
 
 // Callers make sure that a call has fewer than 2^31 units.
+template <class Plan, class Seq>
+__device__ __forceinline__ uint32_t segment_units(const Plan&, const Seq& s) {
+    return s.tiles > 0 ? uint32_t(s.tiles + Plan::kPieceUnits) : 0u;
+}
 template <class Plan>
 __device__ __forceinline__ uint32_t units_of(const Plan& P, int b) {
     const auto s = P.sequence(b);
-    return uint32_t(P.kv_heads) * uint32_t(s.groups) * uint32_t(s.tiles);
+    return uint32_t(P.kv_heads) * uint32_t(s.groups) * segment_units(P, s);
 }
 // CTAs with a share: every share holds at least one unit.
 __device__ __forceinline__ uint32_t share_count(uint32_t total, int ctas) { return min(total, uint32_t(ctas)); }
@@ -87,10 +95,11 @@ __device__ __forceinline__ void find_share(const Plan& P, Share* share) {
     }
 }
 
-// A CTA's pieces in order (CTAs with a share only).
+// A CTA's pieces in order (CTAs with a share only; there may be none).
 template <class Plan>
 struct Walk {
     int left;                   // units of the share still to come
+    int at;                     // units of the segment that are done
     int b, g, group;            // the piece's segment
     decltype(((const Plan*)nullptr)->sequence(0)) s;
     int t0, t1;                 // its key tiles
@@ -101,30 +110,36 @@ struct Walk {
         piece = -1;
         b = share->first_b;
         s = P.sequence(b);
-        const uint32_t off = u - share->first_u, seg = off / uint32_t(s.tiles);
+        const uint32_t off = u - share->first_u, units = segment_units(P, s), seg = off / units;
         g = int(seg / uint32_t(s.groups));
         group = int(seg) - g * s.groups;
-        t1 = int(off - seg * uint32_t(s.tiles));        // as if a piece had ended here
+        at = int(off - seg * units);
     }
     // Moves to the next piece; false when the share is done.
     __device__ __forceinline__ bool next(const Plan& P) {
-        if (left == 0) return false;
-        if (t1 >= s.tiles) {
-            t1 = 0;
-            if (++group >= s.groups) {
-                group = 0;
-                if (++g >= P.kv_heads) {
-                    g = 0;
-                    do s = P.sequence(++b);
-                    while ((s.groups == 0 || s.tiles == 0) && b + 1 < P.batch);
+        for (; left > 0;) {
+            if (at >= s.tiles + Plan::kPieceUnits) {
+                at = 0;
+                if (++group >= s.groups) {
+                    group = 0;
+                    if (++g >= P.kv_heads) {
+                        g = 0;
+                        do s = P.sequence(++b);
+                        while ((s.groups == 0 || s.tiles == 0) && b + 1 < P.batch);
+                    }
                 }
             }
+            t0 = max(at - Plan::kPieceUnits, 0);
+            const int step = min(s.tiles + Plan::kPieceUnits - at, left);
+            at += step;
+            left -= step;
+            t1 = at - Plan::kPieceUnits;
+            if (t1 > t0) {
+                ++piece;
+                return true;
+            }
         }
-        t0 = t1;
-        t1 = min(s.tiles, t0 + left);
-        left -= t1 - t0;
-        ++piece;
-        return true;
+        return false;
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == s.tiles; }
 };

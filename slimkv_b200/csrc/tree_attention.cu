@@ -113,6 +113,9 @@ struct Seq {
 };
 template <int NQ>
 struct Plan {
+    // A piece's end and the next one's first products take 3 to 5 us, a tile 1.  (None: 36.6 us
+    // for the ragged pages, 71 for 64 short sequences; two: 31.7 and 56.7; three: 31.2 and 55.8; six: 32.1 and 55.9.)
+    static constexpr int kPieceUnits = 3;
     const Job& J;
     int batch, kv_heads, ctas;
     __device__ __forceinline__ explicit Plan(const Job& j) : J(j), batch(j.batch), kv_heads(j.kv_heads), ctas(j.ctas) {}
@@ -444,7 +447,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             while (all_lanes(ok && f.more)) issue_s();
         } else {
             if constexpr (NQ == 2) {
-                issue_s();
+                if (f.more) issue_s();
                 if (f.more) issue_s();
             }
             int slot = 0;
@@ -760,11 +763,11 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
         uint32_t total, before;
         sum_units(plan, b, total, before);
         if (lane == 0) {
-            const uint32_t u0 = before + uint32_t(g * s.groups + group) * uint32_t(s.tiles);
-            const uint32_t ctas = share_count(total, J.ctas), c0 = share_of(total, u0, ctas);
+            const uint32_t units = segment_units(plan, s), u0 = before + uint32_t(g * s.groups + group) * units;
+            const uint32_t ctas = share_count(total, J.ctas), c0 = share_of(total, u0 + Plan<NQ>::kPieceUnits, ctas);
             range[0] = int(c0);
-            range[1] = int(share_of(total, u0 + s.tiles - 1, ctas));
-            range[2] = 2 * int(c0) + (share_begin(total, c0, ctas) != u0 ? 1 : 0);
+            range[1] = int(share_of(total, u0 + units - 1, ctas));
+            range[2] = 2 * int(c0) + (share_begin(total, c0, ctas) < u0 ? 1 : 0);   // a piece of another segment before it
         }
     }
     if (threadIdx.x == 32 && g == 0 && group == 0 && blockIdx.y == 0) {
@@ -969,7 +972,7 @@ extern "C" int slimkv_tree_attention(const slimkv_tree_attention_args* a, void* 
     J.paged = paged;
     J.cache = cache_view(cache);
     J.capacity = cache_capacity(J.cache);
-    if (double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / kKeys + 1) >= 2147483648.0)
+    if (double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / kKeys + 1 + Plan<1>::kPieceUnits) >= 2147483648.0)
         return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "tree attention: too many rows in one call");
     J.lengths = a->lengths;
     J.nodes_len = a->nodes_len;
