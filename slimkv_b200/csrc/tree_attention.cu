@@ -48,7 +48,6 @@ constexpr int kRows = 128;
 constexpr int kKeys = 64;                        // keys of a tile
 constexpr uint32_t kQChunk = 128 * 128;          // [128 rows x 64] 16-bit elements
 constexpr uint32_t kChunk = kKeys * 128;         // [64 keys x 64]
-constexpr uint32_t kTileArea = 224 * 1024;
 constexpr int kMaxRing = 12;
 constexpr int kMaxChunks = 5;                    // dims <= 320
 constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a row's maximum grows by more than 2^8
@@ -61,6 +60,16 @@ template <int NQ>
 constexpr int kHalvesOf = NQ == 1 ? 2 : 1;
 template <int NQ>
 constexpr int kSoftmaxThreads = 128 * NQ * kHalvesOf<NQ>;
+// Whether the kernel leaves a block of the merge room next to it, so that this
+// one is there and has done its planning when the last piece ends (one token
+// over 517 rows 14.5 -> 13.6 us, 16 sequences of 8k 113.5 -> 110.7).  Rows of
+// more than 256 dims need the shared memory for their rings (latents 34.4 ->
+// 38.4), two row tiles their threads' registers.
+template <int NQ, int C>
+constexpr bool kEarlyMerge = NQ == 1 && C <= 4;
+// Q and the rings.
+template <int NQ, int C>
+constexpr uint32_t kTileArea = (kEarlyMerge<NQ, C> ? 216 : 224) * 1024;
 
 struct Bars {
     uint64_t kfull[kMaxRing], kempty[kMaxRing], vfull[kMaxRing], vempty[kMaxRing], vfixed[kMaxRing];
@@ -73,8 +82,9 @@ struct Bars {
     float exchange[kRows];       // between a row's two threads
     Share share;
 };
-constexpr uint32_t kSmemBytes = 1024 + kTileArea + uint32_t(sizeof(Bars));
-static_assert(kSmemBytes <= 232448, "shared memory budget");
+template <int NQ, int C>
+constexpr uint32_t kSmemBytes = 1024 + kTileArea<NQ, C> + uint32_t(sizeof(Bars));
+static_assert(kSmemBytes<2, 2> <= 232448, "shared memory budget");
 
 struct Job {
     int batch, nodes, heads, kv_heads, group;
@@ -272,7 +282,7 @@ __device__ __forceinline__ bool fix_values(uint8_t* chunk, int r, int u0, bool s
 // wide rows' MMAs took 100 cycles each.
 template <int NQ, int C>
 struct Rings {
-    static constexpr int kFree = int((kTileArea - uint32_t(NQ * C) * kQChunk) / kChunk);
+    static constexpr int kFree = int((kTileArea<NQ, C> - uint32_t(NQ * C) * kQChunk) / kChunk);
     static constexpr int kGroup = C > 2 ? 1 : C;             // chunks of a K slot
     static constexpr int kPer = C / kGroup;                  // K slots of a tile
     static constexpr int kV = kFree / 2 / C < 2 ? 2 : kFree / 2 / C < kMaxRing ? kFree / 2 / C : kMaxRing;
@@ -282,7 +292,7 @@ struct Rings {
 
 // ----------------------------------------------------------------- kernel --
 template <int NQ, int C, bool kHalf>
-__global__ void __launch_bounds__(128 + kSoftmaxThreads<NQ>, 1)
+__global__ void __launch_bounds__(kEarlyMerge<NQ, C> ? 512 : 128 + kSoftmaxThreads<NQ>, 1)     // (512: 128 registers a thread)
 tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Job J) {
     constexpr int kThreads = 128 + kSoftmaxThreads<NQ>;
@@ -291,7 +301,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     using R = Rings<NQ, C>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    Bars* bs = reinterpret_cast<Bars*>(smem + kTileArea);
+    Bars* bs = reinterpret_cast<Bars*>(smem + kTileArea<NQ, C>);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // Layout: Q (NQ x C chunks) | K ring | V ring.
     const uint32_t off_k = uint32_t(NQ * C) * kQChunk;
@@ -323,6 +333,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         tmem_alloc(&bs->tmem_base, 512);
         tmem_relinquish();
     }
+    if (kEarlyMerge<NQ, C>) grid_launch_dependents();
     const Plan<NQ> plan(J);
     if (warp == 3) find_share(plan, &bs->share);
     tc_fence_before();
@@ -711,7 +722,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         }
     }
     __syncthreads();
-    grid_launch_dependents();
+    if (!kEarlyMerge<NQ, C>) grid_launch_dependents();
     if (any) {
         // Nothing of this CTA is in flight when its tensor memory goes: the
         // MMAs (they follow every copy that was waited for), and after a wait
@@ -748,7 +759,7 @@ constexpr int kCombineThreads = 256;
 // (16: 23 us for 8 segments of 128 rows in 19 pieces); and many blocks to a
 // segment cost many short segments more than the merge.
 template <int NQ, bool kHalf>
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Job J) {
+__global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const __grid_constant__ Job J) {
     __shared__ int range[3];                // first and last CTA of the segment's pieces, slot of the first
     __shared__ uint2 tile[32][17];          // the merged rows, 4 dims to an entry (17: no bank twice)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -887,11 +898,11 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
     static bool configured[64] = {};
     const int dev = device_info().device;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)) != cudaSuccess)
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes<NQ, C>)) != cudaSuccess)
             return fail(SLIMKV_ERR_CUDA, "cudaFuncSetAttribute (tree attention) failed");
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    kernel<<<J.ctas, 128 + kSoftmaxThreads<NQ>, kSmemBytes, stream>>>(qm, km, vm, J);
+    kernel<<<J.ctas, 128 + kSoftmaxThreads<NQ>, kSmemBytes<NQ, C>, stream>>>(qm, km, vm, J);
     cudaLaunchConfig_t cfg{};
     const int segments = J.batch * J.kv_heads * J.row_groups;
     const int parts = (std::min(NQ * J.tile_rows, J.nodes * J.group) + 31) / 32 * ((J.dim_v + 63) / 64);
