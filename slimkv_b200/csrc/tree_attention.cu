@@ -802,18 +802,11 @@ __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const __gri
     for (int part = blockIdx.y; part < parts; part += gridDim.y) {
         const int r0 = part / dim_parts * 32, r = r0 + lane, dim0 = part % dim_parts * 64, d0 = dim0 + 8 * warp;
         const bool live = some && mine(r) && node_of(r) < s.nodes && d0 < J.dim_v;
+        // In one pass, the largest exponent so far taken out: a piece's lse and rows are one latency.
         float m = -INFINITY, sum = 0.f, shift = 0.f;
         float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
         if (live) {
             constexpr int kAhead = 4;
-            for (int c = c0; c <= c1; c += kAhead) {
-                float l[kAhead];
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) l[k] = c + k <= c1 ? J.part_lse[slot_of(c + k) * rows + r] : -INFINITY;
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) m = fmaxf(m, l[k]);
-            }
-            shift = m == -INFINITY ? 0.f : m;
             const float4* part = reinterpret_cast<const float4*>(J.part_o) + int64_t(d0 / 4) * rows + r;
             const int64_t step = int64_t(J.dim_v / 4) * rows;
             for (int c = c0; c <= c1; c += kAhead) {
@@ -828,6 +821,14 @@ __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const __gri
                     x[k][0] = part[slot * step];
                     x[k][1] = part[slot * step + rows];
                 }
+                const float before = shift;
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) m = fmaxf(m, w[k]);
+                shift = m == -INFINITY ? 0.f : m;
+                const float old = sum != 0.f ? sfu_exp2(before - shift) : 0.f;
+                sum *= old;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) { acc[u].x *= old; acc[u].y *= old; acc[u].z *= old; acc[u].w *= old; }
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     const float f = sfu_exp2(w[k] - shift);
