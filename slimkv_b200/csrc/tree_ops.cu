@@ -33,10 +33,9 @@ __global__ void tree_masks_kernel(const int32_t* parents, int nodes, int words, 
 // The largest logit of a row as one 64-bit number: its order-preserving bits
 // (NaN above everything, the two zeros equal) over the complement of its
 // index, so that a maximum of them takes the lowest index of equal values.
-__device__ __forceinline__ uint64_t rank_of(float x, uint32_t index) {
+__device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.f);
-    const uint32_t o = x != x ? 0xffffffffu : (u >> 31 ? ~u : u | 0x80000000u);
-    return uint64_t(o) << 32 | uint32_t(~index);
+    return x != x ? 0xffffffffu : (u >> 31 ? ~u : u | 0x80000000u);
 }
 __device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
@@ -45,51 +44,75 @@ template <> __device__ __forceinline__ float to_float(float x) { return x; }
 template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A vector is looked into only when its largest value (NaN above all) is above
-// the thread's largest so far: a thread's elements come in ascending order, so
-// an equal one is not wanted.
-template <typename T>
-__device__ __forceinline__ void scan_vector(const uint4& w, uint32_t at, float& top, uint64_t& best) {
-    constexpr int kN = 16 / int(sizeof(T));
-    const T* x = reinterpret_cast<const T*>(&w);
-    float m = to_float(x[0]);
-#pragma unroll
-    for (int i = 1; i < kN; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(to_float(x[i])));
-    if (best && (m <= top || top != top)) return;
-    top = m;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) best = max_u64(best, rank_of(to_float(x[i]), at + i));
-}
+// What the threads of a block exchange in scan_row.
+template <int kThreads>
+struct ScanScratch {
+    uint32_t keys[kThreads / 32];
+    uint32_t index;
+};
 
-// The best of elements [lo, hi) of a row, over the threads of a block.
+// The best of elements [lo, hi) of a row, over the threads of a block (0: no
+// elements).  A thread keeps its largest value and the vector that holds it
+// (its elements come in ascending order, so an equal one is not wanted); only
+// the thread with the block's largest looks for the element.
 template <typename T, int kThreads>
-__device__ __forceinline__ uint64_t scan_row(const T* row, int lo, int hi, uint64_t* part) {
+__device__ __forceinline__ uint64_t scan_row(const T* row, int lo, int hi, ScanScratch<kThreads>* scratch) {
     constexpr int kN = 16 / int(sizeof(T));
-    uint64_t best = 0;
     const int lead = int(((16 - (reinterpret_cast<uintptr_t>(row + lo) & 15)) & 15) / sizeof(T));
-    const int body = std::min(lo + lead, hi);
+    const int body = min(lo + lead, hi);
     const int vectors = (hi - body) / kN, tail = body + vectors * kN;
-    for (int i = lo + int(threadIdx.x); i < body; i += kThreads) best = max_u64(best, rank_of(to_float(row[i]), i));
+    float top = 0.f;
+    bool some = false;
+    uint32_t at = 0;
+    alignas(16) T best[kN];
+    auto better = [&](float m) { return !some || m > top || (m != m && top == top); };
+    auto one = [&](int i) {
+        const T x = row[i];
+        if (!better(to_float(x))) return;
+        some = true;
+        top = to_float(x);
+        at = uint32_t(i);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) best[e] = x;
+    };
+    if (threadIdx.x == 0) scratch->index = 0xffffffffu;
+    for (int i = lo + int(threadIdx.x); i < body; i += kThreads) one(i);
     const uint4* v = reinterpret_cast<const uint4*>(row + body);
-    float top = __int_as_float(0xff800000);
     for (int i = threadIdx.x; i < vectors; i += 4 * kThreads) {
         uint4 w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (i + k * kThreads < vectors) w[k] = __ldg(v + i + k * kThreads);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i + k * kThreads < vectors) scan_vector<T>(w[k], body + (i + k * kThreads) * kN, top, best);
+        for (int k = 0; k < 4; ++k) {
+            if (i + k * kThreads >= vectors) continue;
+            const T* x = reinterpret_cast<const T*>(&w[k]);
+            float m = to_float(x[0]);
+#pragma unroll
+            for (int e = 1; e < kN; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(to_float(x[e])));
+            if (better(m)) {
+                some = true;
+                top = m;
+                at = uint32_t(body + (i + k * kThreads) * kN);
+                *reinterpret_cast<uint4*>(best) = w[k];
+            }
+        }
     }
-    for (int i = tail + int(threadIdx.x); i < hi; i += kThreads) best = max_u64(best, rank_of(to_float(row[i]), i));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = best;
+    for (int i = tail + int(threadIdx.x); i < hi; i += kThreads) one(i);
+    const uint32_t key = some ? key_of(top) : 0u, of_warp = __reduce_max_sync(0xffffffffu, key);
+    if ((threadIdx.x & 31) == 0) scratch->keys[threadIdx.x >> 5] = of_warp;
     __syncthreads();
-    best = part[0];
+    const int lane = threadIdx.x & 31;
+    const uint32_t largest = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? scratch->keys[lane] : 0u);
+    if (some && key == largest) {
+        uint32_t first = 0;
 #pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) best = max_u64(best, part[w]);
-    return best;
+        for (int e = kN - 1; e >= 0; --e)
+            if (key_of(to_float(best[e])) == largest) first = uint32_t(e);
+        atomicMin(&scratch->index, at + first);
+    }
+    __syncthreads();
+    return uint64_t(largest) << 32 | uint32_t(~scratch->index);
 }
 
 struct AcceptArgs {
@@ -110,12 +133,12 @@ constexpr int kScanThreads = 256;
 // Every node's argmax, its vocabulary split over gridDim.x blocks.
 template <typename T>
 __global__ void __launch_bounds__(kScanThreads) accept_scan_kernel(AcceptArgs a) {
-    __shared__ uint64_t part[kScanThreads / 32];
+    __shared__ ScanScratch<kScanThreads> scratch;
     const int t = blockIdx.y, b = blockIdx.z;
     if (a.nodes_len && t >= __ldg(a.nodes_len + b)) return;
     const T* row = static_cast<const T*>(a.logits) + b * a.stride_batch + t * a.stride_node;
     const int lo = int(int64_t(a.vocab) * blockIdx.x / a.splits), hi = int(int64_t(a.vocab) * (blockIdx.x + 1) / a.splits);
-    const uint64_t best = scan_row<T, kScanThreads>(row, lo, hi, part);
+    const uint64_t best = scan_row<T, kScanThreads>(row, lo, hi, &scratch);
     if (threadIdx.x == 0) a.best[(int64_t(b) * a.nodes + t) * a.splits + blockIdx.x] = best;
     grid_launch_dependents();
 }
@@ -173,7 +196,7 @@ template <typename T>
 __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a) {
     __shared__ int64_t tokens[kMaxNodes];
     __shared__ int32_t parents[kMaxNodes];
-    __shared__ uint64_t part[kPathThreads / 32];
+    __shared__ ScanScratch<kPathThreads> scratch;
     __shared__ uint64_t of_rank[2][kPathCtas];          // by the step's parity
     __shared__ int child[2];
     const uint32_t rank = cluster_rank();
@@ -196,7 +219,7 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
         ++len;
         __syncthreads();
         const uint64_t best = scan_row<T, kPathThreads>(
-            static_cast<const T*>(a.logits) + b * a.stride_batch + cur * a.stride_node, lo, hi, part);
+            static_cast<const T*>(a.logits) + b * a.stride_batch + cur * a.stride_node, lo, hi, &scratch);
         if (tid < kPathCtas) cluster_store(&of_rank[parity][rank], tid, best);
         cluster_sync();
         uint64_t all = of_rank[parity][0];
@@ -219,11 +242,14 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
     cluster_sync();                                     // no CTA leaves while another may still store to it
 }
 
-// Scanning every node reads all the logits, the walk with its argmaxes takes
-// 3 to 4 us a step.  Measured (vocabulary 128256, bf16, scan / walk): 1 x 8
-// nodes 7.4 / 13.9 us, 1 x 64 (16 MB) 15.7 / 23.2, 16 x 8 (33 MB) 18.7 / 18.2,
-// 16 x 64 (263 MB) 89.9 / 29.1.
-constexpr int64_t kScanAllBytes = int64_t(32) << 20;
+// Scanning every node reads all the logits, the walk with its argmaxes takes 2
+// us a step.  Measured (bf16, logits up to L2's size read again from there, as
+// after the product that wrote them; scan / walk): 1 x 8 nodes of 128256 logits
+// 6.1 / 10.6 us, 1 x 64 (16 MB) 9.2 / 17.2, 16 x 8 (33 MB) 9.7 / 11.6, 16 x 16
+// (66 MB) 12.4 / 14.6, 64 x 16 of 32000 (66 MB) 12.7 / 27.0, 64 x 8 of 128256
+// (131 MB) 26.0 / 19.7, 16 x 64 (263 MB) 47.0 / 18.9.  (Fetching the children's
+// logits into L2 ahead of the walk made its steps longer: 20.2 us.)
+constexpr int64_t kScanAllBytes = int64_t(64) << 20;
 bool accept_scans_all(const slimkv_tree_accept_args* a) {
     return int64_t(a->batch) * a->nodes * a->vocab * (a->type == SLIMKV_FP32 ? 4 : 2) <= kScanAllBytes;
 }

@@ -305,6 +305,30 @@ def test_tree_accept(B, T, V, dtype, offset):
         assert torch.equal(x.cpu(), y)
 
 
+@pytest.mark.parametrize('B,T,V,dtype', [(17, 64, 32003, BF16), (4, 70, 64001, torch.float32), (3, 90, 130003, FP16), (1, 1024, 33001, BF16),
+                                         (70, 2, 240007, BF16)])
+@pytest.mark.parametrize('offset', [0, 1])
+def test_tree_accept_along_the_path(B, T, V, dtype, offset):
+    """More than 64 MB of logits: argmaxes taken as the walk gets to them."""
+    test_tree_accept(B, T, V, dtype, offset)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, BF16, FP16])
+def test_accept_ties_along_the_path(dtype):
+    V = 3000005
+    x = torch.full((6, 2, V), -math.inf, device='cuda', dtype=dtype)
+    x[0, 0, [17, 375000, 375001, 2999999]] = 3.0         # a tie, within and across blocks
+    x[1, 0, 2000005], x[1, 0, 4] = 0.0, -0.0
+    x[2, 0, 3000004], x[2, 0, 3] = math.nan, math.inf
+    x[3, 0, 1500000] = math.inf
+    x[5, 0, [80000, 600000]] = math.nan
+    x[5, 0, 600000] = -math.nan
+    tokens = torch.tensor([[0, 17], [0, 4], [0, 3000004], [0, 1500000], [0, 0], [0, 80000]], device='cuda')
+    parents = torch.tensor([[-1, 0]] * 6, dtype=torch.int32, device='cuda')
+    path, count, _ = tree.tree_accept(x, tokens, parents)
+    assert count.tolist() == [2] * 6 and path.tolist() == [[0, 1]] * 6
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, BF16, FP16])
 def test_accept_ties_zeros_nan_and_infinities(dtype):
     V = 9000
