@@ -754,8 +754,9 @@ SLIMKV_API int slimkv_tree_commit(const slimkv_tree_commit_args* args, void* str
  * for n < lengths[b] (old keys) and, unless context_only, the keys
  * lengths[b] + i of the rows themselves (chain order: row i sees the keys
  * n <= lengths[b] + i; their old mass counts as 0).  Other entries of mass keep
- * their values.  rows null: r_i = i; counts null: every row.  A row whose lse
- * is infinite (it saw no key) gives nothing.
+ * their values.  rows null: r_i = i; counts null: every row.  The lse is taken
+ * as it is: at +inf a row gives nothing, at -inf (a row that saw no key, which
+ * an accepted row is not: it sees itself) the masses of its keys are infinite.
  * q [batch][nodes][heads][dim], lse fp32 [batch][nodes][heads] contiguous,
  * mass fp32, element strides {batch, head}, at least the used rows long.  Only
  * cache.k is read.  Types, dims and pages as slimkv_tree_attention.

@@ -248,8 +248,7 @@ key_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant_
                     const int h = w.g * J.group + at - row * J.group;
                     float off = INFINITY;
                     if (some) {
-                        const float x = __ldg(J.lse + (int64_t(w.b) * J.nodes + r) * J.heads + h);
-                        if (x != -INFINITY) off = x * kLog2e;
+                        off = __ldg(J.lse + (int64_t(w.b) * J.nodes + r) * J.heads + h) * kLog2e;
                     } else if (col < cols) {
                         report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
                     }

@@ -89,7 +89,8 @@ def test_masses_of_a_row_sum_to_its_heads():
 
 
 def test_empty_rows_and_unseen_keys():
-    """Rows without a key (infinite lse) give nothing; NaN keys past the end stay out."""
+    """Rows with lse +inf give nothing, the lse -inf of a row infinite masses to the keys that it sees and no others;
+    NaN keys past the end stay out."""
     q, k, mass, lens, _ = make(2, 3, 4, 2, 64, [100, 128])
     k[0, 103:], k[1, 131:] = math.nan, math.inf
     mass[:, :, 131:] = math.nan
@@ -99,8 +100,11 @@ def test_empty_rows_and_unseen_keys():
     eviction.key_mass(q, k, lse, mass, lens, 0.125)
     want, tol = oracle.mass(q, k, lse, keep, [100, 128], 0.125)
     live = tol > 0
-    assert ((mass.double().cpu() - want).abs() <= 1.05 * tol)[live].all()
+    got, infinite = mass.double().cpu(), want == math.inf
+    assert torch.equal(got == math.inf, infinite)
+    assert ((got - want).abs() <= 1.05 * tol)[live & ~infinite].all()
     assert torch.equal(mass.cpu()[~live].isnan(), keep.cpu()[~live].isnan())
+    assert (mass[0, :, :102] == math.inf).all() and mass[0, :, 102].isfinite().all()
 
 
 def test_mass_refusals():

@@ -110,7 +110,7 @@ def mass(q, k, lse, old, lengths, scale, rows=None, counts=None, decay=1.0, tabl
             m = n if context_only else n + i + 1
             for h in range(H):
                 x = lse[b, r, h]
-                if x.isinf():
+                if x == math.inf:
                     continue
                 g = h * G // H
                 p = torch.exp(kb[:m, g] @ q[b, r, h] * scale - x)
