@@ -17,13 +17,13 @@ from . import _lib
 from .tree import _TYPES, _check_rows, _i32, _refuse, _run, _run_in_workspace, fill_cache
 
 
-def _plane(t, dtype, batch, heads, rows, strides, what):
+def _plane(t, dtype, device, batch, heads, rows, strides, what):
     """Pointer of a [B, Hkv, rows] plane (``rows``: at least so many), its strides into ``strides``."""
     shape = t.shape
     st = t.stride()
-    if not (t.is_cuda and t.dtype == dtype and len(shape) == 3 and shape[0] == batch and shape[1] == heads and
+    if not (t.device == device and t.dtype == dtype and len(shape) == 3 and shape[0] == batch and shape[1] == heads and
             shape[2] >= rows and st[2] == 1):
-        _refuse('%s must be %s [%d, %d, >= %d] on CUDA with contiguous rows', what, dtype, batch, heads, rows)
+        _refuse('%s must be %s [%d, %d, >= %d] on %s with contiguous rows', what, dtype, batch, heads, rows, device)
     strides[0], strides[1] = st[0], st[1]
     return t.data_ptr()
 
@@ -59,14 +59,14 @@ def key_mass(q, k, lse, mass, lengths, scale, rows=None, counts=None, decay=1.0,
     fill_cache(a.cache, k, k, block_tables, batch)
     kv_heads = k.shape[2]
     a.batch, a.nodes, a.heads, a.kv_heads, a.dim, a.type = batch, t, heads, kv_heads, dim, _TYPES[kind]
-    a.q, a.lse, a.lengths = q.data_ptr(), lse.data_ptr(), _i32(lengths, (batch,), 'lengths')
+    a.q, a.lse, a.lengths = q.data_ptr(), lse.data_ptr(), _i32(lengths, (batch,), dev, 'lengths')
     x = a.q_stride
     x[0], x[1], x[2] = qs[:3]
     if rows is not None:
-        a.rows = _i32(rows, (batch, t), 'rows')
+        a.rows = _i32(rows, (batch, t), dev, 'rows')
     if counts is not None:
-        a.counts = _i32(counts, (batch,), 'counts')
-    a.mass = _plane(mass, torch.float32, batch, kv_heads, 0, a.mass_stride, 'mass')
+        a.counts = _i32(counts, (batch,), dev, 'counts')
+    a.mass = _plane(mass, torch.float32, dev, batch, kv_heads, 0, a.mass_stride, 'mass')
     a.mass_rows, a.context_only, a.scale, a.decay, a.wait_limit_ns = mass.shape[2], bool(context_only), scale, decay, wait_limit_ns
     _run(dev, _lib.load().slimkv_key_mass, byref(a))
     return mass
@@ -95,12 +95,22 @@ def evict(k, v, mass, positions, lengths, keep, sinks=0, recent=0, block_tables=
         _refuse('keep must be positive')
     if out is None:
         # Each (sequence, head) a contiguous run of rows.
-        out_k = torch.empty_strided((batch, keep, heads, dim), (heads * keep * dim, dim, keep * dim, 1), dtype=k.dtype, device=dev)
-        out_v = torch.empty_strided((batch, keep, heads, dim_v), (heads * keep * dim_v, dim_v, keep * dim_v, 1), dtype=k.dtype,
-                                    device=dev)
-        plane = (batch, heads, keep), (heads * keep, keep, 1)
+        rows = heads * keep
+        out_k = torch.empty_strided((batch, keep, heads, dim), (rows * dim, dim, keep * dim, 1), dtype=k.dtype, device=dev)
+        out_v = torch.empty_strided((batch, keep, heads, dim_v), (rows * dim_v, dim_v, keep * dim_v, 1), dtype=k.dtype, device=dev)
+        plane = (batch, heads, keep), (rows, keep, 1)
         out_mass = torch.empty_strided(*plane, dtype=torch.float32, device=dev)
         out_positions = None if positions is None else torch.empty_strided(*plane, dtype=torch.int32, device=dev)
+        c = a.dst
+        c.k, c.v, c.rows = out_k.data_ptr(), out_v.data_ptr(), keep
+        x, y = c.k_stride, c.v_stride
+        x[0], x[1], x[2] = rows * dim, dim, keep * dim
+        y[0], y[1], y[2] = rows * dim_v, dim_v, keep * dim_v
+        a.out_mass = out_mass.data_ptr()
+        a.out_mass_stride[0], a.out_mass_stride[1] = rows, keep
+        if positions is not None:
+            a.out_positions = out_positions.data_ptr()
+            a.out_positions_stride[0], a.out_positions_stride[1] = rows, keep
     else:
         out_k, out_v, out_mass, out_positions = out
         _check_rows(out_k, out_v, 4)
@@ -109,15 +119,16 @@ def evict(k, v, mass, positions, lengths, keep, sinks=0, recent=0, block_tables=
             _refuse('out caches must be like the caches, with keep rows')
         if (positions is None) != (out_positions is None):
             _refuse('positions and their output go together')
-    fill_cache(a.dst, out_k, out_v, None, batch)
+        fill_cache(a.dst, out_k, out_v, None, batch)
+        a.out_mass = _plane(out_mass, torch.float32, dev, batch, heads, keep, a.out_mass_stride, 'out mass')
+        if positions is not None:
+            a.out_positions = _plane(out_positions, torch.int32, dev, batch, heads, keep, a.out_positions_stride, 'out positions')
     a.batch, a.kv_heads, a.dim_qk, a.dim_v, a.elem_bytes = batch, heads, dim, dim_v, k.element_size()
-    a.mass, a.mass_rows = _plane(mass, torch.float32, batch, heads, 0, a.mass_stride, 'mass'), mass.shape[2]
-    a.out_mass = _plane(out_mass, torch.float32, batch, heads, keep, a.out_mass_stride, 'out mass')
+    a.mass, a.mass_rows = _plane(mass, torch.float32, dev, batch, heads, 0, a.mass_stride, 'mass'), mass.shape[2]
     if positions is not None:
-        a.positions = _plane(positions, torch.int32, batch, heads, mass.shape[2], a.positions_stride, 'positions')
-        a.out_positions = _plane(out_positions, torch.int32, batch, heads, keep, a.out_positions_stride, 'out positions')
+        a.positions = _plane(positions, torch.int32, dev, batch, heads, mass.shape[2], a.positions_stride, 'positions')
     new_lengths = torch.empty_strided((batch,), (1,), dtype=torch.int32, device=dev)
-    a.lengths, a.new_lengths = _i32(lengths, (batch,), 'lengths'), new_lengths.data_ptr()
+    a.lengths, a.new_lengths = _i32(lengths, (batch,), dev, 'lengths'), new_lengths.data_ptr()
     a.keep, a.sinks, a.recent = keep, sinks, recent
     lib = _lib.load()
     _run_in_workspace(dev, lib.slimkv_evict_workspace_size, lib.slimkv_evict, a)

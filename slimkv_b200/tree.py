@@ -35,9 +35,9 @@ def _refuse(msg, *args):
     raise RuntimeError(msg % args)
 
 
-def _i32(t, shape, what):
-    if not (t.is_cuda and t.dtype == torch.int32 and t.shape == shape and t.is_contiguous()):
-        _refuse('%s must be contiguous int32 %s on CUDA', what, list(shape))
+def _i32(t, shape, device, what):
+    if not (t.device == device and t.dtype == torch.int32 and t.shape == shape and t.is_contiguous()):
+        _refuse('%s must be contiguous int32 %s on %s', what, list(shape), device)
     return t.data_ptr()
 
 
@@ -91,9 +91,9 @@ def fill_cache(c, k, v, block_tables, batch, first=0):
                 _refuse('one cache for each sequence, or one for all')
             x[0] = y[0] = 0
     else:
-        if not (block_tables.is_cuda and block_tables.dtype == torch.int32 and block_tables.dim() == 2 and
+        if not (block_tables.device == k.device and block_tables.dtype == torch.int32 and block_tables.dim() == 2 and
                 block_tables.shape[0] == batch and block_tables.stride(1) == 1):
-            _refuse('block tables must be int32 [B, n] on CUDA')
+            _refuse('block tables must be int32 [B, n] on the caches\' device')
         c.table, c.table_stride = block_tables.data_ptr(), block_tables.stride(0)
         c.table_pages, c.num_pages = block_tables.shape[1], sequences
 
@@ -103,9 +103,9 @@ def tree_masks(parents):
     T]`` int32 (a parent before its children; -1: a root) -> int32 ``[B, T,
     (T + 31) // 32]``, bit i of node t set when t sees i (its ancestors and
     itself)."""
-    if parents.dim() != 2:
-        _refuse('parents must be [B, T]')
-    p = _i32(parents, parents.shape, 'parents')
+    if not (parents.is_cuda and parents.dim() == 2):
+        _refuse('parents must be [B, T] on CUDA')
+    p = _i32(parents, parents.shape, parents.device, 'parents')
     batch, nodes = parents.shape
     out = torch.empty((batch, nodes, (nodes + 31) // 32), dtype=torch.int32, device=parents.device)
     _run(parents.device, _lib.load().slimkv_tree_masks, p, batch, nodes, out.data_ptr())
@@ -149,19 +149,19 @@ def tree_attention(q, k, v, lengths, scale, mask=None, nodes=None, block_tables=
         _refuse('lse must be contiguous fp32 [B, T, H]')
     a.batch, a.nodes, a.heads, a.kv_heads = batch, t, heads, k.shape[2]
     a.dim_qk, a.dim_v, a.type = dim, dim_v, _TYPES[kind]
-    a.q, a.out, a.lse, a.lengths = q.data_ptr(), out.data_ptr(), lse.data_ptr(), _i32(lengths, (batch,), 'lengths')
+    a.q, a.out, a.lse, a.lengths = q.data_ptr(), out.data_ptr(), lse.data_ptr(), _i32(lengths, (batch,), dev, 'lengths')
     x, y = a.q_stride, a.out_stride
     x[0], x[1], x[2] = qs[:3]
     y[0], y[1], y[2] = out.stride()[:3]
     if nodes is not None:
-        a.nodes_len = _i32(nodes, (batch,), 'nodes')
+        a.nodes_len = _i32(nodes, (batch,), dev, 'nodes')
     if mask is not None:
         if context_only:
             _refuse('the nodes\' own rows are not in a context_only cache: no mask')
         many = mask.shape[0] if mask.dim() == 3 else 0
         if many not in (1, batch):
             _refuse('mask must be [B or 1, T, words]')
-        a.mask = _i32(mask, (many, t, (t + 31) // 32), 'mask')
+        a.mask = _i32(mask, (many, t, (t + 31) // 32), dev, 'mask')
         a.mask_stride = mask.stride(0) if many > 1 else 0
     a.context_only, a.scale, a.wait_limit_ns = bool(context_only), scale, wait_limit_ns
     lib = _lib.load()
@@ -188,10 +188,10 @@ def tree_accept(logits, tokens, parents, nodes=None):
         _refuse('tokens must be contiguous int64 [B, T] on the logits\' device')
     a = _lib.TreeAcceptArgs()
     a.batch, a.nodes, a.vocab, a.type = batch, t, vocab, _TYPES[logits.dtype]
-    a.logits, a.tokens, a.parents = logits.data_ptr(), tokens.data_ptr(), _i32(parents, (batch, t), 'parents')
+    a.logits, a.tokens, a.parents = logits.data_ptr(), tokens.data_ptr(), _i32(parents, (batch, t), dev, 'parents')
     a.logits_stride[0], a.logits_stride[1] = logits.stride()[:2]
     if nodes is not None:
-        a.nodes_len = _i32(nodes, (batch,), 'nodes')
+        a.nodes_len = _i32(nodes, (batch,), dev, 'nodes')
     path = torch.empty_strided((batch, t), (t, 1), dtype=torch.int32, device=dev)
     count = torch.empty_strided((batch,), (1,), dtype=torch.int32, device=dev)
     following = torch.empty_strided((batch,), (1,), dtype=torch.int64, device=dev)
@@ -226,8 +226,8 @@ def tree_commit(k, v, lengths, path, count, block_tables=None):
     if first:
         a.k_layer_stride, a.v_layer_stride = k.stride(0), v.stride(0)
     new_lengths = torch.empty_strided((batch,), (1,), dtype=torch.int32, device=dev)
-    a.lengths, a.path, a.count = (_i32(lengths, (batch,), 'lengths'), _i32(path, (batch, t), 'path'),
-                                  _i32(count, (batch,), 'count'))
+    a.lengths, a.path, a.count = (_i32(lengths, (batch,), dev, 'lengths'), _i32(path, (batch, t), dev, 'path'),
+                                  _i32(count, (batch,), dev, 'count'))
     a.new_lengths = new_lengths.data_ptr()
     _run(dev, _lib.load().slimkv_tree_commit, byref(a))
     return new_lengths

@@ -229,3 +229,23 @@ def test_a_bounded_cache_step():
     got = eviction.evict(k, v, mass, positions, new, 40, sinks=4, recent=8)
     same(got, oracle.evict(k, v, mass, positions, new.tolist(), 40, 4, 8))
     assert got[4].tolist() == [40, 40] and (got[3][0, :, -8:].cpu() == torch.arange(55, 63)).all()
+
+
+def test_refusals_of_tensors_elsewhere():
+    """What lies on the CPU (or on another GPU) is refused before a launch."""
+    q, k, mass, lens, _ = make(2, 3, 4, 2, 64, [30, 20])
+    lse = torch.zeros(2, 3, 4, device='cuda')
+    path = torch.zeros(2, 3, dtype=torch.int32, device='cuda')
+    tables = torch.zeros(2, 4, dtype=torch.int32)
+    pages = torch.zeros(8, 16, 2, 64, dtype=BF16, device='cuda')
+    for call in (lambda: eviction.key_mass(q, k, lse, mass.cpu(), lens, 0.1), lambda: eviction.key_mass(q, k, lse, mass, lens.cpu(), 0.1),
+                 lambda: eviction.key_mass(q, k, lse, mass, lens, 0.1, rows=path.cpu()),
+                 lambda: eviction.key_mass(q, k, lse.cpu(), mass, lens, 0.1),
+                 lambda: eviction.evict(k, k, mass.cpu(), None, lens, 8), lambda: eviction.evict(k, k, mass, None, lens.cpu(), 8),
+                 lambda: eviction.evict(k, k, mass, mass.int().cpu(), lens, 8),
+                 lambda: tree.tree_attention(q, k, k, lens.cpu(), 0.1), lambda: tree.tree_attention(q.cpu(), k, k, lens, 0.1),
+                 lambda: tree.tree_attention(q, pages, pages, lens, 0.1, block_tables=tables),
+                 lambda: tree.tree_commit(k, k.clone(), lens, path.cpu(), lens), lambda: tree.tree_commit(k, k.clone(), lens, path, lens.cpu()),
+                 lambda: tree.tree_masks(path.cpu()), lambda: tree.tree_accept(lse, path.long(), path.cpu())):
+        with pytest.raises(RuntimeError):
+            call()
