@@ -28,7 +28,7 @@
 // 195 us = 5.5 TB/s, 16 x 16 over 8k 111 us = 4.9 TB/s, 16 x 64 nodes (256 rows
 // a KV head) over 8k 166 to 172 us = 870 TFLOP/s, one token over 517 rows 13 us.
 // (In calls back to back the last of the three large ones draws the board's
-// 1000 W and runs at 1.65 GHz, 206 us.)
+// 1000 W and runs at 1.65 GHz, 200 to 206 us.)
 //
 // Why 64 keys: S and P of a tile fit 64 tensor-memory columns, so two to four
 // tiles are under way for each row tile next to O (320 + 3 x 64, or 2 x (128 +
