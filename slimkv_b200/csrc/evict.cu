@@ -12,8 +12,8 @@
 //     K, V, mass and position of the listed rows moved, 16 bytes a lane.
 // Bound: HBM, the masses once (later readings come from L2) and each kept row
 // read and written.  Measured: 16 segments of 32k latents cut to 8k (336 MB
-// moved) 76 us in a graph, the selection 20 and the gather 62 alone (5.4 TB/s);
-// two sequences of 1.2k rows cut to 1028, 12.5 us.
+// moved) 74 us in a graph, the selection 20 and the gather 52 alone (6.5 TB/s);
+// two sequences of 1.2k rows cut to 1028, 12.3 us.
 #include <algorithm>
 
 #include "cache_view.cuh"
@@ -238,9 +238,11 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
     __shared__ int64_t from[2][kRows], to[2][kRows];
     const int d0 = blockIdx.x * kRows, g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int kept = min(segment_length(a, b), a.keep), rows = min(kRows, a.keep - d0);
+    const int d = d0 + tid;
+    float mass = 0.f;
+    int position = 0;
     grid_dependency_wait();
     if (tid < rows) {
-        const int d = d0 + tid;
         const bool some = d < kept;
         const int n = some ? a.kept[int64_t(b * a.kv_heads + g) * a.list_rows + d] : 0;
         int64_t ip = 0, op;
@@ -251,16 +253,14 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
         to[0][tid] = in && out ? op * a.out.k_stride[0] + orow * a.out.k_stride[1] + g * a.out.k_stride[2] : -1;
         to[1][tid] = in && out ? op * a.out.v_stride[0] + orow * a.out.v_stride[1] + g * a.out.v_stride[2] : -1;
         if (!in || !out) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
-        if (a.out_mass)
-            a.out_mass[b * a.out_mass_stride[0] + g * a.out_mass_stride[1] + d] =
-                some ? __ldg(a.mass + b * a.mass_stride[0] + g * a.mass_stride[1] + n) : 0.f;
-        if (a.out_positions)
-            a.out_positions[b * a.out_positions_stride[0] + g * a.out_positions_stride[1] + d] =
-                some ? __ldg(a.positions + b * a.positions_stride[0] + g * a.positions_stride[1] + n) : 0;
+        // On their way while the rows move.
+        if (some && a.out_mass) mass = __ldg(a.mass + b * a.mass_stride[0] + g * a.mass_stride[1] + n);
+        if (some && a.out_positions) position = __ldg(a.positions + b * a.positions_stride[0] + g * a.positions_stride[1] + n);
     }
     __syncthreads();
     // 16-byte units of the rows' K and V, kUnits of a thread under way at a time.
-    constexpr int kUnits = 8;
+    // (16 segments of 32k latents in a graph: 5 of them 73.8 us, 8 and 10 74.5.)
+    constexpr int kUnits = 5;
     const int units = a.k_units + a.v_units, total = rows * units;
     // p / units by multiplication: exact while p units < 2^20 (p < kRows units, units <= 181).
     const uint32_t inverse = (1u << 20) / uint32_t(units) + 1u;
@@ -285,6 +285,10 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
 #pragma unroll
         for (int k = 0; k < kUnits; ++k)
             if (dst[k]) __stcs(dst[k], w[k]);
+    }
+    if (tid < rows) {
+        if (a.out_mass) a.out_mass[b * a.out_mass_stride[0] + g * a.out_mass_stride[1] + d] = mass;
+        if (a.out_positions) a.out_positions[b * a.out_positions_stride[0] + g * a.out_positions_stride[1] + d] = position;
     }
 }
 
