@@ -234,7 +234,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2) evict_select_kernel(EvictAr
 }
 
 __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs a) {
-    // Byte offsets of the rows: K, V (from -1: zeros, to -1: nothing).
+    // Byte offsets of the rows: K, V (from -1: zeros, to -1: nothing).  A row of a page outside
+    // the pool is read from the page that cache_row puts in its place, never written there.
     __shared__ int64_t from[2][kRows], to[2][kRows];
     const int d0 = blockIdx.x * kRows, g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int kept = min(segment_length(a, b), a.keep), rows = min(kRows, a.keep - d0);
@@ -250,8 +251,8 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
         const bool in = !some || cache_row(a.in, b, n, ip, ir), out = cache_row(a.out, b, d, op, orow);
         from[0][tid] = some ? ip * a.in.k_stride[0] + ir * a.in.k_stride[1] + g * a.in.k_stride[2] : -1;
         from[1][tid] = some ? ip * a.in.v_stride[0] + ir * a.in.v_stride[1] + g * a.in.v_stride[2] : -1;
-        to[0][tid] = in && out ? op * a.out.k_stride[0] + orow * a.out.k_stride[1] + g * a.out.k_stride[2] : -1;
-        to[1][tid] = in && out ? op * a.out.v_stride[0] + orow * a.out.v_stride[1] + g * a.out.v_stride[2] : -1;
+        to[0][tid] = out ? op * a.out.k_stride[0] + orow * a.out.k_stride[1] + g * a.out.k_stride[2] : -1;
+        to[1][tid] = out ? op * a.out.v_stride[0] + orow * a.out.v_stride[1] + g * a.out.v_stride[2] : -1;
         if (!in || !out) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
         // On their way while the rows move.
         if (some && a.out_mass) mass = __ldg(a.mass + b * a.mass_stride[0] + g * a.mass_stride[1] + n);

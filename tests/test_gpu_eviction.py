@@ -249,3 +249,16 @@ def test_refusals_of_tensors_elsewhere():
                  lambda: tree.tree_masks(path.cpu()), lambda: tree.tree_accept(lse, path.long(), path.cpu())):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_evict_reads_a_clamped_page_for_one_outside_the_pool():
+    """It is reported, and every row of the output is written."""
+    pages = torch.randn(6, 16, 2, 64, device='cuda').to(BF16)
+    tables = torch.tensor([[3, -7, 1], [99, 0, 5]], dtype=torch.int32, device='cuda')
+    mass = torch.rand(2, 2, 48, device='cuda')
+    lens = torch.tensor([40, 48], dtype=torch.int32, device='cuda')
+    out = [torch.full((2, 20, 2, 64), 7.0, device='cuda', dtype=BF16) for _ in range(2)] + [torch.full((2, 2, 20), 7.0, device='cuda')]
+    _lib.device_status(clear=True)
+    got = eviction.evict(pages, pages, mass, None, lens, 20, sinks=2, recent=4, block_tables=tables, out=(*out, None))
+    assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH
+    same(got, oracle.evict(pages, pages, mass, None, [40, 48], 20, 2, 4, tables.clamp(0, 5)))
