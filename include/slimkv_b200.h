@@ -731,8 +731,11 @@ SLIMKV_API int slimkv_tree_accept(const slimkv_tree_accept_args* args, void* wor
 /* ------------------------------------------------------------------------
  * Commit of the accepted nodes: cache row lengths[b] + path[b][i] moves to
  * lengths[b] + i for i < count[b], in place, for `layers` caches whose K / V
- * lie layer_stride elements apart, and new_lengths[b] = lengths[b] + count[b].
- * path ascends (a path of slimkv_tree_accept).  elem_bytes 1, 2 or 4;
+ * lie layer_stride elements apart, and new_lengths[b] = lengths[b] + count[b]
+ * (cut to the rows of the cache).  path ascends (a path of slimkv_tree_accept).
+ * An accepted row that its cache cannot hold, or whose old or new place is in a
+ * page outside the pool, does not move and is reported as
+ * SLIMKV_DEVICE_BAD_LENGTH.  elem_bytes 1, 2 or 4;
  * new_lengths must not be lengths.
  * ---------------------------------------------------------------------- */
 typedef struct {

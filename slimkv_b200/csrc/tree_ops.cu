@@ -294,9 +294,11 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(CommitArgs a) {
     const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
     const int len = __ldg(a.lengths + b), want = __ldg(a.count + b);
     const int count = min(max(want, 0), a.nodes);
+    const int64_t cap = cache_capacity(a.cache);
     if (at == 0) {
-        a.new_lengths[b] = len + count;
-        if (want != count || len < 0) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
+        const int64_t end = int64_t(max(len, 0)) + count;
+        a.new_lengths[b] = int(min(end, cap));
+        if (want != count || len < 0 || end > cap) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
     }
     if (at >= int64_t(a.layers) * a.lanes || len < 0) return;
     const int layer = int(at / a.lanes);
@@ -306,7 +308,6 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(CommitArgs a) {
     const int units = is_v ? a.v_units : a.k_units, head = lane / units;
     const int64_t* st = is_v ? a.cache.v_stride : a.cache.k_stride;
     uint8_t* base = (is_v ? a.v + layer * a.v_layer : a.k + layer * a.k_layer) + head * st[2] + int64_t(lane - head * units) * 16;
-    const int64_t cap = cache_capacity(a.cache);
     const int32_t* path = a.path + int64_t(b) * a.nodes;
     for (int i0 = 0; i0 < count; i0 += kCommitRows) {
         uint4 row[kCommitRows];
@@ -314,16 +315,20 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(CommitArgs a) {
 #pragma unroll
         for (int j = 0; j < kCommitRows; ++j) {
             const int i = i0 + j;
-            const int p = i < count ? __ldg(path + i) : i;
+            move[j] = i < count;
+            if (!move[j]) continue;
+            const int p = __ldg(path + i);
             int64_t page;
             int r;
-            move[j] = p != i;
-            if (!move[j]) continue;
-            if (p < i || p >= a.nodes || int64_t(len) + p >= cap || !cache_row(a.cache, b, len + p, page, r)) {
+            // Both the row's place and its source (the same when p == i) have to exist.
+            if (p < i || p >= a.nodes || int64_t(len) + p >= cap || !cache_row(a.cache, b, len + i, page, r) ||
+                !cache_row(a.cache, b, len + p, page, r)) {
                 report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
                 move[j] = false;
                 continue;
             }
+            move[j] = p != i;
+            if (!move[j]) continue;
             row[j] = *reinterpret_cast<const uint4*>(base + page * st[0] + r * st[1]);
         }
 #pragma unroll

@@ -414,3 +414,24 @@ def test_commit_refusals_and_reports():
     before = k.clone()
     tree.tree_commit(k, k.clone(), lens, torch.tensor([[0, 9], [0, 1]], **i32), count)     # a node that the tree has not
     assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH and torch.equal(k, before)
+
+
+def test_commit_reports_rows_without_a_place():
+    """A destination in a page outside the pool, and accepted rows past the cache, moved or not."""
+    i32 = dict(dtype=torch.int32, device='cuda')
+    pages = torch.randn(6, 8, 2, 64, device='cuda').to(BF16)
+    v, before = pages.clone(), pages.clone()
+    _lib.device_status(clear=True)
+    path = torch.tensor([[4, 5, 6, -1, -1, -1, -1]], **i32)
+    new = tree.tree_commit(pages, v, torch.tensor([12], **i32), path, torch.tensor([2], **i32),
+                           block_tables=torch.tensor([[0, 9, 2]], **i32))         # 16 and 17 to 12 and 13, in no page
+    assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH and new.tolist() == [14]
+    assert torch.equal(pages, before) and torch.equal(v, before)
+    new = tree.tree_commit(pages, v, torch.tensor([12], **i32), torch.tensor([[0, 1, -1]], **i32), torch.tensor([2], **i32),
+                           block_tables=torch.tensor([[0, -1, 2]], **i32))        # rows that stay, in no page
+    assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH and new.tolist() == [14]
+    k = pages[:1].contiguous()
+    new = tree.tree_commit(k, k.clone(), torch.tensor([6], **i32), torch.tensor([[0, 1, 2, -1]], **i32), torch.tensor([3], **i32))
+    assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH and new.tolist() == [8]
+    new = tree.tree_commit(k, k.clone(), torch.tensor([6], **i32), torch.tensor([[0, 1, 2, -1]], **i32), torch.tensor([2], **i32))
+    assert _lib.device_status(clear=True) == 0 and new.tolist() == [8]
