@@ -373,6 +373,10 @@ extern "C" int slimkv_evict(const slimkv_evict_args* a, void* workspace, size_t 
     carve(c, a, k);
     if (!workspace || !c.fits() || reinterpret_cast<uintptr_t>(workspace) % 8)
         return fail(SLIMKV_ERR_WORKSPACE, "evict: workspace of %zu bytes needed", c.used);
+    // A block would read a length that another has written.
+    const size_t lengths_bytes = size_t(a->batch) * sizeof(int32_t);
+    if (share_bytes(a->lengths, lengths_bytes, a->new_lengths, lengths_bytes))
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "evict: new_lengths must not be lengths");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // CTAs of a cluster as many (up to 8) as keep their keys in registers.
     int ranks = 1;

@@ -61,6 +61,12 @@ unsigned int* status_word();
 int check_cache(const slimkv_cache& cache, int batch, int dim_k, int dim_v, int elem_bytes, bool need_v,
                 const char* what);
 
+// Whether two arrays have a byte in common (null: no array).
+inline bool share_bytes(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace slimkv

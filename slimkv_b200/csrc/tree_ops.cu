@@ -431,6 +431,10 @@ extern "C" int slimkv_tree_commit(const slimkv_tree_commit_args* a, void* stream
     const int e = a->elem_bytes;
     if (a->k_layer_stride * e % 16 || a->v_layer_stride * e % 16)
         return fail(SLIMKV_ERR_ALIGNMENT, "tree commit: layer strides must be multiples of 16 bytes");
+    // A block would read a length that another has written.
+    const size_t lengths_bytes = size_t(a->batch) * sizeof(int32_t);
+    if (share_bytes(a->lengths, lengths_bytes, a->new_lengths, lengths_bytes))
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree commit: new_lengths must not be lengths");
     CommitArgs k{};
     k.k = static_cast<uint8_t*>(const_cast<void*>(a->cache.k));
     k.v = static_cast<uint8_t*>(const_cast<void*>(a->cache.v));

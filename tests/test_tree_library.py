@@ -143,3 +143,11 @@ def test_masks_refusals():
     lib = _lib.load()
     for args in ((None, 2, 4, P), (P, 2, 4, None), (P, 0, 4, P), (P, 2, 1025, P), (P, 2, 0, P)):
         assert lib.slimkv_tree_masks(*args, None) == INVALID
+
+
+@pytest.mark.parametrize('entry,make,workspace', [('slimkv_tree_commit', commit, ()), ('slimkv_evict', evict, (P, 1 << 20))])
+@pytest.mark.parametrize('apart', [0, 4, -4])
+def test_new_lengths_are_not_the_lengths(entry, make, workspace, apart):
+    """Two sequences' lengths: the arrays are the same, or share one entry."""
+    assert getattr(_lib.load(), entry)(ctypes.byref(make(new_lengths=P + apart)), *workspace, None) == INVALID
+    assert b'new_lengths' in _lib.load().slimkv_last_error()
