@@ -2,6 +2,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <mutex>
 
 namespace slimkv {
@@ -92,6 +93,57 @@ int encode_map_f32_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t 
         return fail(SLIMKV_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled (f32) failed (%d): dims {%llu,%llu,%llu}", int(r),
                     (unsigned long long)d0, (unsigned long long)d1, (unsigned long long)d2);
     return SLIMKV_OK;
+}
+
+Rows cache_rows(const void* at, const int64_t* strides, int64_t width_bytes, int elem_bytes, const slimkv_cache& cache,
+                int batch, int heads, int layers, int64_t layer_stride) {
+    return Rows{at, width_bytes, {layers, cache.table ? cache.num_pages : batch, cache.rows, heads},
+                {layer_stride * elem_bytes, strides[0] * elem_bytes, strides[1] * elem_bytes, strides[2] * elem_bytes}};
+}
+
+namespace {
+
+using Wide = __int128;          // strides are the caller's: no product of them may overflow
+
+// A set of rows with its dimensions (of more than one entry, positive strides) from the widest on.
+struct Sorted {
+    int dims = 0;
+    Wide at, width, n[4], stride[4], span[5];       // span[d]: bytes from the first to the last of dimensions d..
+    explicit Sorted(const Rows& r) : at(reinterpret_cast<uintptr_t>(r.at)), width(r.width) {
+        for (int i = 0; i < 4; ++i) {
+            if (r.n[i] <= 1) continue;
+            const Wide s = r.stride[i];
+            if (s < 0) at += s * (r.n[i] - 1);
+            int d = dims++;
+            for (; d > 0 && stride[d - 1] < (s < 0 ? -s : s); --d) { stride[d] = stride[d - 1]; n[d] = n[d - 1]; }
+            stride[d] = s < 0 ? -s : s;
+            n[d] = r.n[i];
+        }
+        span[dims] = width;
+        for (int d = dims - 1; d >= 0; --d) span[d] = span[d + 1] + stride[d] * (n[d] - 1);
+    }
+};
+
+// The dimensions d.. of a and b, b `gap` bytes behind a.
+bool share_from(const Sorted& a, const Sorted& b, int d, Wide gap) {
+    if (gap >= a.span[std::min(d, a.dims)] || -gap >= b.span[std::min(d, b.dims)]) return false;
+    if (d >= a.dims || d >= b.dims) return true;    // (one row against several: taken as shared)
+    const Wide s = a.stride[d];
+    if (s != b.stride[d] || s < a.span[d + 1] || s < b.span[d + 1]) return true;
+    // Entry i of a and j of b are gap - (i - j) s apart: only the two differences that leave
+    // less than s can share bytes.
+    Wide q = gap / s;
+    if (gap % s < 0) --q;
+    for (Wide m = q; m <= q + 1; ++m)
+        if (m > -b.n[d] && m < a.n[d] && share_from(a, b, d + 1, gap - m * s)) return true;
+    return false;
+}
+
+}  // namespace
+
+bool share_rows(const Rows& a, const Rows& b) {
+    const Sorted x(a), y(b);
+    return share_from(x, y, 0, y.at - x.at);
 }
 
 }  // namespace slimkv

@@ -67,6 +67,20 @@ inline bool share_bytes(const void* a, size_t a_bytes, const void* b, size_t b_b
     return a && b && x < y + b_bytes && y < x + a_bytes;
 }
 
+// `width` bytes at every place of a strided array (strides in bytes).
+struct Rows {
+    const void* at;
+    int64_t width;
+    int64_t n[4], stride[4];
+};
+// The K or V rows of a cache (`strides` in elements) in `layers` planes.
+Rows cache_rows(const void* at, const int64_t* strides, int64_t width_bytes, int elem_bytes, const slimkv_cache& cache,
+                int batch, int heads, int layers = 1, int64_t layer_stride = 0);
+// Whether two sets of rows have a byte in common.  Exact where the strides of
+// both agree from the largest on, or where their address ranges are apart; true
+// for the others.
+bool share_rows(const Rows& a, const Rows& b);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace slimkv

@@ -2,6 +2,7 @@
 // slimkv_tree_accept, slimkv_tree_commit): the ancestor words of a tree, its
 // greedy acceptance, and the move of the accepted rows next to the context.
 #include <algorithm>
+#include <cstdlib>
 
 #include "cache_view.cuh"
 #include "host_utils.h"
@@ -435,16 +436,33 @@ extern "C" int slimkv_tree_commit(const slimkv_tree_commit_args* a, void* stream
     const size_t lengths_bytes = size_t(a->batch) * sizeof(int32_t);
     if (share_bytes(a->lengths, lengths_bytes, a->new_lengths, lengths_bytes))
         return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree commit: new_lengths must not be lengths");
+    // K and V may be (parts of) the same rows, which then move once: two threads would each read
+    // what the other has moved.
+    const slimkv_cache& c = a->cache;
+    const Rows k_rows = cache_rows(c.k, c.k_stride, int64_t(a->dim_qk) * e, e, c, a->batch, a->kv_heads, a->layers, a->k_layer_stride);
+    const Rows v_rows = cache_rows(c.v, c.v_stride, int64_t(a->dim_v) * e, e, c, a->batch, a->kv_heads, a->layers, a->v_layer_stride);
+    int64_t k_bytes = k_rows.width, v_bytes = v_rows.width;
+    uint8_t *first = static_cast<uint8_t*>(const_cast<void*>(c.k)), *v = static_cast<uint8_t*>(const_cast<void*>(c.v));
+    if (share_rows(k_rows, v_rows)) {
+        bool same = share_bytes(first, k_bytes, v, v_bytes);
+        uint8_t* end = std::max(first + k_bytes, v + v_bytes);
+        first = std::min(first, v);
+        k_bytes = end - first;
+        v_bytes = 0;
+        for (int i = 0; i < 4; ++i)
+            same = same && (k_rows.n[i] == 1 || (k_rows.stride[i] == v_rows.stride[i] && std::abs(k_rows.stride[i]) >= k_bytes));
+        if (!same) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree commit: K and V must be apart, or (parts of) the same rows");
+    }
     CommitArgs k{};
-    k.k = static_cast<uint8_t*>(const_cast<void*>(a->cache.k));
-    k.v = static_cast<uint8_t*>(const_cast<void*>(a->cache.v));
+    k.k = first;
+    k.v = v;
     k.cache = cache_view(a->cache);
     for (int i = 0; i < 3; ++i) { k.cache.k_stride[i] *= e; k.cache.v_stride[i] *= e; }
     k.k_layer = a->k_layer_stride * e;
     k.v_layer = a->v_layer_stride * e;
     k.kv_heads = a->kv_heads;
-    k.k_units = a->dim_qk * e / 16;
-    k.v_units = a->dim_v * e / 16;
+    k.k_units = int(k_bytes / 16);
+    k.v_units = int(v_bytes / 16);
     k.lanes = a->kv_heads * (k.k_units + k.v_units);
     k.layers = a->layers;
     k.nodes = a->nodes;

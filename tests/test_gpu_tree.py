@@ -435,3 +435,38 @@ def test_commit_reports_rows_without_a_place():
     assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH and new.tolist() == [8]
     new = tree.tree_commit(k, k.clone(), torch.tensor([6], **i32), torch.tensor([[0, 1, 2, -1]], **i32), torch.tensor([2], **i32))
     assert _lib.device_status(clear=True) == 0 and new.tolist() == [8]
+
+
+@pytest.mark.parametrize('form', ['same', 'front', 'back', 'overlap', 'pages', 'planes', 'halves'])
+def test_commit_of_keys_and_values_in_one_buffer(form):
+    """K and V that are (parts of) the same rows move once; those that lie between each other's rows move each."""
+    B, T, cap, G, D = 5, 40, 60, 2, 128
+    rng = random.Random(11)
+    lengths = [rng.randint(0, 20) for _ in range(B)]
+    paths = [[0] + sorted(rng.sample(range(1, T), rng.randint(15, T - 1))) for _ in range(B)]
+    tables = None
+    if form == 'pages':
+        x = torch.randn(B * 4, 15, 2, G, D, device='cuda').to(BF16)
+        tables = torch.randperm(B * 4)[:B * 4].view(B, 4).to(torch.int32).cuda()
+        k, v = x[:, :, 0], x[:, :, 1]
+    elif form == 'planes':
+        x = torch.randn(B, 2, cap, G, D, device='cuda').to(BF16)
+        k, v = x[:, 0], x[:, 1]
+    else:
+        x = torch.randn(B, cap, G, D, device='cuda').to(BF16)
+        k, v = {'same': (x, x), 'front': (x, x[..., :64]), 'back': (x, x[..., 64:]), 'overlap': (x[..., :96], x[..., 32:]),
+                'halves': (x[..., :64], x[..., 64:])}[form]
+    want = x.clone()
+    for b in range(B):
+        for i, p in enumerate(paths[b]):
+            if form == 'pages':
+                (pd, rd), (ps, rs) = (divmod(lengths[b] + j, 15) for j in (i, p))
+                want[tables[b, pd].long(), rd] = x[tables[b, ps].long(), rs]
+            elif form == 'planes':
+                want[b, :, lengths[b] + i] = x[b, :, lengths[b] + p]
+            else:
+                want[b, lengths[b] + i] = x[b, lengths[b] + p]
+    i32 = dict(dtype=torch.int32, device='cuda')
+    tree.tree_commit(k, v, torch.tensor(lengths, **i32), torch.tensor([p + [-1] * (T - len(p)) for p in paths], **i32),
+                     torch.tensor([len(p) for p in paths], **i32), block_tables=tables)
+    assert torch.equal(x, want) and _lib.device_status() == 0

@@ -151,3 +151,15 @@ def test_new_lengths_are_not_the_lengths(entry, make, workspace, apart):
     """Two sequences' lengths: the arrays are the same, or share one entry."""
     assert getattr(_lib.load(), entry)(ctypes.byref(make(new_lengths=P + apart)), *workspace, None) == INVALID
     assert b'new_lengths' in _lib.load().slimkv_last_error()
+
+
+@pytest.mark.parametrize('change', [
+    dict(cache__v=P + 128),                                     # V a head of K's further on
+    dict(cache__v=P + 2 * 64 * 2),                              # a row further on
+    dict(cache__v=P + 64 * 2 * 64 * 2),                         # a sequence further on
+    dict(cache__v_stride__x1=64),                               # the same place in another order
+    dict(cache__v=P + 64, dim_v=96),                            # V past the end of K's head, into the next
+    dict(layers=2, k_layer_stride=2 * 64 * 2 * 64, v_layer_stride=64 * 2 * 64)])
+def test_commit_refuses_keys_and_values_that_share_rows_in_part(change):
+    assert _lib.load().slimkv_tree_commit(ctypes.byref(commit(**dict(dict(new_lengths=2 * P), **change))), None) == INVALID
+    assert b'K and V' in _lib.load().slimkv_last_error()
