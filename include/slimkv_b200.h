@@ -736,8 +736,8 @@ SLIMKV_API int slimkv_tree_accept(const slimkv_tree_accept_args* args, void* wor
  * An accepted row that its cache cannot hold, or whose old or new place is in a
  * page outside the pool, does not move and is reported as
  * SLIMKV_DEVICE_BAD_LENGTH.  K and V are apart or (parts of) the same rows.
- * elem_bytes 1, 2 or 4;
- * new_lengths must not be lengths.
+ * Each sequence has rows of its own (no sequence stride of 0).  elem_bytes 1, 2
+ * or 4; new_lengths must not be lengths.
  * ---------------------------------------------------------------------- */
 typedef struct {
     int layers, batch, nodes, kv_heads, dim_qk, dim_v, elem_bytes;

@@ -432,6 +432,8 @@ extern "C" int slimkv_tree_commit(const slimkv_tree_commit_args* a, void* stream
     const int e = a->elem_bytes;
     if (a->k_layer_stride * e % 16 || a->v_layer_stride * e % 16)
         return fail(SLIMKV_ERR_ALIGNMENT, "tree commit: layer strides must be multiples of 16 bytes");
+    if (a->batch > 1 && !a->cache.table && (a->cache.k_stride[0] == 0 || a->cache.v_stride[0] == 0))
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree commit: one cache for each sequence, none shared by the batch");
     // A block would read a length that another has written.
     const size_t lengths_bytes = size_t(a->batch) * sizeof(int32_t);
     if (share_bytes(a->lengths, lengths_bytes, a->new_lengths, lengths_bytes))

@@ -163,3 +163,11 @@ def test_new_lengths_are_not_the_lengths(entry, make, workspace, apart):
 def test_commit_refuses_keys_and_values_that_share_rows_in_part(change):
     assert _lib.load().slimkv_tree_commit(ctypes.byref(commit(**dict(dict(new_lengths=2 * P), **change))), None) == INVALID
     assert b'K and V' in _lib.load().slimkv_last_error()
+
+
+@pytest.mark.parametrize('which', ['k', 'v'])
+def test_commit_refuses_a_cache_shared_by_the_batch(which):
+    """Every sequence would move the same rows."""
+    a = commit(new_lengths=2 * P, cache__v=64 * P, **{f'cache__{which}_stride__x0': 0})
+    assert _lib.load().slimkv_tree_commit(ctypes.byref(a), None) == INVALID
+    assert b'each sequence' in _lib.load().slimkv_last_error()
