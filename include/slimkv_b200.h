@@ -792,8 +792,8 @@ SLIMKV_API int slimkv_key_mass(const slimkv_key_mass_args* args, void* stream);
  * there to `keep` are zeroed.  The masses move along into out_mass (nullable),
  * positions (int32) into out_positions (both or neither).  new_lengths[b] =
  * min(lengths[b], keep).
- * sinks + recent <= keep.  The output must not overlap the input, nor
- * new_lengths be lengths.
+ * sinks + recent <= keep.  The output must not overlap the input (any row that
+ * the caches and masses hold, used or not), nor new_lengths be lengths.
  * elem_bytes 1, 2 or 4; mass strides {batch, head} elements, mass_rows long.
  * ---------------------------------------------------------------------- */
 typedef struct {

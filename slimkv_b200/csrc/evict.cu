@@ -308,6 +308,25 @@ int check_evict(const slimkv_evict_args* a) {
     return SLIMKV_OK;
 }
 
+// Rows are read while others are written, so no output row may lie over an input row (`rows` to a segment).
+bool output_shares_input(const slimkv_evict_args* a, int rows) {
+    const int e = a->elem_bytes;
+    slimkv_cache in = a->in, out = a->out;
+    if (!in.table) in.rows = rows;
+    if (!out.table) out.rows = a->keep;
+    auto part = [&](const slimkv_cache& c, bool is_v) {
+        return cache_rows(is_v ? c.v : c.k, is_v ? c.v_stride : c.k_stride, int64_t(is_v ? a->dim_v : a->dim_qk) * e, e, c, a->batch, a->kv_heads);
+    };
+    auto plane = [&](const void* at, const int64_t* strides, int n) {
+        return Rows{at, int64_t(n) * 4, {1, 1, a->batch, a->kv_heads}, {0, 0, strides[0] * 4, strides[1] * 4}};
+    };
+    for (bool o : {false, true})
+        for (bool i : {false, true})
+            if (share_rows(part(out, o), part(in, i))) return true;
+    return (a->out_mass && share_rows(plane(a->out_mass, a->out_mass_stride, a->keep), plane(a->mass, a->mass_stride, rows))) ||
+           (a->positions && share_rows(plane(a->out_positions, a->out_positions_stride, a->keep), plane(a->positions, a->positions_stride, rows)));
+}
+
 void carve(Carver& c, const slimkv_evict_args* a, EvictArgs& k) {
     k.list_rows = std::min(evict_rows(a), a->keep);
     k.kept = c.take<int32_t>(size_t(a->batch) * a->kv_heads * k.list_rows);
@@ -377,6 +396,8 @@ extern "C" int slimkv_evict(const slimkv_evict_args* a, void* workspace, size_t 
     const size_t lengths_bytes = size_t(a->batch) * sizeof(int32_t);
     if (share_bytes(a->lengths, lengths_bytes, a->new_lengths, lengths_bytes))
         return fail(SLIMKV_ERR_INVALID_ARGUMENT, "evict: new_lengths must not be lengths");
+    if (output_shares_input(a, k.rows))
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "evict: the output must not overlap the input");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // CTAs of a cluster as many (up to 8) as keep their keys in registers.
     int ranks = 1;

@@ -262,3 +262,34 @@ def test_evict_reads_a_clamped_page_for_one_outside_the_pool():
     got = eviction.evict(pages, pages, mass, None, lens, 20, sinks=2, recent=4, block_tables=tables, out=(*out, None))
     assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH
     same(got, oracle.evict(pages, pages, mass, None, [40, 48], 20, 2, 4, tables.clamp(0, 5)))
+
+
+@pytest.mark.parametrize('form', ['planes', 'behind', 'sides', 'before'])
+def test_evict_within_one_buffer(form):
+    """Outputs between or behind the input's rows, none over them."""
+    n, keep = 300, 100
+    k, v, mass, out = {
+        # Two caches of each sequence side by side, their masses too.
+        'planes': lambda x, m: (x[:, 0], x[:, 1], m[:, 0], (x[:, 2], x[:, 3], m[:, 1], None)),
+        # The rows behind the input's.
+        'behind': lambda x, m: (x[:, 0, :n], x[:, 1, :n], m[:, 0, :, :n], (x[:, 0, n:], x[:, 1, n:], m[:, 0, :, n:], None)),
+        # Input and output in the halves of each row.
+        'sides': lambda x, m: (x[:, 0, ..., :32], x[:, 1, ..., :32], m[:, 0], (x[:, 0, ..., 32:], x[:, 1, ..., 32:], m[:, 1], None)),
+        'before': lambda x, m: (x[1:, 0], x[1:, 1], m[1:, 0], (x[:1, 0], x[:1, 1], m[:1, 0], None))}[form](
+            torch.randn(2, 4, 500, 3, 64, device='cuda').to(BF16), torch.rand(2, 2, 3, 500, device='cuda'))
+    B = k.shape[0]
+    lengths = [n, 250][:B]
+    lens = torch.tensor(lengths, dtype=torch.int32, device='cuda')
+    want = oracle.evict(k.clone(), v.clone(), mass.clone(), None, lengths, keep, 4, 16)
+    got = eviction.evict(k, v, mass, None, lens, keep, sinks=4, recent=16, out=out)
+    same((got[0][:, :keep], got[1][:, :keep], got[2][..., :keep], None, got[4]), want)
+
+
+def test_evict_refuses_outputs_over_their_inputs():
+    k, v = (torch.randn(2, 300, 2, 64, device='cuda').to(BF16) for _ in range(2))
+    mass, spare = torch.rand(2, 2, 300, device='cuda'), torch.rand(2, 2, 300, device='cuda')
+    lens = torch.tensor([300, 250], dtype=torch.int32, device='cuda')
+    for out in ((k[:, 4:], v.clone(), spare, None), (k.clone(), v[:, 299 - 100:], spare, None), (v[:, 7:], k.clone(), spare, None),
+                (k.clone(), v.clone(), mass[..., 100:], None)):
+        with pytest.raises(RuntimeError):
+            eviction.evict(k, v, mass, None, lens, 100, out=out)

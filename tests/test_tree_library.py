@@ -171,3 +171,20 @@ def test_commit_refuses_a_cache_shared_by_the_batch(which):
     a = commit(new_lengths=2 * P, cache__v=64 * P, **{f'cache__{which}_stride__x0': 0})
     assert _lib.load().slimkv_tree_commit(ctypes.byref(a), None) == INVALID
     assert b'each sequence' in _lib.load().slimkv_last_error()
+
+
+I = 16 * P      # where an input lies
+
+
+@pytest.mark.parametrize('change', [
+    dict(dst__k=I + 2 * 64 * 2 * 4),                            # the input from its fourth row on
+    dict(dst__v=I + 2 * 64 * 2 * 63),                           # from its last row on
+    dict(dst__k=I - 2 * 64 * 2 * 31),                           # up to its first row
+    dict(dst__k=I + 64 * 2 * 64 * 2),                           # from its second sequence on
+    dict(dst__k_stride__x1=64, dst__k_stride__x2=64 * 64, dst__k=I + 64 * 2 * 64 * 2),      # the same in another order
+    dict(out_mass=I + 4 * 63), dict(out_mass=I - 4 * 31), dict(positions=I, out_positions=I + 4 * 32)])
+def test_evict_refuses_an_output_over_its_input(change):
+    far = dict(src__k=I, src__v=I, mass=I, dst__k=4 * I, dst__v=8 * I, out_mass=12 * I, new_lengths=16 * I)
+    a = evict(**dict(far, **change))
+    assert _lib.load().slimkv_evict(ctypes.byref(a), P, 1 << 20, None) == INVALID
+    assert b'overlap' in _lib.load().slimkv_last_error()
