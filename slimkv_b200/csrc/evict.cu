@@ -396,6 +396,10 @@ extern "C" int slimkv_evict(const slimkv_evict_args* a, void* workspace, size_t 
     const size_t lengths_bytes = size_t(a->batch) * sizeof(int32_t);
     if (share_bytes(a->lengths, lengths_bytes, a->new_lengths, lengths_bytes))
         return fail(SLIMKV_ERR_INVALID_ARGUMENT, "evict: new_lengths must not be lengths");
+    const int64_t *ks = a->out.k_stride, *vs = a->out.v_stride;
+    if (!a->out.table && ((a->batch > 1 && (ks[0] == 0 || vs[0] == 0)) || (a->keep > 1 && (ks[1] == 0 || vs[1] == 0)) ||
+                          (a->kv_heads > 1 && (ks[2] == 0 || vs[2] == 0))))
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "evict: each output row needs its own place (no stride of 0)");
     if (output_shares_input(a, k.rows))
         return fail(SLIMKV_ERR_INVALID_ARGUMENT, "evict: the output must not overlap the input");
     cudaStream_t st = static_cast<cudaStream_t>(stream);

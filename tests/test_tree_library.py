@@ -188,3 +188,12 @@ def test_evict_refuses_an_output_over_its_input(change):
     a = evict(**dict(far, **change))
     assert _lib.load().slimkv_evict(ctypes.byref(a), P, 1 << 20, None) == INVALID
     assert b'overlap' in _lib.load().slimkv_last_error()
+
+
+@pytest.mark.parametrize('which', ['k', 'v'])
+@pytest.mark.parametrize('dim', [0, 1, 2])
+def test_evict_refuses_output_rows_in_one_place(which, dim):
+    a = evict(src__k=I, src__v=I, mass=I, dst__k=4 * I, dst__v=8 * I, out_mass=12 * I, new_lengths=16 * I,
+              **{f'dst__{which}_stride__x{dim}': 0})
+    assert _lib.load().slimkv_evict(ctypes.byref(a), P, 1 << 20, None) == INVALID
+    assert b'own place' in _lib.load().slimkv_last_error()
