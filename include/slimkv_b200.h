@@ -671,7 +671,9 @@ SLIMKV_API int slimkv_tree_masks(const int32_t* parents, int batch, int nodes, i
  * context_only: the cache holds no rows of the nodes; every node sees the
  * context.  A row that sees no key gets zero output and lse -inf.  What a key
  * or value that a row does not see holds (infinities and NaN too) does not
- * reach that row.
+ * reach that row.  Scores, sums and lse are fp32; a probability is rounded to
+ * the tensors' type once (in fp16 by at most 2^-32 of the row's largest where
+ * it is that small), and the output once.
  * q [batch][nodes][heads][dim_qk], out [batch][nodes][heads][dim_v], element
  * strides {batch, node, head}, type bf16 or fp16 like the cache; lse fp32
  * [batch][nodes][heads] contiguous, natural log.  mask: int32, words of node t

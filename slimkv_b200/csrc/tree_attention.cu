@@ -10,8 +10,9 @@
 //   S [128 rows x 64 keys] = Q . K^T,   O [128 rows x dim_v] += P . V
 // with tcgen05 (fp32 accumulators in TMEM; P = 2^(s - m) written back to TMEM
 // in the inputs' 16-bit type as the A operand of the second product, which
-// costs about what rounding the output costs; the row sums stay in fp32
-// before that rounding, so lse keeps fp32 accuracy).
+// costs about what rounding the output costs (1.25 to 1.4 times the error of a
+// rounded fp32 result in all); the row sums stay in fp32 before that rounding,
+// so lse keeps fp32 accuracy).
 //
 // Work: a unit is one 64-key tile of one (sequence, KV head, group of NQ row
 // tiles) segment: the context rows, then the nodes' own rows, of which each
@@ -56,6 +57,12 @@ constexpr uint32_t kChunk = kKeys * 128;         // [64 keys x 64]
 constexpr int kMaxRing = 12;
 constexpr int kMaxChunks = 5;                    // dims <= 320
 constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a row's maximum grows by more than 2^8
+// P = 2^(s - m) with m this far below the row's maximum.  Of fp16's exponents P then uses those
+// up to 2^15 (with the 2^8 above), and what it loses below its smallest number is 2^-32 of the
+// largest probability for each key (2^-25 with m at the maximum, up to 0.4 % of the weight of
+// 131,000 keys behind one dominant one); bf16 has fp32's exponents.
+template <bool kHalf>
+constexpr float kDownLog2 = kHalf ? 7.f : 0.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -544,7 +551,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
             const bool live = r < J.tile_rows && t < w.s.nodes;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const int32_t* words = J.mask ? J.mask + w.b * J.mask_stride + int64_t(min(t, J.nodes - 1)) * J.words : nullptr;
-            float m_run = -INFINITY, l_run = 0.f;
+            float m_run = -INFINITY, l_run = 0.f;               // the exponent m taken out, and the sum of P
             for (int tile = w.t0; tile < w.t1; ++tile, ++i) {
                 const bool masked = needs_fix(w.s, tile);
                 uint32_t seen[kCols / 32];                      // which of its keys the row sees
@@ -583,7 +590,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 mx *= J.scale_log2;                             // scale > 0
                 // Two threads of a row: all have read this tile's S when they pass here, so P may
                 // go over it.
-                const bool more = live && mx > m_run + kLazyLog2;
+                const bool more = live && mx > m_run + (kLazyLog2 + kDownLog2<kHalf>);
                 const bool grown = kHalves == 2 ? any_of_row_tile(1 + qt, more) : __any_sync(0xffffffffu, more);
                 const bool fix = qt == 0 && masked;
                 // (A ring of more V slots than S buffers: the slot's last tile is over, S(i) came after it.)
@@ -594,9 +601,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
                 if (grown) {
                     mx = over_row(mx, [](float a, float b) { return fmaxf(a, b); });
                     float alpha = 1.f;
-                    if (mx > m_run + kLazyLog2) {
-                        alpha = m_run == -INFINITY ? 1.f : exp2f(m_run - mx);
-                        m_run = mx;
+                    if (mx > m_run + (kLazyLog2 + kDownLog2<kHalf>)) {
+                        const float m = mx - kDownLog2<kHalf>;
+                        alpha = m_run == -INFINITY ? 1.f : exp2f(m_run - m);
+                        m_run = m;
                         l_run *= alpha;
                     }
                     if (ok && tile > w.t0 && __any_sync(0xffffffffu, alpha != 1.f)) {

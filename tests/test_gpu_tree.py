@@ -470,3 +470,37 @@ def test_commit_of_keys_and_values_in_one_buffer(form):
     tree.tree_commit(k, v, torch.tensor(lengths, **i32), torch.tensor([p + [-1] * (T - len(p)) for p in paths], **i32),
                      torch.tensor([len(p) for p in paths], **i32), block_tables=tables)
     assert torch.equal(x, want) and _lib.device_status() == 0
+
+
+@pytest.mark.parametrize('T,G', [(1, 8), (5, 8), (40, 8)])
+@pytest.mark.parametrize('dtype', [FP16, BF16])
+def test_many_small_probabilities_behind_a_dominant_one(T, G, dtype):
+    """One key 17.5 to 20 nats above thousands: their weight of some 2^-26 each does not get lost.  The values' bound is
+    the oracle's with a probability's fp16 rounding below 2^-32 of the largest (not 2^-25)."""
+    n, D, H, B = 4000, 64, 8, 16
+    q = torch.zeros(B, T, H, D, device='cuda', dtype=dtype)
+    q[..., 0] = 8
+    k = torch.zeros(1, n, G, D, device='cuda', dtype=dtype)
+    k[..., 0] = -torch.empty(1, n, G, device='cuda').uniform_(17.5, 20)
+    k[:, 0] = 0
+    v = torch.rand(1, n, G, D, device='cuda').to(dtype)
+    v[:, 0] = 0
+    lens = torch.full((B,), n, dtype=torch.int32, device='cuda')
+    got = tree.tree_attention(q, k, v, lens, 0.125, context_only=True)
+    out, lse, tol, tol_lse = oracle.attention(q[:1, :1], k, v, [n], 0.125, context_only=True)
+    if dtype == FP16:
+        tol = tol - n * (2.0 ** -25 - 2.0 ** -32) * v.double().cpu()[0].amax(0)[torch.arange(H) * G // H]
+    for b in range(0, B, 5):
+        for t in range(T):
+            oracle.check_attention((got[0][b:b + 1, t:t + 1], got[1][b:b + 1, t:t + 1]), (out, lse, tol, tol_lse))
+
+
+@pytest.mark.parametrize('step', [5.4, 5.6, 11.0])
+@pytest.mark.parametrize('T', [3, 40])
+def test_fp16_probabilities_above_the_running_maximum(T, step):
+    """Maxima that grow by a little less and more than 2^8 and 2^15 from one key tile to the next."""
+    q, k, v, lens, _ = make(1, T, 8, 2, 64, [700], dtype=FP16)
+    q.zero_()
+    q[..., 0] = 8
+    k[:, :700 + T, :, 0] = (torch.arange(700 + T, device='cuda') // 64 * step - 30)[None, :, None].to(FP16)
+    run(q, k, v, lens, scale=0.125)
