@@ -127,21 +127,31 @@ struct AcceptArgs {
     int32_t* count;
     int64_t* next;
     uint64_t* best;             // [batch][nodes][splits]
+    // The walk with its argmaxes ends after max_steps nodes and leaves the node it would go on
+    // with (-1: it is over) and the steps taken; null: no such walk comes before.
+    int max_steps;
+    int2* resume;               // [batch]
 };
 
 constexpr int kScanThreads = 256;
 
-// Every node's argmax, its vocabulary split over gridDim.x blocks.
+// Every node's argmax, its vocabulary split over gridDim.x blocks; after a walk
+// that stopped, of the nodes from its last on (children come after their parents).
 template <typename T>
 __global__ void __launch_bounds__(kScanThreads) accept_scan_kernel(AcceptArgs a) {
     __shared__ ScanScratch<kScanThreads> scratch;
     const int t = blockIdx.y, b = blockIdx.z;
+    grid_launch_dependents();               // the walk over the argmaxes, which waits for this grid
+    if (a.resume) {
+        grid_dependency_wait();
+        const int from = a.resume[b].x;
+        if (from < 0 || t < from) return;
+    }
     if (a.nodes_len && t >= __ldg(a.nodes_len + b)) return;
     const T* row = static_cast<const T*>(a.logits) + b * a.stride_batch + t * a.stride_node;
     const int lo = int(int64_t(a.vocab) * blockIdx.x / a.splits), hi = int(int64_t(a.vocab) * (blockIdx.x + 1) / a.splits);
     const uint64_t best = scan_row<T, kScanThreads>(row, lo, hi, &scratch);
     if (threadIdx.x == 0) a.best[(int64_t(b) * a.nodes + t) * a.splits + blockIdx.x] = best;
-    grid_launch_dependents();
 }
 
 // The walk over every node's argmax, in shared memory: a block per sequence
@@ -159,7 +169,9 @@ __global__ void __launch_bounds__(kWalkThreads) accept_walk_kernel(AcceptArgs a)
         tokens[i] = token >= 0 && token < a.vocab ? int(token) : -1;
     }
     grid_dependency_wait();
-    for (int i = tid; i < n; i += kWalkThreads) {
+    const int2 start = a.resume ? a.resume[b] : make_int2(n > 0 ? 0 : -1, 0);
+    if (a.resume && start.x < 0) return;                // that walk has written everything
+    for (int i = max(start.x, 0) + tid; i < n; i += kWalkThreads) {
         uint64_t top = 0;
         for (int k = 0; k < a.splits; ++k) top = max_u64(top, a.best[(int64_t(b) * a.nodes + i) * a.splits + k]);
         best[i] = int(~uint32_t(top));
@@ -167,7 +179,7 @@ __global__ void __launch_bounds__(kWalkThreads) accept_walk_kernel(AcceptArgs a)
     __syncthreads();
     if (tid >= 32) return;
     int32_t* path = a.path + int64_t(b) * a.nodes;
-    int cur = n > 0 ? 0 : -1, len = 0, next = -1;
+    int cur = start.x, len = start.y, next = -1;
     while (cur >= 0) {
         if (lane == 0) path[len] = cur;
         ++len;
@@ -190,7 +202,8 @@ __global__ void __launch_bounds__(kWalkThreads) accept_walk_kernel(AcceptArgs a)
 // The walk with each node's argmax taken when the walk gets there: a cluster of
 // CTAs per sequence, each scanning its part of the vocabulary, their results
 // exchanged over distributed shared memory.  Reads the logits of the accepted
-// path alone; a step is one pass over V / 8 logits and one cluster barrier.
+// path alone; a step is one pass over V / 8 logits and one cluster barrier.  After
+// max_steps nodes it leaves the rest to the two kernels above.
 constexpr int kPathCtas = 8, kPathThreads = 512;
 
 template <typename T>
@@ -214,7 +227,8 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
     int cur = n > 0 ? 0 : -1, len = 0;
     int64_t next = -1;
     cluster_wait();
-    while (cur >= 0) {
+    if (a.resume) grid_launch_dependents();
+    while (cur >= 0 && len < a.max_steps) {
         const int parity = len & 1;
         if (rank == 0 && tid == 0) path[len] = cur;
         ++len;
@@ -233,7 +247,8 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
         __syncthreads();
         cur = child[parity] < kMaxNodes ? child[parity] : -1;
     }
-    if (rank == 0) {
+    if (rank == 0 && tid == 0 && a.resume) a.resume[b] = make_int2(cur, len);
+    if (rank == 0 && cur < 0) {
         for (int i = len + tid; i < a.nodes; i += kPathThreads) path[i] = -1;
         if (tid == 0) {
             a.count[b] = len;
@@ -243,16 +258,32 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
     cluster_sync();                                     // no CTA leaves while another may still store to it
 }
 
-// Scanning every node reads all the logits, the walk with its argmaxes takes 2
-// us a step.  Measured (bf16, logits up to L2's size read again from there, as
-// after the product that wrote them; scan / walk): 1 x 8 nodes of 128256 logits
-// 6.1 / 10.6 us, 1 x 64 (16 MB) 9.2 / 17.2, 16 x 8 (33 MB) 9.7 / 11.6, 16 x 16
-// (66 MB) 12.4 / 14.6, 64 x 16 of 32000 (66 MB) 12.7 / 27.0, 64 x 8 of 128256
-// (131 MB) 26.0 / 19.7, 16 x 64 (263 MB) 47.0 / 18.9.  (Fetching the children's
-// logits into L2 ahead of the walk made its steps longer: 20.2 us.)
+// Scanning every node reads all the logits, the walk with its argmaxes takes 2.3
+// us a step (bf16, in a graph, logits up to L2's size read again from there, as
+// after the product that wrote them).  Scan / walk with so many nodes accepted:
+//   1 x 64 of 128256 (16 MB)     8 / 18.5 (7)
+//   64 x 16 of 32000 (66 MB)     14.0 / 41.6 (8)
+//   8 x 32 of 128256 (66 MB)     14.0 / 21.0 (8)    18.2 / 73.2 (all 32)
+//   64 x 8 of 128256 (131 MB)    26.6 / 10.4 (1)    27.7 / 56.2 (all 8)
+//   16 x 64 of 128256 (263 MB)   48.3 / 22.8 (8)    58.1 / 185 (all 64)
+//   1 x 1024 of 33001 (68 MB)    22.6 / 21.6 (8)    197 / 2521 (all 1024)
+// So small logits are scanned.  Of larger ones most trees' paths are cheaper to
+// walk, but nothing on the host bounds a path below the number of nodes: where a
+// walk over all of them could cost more than four scans, it stops after as many
+// steps as cost about one scan, and a scan of the nodes behind it ends the path
+// (1 x 1024 of 33001: 25.2 (8), 210 (all); 4 x 70 of 64001 fp32, 72 MB: 24.1 (8),
+// 42.4 (all), 164 by walking alone).  The launches that have nothing left to do
+// cost 3 to 4 us.
 constexpr int64_t kScanAllBytes = int64_t(64) << 20;
-bool accept_scans_all(const slimkv_tree_accept_args* a) {
-    return int64_t(a->batch) * a->nodes * a->vocab * (a->type == SLIMKV_FP32 ? 4 : 2) <= kScanAllBytes;
+constexpr int64_t kStepBytes = 13000000;    // scanned in a step's time
+int64_t accept_bytes(const slimkv_tree_accept_args* a) {
+    return int64_t(a->batch) * a->nodes * a->vocab * (a->type == SLIMKV_FP32 ? 4 : 2);
+}
+bool accept_scans_all(const slimkv_tree_accept_args* a) { return accept_bytes(a) <= kScanAllBytes; }
+// Steps of a walk: all, or those that cost about a scan.
+int accept_steps(const slimkv_tree_accept_args* a) {
+    const int64_t of_a_scan = std::max<int64_t>(8, accept_bytes(a) / kStepBytes);
+    return a->nodes <= 4 * of_a_scan ? a->nodes : int(of_a_scan);
 }
 
 int accept_splits(const slimkv_tree_accept_args* a) {
@@ -260,6 +291,13 @@ int accept_splits(const slimkv_tree_accept_args* a) {
     const int64_t rows = int64_t(a->batch) * a->nodes;
     const int64_t want = (int64_t(device_info().sm_count) * 8 + rows - 1) / rows;
     return int(std::max<int64_t>(1, std::min<int64_t>(want, a->vocab / 4096)));
+}
+
+void carve_accept(Carver& c, const slimkv_tree_accept_args* a, AcceptArgs& k) {
+    k.splits = accept_splits(a);
+    const bool all = accept_scans_all(a), stops = !all && accept_steps(a) < a->nodes;
+    if (all || stops) k.best = c.take<uint64_t>(size_t(a->batch) * a->nodes * k.splits);
+    if (stops) k.resume = c.take<int2>(a->batch);
 }
 
 int check_accept(const slimkv_tree_accept_args* a) {
@@ -378,7 +416,10 @@ extern "C" int slimkv_tree_masks(const int32_t* parents, int batch, int nodes, i
 
 extern "C" size_t slimkv_tree_accept_workspace_size(const slimkv_tree_accept_args* a) {
     if (check_accept(a) != SLIMKV_OK) return 0;
-    return accept_scans_all(a) ? size_t(a->batch) * a->nodes * accept_splits(a) * sizeof(uint64_t) : 256;
+    AcceptArgs k{};
+    Carver c(nullptr, 0);
+    carve_accept(c, a, k);
+    return std::max<size_t>(c.used, 256);
 }
 
 extern "C" int slimkv_tree_accept(const slimkv_tree_accept_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -387,36 +428,48 @@ extern "C" int slimkv_tree_accept(const slimkv_tree_accept_args* a, void* worksp
         return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree accept: null pointer");
     if (a->logits_stride[0] < 0 || a->logits_stride[1] < 0)
         return fail(SLIMKV_ERR_INVALID_ARGUMENT, "tree accept: negative strides");
-    AcceptArgs k{a->nodes, a->vocab, accept_splits(a), a->logits, a->logits_stride[0], a->logits_stride[1], a->tokens,
-                 a->parents, a->nodes_len, a->path, a->count, a->next, static_cast<uint64_t*>(workspace)};
+    AcceptArgs k{};
+    Carver c(workspace, workspace_bytes);
+    carve_accept(c, a, k);
     if (!workspace || workspace_bytes < slimkv_tree_accept_workspace_size(a) || reinterpret_cast<uintptr_t>(workspace) % 8)
         return fail(SLIMKV_ERR_WORKSPACE, "tree accept: workspace too small or misaligned");
+    k.nodes = a->nodes;
+    k.vocab = a->vocab;
+    k.logits = a->logits;
+    k.stride_batch = a->logits_stride[0];
+    k.stride_node = a->logits_stride[1];
+    k.tokens = a->tokens;
+    k.parents = a->parents;
+    k.nodes_len = a->nodes_len;
+    k.path = a->path;
+    k.count = a->count;
+    k.next = a->next;
+    k.max_steps = accept_steps(a);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e;
+    cudaError_t e = cudaSuccess;
+    cudaLaunchAttribute cluster{}, dependent{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = kPathCtas;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dependent.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
     cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (accept_scans_all(a)) {
-        const dim3 grid(k.splits, a->nodes, a->batch);
-        if (a->type == SLIMKV_BF16) accept_scan_kernel<__nv_bfloat16><<<grid, kScanThreads, 0, st>>>(k);
-        else if (a->type == SLIMKV_FP16) accept_scan_kernel<__half><<<grid, kScanThreads, 0, st>>>(k);
-        else accept_scan_kernel<float><<<grid, kScanThreads, 0, st>>>(k);
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cfg.gridDim = dim3(a->batch);
-        cfg.blockDim = dim3(kWalkThreads);
-        e = cudaLaunchKernelEx(&cfg, accept_walk_kernel, k);
-    } else {
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = kPathCtas;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.gridDim = dim3(unsigned(a->batch) * kPathCtas);
-        cfg.blockDim = dim3(kPathThreads);
-        if (a->type == SLIMKV_BF16) e = cudaLaunchKernelEx(&cfg, accept_path_kernel<__nv_bfloat16>, k);
-        else if (a->type == SLIMKV_FP16) e = cudaLaunchKernelEx(&cfg, accept_path_kernel<__half>, k);
-        else e = cudaLaunchKernelEx(&cfg, accept_path_kernel<float>, k);
+    auto launch = [&](dim3 grid, int threads, cudaLaunchAttribute* attr, auto bf16, auto fp16, auto fp32) {
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads);
+        cfg.attrs = attr;
+        cfg.numAttrs = attr ? 1 : 0;
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, a->type == SLIMKV_BF16 ? bf16 : a->type == SLIMKV_FP16 ? fp16 : fp32, k);
+    };
+    const bool walks = !accept_scans_all(a);
+    if (walks)
+        launch(dim3(unsigned(a->batch) * kPathCtas), kPathThreads, &cluster, accept_path_kernel<__nv_bfloat16>, accept_path_kernel<__half>,
+               accept_path_kernel<float>);
+    if (!walks || k.resume) {
+        launch(dim3(k.splits, a->nodes, a->batch), kScanThreads, walks ? &dependent : nullptr, accept_scan_kernel<__nv_bfloat16>,
+               accept_scan_kernel<__half>, accept_scan_kernel<float>);
+        launch(dim3(a->batch), kWalkThreads, &dependent, accept_walk_kernel, accept_walk_kernel, accept_walk_kernel);
     }
     return e == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "tree accept launch failed: %s", cudaGetErrorString(e));
 }

@@ -504,3 +504,25 @@ def test_fp16_probabilities_above_the_running_maximum(T, step):
     q[..., 0] = 8
     k[:, :700 + T, :, 0] = (torch.arange(700 + T, device='cuda') // 64 * step - 30)[None, :, None].to(FP16)
     run(q, k, v, lens, scale=0.125)
+
+
+@pytest.mark.parametrize('B,T,V,dtype', [(4, 70, 64001, torch.float32), (1, 1024, 33001, BF16), (20, 33, 60001, FP16), (16, 64, 33001, BF16)])
+def test_accepted_chains_of_every_length(B, T, V, dtype):
+    """Chains accepted up to each length around the number of steps after which a walk may stop, or whole."""
+    gen = torch.Generator(device='cuda').manual_seed(V)
+    logits = torch.randn(B, T, V, generator=gen, device='cuda').to(dtype)
+    best = torch.stack([x.float().argmax(-1) for x in logits])
+    parents = torch.arange(-1, T - 1, dtype=torch.int32, device='cuda').expand(B, T).contiguous()
+    lengths = [1, 2, 6, 7, 8, 9, 10, 17, T - 1, T]
+    for turn in range(0, len(lengths), B) if B < len(lengths) else range(1):
+        tokens = torch.cat([best[:, :1], best[:, :-1]], 1)
+        want = [lengths[(turn + b) % len(lengths)] for b in range(B)]
+        for b, n in enumerate(want):
+            if n < T:
+                tokens[b, n] = (tokens[b, n] + 1) % V
+        nodes = [T if b % 3 else max(1, T - 1 - b) for b in range(B)]
+        for given in (None, torch.tensor(nodes, dtype=torch.int32, device='cuda')):
+            path, count, after = tree.tree_accept(logits, tokens, parents, nodes=given)
+            counts = [min(n, T if given is None else m) for n, m in zip(want, nodes)]
+            assert count.tolist() == counts and after.tolist() == [int(best[b, c - 1]) for b, c in enumerate(counts)]
+            assert path.tolist() == [list(range(c)) + [-1] * (T - c) for c in counts]

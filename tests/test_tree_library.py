@@ -197,3 +197,10 @@ def test_evict_refuses_output_rows_in_one_place(which, dim):
               **{f'dst__{which}_stride__x{dim}': 0})
     assert _lib.load().slimkv_evict(ctypes.byref(a), P, 1 << 20, None) == INVALID
     assert b'own place' in _lib.load().slimkv_last_error()
+
+
+@pytest.mark.parametrize('batch,nodes,vocab,kind', [(1, 1024, 33001, 0), (4, 70, 64001, 2), (2, 256, 128256, 0), (8, 1024, 128256, 0)])
+def test_long_paths_are_not_left_to_serial_steps(batch, nodes, vocab, kind):
+    """Where every node may be accepted and walking them costs many scans of all, the call has room for the scan's argmaxes."""
+    a = accept(batch=batch, nodes=nodes, vocab=vocab, type=kind)
+    assert _lib.load().slimkv_tree_accept_workspace_size(ctypes.byref(a)) >= 8 * batch * nodes
