@@ -25,6 +25,7 @@
 // 8-11 of its odd ones.  Every wait is bounded.
 #include <algorithm>
 
+#include "bounded_wait.cuh"
 #include "cache_view.cuh"
 #include "host_utils.h"
 #include "key_shares.cuh"
@@ -90,24 +91,6 @@ struct Plan {
     }
 };
 
-// A wait that is over costs one test; one that is not looks for an abort of
-// another warp and for its limit.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
-    if (mbar_test(bar, parity)) return true;
-    for (uint64_t waited = 0; waited < J.wait_ns;) {
-        const uint64_t step = min(J.wait_ns - waited, uint64_t(100000));
-        if (mbar_wait(bar, parity, step)) return true;
-        if (*const_cast<volatile int*>(&bs->abort)) return false;
-        waited += step;
-    }
-    bs->abort = 1;
-    report(J.status, SLIMKV_DEVICE_TIMEOUT);
-    return false;
-}
-__device__ __forceinline__ bool all_lanes(bool x) { return __all_sync(0xffffffffu, x); }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
-    return __all_sync(0xffffffffu, wait_bar(bar, parity, bs, J));
-}
 // 16 bytes global -> shared, or zeros.
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool some) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(some ? 16 : 0) : "memory");

@@ -43,6 +43,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "bounded_wait.cuh"
 #include "cache_view.cuh"
 #include "host_utils.h"
 #include "key_shares.cuh"
@@ -184,20 +185,6 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
         : "memory");
 }
 
-// A wait that is over costs one test; one that is not looks for an abort of
-// another warp and for its limit.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
-    if (mbar_test(bar, parity)) return true;
-    for (uint64_t waited = 0; waited < J.wait_ns;) {
-        const uint64_t step = min(J.wait_ns - waited, uint64_t(100000));
-        if (mbar_wait(bar, parity, step)) return true;
-        if (*const_cast<volatile int*>(&bs->abort)) return false;
-        waited += step;
-    }
-    bs->abort = 1;
-    report(J.status, SLIMKV_DEVICE_TIMEOUT);
-    return false;
-}
 // Whether `x` holds for any of the 256 softmax threads of a row tile (their
 // barrier `id`).
 __device__ __forceinline__ bool any_of_row_tile(int id, bool x) {
@@ -208,10 +195,6 @@ __device__ __forceinline__ bool any_of_row_tile(int id, bool x) {
         : "r"(uint32_t(x)), "r"(id)
         : "memory");
     return any != 0;
-}
-__device__ __forceinline__ bool all_lanes(bool x) { return __all_sync(0xffffffffu, x); }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Bars* bs, const Job& J) {
-    return __all_sync(0xffffffffu, wait_bar(bar, parity, bs, J));
 }
 
 // Tensor memory columns: O of each row tile, then its S buffers, as many as

@@ -293,3 +293,17 @@ def test_evict_refuses_outputs_over_their_inputs():
                 (k.clone(), v.clone(), mass[..., 100:], None)):
         with pytest.raises(RuntimeError):
             eviction.evict(k, v, mass, None, lens, 100, out=out)
+
+
+@pytest.mark.parametrize('T,H,D', [(4, 32, 320), (70, 8, 128)])
+def test_waits_of_the_masses_that_run_out_are_reported(T, H, D):
+    """With a limit of 1 ns the waits run out while the ring is full (one and several column blocks): the timeout is
+    reported, and the next call, with the usual limit, gives what the one before gave."""
+    q, k, mass, lens, _ = make(1, T, H, 1, D, [60000])
+    lse = torch.full((1, T, H), 5.0, device='cuda')
+    want = eviction.key_mass(q, k, lse, mass.clone(), lens, 0.1)
+    assert _lib.device_status(clear=True) == 0
+    eviction.key_mass(q, k, lse, mass.clone(), lens, 0.1, wait_limit_ns=1)
+    assert _lib.device_status(clear=True) & _lib.DEVICE_TIMEOUT
+    assert torch.equal(eviction.key_mass(q, k, lse, mass, lens, 0.1), want)
+    assert _lib.device_status(clear=True) == 0

@@ -526,3 +526,17 @@ def test_accepted_chains_of_every_length(B, T, V, dtype):
             counts = [min(n, T if given is None else m) for n, m in zip(want, nodes)]
             assert count.tolist() == counts and after.tolist() == [int(best[b, c - 1]) for b, c in enumerate(counts)]
             assert path.tolist() == [list(range(c)) + [-1] * (T - c) for c in counts]
+
+
+@pytest.mark.parametrize('T,H,G,D,n,context_only', [(2, 8, 2, 128, 60000, False), (20, 8, 1, 128, 60000, False), (4, 32, 1, 320, 60000, True)])
+def test_waits_that_run_out_end_every_pipeline(T, H, G, D, n, context_only):
+    """With a limit of 1 ns the waits run out while the rings are full (one and two row tiles, K slots of a row and of a
+    chunk): the timeout is reported, and the next call, with the usual limit, gives what the one before gave."""
+    q, k, v, lens, _ = make(1, T, H, G, D, [n], context_only=context_only)
+    want = tree.tree_attention(q, k, v, lens, 0.1, context_only=context_only)
+    assert _lib.device_status(clear=True) == 0
+    tree.tree_attention(q, k, v, lens, 0.1, context_only=context_only, wait_limit_ns=1)
+    assert _lib.device_status(clear=True) & _lib.DEVICE_TIMEOUT
+    got = tree.tree_attention(q, k, v, lens, 0.1, context_only=context_only)
+    assert _lib.device_status(clear=True) == 0
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
