@@ -763,6 +763,8 @@ SLIMKV_API int slimkv_tree_commit(const slimkv_tree_commit_args* args, void* str
  * their values.  rows null: r_i = i; counts null: every row.  The lse is taken
  * as it is: at +inf a row gives nothing, at -inf (a row that saw no key, which
  * an accepted row is not: it sees itself) the masses of its keys are infinite.
+ * Where slimkv_tree_attention had nodes_len and rows is null, counts = nodes_len
+ * leaves those rows out.
  * q [batch][nodes][heads][dim], lse fp32 [batch][nodes][heads] contiguous,
  * mass fp32, element strides {batch, head}, at least the used rows long.  Only
  * cache.k is read.  Types, dims and pages as slimkv_tree_attention.

@@ -41,9 +41,11 @@ def key_mass(q, k, lse, mass, lengths, scale, rows=None, counts=None, decay=1.0,
     (row i sees n <= lengths[b] + i; a new row's mass starts from 0).
     ``context_only``: only the ``lengths[b]`` rows (Beacon latents).  ``q [B, T,
     H, D]`` and ``lse [B, T, H]`` as ``tree.tree_attention`` took and returned
-    them; for a key set attended in parts, pass the merged lse (a row that saw
-    no key, lse -inf, has no weights: leave it out of ``rows``).  Other entries
-    of ``mass`` keep their values.  Returns ``mass``.
+    them; for a key set attended in parts, pass the merged lse.  The lse is taken
+    as it is: a row that saw no key (lse -inf) would make the masses of its keys
+    infinite for good, so leave it out of ``rows``; where ``tree_attention`` had
+    ``nodes`` and every row counts, ``counts=nodes`` does.  Other entries of
+    ``mass`` keep their values.  Returns ``mass``.
     """
     kind = q.dtype
     if not (q.is_cuda and q.dim() == 4 and kind in (torch.bfloat16, torch.float16)):

@@ -1,5 +1,6 @@
 """Accumulated attention weight and eviction (``slimkv_b200.eviction``)
 against plain 64-bit forms."""
+import ctypes
 import math
 import random
 
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 import tree_oracle as oracle
-from slimkv_b200 import _lib, eviction, tree
+from slimkv_b200 import _lib, eviction, kernels, tree
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -307,3 +308,106 @@ def test_waits_of_the_masses_that_run_out_are_reported(T, H, D):
     assert _lib.device_status(clear=True) & _lib.DEVICE_TIMEOUT
     assert torch.equal(eviction.key_mass(q, k, lse, mass, lens, 0.1), want)
     assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize('T,page,rank', [(5, 48, 320), (3, 96, 160), (1, 16, 64)])
+def test_masses_over_latent_pages(T, page, rank):
+    """Only the context has masses; NaN rows past it and table entries of no page stay out."""
+    q, k, mass, lens, tables = make(3, T, 32, 1, rank, [0, 700, 129], page=page)
+    for b, n in enumerate(lens.tolist()):
+        k[tables[b, n // page].long(), n % page:] = math.nan
+        tables[b, -(-n // page):] = -7
+    lse = torch.full((3, T, 32), 4.0, device='cuda')
+    check_mass(q, k, lse, mass, lens, rank ** -0.5, block_tables=tables, context_only=True, decay=0.5)
+
+
+def test_masses_over_a_cache_shared_by_the_batch():
+    q, _, mass, lens, _ = make(3, 4, 8, 2, 128, [50, 60, 170])
+    k = torch.randn(1, mass.shape[2], 2, 128, device='cuda').to(BF16)
+    check_mass(q, k, torch.full((3, 4, 8), 4.0, device='cuda'), mass, lens, 0.1, decay=0.9)
+
+
+def test_counts_leave_out_rows_that_saw_nothing():
+    """A batch of smaller trees: rows past a sequence's nodes have lse -inf, and its count of nodes keeps them out."""
+    q, k, mass, lens, _ = make(3, 4, 8, 2, 128, [50, 60, 170])
+    nodes = torch.tensor([4, 0, 2], dtype=torch.int32, device='cuda')
+    _, lse = tree.tree_attention(q, k, k, lens, 0.1, nodes=nodes)
+    assert (lse[1] == -math.inf).all() and (lse[2, 2:] == -math.inf).all()
+    check_mass(q, k, lse, mass, lens, 0.1, counts=nodes, decay=0.9)
+    assert mass.isfinite().all()
+
+
+@pytest.mark.parametrize('page', [16, 5])
+def test_evict_from_pages_into_pages_without_masses(page):
+    """The C entry alone: an output with block tables, and no output of masses or positions."""
+    B, G, D, lengths, keep = 2, 2, 64, [90, 40], 64
+    i32 = dict(dtype=torch.int32, device='cuda')
+    pages = torch.randn(B * 20, page, G, D, device='cuda').to(BF16)
+    tables = torch.randperm(B * 20, device='cuda')[:B * 20].view(B, 20).to(torch.int32)
+    per = -(-keep // page)
+    new = torch.full((B * per + 1, page, G, D), 7.0, device='cuda', dtype=BF16)
+    new_v = new.clone()
+    new_tables = torch.randperm(B * per + 1, device='cuda')[:B * per].view(B, per).to(torch.int32)
+    mass, lens, after = torch.rand(B, G, 100, device='cuda'), torch.tensor(lengths, **i32), torch.zeros(B, **i32)
+    a = _lib.EvictArgs()
+    tree.fill_cache(a.src, pages, pages, tables, B)
+    tree.fill_cache(a.dst, new, new_v, new_tables, B)
+    a.batch, a.kv_heads, a.dim_qk, a.dim_v, a.elem_bytes, a.mass_rows = B, G, D, D, 2, 100
+    a.mass, a.lengths, a.new_lengths = mass.data_ptr(), lens.data_ptr(), after.data_ptr()
+    a.mass_stride[0], a.mass_stride[1] = mass.stride()[:2]
+    a.keep, a.sinks, a.recent = keep, 4, 8
+    lib = _lib.load()
+    workspace = torch.empty(lib.slimkv_evict_workspace_size(ctypes.byref(a)), dtype=torch.uint8, device='cuda')
+    _lib.check(lib.slimkv_evict(ctypes.byref(a), workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream))
+    want = oracle.evict(pages, pages, mass, None, lengths, keep, 4, 8, tables)
+    for x in (new, new_v):
+        rows = x[new_tables.long()].flatten(1, 2)
+        assert torch.equal(rows[:, :keep].double().cpu(), want[0]) and (rows[:, keep:] == 7).all()
+        left = torch.ones(len(x), dtype=torch.bool, device='cuda').index_fill(0, new_tables.flatten().long(), False)
+        assert (x[left] == 7).all()
+    assert after.tolist() == [min(n, keep) for n in lengths] and _lib.device_status() == 0
+
+
+def test_a_step_over_latents_and_raw_rows():
+    """SlimKV's cache in its two parts: attention over each, merged, the accepted rows committed, and the masses of both
+    as shares of one softmax."""
+    B, T, H, G, D, R = 2, 6, 8, 2, 64, 160
+    raw_n, lat_n, scale = [70, 33], [300, 129], 0.125
+    q, raw_k, raw_mass, raw_lens, _ = make(B, T, H, G, D, raw_n)
+    raw_v = torch.randn_like(raw_k)
+    lat = torch.randn(B, 2, 310, R, device='cuda').to(BF16)
+    lat_k, lat_v = lat[:, 0].unsqueeze(2), lat[:, 1].unsqueeze(2)
+    up_k, up_v = (torch.randn(H, R, D, device='cuda').mul_(R ** -0.5).to(BF16) for _ in range(2))
+    absorbed = torch.einsum('bthd,hrd->bthr', q.float(), up_k.float()).to(BF16)
+    lat_lens = torch.tensor(lat_n, dtype=torch.int32, device='cuda')
+    parents = torch.tensor([[-1, 0, 0, 1, 1, 3], [-1, 0, 1, 2, 0, 4]], dtype=torch.int32, device='cuda')
+    seen = torch.stack([oracle.ancestors(p) for p in parents.tolist()])
+    raw, raw_lse = tree.tree_attention(q, raw_k, raw_v, raw_lens, scale, mask=tree.tree_masks(parents))
+    part, lat_lse = tree.tree_attention(absorbed, lat_k, lat_v, lat_lens, scale, context_only=True)
+    up = torch.einsum('bthr,hrd->bthd', part.float(), up_v.float()).to(BF16)
+    out = kernels.merge(raw.transpose(1, 2), raw_lse.transpose(1, 2), up.transpose(1, 2), lat_lse.transpose(1, 2)).transpose(1, 2)
+    lse = torch.logaddexp(raw_lse, lat_lse)
+    # In 64 bits, each part's bound weighted by its share; a share is off by the two lse's bounds, the up-projected part
+    # and the output are rounded to bf16 once.
+    ro, rl, rt, rlt = oracle.attention(q, raw_k, raw_v, raw_n, scale, seen)
+    lo, ll, lt, llt = oracle.attention(absorbed, lat_k, lat_v, lat_n, scale, context_only=True)
+    lo = torch.einsum('bthr,hrd->bthd', lo, up_v.double().cpu())
+    lt = torch.einsum('bthr,hrd->bthd', lt, up_v.double().cpu().abs()) + 2.0 ** -8 * lo.abs() + 1e-5
+    total = torch.logaddexp(rl, ll)
+    wr, wl = (rl - total).exp()[..., None], (ll - total).exp()[..., None]
+    want = wr * ro + wl * lo
+    tol = wr * rt + wl * lt + (rlt + llt + 1e-5)[..., None] * (wr * ro.abs() + wl * lo.abs()) + 2.0 ** -8 * want.abs() + 1e-6
+    assert ((out.double().cpu() - want).abs() <= 1.05 * tol).all()
+    assert ((lse.double().cpu() - total).abs() <= 1.05 * (rlt + llt + 1e-6)).all()
+    path = torch.tensor([[0, 1, 3, 5, -1, -1], [0, 4, -1, -1, -1, -1]], dtype=torch.int32, device='cuda')
+    count = torch.tensor([4, 2], dtype=torch.int32, device='cuda')
+    new = tree.tree_commit(raw_k, raw_v, raw_lens, path, count)
+    assert new.tolist() == [74, 35]
+    lat_mass = torch.rand(B, 1, 310, device='cuda')
+    check_mass(absorbed, lat_k, lse, lat_mass.clone(), lat_lens, scale, rows=path, counts=count, context_only=True)
+    check_mass(q, raw_k, lse, raw_mass.clone(), raw_lens, scale, rows=path, counts=count)
+    # Every accepted row has given each head's weight once, over both parts.
+    eviction.key_mass(absorbed, lat_k, lse, lat_mass.zero_(), lat_lens, scale, rows=path, counts=count, context_only=True)
+    eviction.key_mass(q, raw_k, lse, raw_mass.zero_(), raw_lens, scale, rows=path, counts=count)
+    given = lat_mass.double().sum((1, 2)) + raw_mass.double().sum((1, 2))
+    assert (given - H * count).abs().max() < 1e-3

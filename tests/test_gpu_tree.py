@@ -540,3 +540,10 @@ def test_waits_that_run_out_end_every_pipeline(T, H, G, D, n, context_only):
     got = tree.tree_attention(q, k, v, lens, 0.1, context_only=context_only)
     assert _lib.device_status(clear=True) == 0
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize('T,page,rank', [(5, 48, 320), (3, 96, 160), (1, 16, 64)])
+def test_latent_pages(T, page, rank):
+    """Latents in pages, which hold no rows of the nodes."""
+    q, k, v, lens, tables = make(3, T, 32, 1, rank, [0, 700, 129], page=page, context_only=True)
+    run(q, k, v, lens, tables, context_only=True)
