@@ -124,6 +124,17 @@ struct Sorted {
     }
 };
 
+// First byte of a set of rows, and the one behind its last.
+void range_of(const Rows& r, Wide& from, Wide& to) {
+    from = reinterpret_cast<uintptr_t>(r.at);
+    to = from + r.width;
+    for (int i = 0; i < 4; ++i) {
+        const Wide far = Wide(r.stride[i]) * (r.n[i] - 1);
+        if (far < 0) from += far;
+        else to += far;
+    }
+}
+
 // The dimensions d.. of a and b, b `gap` bytes behind a.
 bool share_from(const Sorted& a, const Sorted& b, int d, Wide gap) {
     if (gap >= a.span[std::min(d, a.dims)] || -gap >= b.span[std::min(d, b.dims)]) return false;
@@ -142,6 +153,10 @@ bool share_from(const Sorted& a, const Sorted& b, int d, Wide gap) {
 }  // namespace
 
 bool share_rows(const Rows& a, const Rows& b) {
+    Wide a0, a1, b0, b1;
+    range_of(a, a0, a1);
+    range_of(b, b0, b1);
+    if (a1 <= b0 || b1 <= a0) return false;         // what nearly every call has
     const Sorted x(a), y(b);
     return share_from(x, y, 0, y.at - x.at);
 }

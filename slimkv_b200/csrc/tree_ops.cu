@@ -116,8 +116,10 @@ __device__ __forceinline__ uint64_t scan_row(const T* row, int lo, int hi, ScanS
     return uint64_t(largest) << 32 | uint32_t(~scratch->index);
 }
 
+// (96 bytes: with 104 a launch cost the host 0.3 us more, the Python call 0.9.)
 struct AcceptArgs {
     int nodes, vocab, splits;
+    int max_steps;              // nodes after which the walk with its argmaxes stops (all: never)
     const void* logits;
     int64_t stride_batch, stride_node;
     const int64_t* tokens;
@@ -126,11 +128,10 @@ struct AcceptArgs {
     int32_t* path;
     int32_t* count;
     int64_t* next;
-    uint64_t* best;             // [batch][nodes][splits]
-    // The walk with its argmaxes ends after max_steps nodes and leaves the node it would go on
-    // with (-1: it is over) and the steps taken; null: no such walk comes before.
-    int max_steps;
-    int2* resume;               // [batch]
+    uint64_t* best;             // [batch][nodes][splits]; before it what resume_of says
+    __device__ __forceinline__ bool stops() const { return max_steps < nodes; }
+    // Where a walk that stops would go on: its next node (-1: it is over) and the steps taken.
+    __device__ __forceinline__ int2& resume_of(int b) const { return reinterpret_cast<int2*>(best)[-1 - b]; }
 };
 
 constexpr int kScanThreads = 256;
@@ -142,9 +143,9 @@ __global__ void __launch_bounds__(kScanThreads) accept_scan_kernel(AcceptArgs a)
     __shared__ ScanScratch<kScanThreads> scratch;
     const int t = blockIdx.y, b = blockIdx.z;
     grid_launch_dependents();               // the walk over the argmaxes, which waits for this grid
-    if (a.resume) {
+    if (a.stops()) {
         grid_dependency_wait();
-        const int from = a.resume[b].x;
+        const int from = a.resume_of(b).x;
         if (from < 0 || t < from) return;
     }
     if (a.nodes_len && t >= __ldg(a.nodes_len + b)) return;
@@ -169,8 +170,8 @@ __global__ void __launch_bounds__(kWalkThreads) accept_walk_kernel(AcceptArgs a)
         tokens[i] = token >= 0 && token < a.vocab ? int(token) : -1;
     }
     grid_dependency_wait();
-    const int2 start = a.resume ? a.resume[b] : make_int2(n > 0 ? 0 : -1, 0);
-    if (a.resume && start.x < 0) return;                // that walk has written everything
+    const int2 start = a.stops() ? a.resume_of(b) : make_int2(n > 0 ? 0 : -1, 0);
+    if (a.stops() && start.x < 0) return;               // the walk before has written everything
     for (int i = max(start.x, 0) + tid; i < n; i += kWalkThreads) {
         uint64_t top = 0;
         for (int k = 0; k < a.splits; ++k) top = max_u64(top, a.best[(int64_t(b) * a.nodes + i) * a.splits + k]);
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
     int cur = n > 0 ? 0 : -1, len = 0;
     int64_t next = -1;
     cluster_wait();
-    if (a.resume) grid_launch_dependents();
+    if (a.stops()) grid_launch_dependents();
     while (cur >= 0 && len < a.max_steps) {
         const int parity = len & 1;
         if (rank == 0 && tid == 0) path[len] = cur;
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
         __syncthreads();
         cur = child[parity] < kMaxNodes ? child[parity] : -1;
     }
-    if (rank == 0 && tid == 0 && a.resume) a.resume[b] = make_int2(cur, len);
+    if (rank == 0 && tid == 0 && a.stops()) a.resume_of(b) = make_int2(cur, len);
     if (rank == 0 && cur < 0) {
         for (int i = len + tid; i < a.nodes; i += kPathThreads) path[i] = -1;
         if (tid == 0) {
@@ -261,7 +262,8 @@ __global__ void __launch_bounds__(kPathThreads) accept_path_kernel(AcceptArgs a)
 // Scanning every node reads all the logits, the walk with its argmaxes takes 2.3
 // us a step (bf16, in a graph, logits up to L2's size read again from there, as
 // after the product that wrote them).  Scan / walk with so many nodes accepted:
-//   1 x 64 of 128256 (16 MB)     8 / 18.5 (7)
+//   1 x 64 of 128256 (16 MB)     10.1 / 17.9 (7)    20.1 / 142 (all 64)
+//   16 x 8 of 128256 (33 MB)     11.4 / 22.8 (all 8)
 //   64 x 16 of 32000 (66 MB)     14.0 / 41.6 (8)
 //   8 x 32 of 128256 (66 MB)     14.0 / 21.0 (8)    18.2 / 73.2 (all 32)
 //   64 x 8 of 128256 (131 MB)    26.6 / 10.4 (1)    27.7 / 56.2 (all 8)
@@ -294,10 +296,13 @@ int accept_splits(const slimkv_tree_accept_args* a) {
 }
 
 void carve_accept(Carver& c, const slimkv_tree_accept_args* a, AcceptArgs& k) {
+    k.nodes = a->nodes;
     k.splits = accept_splits(a);
-    const bool all = accept_scans_all(a), stops = !all && accept_steps(a) < a->nodes;
-    if (all || stops) k.best = c.take<uint64_t>(size_t(a->batch) * a->nodes * k.splits);
-    if (stops) k.resume = c.take<int2>(a->batch);
+    const bool all = accept_scans_all(a);
+    k.max_steps = all ? a->nodes : accept_steps(a);
+    const bool stops = k.max_steps < k.nodes;
+    const size_t first = stops ? a->batch : 0;          // resume_of's entries
+    if (all || stops) k.best = c.take<uint64_t>(first + size_t(a->batch) * a->nodes * k.splits) + first;
 }
 
 int check_accept(const slimkv_tree_accept_args* a) {
@@ -431,9 +436,8 @@ extern "C" int slimkv_tree_accept(const slimkv_tree_accept_args* a, void* worksp
     AcceptArgs k{};
     Carver c(workspace, workspace_bytes);
     carve_accept(c, a, k);
-    if (!workspace || workspace_bytes < slimkv_tree_accept_workspace_size(a) || reinterpret_cast<uintptr_t>(workspace) % 8)
+    if (!workspace || workspace_bytes < std::max<size_t>(c.used, 256) || reinterpret_cast<uintptr_t>(workspace) % 8)
         return fail(SLIMKV_ERR_WORKSPACE, "tree accept: workspace too small or misaligned");
-    k.nodes = a->nodes;
     k.vocab = a->vocab;
     k.logits = a->logits;
     k.stride_batch = a->logits_stride[0];
@@ -444,32 +448,32 @@ extern "C" int slimkv_tree_accept(const slimkv_tree_accept_args* a, void* worksp
     k.path = a->path;
     k.count = a->count;
     k.next = a->next;
-    k.max_steps = accept_steps(a);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
-    cudaLaunchAttribute cluster{}, dependent{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = kPathCtas;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    dependent.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.stream = st;
-    auto launch = [&](dim3 grid, int threads, cudaLaunchAttribute* attr, auto bf16, auto fp16, auto fp32) {
+    cudaLaunchAttribute attr{};
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = &attr;
+    // The kernel of the logits' type.
+    auto launch = [&](int attrs, dim3 grid, int threads, auto bf16, auto fp16, auto fp32) {
         cfg.gridDim = grid;
         cfg.blockDim = dim3(threads);
-        cfg.attrs = attr;
-        cfg.numAttrs = attr ? 1 : 0;
+        cfg.numAttrs = attrs;
         if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, a->type == SLIMKV_BF16 ? bf16 : a->type == SLIMKV_FP16 ? fp16 : fp32, k);
     };
     const bool walks = !accept_scans_all(a);
-    if (walks)
-        launch(dim3(unsigned(a->batch) * kPathCtas), kPathThreads, &cluster, accept_path_kernel<__nv_bfloat16>, accept_path_kernel<__half>,
+    if (walks) {
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = kPathCtas;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        launch(1, dim3(unsigned(a->batch) * kPathCtas), kPathThreads, accept_path_kernel<__nv_bfloat16>, accept_path_kernel<__half>,
                accept_path_kernel<float>);
-    if (!walks || k.resume) {
-        launch(dim3(k.splits, a->nodes, a->batch), kScanThreads, walks ? &dependent : nullptr, accept_scan_kernel<__nv_bfloat16>,
-               accept_scan_kernel<__half>, accept_scan_kernel<float>);
-        launch(dim3(a->batch), kWalkThreads, &dependent, accept_walk_kernel, accept_walk_kernel, accept_walk_kernel);
+    }
+    if (!walks || k.max_steps < k.nodes) {
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        launch(walks, dim3(k.splits, a->nodes, a->batch), kScanThreads, accept_scan_kernel<__nv_bfloat16>, accept_scan_kernel<__half>,
+               accept_scan_kernel<float>);
+        launch(1, dim3(a->batch), kWalkThreads, accept_walk_kernel, accept_walk_kernel, accept_walk_kernel);
     }
     return e == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "tree accept launch failed: %s", cudaGetErrorString(e));
 }
