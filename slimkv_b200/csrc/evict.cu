@@ -259,8 +259,10 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
         if (some && a.out_positions) position = __ldg(a.positions + b * a.positions_stride[0] + g * a.positions_stride[1] + n);
     }
     __syncthreads();
-    // 16-byte units of the rows' K and V, kUnits of a thread under way at a time.
-    // (16 segments of 32k latents in a graph: 5 of them 73.8 us, 8 and 10 74.5.)
+    // 16-byte units of the rows' K and V, kUnits of a thread under way at a time.  In a graph, 3 / 4 /
+    // 5 / 8 of them: 16 x 32k rows of 320 dims 75.6 / 74.7 / 73.8 / 74.2 us, 16 x 8 heads of 8k rows of
+    // 128 dims 112 / 106 / 106 / 116, 4 x 4 heads of 40k rows of 64 dims 63 / 66 / 66 / 72, 8 x 50k rows of
+    // 160 dims 76.6 / 80.7 / 75.0 / 78.4 (best where they divide the 32 rows' units), 1.2k rows 12.4 with all.
     constexpr int kUnits = 5;
     const int units = a.k_units + a.v_units, total = rows * units;
     // p / units by multiplication: exact while p units < 2^20 (p < kRows units, units <= 181).

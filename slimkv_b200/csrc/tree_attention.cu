@@ -24,10 +24,11 @@
 // Lengths are read on the device; nothing on the host depends on them.
 //
 // Bound: with few rows per KV head HBM (each K / V row read once); with 128
-// rows or more the tensor cores and the exponentials.  Measured (bf16, 8 KV
-// heads of 128 dims, with the merge, in a graph): 2 x 8 nodes over 131,000 rows
-// 195 us = 5.5 TB/s, 16 x 16 over 8k 111 us = 4.9 TB/s, 16 x 64 nodes (256 rows
-// a KV head) over 8k 166 to 172 us = 870 TFLOP/s, one token over 517 rows 13 us.
+// rows or more the tensor cores and the exponentials; with few tiles to a CTA
+// its start, the ends of its pieces and the merge.  Measured (bf16, 8 KV heads
+// of 128 dims, with the merge, in a graph): 2 x 8 nodes over 131,000 rows
+// 192 us = 5.6 TB/s, 16 x 16 over 8k 111 us = 4.9 TB/s, 16 x 64 nodes (256 rows
+// a KV head) over 8k 167 us = 820 TFLOP/s, one token over 517 rows 13 us.
 // (In calls back to back the last of the three large ones draws the board's
 // 1000 W and runs at 1.65 GHz, 200 to 206 us.)
 //
@@ -751,9 +752,10 @@ constexpr int kCombineThreads = 256;
 // of 32 rows (a lane each) and 64 dims (8 to a warp) by turns, four pieces'
 // loads under way at a time.  Segments have two or three pieces when there are
 // many, tens when there are few: fewer dims to a warp cost the first case
-// instructions (4: 34 us for 128 segments of 256 rows), more the second latency
-// (16: 23 us for 8 segments of 128 rows in 19 pieces); and many blocks to a
-// segment cost many short segments more than the merge.
+// instructions, more the second latency; and many blocks to a segment cost many
+// short segments more than the merge.  Alone, caches cold: 10.7 us for 8 segments
+// of 128 rows x 320 dims in 19 pieces each (24 MB), 17 us for 128 segments of 256
+// rows x 128 dims, 7.5 us for 64 segments of 65 rows, 7 us for one token.
 template <int NQ, bool kHalf>
 __global__ void __launch_bounds__(kCombineThreads, 4) combine_kernel(const __grid_constant__ Job J) {
     __shared__ int range[3];                // first and last CTA of the segment's pieces, slot of the first

@@ -326,8 +326,8 @@ struct CommitArgs {
     unsigned int* status;
 };
 
-// Latency and HBM: one layer of one sequence 3.2 us in a graph, 32 layers of 16
-// sequences with 1 to 8 accepted rows 5.7 us (2.1 us for their bytes).
+// Latency and HBM: one layer of one sequence 3.0 us in a graph, 32 layers of 16
+// sequences with 1 to 7 accepted rows 5.6 us (2.1 us for their bytes).
 constexpr int kCommitRows = 8;
 
 // One thread per 16-byte column of a (layer, K or V, head): rows move in

@@ -84,7 +84,7 @@ def evict(k, v, mass, positions, lengths, keep, sinks=0, recent=0, block_tables=
     those of the largest mass (ties: the lowest row), all in their order.
     Returns ``(k, v, mass, positions, lengths)`` of ``keep`` rows, zeros past a
     sequence's new length; ``out = (k, v, mass, positions)`` gives buffers (at
-    least ``keep`` rows, not the inputs) to write instead of new ones.
+    least ``keep`` rows, nowhere over the inputs') to write instead of new ones.
     """
     _check_rows(k, v, 4)
     if mass.dim() != 3:

@@ -208,7 +208,8 @@ def tree_commit(k, v, lengths, path, count, block_tables=None):
 
     ``k`` / ``v`` one layer ``[B, rows, Hkv, D]`` (or pages with
     ``block_tables``), or every layer at once with a leading layer dimension;
-    any 1-, 2- or 4-byte type.  ``path`` / ``count`` as :func:`tree_accept`
+    any 1-, 2- or 4-byte type.  K and V may be (parts of) the same rows; each
+    sequence has rows of its own.  ``path`` / ``count`` as :func:`tree_accept`
     returns them.  Returns the new lengths (int32 ``[B]``).
     """
     first = k.dim() - 4
