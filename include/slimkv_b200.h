@@ -820,6 +820,67 @@ typedef struct {
 SLIMKV_API size_t slimkv_evict_workspace_size(const slimkv_evict_args* args);
 SLIMKV_API int slimkv_evict(const slimkv_evict_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 4-bit cache.  A row of D dims (a multiple of 32 up to 320) of bf16 or fp16
+ * values x is held in slimkv_row4_bytes(D) bytes: D / 2 bytes of codes, the
+ * pairs (scale, low) of its groups of 32 dims in the rows' type T, and what
+ * fills it up to a multiple of 16 bytes (never written).  Of a group
+ *   low = min x,  scale = T((max x - low) / 15) (one step less where 15 scale +
+ *   low would pass T's largest value; 0 below 2^-126),
+ *   code = the whole number in 0..15 nearest to (x - low) / scale, x - low
+ *   rounded to fp32 (ties: the even one; 0 for a scale of 0),
+ * and a code stands for T(code * scale + low), one rounding.  A group with an
+ * infinity or a NaN is NaN throughout.  Word w of the codes (little-endian)
+ * holds the dims 8w..8w+7: dim 8w + 2j + h at bits 16h + 4j.
+ *
+ * In slimkv_cache of the entries below K and V rows are such rows: the strides
+ * are in bytes, and pointers and strides multiples of 16 bytes.  A row's bytes
+ * can be moved as they are: slimkv_tree_commit and slimkv_evict take the cache
+ * with elem_bytes 1 and slimkv_row4_bytes as its dims.
+ * ---------------------------------------------------------------------- */
+SLIMKV_API int slimkv_row4_bytes(int dim);     /* 0: no dim of a 4-bit row */
+
+/* ------------------------------------------------------------------------
+ * Writes rows into the 4-bit cache, or reads them back: row i of sequence b,
+ * i < counts[b] (null: rows), is cache row starts[b] + i (null: i).
+ * k, v: 16-bit rows [batch][rows][kv_heads][dim], element strides {batch, row,
+ * head} (multiples of 8).  Read leaves rows past a sequence's count as they
+ * are, or fills them with zeros (zero_rest).  A count outside [0, rows], a
+ * negative start and rows that the cache does not hold are reported as
+ * SLIMKV_DEVICE_BAD_LENGTH and left out; of a page outside the pool, write
+ * leaves the rows out and read takes the page put in its place.  Two sequences
+ * that write the same cache row leave either's.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    int batch, rows, kv_heads, dim_qk, dim_v, type;
+    const void* k;
+    int64_t k_stride[3];
+    const void* v;
+    int64_t v_stride[3];
+    slimkv_cache cache;
+    const int32_t* starts;
+    const int32_t* counts;
+    int zero_rest;
+} slimkv_cache4_rows_args;
+
+SLIMKV_API int slimkv_cache4_write(const slimkv_cache4_rows_args* args, void* stream);
+SLIMKV_API int slimkv_cache4_read(const slimkv_cache4_rows_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * slimkv_tree_attention over a 4-bit cache: the same arguments and results
+ * (args->cache as above; dims multiples of 32; at most 128 query heads per KV
+ * head), as if over the 16-bit rows that slimkv_cache4_read gives.
+ * ---------------------------------------------------------------------- */
+SLIMKV_API size_t slimkv_cache4_attention_workspace_size(const slimkv_tree_attention_args* args);
+SLIMKV_API int slimkv_cache4_attention(const slimkv_tree_attention_args* args, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* ------------------------------------------------------------------------
+ * slimkv_key_mass over the keys of a 4-bit cache: the same arguments and
+ * results (args->cache as above, dim a multiple of 32).
+ * ---------------------------------------------------------------------- */
+SLIMKV_API int slimkv_cache4_key_mass(const slimkv_key_mass_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

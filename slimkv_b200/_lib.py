@@ -202,6 +202,15 @@ class EvictArgs(ctypes.Structure):
     ]
 
 
+class Cache4RowsArgs(ctypes.Structure):
+    """Mirror of ``slimkv_cache4_rows_args``."""
+    _fields_ = [
+        ('batch', _I), ('rows', _I), ('kv_heads', _I), ('dim_qk', _I), ('dim_v', _I), ('type', _I), ('k', _P),
+        ('k_stride', _L * 3), ('v', _P), ('v_stride', _L * 3), ('cache', Cache), ('starts', _P), ('counts', _P),
+        ('zero_rest', _I),
+    ]
+
+
 _PL = ctypes.POINTER(ctypes.c_int64)
 
 SIGNATURES = {
@@ -244,6 +253,12 @@ SIGNATURES = {
     'slimkv_key_mass': (_I, [ctypes.POINTER(KeyMassArgs), _P]),
     'slimkv_evict_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(EvictArgs)]),
     'slimkv_evict': (_I, [ctypes.POINTER(EvictArgs), _P, ctypes.c_size_t, _P]),
+    'slimkv_row4_bytes': (_I, [_I]),
+    'slimkv_cache4_write': (_I, [ctypes.POINTER(Cache4RowsArgs), _P]),
+    'slimkv_cache4_read': (_I, [ctypes.POINTER(Cache4RowsArgs), _P]),
+    'slimkv_cache4_attention_workspace_size': (ctypes.c_size_t, [ctypes.POINTER(TreeAttentionArgs)]),
+    'slimkv_cache4_attention': (_I, [ctypes.POINTER(TreeAttentionArgs), _P, ctypes.c_size_t, _P]),
+    'slimkv_cache4_key_mass': (_I, [ctypes.POINTER(KeyMassArgs), _P]),
     'slimkv_rms_norm': (_I, [_P, _L, _P, _P, _L, _I, _I, ctypes.c_float, _P]),
     'slimkv_silu_mul': (_I, [_P, _L, _P, _L, _I, _I, _P]),
 }

@@ -1,0 +1,786 @@
+// Attention over a 4-bit cache, split over the keys (C ABI
+// slimkv_cache4_attention).
+//
+// For every query row (node t, head h) over the keys n that the node sees
+//   s_n = scale q . k_n,   lse = log sum_n e^{s_n},   out = sum_n e^{s_n - lse} v_n,
+// k_n and v_n being the 16-bit rows that the codes stand for (cache4.cuh).
+//
+// A decode step has few query rows to a KV head and must read 0.625 bytes a
+// value, so what counts is how few instructions a value costs between its load
+// and the tensor core.  Codes never go back to shared memory: a warp takes 16
+// keys, turns their codes into MMA operands in its registers, and has the keys
+// (for V: the dims) on the 16 side of mma.sync.m16n8k16 and 8 query rows on the
+// other:
+//   S [16 keys x 8 rows] += K [16 x 16 dims] . Q^T,   O^T [16 dims x 8 rows] += V^T [16 x 16 keys] . P^T
+// Any order of the dims serves as the products' inner (outer) index as long as
+// both sides have the same one, so each lane reads whole words of one group:
+// one (scale, low) pair serves up to 32 values.  The softmax keeps a row's
+// maximum until a score passes it by 2^8, so a vote replaces the reduction over
+// keys; P goes from the layout of S to that of the second product by two
+// transpositions of 8 x 8 blocks in registers.
+//
+// Work: equal shares of all segments' 64-key tiles (key_shares.cuh), a segment
+// being the keys of one (sequence, KV head, 8 or 16 query rows); in a CTA's
+// piece of a segment each of its four warps takes a quarter of every tile, with
+// its own ring of TMA loads and its own running softmax, and the warps meet only
+// at the piece's end.  Pieces that are not a whole segment leave normalised
+// partial rows, which a dependent launch merges.  Lengths are read on the device.
+#include <algorithm>
+#include <type_traits>
+
+#include "bounded_wait.cuh"
+#include "cache4.cuh"
+#include "cache_view.cuh"
+#include "host_utils.h"
+#include "key_shares.cuh"
+#include "node_mask.cuh"
+
+namespace slimkv {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kSlab = 16;                        // keys of a warp's step
+constexpr int kKeys = kSlab * kWarps;            // keys of a tile
+constexpr int kStages = 4;                       // slabs of a warp's ring
+constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a score passes the row's maximum by 2^8
+// P = 2^(s - m), m this far below the maximum: of fp16's exponents P uses those up to 2^15.
+template <bool kHalf>
+constexpr float kDownLog2 = kHalf ? 7.f : 0.f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+struct Job {
+    int batch, nodes, heads, kv_heads, group;
+    int rows, row_groups;       // query rows of a KV head, and groups of 8 NT of them
+    int kg, vg;                 // groups of 32 dims of a K and a V row
+    int k_pitch, v_pitch;       // bytes of a row
+    int context_only, paged, shared_cache, box;
+    CacheView cache;
+    int64_t capacity;
+    const int32_t *lengths, *nodes_len, *mask;
+    int64_t mask_stride;
+    int words;
+    float scale_log2;
+    const uint16_t* q;
+    int64_t q_sb, q_st, q_sh;
+    uint16_t* out;
+    int64_t o_sb, o_st, o_sh;
+    float* lse;
+    float* part_o;              // [2 ctas][8 NT][dim_v]
+    float* part_lse;            // [2 ctas][8 NT], log2
+    int ctas;
+    unsigned int* status;
+    uint64_t wait_ns;
+};
+
+// ------------------------------------------------------------- schedule --
+struct Seq {
+    int len, nodes, end;        // keys: rows [0, end), the context and then the nodes' own
+    int tiles, groups;          // groups of row tiles with live rows
+};
+template <int NT>
+struct Plan {
+    static constexpr int kPieceUnits = 2;
+    const Job& J;
+    int batch, kv_heads, ctas;
+    __device__ __forceinline__ explicit Plan(const Job& j) : J(j), batch(j.batch), kv_heads(j.kv_heads), ctas(j.ctas) {}
+    __device__ __forceinline__ Seq sequence(int b) const {
+        Seq s;
+        s.nodes = J.nodes_len ? min(max(__ldg(J.nodes_len + b), 0), J.nodes) : J.nodes;
+        // A sequence that its cache cannot hold is cut to what fits (and reported).
+        const int64_t own = J.context_only ? 0 : min(int64_t(s.nodes), J.capacity);
+        s.len = int(min(int64_t(max(__ldg(J.lengths + b), 0)), J.capacity - own));
+        s.end = s.len + int(own);
+        s.tiles = (s.end + kKeys - 1) / kKeys;
+        s.groups = (s.nodes * J.group + 8 * NT - 1) / (8 * NT);
+        return s;
+    }
+};
+
+// ---------------------------------------------------------------- layout --
+// The words of a V row that lane row g takes: of every eight groups one, then
+// half, a quarter; of a last single group lanes 0 to 3 one each.
+template <int G>
+struct ValueWords {
+    static constexpr int kOcts = G / 8, kQuad = G / 4 % 2, kPair = G / 2 % 2, kOne = G % 2;
+    static constexpr int kWords = 4 * kOcts + 2 * kQuad + kPair + kOne;
+    __device__ __forceinline__ static constexpr int dim(int i, int g) {
+        return i < 4 * kOcts               ? 256 * (i / 4) + 32 * g + 8 * (i % 4)
+               : i < 4 * kOcts + 2 * kQuad ? 256 * kOcts + 16 * g + 8 * (i - 4 * kOcts)
+               : kPair && i == 4 * kOcts + 2 * kQuad ? 256 * kOcts + 128 * kQuad + 8 * g
+                                           : 256 * kOcts + 128 * kQuad + 64 * kPair + 8 * g;
+    }
+};
+
+template <int G, int NT>
+struct Shape {
+    static constexpr int kWordsV = ValueWords<G>::kWords;
+    // Q operands in registers where there is room for them, else in shared memory.
+    static constexpr bool kQShared = NT * G > 10;
+    static constexpr int kBlocks = G <= 4 ? (NT == 1 ? 4 : 3) : G <= 6 && NT == 1 ? 3 : 2;
+    // What the four warps' O takes when they are added up (over the rings).
+    static constexpr uint32_t kMerge = uint32_t(kWordsV) * 2 * NT * kWarps * 32 * 32;
+    static constexpr uint32_t kQBytes = kQShared ? uint32_t(NT) * G * 512 : 0;
+};
+
+template <int kRows>
+struct Bars {
+    uint64_t full[kWarps][kStages];
+    int abort;
+    Share share;
+    float top[kWarps][kRows], sum[kWarps][kRows];
+};
+template <int G, int NT>
+uint32_t smem_bytes(int k_pitch, int v_pitch) {
+    const uint32_t ring = uint32_t(kWarps * kStages * kSlab) * uint32_t(k_pitch + v_pitch) + 512;    // 512: words behind a short row
+    return 128 + std::max(ring, Shape<G, NT>::kMerge) + Shape<G, NT>::kQBytes + uint32_t(sizeof(Bars<8 * NT>)) + 128;
+}
+
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (kHalf) {
+        __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&v);
+    } else {
+        return pack_bf16x2(lo, hi);
+    }
+}
+// ----------------------------------------------------------------- kernel --
+template <int G, int NT, bool kHalf>
+__global__ void __launch_bounds__(kThreads, Shape<G, NT>::kBlocks)
+cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Job J) {
+    using P = Pair<kHalf>;
+    using VW = ValueWords<G>;
+    using S = Shape<G, NT>;
+    constexpr int kRows = 8 * NT, kWordsV = VW::kWords;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t k_bytes = uint32_t(kSlab * J.k_pitch), stage_bytes = k_bytes + uint32_t(kSlab * J.v_pitch);
+    const uint32_t area = max(uint32_t(kWarps * kStages) * stage_bytes + 512u, S::kMerge);
+    uint8_t* ring = smem + uint32_t(warp * kStages) * stage_bytes;
+    uint4* q_shared = reinterpret_cast<uint4*>(smem + area);
+    Bars<kRows>* bs = reinterpret_cast<Bars<kRows>*>(smem + area + S::kQBytes);
+
+    if (tid < kWarps * kStages) mbar_init(&bs->full[tid / kStages][tid % kStages], 1);
+    if (tid == 0) bs->abort = 0;
+    if (tid < 32) fence_barrier_init();
+    if (tid == 32) {
+        tma_prefetch_desc(&kmap);
+        tma_prefetch_desc(&vmap);
+    }
+    grid_launch_dependents();
+    const Plan<NT> plan(J);
+    if (warp == 0) find_share(plan, &bs->share);
+    __syncthreads();
+    if (int(blockIdx.x) >= bs->share.ctas) return;
+
+    const int boxes = kSlab / J.box;
+    int stage = 0;                               // of the next slab to be used
+    uint32_t lap = 0;
+    uint32_t pending = 0;                        // stages with a load under way
+    bool ok = true;
+    Walk<Plan<NT>> w;
+    w.start(plan, &bs->share);
+    while (w.next(plan)) {
+        // The piece's slabs of this warp: keys [64 tile + 16 warp, + 16), the last may lie behind the keys.
+        const int first_key = w.t0 * kKeys + warp * kSlab;
+        const int slabs = max(0, min(w.t1 - w.t0, (w.s.end - first_key + kKeys - 1) / kKeys));
+        // Where a slab's box of this lane lies: its page (dense: its sequence) and row.  Boxes
+        // past the last used row repeat that row's (they are masked).
+        auto locate = [&](int slab, int& row) {
+            row = first_key + slab * kKeys + lane * J.box;
+            if (!J.paged) return J.shared_cache ? 0 : w.b;
+            int64_t page = 0;
+            if (lane < boxes && slab < slabs) {
+                if (!cache_row(J.cache, w.b, min(row, (w.s.end - 1) / J.box * J.box), page, row)) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+            }
+            return int(page);
+        };
+        auto issue = [&](int st, int page, int row) {
+            uint64_t* bar = &bs->full[warp][st];
+            if (lane == 0) mbar_expect_tx(bar, stage_bytes);
+            __syncwarp();
+            if (lane < boxes) {
+                uint8_t* at = ring + uint32_t(st) * stage_bytes;
+                tma_load_4d(at + lane * J.box * J.k_pitch, &kmap, bar, 0, w.g, row, page);
+                tma_load_4d(at + k_bytes + lane * J.box * J.v_pitch, &vmap, bar, 0, w.g, row, page);
+            }
+            pending |= 1u << st;
+        };
+        if (ok) {
+            int page[kStages], row[kStages];
+#pragma unroll
+            for (int s = 0; s < kStages; ++s) page[s] = locate(s, row[s]);
+#pragma unroll
+            for (int s = 0; s < kStages; ++s)
+                if (s < slabs) issue((stage + s) % kStages, page[s], row[s]);
+        }
+
+        // ---- Q: row g of each row tile, the dims of lane column t ----
+        const int row0 = w.group * kRows;
+        uint4 qf[S::kQShared ? 1 : NT * G];
+        auto load_q = [&](int n, int i) {
+            const int r = row0 + 8 * n + g, d = KeyWords<G>::dim(i, t);
+            if (r >= J.rows || d >= J.kg * kGroupDims) return make_uint4(0, 0, 0, 0);
+            const int node = r / J.group, h = w.g * J.group + r - node * J.group;
+            return __ldg(reinterpret_cast<const uint4*>(J.q + w.b * J.q_sb + node * J.q_st + h * J.q_sh + d));
+        };
+        if constexpr (S::kQShared) {
+            for (int i = warp; i < NT * G; i += kWarps) q_shared[i * 32 + lane] = load_q(i / G, i % G);
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < G; ++i) qf[n * G + i] = load_q(n, i);
+        }
+        float o[4 * kWordsV][NT][4];
+#pragma unroll
+        for (int m = 0; m < 4 * kWordsV; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
+        // Of the rows 2t and 2t + 1 of each row tile.
+        float top[NT][2], sum[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            top[n][0] = top[n][1] = -INFINITY;
+            sum[n][0] = sum[n][1] = 0.f;
+        }
+
+        for (int i = 0; i < slabs && ok; ++i) {
+            const int key0 = first_key + i * kKeys;
+            int next_row;
+            const int next_page = locate(i + kStages, next_row);
+            if (!(ok = warp_wait(&bs->full[warp][stage], lap, bs, J))) break;
+            pending &= ~(1u << stage);
+            const uint8_t* ks = ring + uint32_t(stage) * stage_bytes;
+            const uint8_t* vs = ks + k_bytes;
+
+            // ---- S ----
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            const uint8_t *k0 = ks + g * J.k_pitch, *k1 = k0 + 8 * J.k_pitch;
+            key_products<G, NT, kHalf>(s, k0, k1, J.kg, t, [&](int n, int i) {
+                if constexpr (S::kQShared) return q_shared[(n * G + i) * 32 + lane];
+                else return qf[n * G + i];
+            });
+
+            // ---- what the rows see of the slab's keys (g and g + 8 here) ----
+            auto seen_of = [&](int r) {
+                const int node = r / J.group;
+                if (node >= w.s.nodes) return 0u;
+                if (J.context_only) return low_bits(w.s.end - key0);
+                const int32_t* words = J.mask ? J.mask + w.b * J.mask_stride + int64_t(node) * J.words : nullptr;
+                return seen_keys(words, J.words, node, w.s.end - w.s.len, key0 - w.s.len);
+            };
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] *= J.scale_log2;
+            const bool whole_slab = key0 + kSlab <= w.s.len;
+            if (!whole_slab) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t seen = seen_of(row0 + 8 * n + 2 * t + e) >> g;
+                        if (!(seen & 1u)) s[n][e] = -INFINITY;
+                        if (!(seen & 256u)) s[n][2 + e] = -INFINITY;
+                    }
+            }
+
+            // ---- softmax ----
+            bool grown = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) grown |= s[n][e] > top[n][e & 1] + (kLazyLog2 + kDownLog2<kHalf>);
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float alpha[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(s[n][e], s[n][2 + e]);
+#pragma unroll
+                        for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+                        const float m = fmaxf(top[n][e], mx - kDownLog2<kHalf>);
+                        alpha[e] = top[n][e] == m ? 1.f : sfu_exp2(top[n][e] - m);      // (both may be -inf)
+                        top[n][e] = m;
+                        sum[n][e] *= alpha[e];
+                    }
+#pragma unroll
+                    for (int m = 0; m < 4 * kWordsV; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[m][n][e] *= alpha[e & 1];
+                }
+            }
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = sfu_exp2(s[n][e] - (top[n][e & 1] == -INFINITY ? 0.f : top[n][e & 1]));
+                sum[n][0] += p[0] + p[2];
+                sum[n][1] += p[1] + p[3];
+                pf[n][0] = transpose8x8(pack2<kHalf>(p[0], p[1]));
+                pf[n][1] = transpose8x8(pack2<kHalf>(p[2], p[3]));
+            }
+
+            // ---- O: the keys 2t, 2t + 1, 2t + 8, 2t + 9 and the dims of lane row g.  A key that
+            // nobody sees counts as zero (its P is 0, and 0 x NaN is not 0); so does a group of a
+            // node's row that is NaN, which the rows that see it get afterwards. ----
+            const uint32_t live = low_bits(w.s.end - key0);
+            const bool nodes_here = !J.context_only && key0 + kSlab > w.s.len;
+            auto pair_of = [&](int key, int grp) { return *reinterpret_cast<const uint32_t*>(vs + key * J.v_pitch + 16 * J.vg + 4 * grp); };
+            bool bad = false;
+            if (nodes_here) {
+                for (int k = lane; k < kSlab * J.vg; k += 32)
+                    if (live >> (k / J.vg) & 1) bad |= !P::finite(pair_of(k / J.vg, k % J.vg));
+                bad = __any_sync(0xffffffffu, bad);
+            }
+            const uint8_t* v0 = vs + 2 * t * J.v_pitch;
+            {
+                auto value_words = [&](auto width, int i0) {
+                    constexpr int W = decltype(width)::value;
+                    const int d0 = VW::dim(i0, g), grp = d0 / kGroupDims;
+                    const int at = J.vg * 16 + 4 * min(grp, J.vg - 1);
+                    uint32_t a[4][W], p[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint8_t* row = v0 + ((k & 1) + 8 * (k >> 1)) * J.v_pitch;
+                        load_words<W>(row + d0 / 2, a[k]);
+                        p[k] = *reinterpret_cast<const uint32_t*>(row + at);
+                        if (grp >= J.vg) p[k] = 0;
+                    }
+                    if (!whole_slab) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (!(live >> (2 * t + (k & 1) + 8 * (k >> 1)) & 1) || (nodes_here && !P::finite(p[k]))) p[k] = 0;
+                    }
+                    const auto sc0 = P::as(low_halves(p[0], p[1])), lo0 = P::as(high_halves(p[0], p[1]));
+                    const auto sc1 = P::as(low_halves(p[2], p[3])), lo1 = P::as(high_halves(p[2], p[3]));
+#pragma unroll
+                    for (int k = 0; k < W; ++k) {
+                        // The codes of the even and of the odd dims, a key in each half.
+                        const uint32_t x0 = low_halves(a[0][k], a[1][k]), y0 = high_halves(a[0][k], a[1][k]);
+                        const uint32_t x1 = low_halves(a[2][k], a[3][k]), y1 = high_halves(a[2][k], a[3][k]);
+                        auto pair = [&](auto which) {
+                            constexpr int j = decltype(which)::value;
+                            const uint32_t x[4] = {P::template values<j>(x0, sc0, lo0), P::template values<j>(y0, sc0, lo0),
+                                                   P::template values<j>(x1, sc1, lo1), P::template values<j>(y1, sc1, lo1)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma<kHalf>(o[4 * (i0 + k) + j][n], x, pf[n][0], pf[n][1]);
+                        };
+                        pair(std::integral_constant<int, 0>());
+                        pair(std::integral_constant<int, 1>());
+                        pair(std::integral_constant<int, 2>());
+                        pair(std::integral_constant<int, 3>());
+                    }
+                };
+#pragma unroll
+                for (int c = 0; c < VW::kOcts; ++c) value_words(std::integral_constant<int, 4>(), 4 * c);
+                if constexpr (VW::kQuad != 0) value_words(std::integral_constant<int, 2>(), 4 * VW::kOcts);
+                if constexpr (VW::kPair != 0) value_words(std::integral_constant<int, 1>(), 4 * VW::kOcts + 2 * VW::kQuad);
+                if constexpr (VW::kOne != 0) value_words(std::integral_constant<int, 1>(), 4 * VW::kOcts + 2 * VW::kQuad + VW::kPair);
+            }
+            if (bad) {
+#pragma unroll 1
+                for (int k = 0; k < kSlab * J.vg; ++k) {
+                    const int key = k / J.vg, grp = k % J.vg;
+                    if (!(live >> key & 1) || P::finite(pair_of(key, grp))) continue;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (seen_of(row0 + 8 * n + 2 * t + e) >> key & 1) {
+#pragma unroll
+                                for (int m = 0; m < 4 * kWordsV; ++m)
+                                    if (VW::dim(m / 4, g) / kGroupDims == grp) o[m][n][e] = o[m][n][2 + e] = NAN;
+                            }
+                }
+            }
+            __syncwarp();
+            if (i + kStages < slabs) issue(stage, next_page, next_row);
+            if (++stage == kStages) { stage = 0; lap ^= 1; }
+        }
+
+        // ---- the piece's end: the warps' O to a common maximum, added up ----
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], k);
+                if (g == 0) {
+                    bs->top[warp][8 * n + 2 * t + e] = top[n][e];
+                    bs->sum[warp][8 * n + 2 * t + e] = sum[n][e];
+                }
+            }
+        __syncthreads();                         // (every slab has been used: the rings are free)
+        auto row_total = [&](int r, float& m) {
+            m = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) m = fmaxf(m, bs->top[k][r]);
+            float l = 0.f;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const float x = bs->top[k][r];
+                l += x == -INFINITY ? bs->sum[k][r] : bs->sum[k][r] * sfu_exp2(x - m);    // (a NaN sum stays)
+            }
+            return l;
+        };
+        float4* merge = reinterpret_cast<float4*>(smem);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float m;
+                const float l = row_total(8 * n + 2 * t + e, m);
+                const float f = l == 0.f ? 0.f : top[n][e] == -INFINITY ? 0.f / l : sfu_exp2(top[n][e] - m) / l;
+#pragma unroll
+                for (int k = 0; k < kWordsV; ++k)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        merge[((((k * NT + n) * 2 + e) * 2 + half) * kWarps + warp) * 32 + lane] =
+                            make_float4(o[4 * k + 2 * half][n][e] * f, o[4 * k + 2 * half][n][2 + e] * f,
+                                        o[4 * k + 2 * half + 1][n][e] * f, o[4 * k + 2 * half + 1][n][2 + e] * f);
+            }
+        __syncthreads();
+        const bool whole = w.whole();
+        const int slot = 2 * blockIdx.x + (w.piece > 0);
+        if (ok) {
+            for (int u = warp; u < kWordsV * NT * 2; u += kWarps) {
+                const int k = u / (2 * NT), n = u / 2 % NT, e = u & 1, r = row0 + 8 * n + 2 * t + e;
+                int d = 0;
+#pragma unroll
+                for (int i = 0; i < kWordsV; ++i)
+                    if (i == k) d = VW::dim(i, g);
+                float4 x[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    x[half] = merge[((u * 2 + half) * kWarps) * 32 + lane];
+#pragma unroll
+                    for (int v = 1; v < kWarps; ++v) {
+                        const float4 y = merge[((u * 2 + half) * kWarps + v) * 32 + lane];
+                        x[half].x += y.x; x[half].y += y.y; x[half].z += y.z; x[half].w += y.w;
+                    }
+                }
+                if (r >= J.rows || d >= J.vg * kGroupDims) continue;
+                const int node = r / J.group, h = w.g * J.group + r - node * J.group;
+                if (whole) {
+                    uint4 y = make_uint4(0, 0, 0, 0);
+                    if (node < w.s.nodes)
+                        y = make_uint4(pack2<kHalf>(x[0].x, x[0].y), pack2<kHalf>(x[0].z, x[0].w), pack2<kHalf>(x[1].x, x[1].y),
+                                       pack2<kHalf>(x[1].z, x[1].w));
+                    *reinterpret_cast<uint4*>(J.out + w.b * J.o_sb + node * J.o_st + h * J.o_sh + d) = y;
+                } else {
+                    float4* part = reinterpret_cast<float4*>(J.part_o + (int64_t(slot) * kRows + r - row0) * (J.vg * kGroupDims) + d);
+                    part[0] = x[0];
+                    part[1] = x[1];
+                }
+            }
+            if (tid < kRows && row0 + tid < J.rows) {
+                float m;
+                const float l = row_total(tid, m);
+                const int r = row0 + tid, node = r / J.group, h = w.g * J.group + r - node * J.group;
+                const float lse2 = l == 0.f || node >= w.s.nodes ? -INFINITY : m + log2f(l);
+                if (whole) J.lse[(int64_t(w.b) * J.nodes + node) * J.heads + h] = lse2 * kLn2;
+                else J.part_lse[int64_t(slot) * kRows + tid] = lse2;
+            }
+        }
+        fence_async_shared();                    // the merge's stores before the next piece's copies
+        __syncthreads();
+    }
+    // After a wait that ran out copies may still be under way.
+    if (bs->abort && lane == 0)
+        for (int s = 0; s < kStages; ++s)
+            if (pending >> s & 1) {
+                mbar_wait(&bs->full[warp][s], 0, 100000000ull);
+                mbar_wait(&bs->full[warp][s], 1, 100000000ull);
+            }
+}
+
+// Merges the pieces of a segment's rows (a block each), and writes the rows
+// that see nothing.  The four warps take the pieces by turns, a lane four dims.
+template <int NT, bool kHalf>
+__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Job J) {
+    constexpr int kRows = 8 * NT;
+    __shared__ int range[3];                // first and last CTA of the segment's pieces, slot of the first
+    __shared__ float4 acc[4][kMaxDims4 / 4];
+    __shared__ float tops[4], sums[4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int at = blockIdx.x;
+    const int group = at % J.row_groups;
+    at /= J.row_groups;
+    const int g = at % J.kv_heads, b = at / J.kv_heads, r = group * kRows + blockIdx.y;
+    const Plan<NT> plan(J);
+    const Seq s = plan.sequence(b);
+    const bool some = group < s.groups && s.tiles > 0;
+    if (some && warp == 0) {
+        uint32_t total, before;
+        sum_units(plan, b, total, before);
+        if (lane == 0) {
+            const uint32_t units = segment_units(plan, s), u0 = before + uint32_t(g * s.groups + group) * units;
+            const uint32_t ctas = share_count(total, J.ctas), c0 = share_of(total, u0 + Plan<NT>::kPieceUnits, ctas);
+            range[0] = int(c0);
+            range[1] = int(share_of(total, u0 + units - 1, ctas));
+            range[2] = 2 * int(c0) + (share_begin(total, c0, ctas) < u0 ? 1 : 0);   // a piece of another segment before it
+        }
+    }
+    if (tid == 32 && g == 0 && group == 0 && blockIdx.y == 0) {
+        const int len = __ldg(J.lengths + b), nodes = J.nodes_len ? __ldg(J.nodes_len + b) : J.nodes;
+        if (len != s.len || nodes != s.nodes || (!J.context_only && s.end != s.len + s.nodes)) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+    }
+    __syncthreads();
+    const int c0 = some ? range[0] : 0, c1 = some ? range[1] : 0, slot0 = some ? range[2] : 0;
+    grid_dependency_wait();                 // every block: what follows this grid counts on the one before it too
+    if (r >= J.rows || (some && c0 == c1)) return;
+    const int node = r / J.group, h = g * J.group + r - node * J.group, dims = J.vg * kGroupDims;
+    uint16_t* out = J.out + b * J.o_sb + node * J.o_st + h * J.o_sh;
+    float* lse = J.lse + (int64_t(b) * J.nodes + node) * J.heads + h;
+    if (!some || node >= s.nodes) {
+        for (int d = 8 * tid; d < dims; d += 8 * 128) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
+        if (tid == 0) *lse = -INFINITY;
+        return;
+    }
+    // In one pass, the largest exponent so far taken out: a piece's lse and rows are one latency.
+    constexpr int kAhead = 4, kSpan = (kMaxDims4 + 127) / 128;
+    float m = -INFINITY, sum = 0.f;
+    float4 x[kSpan];
+#pragma unroll
+    for (int k = 0; k < kSpan; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0 + warp; c <= c1; c += 4 * kAhead) {
+        float w[kAhead];
+        float4 y[kAhead][kSpan];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            w[a] = -INFINITY;
+            const int cc = c + 4 * a;
+            if (cc > c1) continue;
+            const int64_t row = int64_t(cc == c0 ? slot0 : 2 * cc) * kRows + blockIdx.y;
+            w[a] = __ldcg(J.part_lse + row);
+#pragma unroll
+            for (int k = 0; k < kSpan; ++k)
+                if (4 * lane + 128 * k < dims) y[a][k] = __ldcg(reinterpret_cast<const float4*>(J.part_o + row * dims) + lane + 32 * k);
+        }
+        const float before = m;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) m = fmaxf(m, w[a]);
+        const float shift = m == -INFINITY ? 0.f : m, old = before == -INFINITY ? 0.f : sfu_exp2(before - shift);
+        if (before != -INFINITY) {
+            sum *= old;
+#pragma unroll
+            for (int k = 0; k < kSpan; ++k) { x[k].x *= old; x[k].y *= old; x[k].z *= old; x[k].w *= old; }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const float f = sfu_exp2(w[a] - shift);
+            sum += f;
+            if (f == 0.f) continue;             // (a piece without weight: its rows stay out)
+#pragma unroll
+            for (int k = 0; k < kSpan; ++k)
+                if (4 * lane + 128 * k < dims) {
+                    x[k].x = fmaf(f, y[a][k].x, x[k].x); x[k].y = fmaf(f, y[a][k].y, x[k].y);
+                    x[k].z = fmaf(f, y[a][k].z, x[k].z); x[k].w = fmaf(f, y[a][k].w, x[k].w);
+                }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSpan; ++k)
+        if (4 * lane + 128 * k < dims) acc[warp][lane + 32 * k] = x[k];
+    if (lane == 0) { tops[warp] = m; sums[warp] = sum; }
+    __syncthreads();
+    const float all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), shift = all == -INFINITY ? 0.f : all;
+    float f[4], l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        f[k] = tops[k] == -INFINITY ? (sums[k] == 0.f ? 0.f : sums[k]) : sfu_exp2(tops[k] - shift);     // (NaN stays)
+        l += tops[k] == -INFINITY ? sums[k] : f[k] * sums[k];
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    for (int d = 8 * tid; d < dims; d += 8 * 128) {
+        float4 y[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            y[half] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (f[k] == 0.f) continue;
+                const float4 z = acc[k][d / 4 + half];
+                y[half].x = fmaf(f[k], z.x, y[half].x); y[half].y = fmaf(f[k], z.y, y[half].y);
+                y[half].z = fmaf(f[k], z.z, y[half].z); y[half].w = fmaf(f[k], z.w, y[half].w);
+            }
+        }
+        *reinterpret_cast<uint4*>(out + d) =
+            make_uint4(pack2<kHalf>(y[0].x * inv, y[0].y * inv), pack2<kHalf>(y[0].z * inv, y[0].w * inv),
+                       pack2<kHalf>(y[1].x * inv, y[1].y * inv), pack2<kHalf>(y[1].z * inv, y[1].w * inv));
+    }
+    if (tid == 0) *lse = l != 0.f ? (shift + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// ------------------------------------------------------------------- host --
+// Two row tiles to a segment where there are rows for them: K and V are read, and their codes
+// turned into operands, once for 16 rows.
+int row_tiles(const slimkv_tree_attention_args* a) { return a->nodes * (a->heads / a->kv_heads) > 8 ? 2 : 1; }
+// Instantiated row lengths in groups of 32 dims (1, 7 and 9 take the next).
+int groups_of(const slimkv_tree_attention_args* a) {
+    const int g = (std::max(a->dim_qk, a->dim_v) + kGroupDims - 1) / kGroupDims;
+    return g == 1 ? 2 : g == 7 ? 8 : g == 9 ? 10 : g;
+}
+
+int check_attention4(const slimkv_tree_attention_args* a) {
+    if (!a) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "null arguments");
+    if (a->batch < 1 || a->batch > 4096 || a->nodes < 1 || a->nodes > 1024 || a->heads < 1 || a->kv_heads < 1 ||
+        a->heads % a->kv_heads)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "4-bit attention: batch in 1..4096, nodes in 1..1024, heads a multiple of kv_heads");
+    if (a->heads / a->kv_heads > 128)
+        return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "4-bit attention: at most 128 query heads per KV head");
+    for (int dim : {a->dim_qk, a->dim_v})
+        if (dim < kGroupDims || dim > kMaxDims4 || dim % kGroupDims)
+            return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "4-bit attention: dims must be multiples of 32 up to 320");
+    if (a->type != SLIMKV_BF16 && a->type != SLIMKV_FP16)
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "4-bit attention: bf16 or fp16 tensors");
+    return SLIMKV_OK;
+}
+
+// Calls f(G, NT) with the constants of a call's kernel.
+template <class F>
+auto with_shape(const slimkv_tree_attention_args* a, F f) {
+    using std::integral_constant;
+    auto rows = [&](auto g) {
+        return row_tiles(a) == 2 ? f(g, integral_constant<int, 2>()) : f(g, integral_constant<int, 1>());
+    };
+    switch (groups_of(a)) {
+        case 2: return rows(integral_constant<int, 2>());
+        case 3: return rows(integral_constant<int, 3>());
+        case 4: return rows(integral_constant<int, 4>());
+        case 5: return rows(integral_constant<int, 5>());
+        case 6: return rows(integral_constant<int, 6>());
+        case 8: return rows(integral_constant<int, 8>());
+        default: return rows(integral_constant<int, 10>());
+    }
+}
+
+void carve(Carver& c, const slimkv_tree_attention_args* a, Job& J) {
+    J.ctas = device_info().sm_count * with_shape(a, [](auto g, auto nt) { return Shape<decltype(g)::value, decltype(nt)::value>::kBlocks; });
+    const size_t rows = size_t(2) * J.ctas * 8 * row_tiles(a);
+    J.part_o = c.take<float>(rows * a->dim_v);
+    J.part_lse = c.take<float>(rows);
+}
+
+template <int G, int NT, bool kHalf>
+int launch(const CUtensorMap& km, const CUtensorMap& vm, const Job& J, cudaStream_t stream) {
+    auto kernel = cache4_attention_kernel<G, NT, kHalf>;
+    const uint32_t bytes = smem_bytes<G, NT>(J.k_pitch, J.v_pitch);
+    static bool configured[64] = {};
+    const int dev = device_info().device;
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 int(smem_bytes<G, NT>(row4_bytes(G * kGroupDims), row4_bytes(G * kGroupDims)))) != cudaSuccess)
+            return fail(SLIMKV_ERR_CUDA, "cudaFuncSetAttribute (4-bit attention) failed");
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    kernel<<<J.ctas, kThreads, bytes, stream>>>(km, vm, J);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(J.batch * J.kv_heads * J.row_groups, std::min(8 * NT, J.rows));
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute dependent{};
+    dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dependent.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &dependent;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, combine_kernel<NT, kHalf>, J);
+    return e == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "4-bit attention launch failed: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace slimkv
+
+using namespace slimkv;
+
+extern "C" size_t slimkv_cache4_attention_workspace_size(const slimkv_tree_attention_args* a) {
+    if (check_attention4(a) != SLIMKV_OK) return 0;
+    Job J{};
+    Carver c(nullptr, 0);
+    carve(c, a, J);
+    return c.used;
+}
+
+extern "C" int slimkv_cache4_attention(const slimkv_tree_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_attention4(a)) return rc;
+    if (!a->q || !a->lengths || !a->out || !a->lse) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "4-bit attention: null pointer");
+    if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(SLIMKV_ERR_INVALID_ARGUMENT, "4-bit attention: scale must be positive");
+    const int k_pitch = row4_bytes(a->dim_qk), v_pitch = row4_bytes(a->dim_v);
+    if (int rc = check_cache(a->cache, a->batch, k_pitch, v_pitch, 1, true, "4-bit attention")) return rc;
+    for (int i = 0; i < 3; ++i)
+        if (a->q_stride[i] % 8 || a->out_stride[i] % 8)
+            return fail(SLIMKV_ERR_ALIGNMENT, "4-bit attention: strides must be multiples of 8 elements");
+    if (!aligned16(a->q) || !aligned16(a->out)) return fail(SLIMKV_ERR_ALIGNMENT, "4-bit attention: 16-byte aligned tensors");
+    const slimkv_cache& cache = a->cache;
+    const bool paged = cache.table != nullptr;
+    if (paged && cache.rows % 8) return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "4-bit attention: pages of a multiple of 8 rows");
+    Job J{};
+    Carver c(workspace, workspace_bytes);
+    carve(c, a, J);
+    if (!workspace || !c.fits() || !aligned16(workspace))
+        return fail(SLIMKV_ERR_WORKSPACE, "4-bit attention: %zu bytes of 16-byte aligned workspace needed", c.used);
+    // A box of TMA rows stays inside a page.
+    J.box = paged && cache.rows % kSlab ? 8 : kSlab;
+    J.shared_cache = !paged && cache.k_stride[0] == 0 && cache.v_stride[0] == 0;
+    if (a->batch > 1 && !paged && !J.shared_cache && (cache.k_stride[0] == 0 || cache.v_stride[0] == 0))
+        return fail(SLIMKV_ERR_INVALID_ARGUMENT, "4-bit attention: K and V are both shared by the batch or neither");
+    const uint64_t planes = paged ? uint64_t(cache.num_pages) : J.shared_cache ? 1 : uint64_t(a->batch);
+    // One tensor map {row, heads, rows, planes}; a dimension of one (or shared) entry takes any valid stride.
+    auto encode = [&](CUtensorMap* m, const void* base, int pitch, const int64_t* st) {
+        return encode_map_words_4d(m, base, pitch / 4, a->kv_heads, cache.rows, planes, a->kv_heads > 1 ? st[2] : pitch,
+                                   cache.rows > 1 ? st[1] : pitch, planes > 1 ? st[0] : pitch, J.box);
+    };
+    CUtensorMap km, vm;
+    int rc;
+    if ((rc = encode(&km, cache.k, k_pitch, cache.k_stride)) || (rc = encode(&vm, cache.v, v_pitch, cache.v_stride))) return rc;
+    J.batch = a->batch;
+    J.nodes = a->nodes;
+    J.heads = a->heads;
+    J.kv_heads = a->kv_heads;
+    J.group = a->heads / a->kv_heads;
+    J.rows = a->nodes * J.group;
+    const int nt = row_tiles(a);
+    J.row_groups = (J.rows + 8 * nt - 1) / (8 * nt);
+    J.kg = a->dim_qk / kGroupDims;
+    J.vg = a->dim_v / kGroupDims;
+    J.k_pitch = k_pitch;
+    J.v_pitch = v_pitch;
+    J.context_only = a->context_only;
+    J.paged = paged;
+    J.cache = cache_view(cache);
+    J.capacity = cache_capacity(J.cache);
+    if (double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / kKeys + 1 + Plan<1>::kPieceUnits) >= 2147483648.0)
+        return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "4-bit attention: too many rows in one call");
+    J.lengths = a->lengths;
+    J.nodes_len = a->nodes_len;
+    J.mask = a->context_only ? nullptr : a->mask;
+    J.mask_stride = a->mask_stride;
+    J.words = (a->nodes + 31) / 32;
+    J.scale_log2 = a->scale * kLog2e;
+    J.q = static_cast<const uint16_t*>(a->q);
+    J.q_sb = a->q_stride[0]; J.q_st = a->q_stride[1]; J.q_sh = a->q_stride[2];
+    J.out = static_cast<uint16_t*>(a->out);
+    J.o_sb = a->out_stride[0]; J.o_st = a->out_stride[1]; J.o_sh = a->out_stride[2];
+    J.lse = a->lse;
+    J.status = status_word();
+    J.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool half = a->type == SLIMKV_FP16;
+    return with_shape(a, [&](auto g, auto nt) {
+        constexpr int kG = decltype(g)::value, kNt = decltype(nt)::value;
+        return half ? launch<kG, kNt, true>(km, vm, J, st) : launch<kG, kNt, false>(km, vm, J, st);
+    });
+}

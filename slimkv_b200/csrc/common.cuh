@@ -336,6 +336,14 @@ __device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The 8 x 8 matrix of 16-bit elements that a warp holds (lane 4r + c: row r,
+// columns 2c and 2c + 1), transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // Byte offset of element (row, col) inside a [rows x 64] bf16 tile stored
 // with the TMA 128-byte swizzle: 16-byte unit u of row r lives at unit
 // u ^ (r % 8).  Tiles start on 1024-byte boundaries.

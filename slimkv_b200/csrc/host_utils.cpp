@@ -78,6 +78,25 @@ int encode_map_4d_box(CUtensorMap* map, const void* base, uint64_t d0, uint64_t 
     return SLIMKV_OK;
 }
 
+int encode_map_words_4d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t d3,
+                        uint64_t s1, uint64_t s2, uint64_t s3, uint32_t box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return fail(SLIMKV_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[4] = {d0, d1, d2, d3};
+    cuuint64_t strides[3] = {s1, s2, s3};
+    cuuint32_t box[4] = {cuuint32_t(d0), 1, box_rows, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(SLIMKV_ERR_TENSOR_MAP,
+                    "cuTensorMapEncodeTiled (words) failed (%d): dims {%llu,%llu,%llu,%llu} strides {%llu,%llu,%llu}", int(r),
+                    (unsigned long long)d0, (unsigned long long)d1, (unsigned long long)d2, (unsigned long long)d3,
+                    (unsigned long long)s1, (unsigned long long)s2, (unsigned long long)s3);
+    return SLIMKV_OK;
+}
+
 int encode_map_f32_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1,
                       uint64_t s2, uint32_t box0, uint32_t box1) {
     auto fn = encode_fn();

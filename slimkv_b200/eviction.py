@@ -28,6 +28,36 @@ def _plane(t, dtype, device, batch, heads, rows, strides, what):
     return t.data_ptr()
 
 
+def mass_args(q, k, lse, mass, lengths, scale, rows, counts, decay, block_tables, context_only, wait_limit_ns,
+              cache_type=None, cache_dim=None):
+    """``slimkv_key_mass_args`` of a call.  ``cache_type``: that of the keys'
+    elements (default: q's), ``cache_dim`` of them a row (default: the queries')."""
+    kind = q.dtype
+    if not (q.is_cuda and q.dim() == 4 and kind in (torch.bfloat16, torch.float16)):
+        _refuse('q must be bf16 or fp16 [B, T, H, D] on CUDA')
+    batch, t, heads, dim = q.shape
+    qs, dev = q.stride(), q.device
+    _check_rows(k, k, 4)
+    if qs[3] != 1 or k.dtype != (cache_type or kind) or k.shape[3] != (cache_dim or dim) or k.device != dev:
+        _refuse('q needs a contiguous last dimension, and a cache of its type, dim and device')
+    if not (lse.device == dev and lse.dtype == torch.float32 and lse.shape == (batch, t, heads) and lse.is_contiguous()):
+        _refuse('lse must be contiguous fp32 [B, T, H] on q\'s device')
+    a = _lib.KeyMassArgs()
+    fill_cache(a.cache, k, k, block_tables, batch)
+    kv_heads = k.shape[2]
+    a.batch, a.nodes, a.heads, a.kv_heads, a.dim, a.type = batch, t, heads, kv_heads, dim, _TYPES[kind]
+    a.q, a.lse, a.lengths = q.data_ptr(), lse.data_ptr(), _i32(lengths, (batch,), dev, 'lengths')
+    x = a.q_stride
+    x[0], x[1], x[2] = qs[:3]
+    if rows is not None:
+        a.rows = _i32(rows, (batch, t), dev, 'rows')
+    if counts is not None:
+        a.counts = _i32(counts, (batch,), dev, 'counts')
+    a.mass = _plane(mass, torch.float32, dev, batch, kv_heads, 0, a.mass_stride, 'mass')
+    a.mass_rows, a.context_only, a.scale, a.decay, a.wait_limit_ns = mass.shape[2], bool(context_only), scale, decay, wait_limit_ns
+    return a
+
+
 def key_mass(q, k, lse, mass, lengths, scale, rows=None, counts=None, decay=1.0, block_tables=None,
              context_only=False, wait_limit_ns=0):
     """Accumulates attention weights per key, in place (``slimkv_key_mass``).
@@ -47,30 +77,8 @@ def key_mass(q, k, lse, mass, lengths, scale, rows=None, counts=None, decay=1.0,
     ``nodes`` and every row counts, ``counts=nodes`` does.  Other entries of
     ``mass`` keep their values.  Returns ``mass``.
     """
-    kind = q.dtype
-    if not (q.is_cuda and q.dim() == 4 and kind in (torch.bfloat16, torch.float16)):
-        _refuse('q must be bf16 or fp16 [B, T, H, D] on CUDA')
-    batch, t, heads, dim = q.shape
-    qs, dev = q.stride(), q.device
-    _check_rows(k, k, 4)
-    if qs[3] != 1 or k.dtype != kind or k.shape[3] != dim or k.device != dev:
-        _refuse('q needs a contiguous last dimension, and a cache of its type, dim and device')
-    if not (lse.device == dev and lse.dtype == torch.float32 and lse.shape == (batch, t, heads) and lse.is_contiguous()):
-        _refuse('lse must be contiguous fp32 [B, T, H] on q\'s device')
-    a = _lib.KeyMassArgs()
-    fill_cache(a.cache, k, k, block_tables, batch)
-    kv_heads = k.shape[2]
-    a.batch, a.nodes, a.heads, a.kv_heads, a.dim, a.type = batch, t, heads, kv_heads, dim, _TYPES[kind]
-    a.q, a.lse, a.lengths = q.data_ptr(), lse.data_ptr(), _i32(lengths, (batch,), dev, 'lengths')
-    x = a.q_stride
-    x[0], x[1], x[2] = qs[:3]
-    if rows is not None:
-        a.rows = _i32(rows, (batch, t), dev, 'rows')
-    if counts is not None:
-        a.counts = _i32(counts, (batch,), dev, 'counts')
-    a.mass = _plane(mass, torch.float32, dev, batch, kv_heads, 0, a.mass_stride, 'mass')
-    a.mass_rows, a.context_only, a.scale, a.decay, a.wait_limit_ns = mass.shape[2], bool(context_only), scale, decay, wait_limit_ns
-    _run(dev, _lib.load().slimkv_key_mass, byref(a))
+    a = mass_args(q, k, lse, mass, lengths, scale, rows, counts, decay, block_tables, context_only, wait_limit_ns)
+    _run(q.device, _lib.load().slimkv_key_mass, byref(a))
     return mass
 
 

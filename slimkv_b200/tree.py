@@ -112,33 +112,22 @@ def tree_masks(parents):
     return out
 
 
-def tree_attention(q, k, v, lengths, scale, mask=None, nodes=None, block_tables=None, context_only=False, out=None,
-                   lse=None, wait_limit_ns=0):
-    """Attention of drafted nodes over a cache (``slimkv_tree_attention``).
-
-    ``q [B, T, H, D]`` (bf16 or fp16, rotated); ``k`` / ``v`` dense ``[B, rows,
-    Hkv, D / Dv]`` (``[1, ...]``: shared) or pages ``[n, page, Hkv, ...]`` with
-    int32 ``block_tables [B, pages]``.  Node t of sequence b sees the
-    ``lengths[b]`` (int32) context rows and, of the rows ``lengths[b] + i``
-    that hold the nodes' own K/V, those whose bit is set in ``mask`` (int32
-    ``[B or 1, T, (T + 31) // 32]``, :func:`tree_masks`); without a mask the
-    nodes are a chain (a single token: T = 1).  ``nodes`` (int32 ``[B]``)
-    limits a sequence to its first nodes.  ``context_only``: the cache holds no
-    rows of the nodes (Beacon latents: absorbed queries, one KV head).
-    Returns ``(out [B, T, H, Dv], lse [B, T, H] fp32 natural log)``; a row that
-    sees nothing gets zeros and -inf.  Dims: multiples of 8 up to 320.
-    """
+def attention_args(q, k, v, lengths, scale, mask, nodes, block_tables, context_only, out, lse, wait_limit_ns,
+                   cache_type=None, dim_qk=None, dim_v=None):
+    """``slimkv_tree_attention_args`` of a call, with its outputs: ``(args, out,
+    lse)``.  ``cache_type``: that of the caches' elements (default: q's), whose
+    rows have ``dim_qk`` / ``dim_v`` elements (default: the queries' and V's)."""
     kind = q.dtype
     if not (q.is_cuda and q.dim() == 4 and kind in (torch.bfloat16, torch.float16)):
         _refuse('q must be bf16 or fp16 [B, T, H, D] on CUDA')
     batch, t, heads, dim = q.shape
     qs, dev = q.stride(), q.device
     _check_rows(k, v, 4)
-    if qs[3] != 1 or k.dtype != kind or k.shape[3] != dim or k.device != dev:
+    if qs[3] != 1 or k.dtype != (cache_type or kind) or k.shape[3] != (dim_qk or dim) or k.device != dev:
         _refuse('q needs a contiguous last dimension, and caches of its type, dim and device')
     a = _lib.TreeAttentionArgs()
     fill_cache(a.cache, k, v, block_tables, batch)
-    dim_v = v.shape[3]
+    dim_v = dim_v or v.shape[3]
     if out is None:
         out = torch.empty_strided((batch, t, heads, dim_v), (t * heads * dim_v, heads * dim_v, dim_v, 1), dtype=kind, device=dev)
     elif not (out.shape == (batch, t, heads, dim_v) and out.dtype == kind and out.device == dev and out.stride(3) == 1):
@@ -164,8 +153,28 @@ def tree_attention(q, k, v, lengths, scale, mask=None, nodes=None, block_tables=
         a.mask = _i32(mask, (many, t, (t + 31) // 32), dev, 'mask')
         a.mask_stride = mask.stride(0) if many > 1 else 0
     a.context_only, a.scale, a.wait_limit_ns = bool(context_only), scale, wait_limit_ns
+    return a, out, lse
+
+
+def tree_attention(q, k, v, lengths, scale, mask=None, nodes=None, block_tables=None, context_only=False, out=None,
+                   lse=None, wait_limit_ns=0):
+    """Attention of drafted nodes over a cache (``slimkv_tree_attention``).
+
+    ``q [B, T, H, D]`` (bf16 or fp16, rotated); ``k`` / ``v`` dense ``[B, rows,
+    Hkv, D / Dv]`` (``[1, ...]``: shared) or pages ``[n, page, Hkv, ...]`` with
+    int32 ``block_tables [B, pages]``.  Node t of sequence b sees the
+    ``lengths[b]`` (int32) context rows and, of the rows ``lengths[b] + i``
+    that hold the nodes' own K/V, those whose bit is set in ``mask`` (int32
+    ``[B or 1, T, (T + 31) // 32]``, :func:`tree_masks`); without a mask the
+    nodes are a chain (a single token: T = 1).  ``nodes`` (int32 ``[B]``)
+    limits a sequence to its first nodes.  ``context_only``: the cache holds no
+    rows of the nodes (Beacon latents: absorbed queries, one KV head).
+    Returns ``(out [B, T, H, Dv], lse [B, T, H] fp32 natural log)``; a row that
+    sees nothing gets zeros and -inf.  Dims: multiples of 8 up to 320.
+    """
+    a, out, lse = attention_args(q, k, v, lengths, scale, mask, nodes, block_tables, context_only, out, lse, wait_limit_ns)
     lib = _lib.load()
-    _run_in_workspace(dev, lib.slimkv_tree_attention_workspace_size, lib.slimkv_tree_attention, a)
+    _run_in_workspace(q.device, lib.slimkv_tree_attention_workspace_size, lib.slimkv_tree_attention, a)
     return out, lse
 
 
