@@ -204,9 +204,10 @@ __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const __grid_cons
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
         if (!dst[k]) continue;
+        const typename P::Constants constants;
         const auto scale = P::as(low_twice(pair[k])), low = P::as(high_twice(pair[k]));
-        __stcs(dst[k], make_uint4(P::template values<0>(code[k], scale, low), P::template values<1>(code[k], scale, low),
-                                  P::template values<2>(code[k], scale, low), P::template values<3>(code[k], scale, low)));
+        __stcs(dst[k], make_uint4(P::template values<0>(constants, code[k], scale, low), P::template values<1>(constants, code[k], scale, low),
+                                  P::template values<2>(constants, code[k], scale, low), P::template values<3>(constants, code[k], scale, low)));
     }
 }
 

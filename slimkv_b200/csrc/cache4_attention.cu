@@ -40,9 +40,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kSlab = 16;                        // keys of a warp's step
-constexpr int kKeys = kSlab * kWarps;            // keys of a tile
-constexpr int kStages = 4;                       // slabs of a warp's ring
+constexpr int kRingKeys = 64;                    // keys of a warp's ring
 constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a score passes the row's maximum by 2^8
 // P = 2^(s - m), m this far below the maximum: of fp16's exponents P uses those up to 2^15.
 template <bool kHalf>
@@ -79,7 +77,8 @@ struct Seq {
     int len, nodes, end;        // keys: rows [0, end), the context and then the nodes' own
     int tiles, groups;          // groups of row tiles with live rows
 };
-template <int NT>
+// NT: row tiles (8 rows) of a segment, kKeys: keys of a tile.
+template <int NT, int kKeys>
 struct Plan {
     static constexpr int kPieceUnits = 2;
     const Job& J;
@@ -116,6 +115,9 @@ struct ValueWords {
 template <int G, int NT>
 struct Shape {
     static constexpr int kWordsV = ValueWords<G>::kWords;
+    // Blocks of 16 keys in a warp's step: two where their scores have room in registers.
+    static constexpr int kHalves = NT * G > 10 ? 1 : 2;
+    static constexpr int kSlab = 16 * kHalves, kKeys = kSlab * kWarps, kStages = kRingKeys / kSlab;
     // Q operands in registers where there is room for them, else in shared memory.
     static constexpr bool kQShared = NT * G > 10;
     static constexpr int kBlocks = G <= 4 ? (NT == 1 ? 4 : 3) : G <= 6 && NT == 1 ? 3 : 2;
@@ -124,7 +126,7 @@ struct Shape {
     static constexpr uint32_t kQBytes = kQShared ? uint32_t(NT) * G * 512 : 0;
 };
 
-template <int kRows>
+template <int kRows, int kStages>
 struct Bars {
     uint64_t full[kWarps][kStages];
     int abort;
@@ -133,8 +135,8 @@ struct Bars {
 };
 template <int G, int NT>
 uint32_t smem_bytes(int k_pitch, int v_pitch) {
-    const uint32_t ring = uint32_t(kWarps * kStages * kSlab) * uint32_t(k_pitch + v_pitch) + 512;    // 512: words behind a short row
-    return 128 + std::max(ring, Shape<G, NT>::kMerge) + Shape<G, NT>::kQBytes + uint32_t(sizeof(Bars<8 * NT>)) + 128;
+    const uint32_t ring = uint32_t(kWarps * kRingKeys) * uint32_t(k_pitch + v_pitch) + 512;    // 512: words behind a short row
+    return std::max(ring, Shape<G, NT>::kMerge) + Shape<G, NT>::kQBytes + uint32_t(sizeof(Bars<8 * NT, Shape<G, NT>::kStages>));
 }
 
 template <bool kHalf>
@@ -147,21 +149,27 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     }
 }
 // ----------------------------------------------------------------- kernel --
-template <int G, int NT, bool kHalf>
+template <int G, int NT, bool kHalf, bool kExact>
 __global__ void __launch_bounds__(kThreads, Shape<G, NT>::kBlocks)
 cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Job J) {
     using P = Pair<kHalf>;
     using VW = ValueWords<G>;
     using S = Shape<G, NT>;
-    constexpr int kRows = 8 * NT, kWordsV = VW::kWords;
-    extern __shared__ __align__(128) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    constexpr int kRows = 8 * NT, kWordsV = VW::kWords, kHalves = S::kHalves, kSlab = S::kSlab, kKeys = S::kKeys, kStages = S::kStages;
+    using Work = Plan<NT, kKeys>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 127) {                  // (TMA writes at multiples of 128 bytes)
+        report(J.status, SLIMKV_DEVICE_MISALIGNED);
+        return;
+    }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t k_bytes = uint32_t(kSlab * J.k_pitch), stage_bytes = k_bytes + uint32_t(kSlab * J.v_pitch);
+    const RowShape<G, kExact> kshape{J.kg}, vshape{J.vg};
+    const uint32_t k_pitch = uint32_t(kshape.pitch()), v_pitch = uint32_t(vshape.pitch());
+    const uint32_t k_bytes = kSlab * k_pitch, stage_bytes = k_bytes + kSlab * v_pitch;
     const uint32_t area = max(uint32_t(kWarps * kStages) * stage_bytes + 512u, S::kMerge);
     uint8_t* ring = smem + uint32_t(warp * kStages) * stage_bytes;
     uint4* q_shared = reinterpret_cast<uint4*>(smem + area);
-    Bars<kRows>* bs = reinterpret_cast<Bars<kRows>*>(smem + area + S::kQBytes);
+    auto* bs = reinterpret_cast<Bars<kRows, kStages>*>(smem + area + S::kQBytes);
 
     if (tid < kWarps * kStages) mbar_init(&bs->full[tid / kStages][tid % kStages], 1);
     if (tid == 0) bs->abort = 0;
@@ -171,20 +179,22 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         tma_prefetch_desc(&vmap);
     }
     grid_launch_dependents();
-    const Plan<NT> plan(J);
+    const Work plan(J);
     if (warp == 0) find_share(plan, &bs->share);
     __syncthreads();
     if (int(blockIdx.x) >= bs->share.ctas) return;
 
     const int boxes = kSlab / J.box;
+    const typename P::Constants constants;
+    const float unscale = 1.f / J.scale_log2;
     int stage = 0;                               // of the next slab to be used
     uint32_t lap = 0;
     uint32_t pending = 0;                        // stages with a load under way
     bool ok = true;
-    Walk<Plan<NT>> w;
+    Walk<Work> w;
     w.start(plan, &bs->share);
     while (w.next(plan)) {
-        // The piece's slabs of this warp: keys [64 tile + 16 warp, + 16), the last may lie behind the keys.
+        // The piece's slabs of this warp, a quarter of each tile; the last may lie behind the keys.
         const int first_key = w.t0 * kKeys + warp * kSlab;
         const int slabs = max(0, min(w.t1 - w.t0, (w.s.end - first_key + kKeys - 1) / kKeys));
         // Where a slab's box of this lane lies: its page (dense: its sequence) and row.  Boxes
@@ -200,12 +210,15 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         };
         auto issue = [&](int st, int page, int row) {
             uint64_t* bar = &bs->full[warp][st];
-            if (lane == 0) mbar_expect_tx(bar, stage_bytes);
-            __syncwarp();
-            if (lane < boxes) {
-                uint8_t* at = ring + uint32_t(st) * stage_bytes;
-                tma_load_4d(at + lane * J.box * J.k_pitch, &kmap, bar, 0, w.g, row, page);
-                tma_load_4d(at + k_bytes + lane * J.box * J.v_pitch, &vmap, bar, 0, w.g, row, page);
+            uint8_t* at = ring + uint32_t(st) * stage_bytes;
+            // One elected thread has the copies: their operands are uniform registers.
+            for (int box = 0; box < boxes; ++box) {
+                const int p = __shfl_sync(0xffffffffu, page, box), r = __shfl_sync(0xffffffffu, row, box);
+                if (elect_one()) {
+                    if (box == 0) mbar_expect_tx(bar, stage_bytes);
+                    tma_load_4d(at + uint32_t(box * J.box) * k_pitch, &kmap, bar, 0, w.g, r, p);
+                    tma_load_4d(at + k_bytes + uint32_t(box * J.box) * v_pitch, &vmap, bar, 0, w.g, r, p);
+                }
             }
             pending |= 1u << st;
         };
@@ -223,7 +236,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         uint4 qf[S::kQShared ? 1 : NT * G];
         auto load_q = [&](int n, int i) {
             const int r = row0 + 8 * n + g, d = KeyWords<G>::dim(i, t);
-            if (r >= J.rows || d >= J.kg * kGroupDims) return make_uint4(0, 0, 0, 0);
+            if (r >= J.rows || !kshape.has(d)) return make_uint4(0, 0, 0, 0);
             const int node = r / J.group, h = w.g * J.group + r - node * J.group;
             return __ldg(reinterpret_cast<const uint4*>(J.q + w.b * J.q_sb + node * J.q_st + h * J.q_sh + d));
         };
@@ -243,11 +256,12 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
-        // Of the rows 2t and 2t + 1 of each row tile.
-        float top[NT][2], sum[NT][2];
+        // Of the rows 2t and 2t + 1 of each row tile: the maximum that P is taken from (log2), the
+        // score (unscaled) that calls for another one, the sum.
+        float top[NT][2], limit[NT][2], sum[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            top[n][0] = top[n][1] = -INFINITY;
+            top[n][0] = top[n][1] = limit[n][0] = limit[n][1] = -INFINITY;
             sum[n][0] = sum[n][1] = 0.f;
         }
 
@@ -257,20 +271,24 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             const int next_page = locate(i + kStages, next_row);
             if (!(ok = warp_wait(&bs->full[warp][stage], lap, bs, J))) break;
             pending &= ~(1u << stage);
-            const uint8_t* ks = ring + uint32_t(stage) * stage_bytes;
-            const uint8_t* vs = ks + k_bytes;
+            // Slabs of context that every row sees whole, all but a sequence's last ones, do without masks.
+            auto step = [&](auto all) {
+            constexpr bool whole_slab = decltype(all)::value;
+            const uint8_t *ks = ring + uint32_t(stage) * stage_bytes, *vs = ks + k_bytes;
 
             // ---- S ----
-            float s[NT][4];
+            float s[kHalves][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-            const uint8_t *k0 = ks + g * J.k_pitch, *k1 = k0 + 8 * J.k_pitch;
-            key_products<G, NT, kHalf>(s, k0, k1, J.kg, t, [&](int n, int i) {
-                if constexpr (S::kQShared) return q_shared[(n * G + i) * 32 + lane];
-                else return qf[n * G + i];
-            });
+            for (int b = 0; b < kHalves; ++b) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
+                key_products<G, NT, kHalf>(s[b], ks + uint32_t(16 * b + g) * k_pitch, kshape, t, constants, [&](int n, int i) {
+                    if constexpr (S::kQShared) return q_shared[(n * G + i) * 32 + lane];
+                    else return qf[n * G + i];
+                });
+            }
 
-            // ---- what the rows see of the slab's keys (g and g + 8 here) ----
+            // ---- what the rows see of the slab's keys (16 b + g and 16 b + g + 8 here) ----
             auto seen_of = [&](int r) {
                 const int node = r / J.group;
                 if (node >= w.s.nodes) return 0u;
@@ -278,40 +296,42 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                 const int32_t* words = J.mask ? J.mask + w.b * J.mask_stride + int64_t(node) * J.words : nullptr;
                 return seen_keys(words, J.words, node, w.s.end - w.s.len, key0 - w.s.len);
             };
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] *= J.scale_log2;
-            const bool whole_slab = key0 + kSlab <= w.s.len;
-            if (!whole_slab) {
+            if constexpr (!whole_slab) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const uint32_t seen = seen_of(row0 + 8 * n + 2 * t + e) >> g;
-                        if (!(seen & 1u)) s[n][e] = -INFINITY;
-                        if (!(seen & 256u)) s[n][2 + e] = -INFINITY;
+#pragma unroll
+                        for (int b = 0; b < kHalves; ++b) {
+                            if (!(seen >> (16 * b) & 1u)) s[b][n][e] = -INFINITY;
+                            if (!(seen >> (16 * b) & 256u)) s[b][n][2 + e] = -INFINITY;
+                        }
                     }
             }
 
             // ---- softmax ----
             bool grown = false;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int b = 0; b < kHalves; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) grown |= s[n][e] > top[n][e & 1] + (kLazyLog2 + kDownLog2<kHalf>);
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) grown |= s[b][n][e] > limit[n][e & 1];
             if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float alpha[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(s[n][e], s[n][2 + e]);
+                        float mx = fmaxf(s[0][n][e], s[0][n][2 + e]);
+                        if constexpr (kHalves == 2) mx = fmaxf(mx, fmaxf(s[1][n][e], s[1][n][2 + e]));
 #pragma unroll
                         for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-                        const float m = fmaxf(top[n][e], mx - kDownLog2<kHalf>);
+                        const float m = fmaxf(top[n][e], mx * J.scale_log2 - kDownLog2<kHalf>);
                         alpha[e] = top[n][e] == m ? 1.f : sfu_exp2(top[n][e] - m);      // (both may be -inf)
                         top[n][e] = m;
+                        limit[n][e] = (m + (kLazyLog2 + kDownLog2<kHalf>)) * unscale;
                         sum[n][e] *= alpha[e];
                     }
 #pragma unroll
@@ -320,48 +340,52 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                         for (int e = 0; e < 4; ++e) o[m][n][e] *= alpha[e & 1];
                 }
             }
-            uint32_t pf[NT][2];
+            uint32_t pf[kHalves][NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float p[4];
+                const float shift[2] = {-fmaxf(top[n][0], -3e38f), -fmaxf(top[n][1], -3e38f)};      // (-inf: nothing seen yet)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[e] = sfu_exp2(s[n][e] - (top[n][e & 1] == -INFINITY ? 0.f : top[n][e & 1]));
-                sum[n][0] += p[0] + p[2];
-                sum[n][1] += p[1] + p[3];
-                pf[n][0] = transpose8x8(pack2<kHalf>(p[0], p[1]));
-                pf[n][1] = transpose8x8(pack2<kHalf>(p[2], p[3]));
+                for (int b = 0; b < kHalves; ++b) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = sfu_exp2(fmaf(s[b][n][e], J.scale_log2, shift[e & 1]));
+                    sum[n][0] += p[0] + p[2];
+                    sum[n][1] += p[1] + p[3];
+                    pf[b][n][0] = transpose8x8(pack2<kHalf>(p[0], p[1]));
+                    pf[b][n][1] = transpose8x8(pack2<kHalf>(p[2], p[3]));
+                }
             }
 
-            // ---- O: the keys 2t, 2t + 1, 2t + 8, 2t + 9 and the dims of lane row g.  A key that
+            // ---- O: the keys 2t, 2t + 1, 2t + 8, 2t + 9 of a half and the dims of lane row g.  A key that
             // nobody sees counts as zero (its P is 0, and 0 x NaN is not 0); so does a group of a
             // node's row that is NaN, which the rows that see it get afterwards. ----
             const uint32_t live = low_bits(w.s.end - key0);
-            const bool nodes_here = !J.context_only && key0 + kSlab > w.s.len;
-            auto pair_of = [&](int key, int grp) { return *reinterpret_cast<const uint32_t*>(vs + key * J.v_pitch + 16 * J.vg + 4 * grp); };
+            const bool nodes_here = !whole_slab && !J.context_only;
+            auto pair_of = [&](int key, int grp) { return load_word(vs + uint32_t(key) * v_pitch + vshape.pair_at(kGroupDims * grp)); };
             bool bad = false;
             if (nodes_here) {
                 for (int k = lane; k < kSlab * J.vg; k += 32)
                     if (live >> (k / J.vg) & 1) bad |= !P::finite(pair_of(k / J.vg, k % J.vg));
                 bad = __any_sync(0xffffffffu, bad);
             }
-            const uint8_t* v0 = vs + 2 * t * J.v_pitch;
-            {
-                auto value_words = [&](auto width, int i0) {
-                    constexpr int W = decltype(width)::value;
-                    const int d0 = VW::dim(i0, g), grp = d0 / kGroupDims;
-                    const int at = J.vg * 16 + 4 * min(grp, J.vg - 1);
+#pragma unroll
+            for (int b = 0; b < kHalves; ++b) {
+                const uint8_t* v0 = vs + uint32_t(16 * b + 2 * t) * v_pitch;
+                auto value_words = [&](auto width, auto first) {
+                    constexpr int W = decltype(width)::value, i0 = decltype(first)::value;
+                    const int d0 = VW::dim(i0, g);
                     uint32_t a[4][W], p[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const uint8_t* row = v0 + ((k & 1) + 8 * (k >> 1)) * J.v_pitch;
+                        const uint8_t* row = v0 + uint32_t((k & 1) + 8 * (k >> 1)) * v_pitch;
                         load_words<W>(row + d0 / 2, a[k]);
-                        p[k] = *reinterpret_cast<const uint32_t*>(row + at);
-                        if (grp >= J.vg) p[k] = 0;
+                        p[k] = load_word(row + vshape.pair_at(d0));
+                        if (!vshape.has(d0) || (G % 2 && d0 >= kGroupDims * G)) p[k] = 0;
                     }
-                    if (!whole_slab) {
+                    if constexpr (!whole_slab) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            if (!(live >> (2 * t + (k & 1) + 8 * (k >> 1)) & 1) || (nodes_here && !P::finite(p[k]))) p[k] = 0;
+                            if (!(live >> (16 * b + 2 * t + (k & 1) + 8 * (k >> 1)) & 1) || (nodes_here && !P::finite(p[k]))) p[k] = 0;
                     }
                     const auto sc0 = P::as(low_halves(p[0], p[1])), lo0 = P::as(high_halves(p[0], p[1]));
                     const auto sc1 = P::as(low_halves(p[2], p[3])), lo1 = P::as(high_halves(p[2], p[3]));
@@ -372,10 +396,10 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                         const uint32_t x1 = low_halves(a[2][k], a[3][k]), y1 = high_halves(a[2][k], a[3][k]);
                         auto pair = [&](auto which) {
                             constexpr int j = decltype(which)::value;
-                            const uint32_t x[4] = {P::template values<j>(x0, sc0, lo0), P::template values<j>(y0, sc0, lo0),
-                                                   P::template values<j>(x1, sc1, lo1), P::template values<j>(y1, sc1, lo1)};
+                            const uint32_t x[4] = {P::template values<j>(constants, x0, sc0, lo0), P::template values<j>(constants, y0, sc0, lo0),
+                                                   P::template values<j>(constants, x1, sc1, lo1), P::template values<j>(constants, y1, sc1, lo1)};
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma<kHalf>(o[4 * (i0 + k) + j][n], x, pf[n][0], pf[n][1]);
+                            for (int n = 0; n < NT; ++n) mma<kHalf>(o[4 * (i0 + k) + j][n], x, pf[b][n][0], pf[b][n][1]);
                         };
                         pair(std::integral_constant<int, 0>());
                         pair(std::integral_constant<int, 1>());
@@ -383,11 +407,12 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                         pair(std::integral_constant<int, 3>());
                     }
                 };
-#pragma unroll
-                for (int c = 0; c < VW::kOcts; ++c) value_words(std::integral_constant<int, 4>(), 4 * c);
-                if constexpr (VW::kQuad != 0) value_words(std::integral_constant<int, 2>(), 4 * VW::kOcts);
-                if constexpr (VW::kPair != 0) value_words(std::integral_constant<int, 1>(), 4 * VW::kOcts + 2 * VW::kQuad);
-                if constexpr (VW::kOne != 0) value_words(std::integral_constant<int, 1>(), 4 * VW::kOcts + 2 * VW::kQuad + VW::kPair);
+                using std::integral_constant;
+                if constexpr (VW::kOcts > 0) value_words(integral_constant<int, 4>(), integral_constant<int, 0>());
+                if constexpr (VW::kQuad != 0) value_words(integral_constant<int, 2>(), integral_constant<int, 4 * VW::kOcts>());
+                if constexpr (VW::kPair != 0) value_words(integral_constant<int, 1>(), integral_constant<int, 4 * VW::kOcts + 2 * VW::kQuad>());
+                if constexpr (VW::kOne != 0)
+                    value_words(integral_constant<int, 1>(), integral_constant<int, 4 * VW::kOcts + 2 * VW::kQuad + VW::kPair>());
             }
             if (bad) {
 #pragma unroll 1
@@ -405,6 +430,9 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                             }
                 }
             }
+            };
+            if (key0 + kSlab <= w.s.len) step(std::true_type());
+            else step(std::false_type());
             __syncwarp();
             if (i + kStages < slabs) issue(stage, next_page, next_row);
             if (++stage == kStages) { stage = 0; lap ^= 1; }
@@ -471,7 +499,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                         x[half].x += y.x; x[half].y += y.y; x[half].z += y.z; x[half].w += y.w;
                     }
                 }
-                if (r >= J.rows || d >= J.vg * kGroupDims) continue;
+                if (r >= J.rows || d >= vshape.groups() * kGroupDims) continue;
                 const int node = r / J.group, h = w.g * J.group + r - node * J.group;
                 if (whole) {
                     uint4 y = make_uint4(0, 0, 0, 0);
@@ -508,7 +536,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
 // Merges the pieces of a segment's rows (a block each), and writes the rows
 // that see nothing.  The four warps take the pieces by turns, a lane four dims.
-template <int NT, bool kHalf>
+template <int NT, int kKeys, bool kHalf>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Job J) {
     constexpr int kRows = 8 * NT;
     __shared__ int range[3];                // first and last CTA of the segment's pieces, slot of the first
@@ -519,7 +547,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
     const int group = at % J.row_groups;
     at /= J.row_groups;
     const int g = at % J.kv_heads, b = at / J.kv_heads, r = group * kRows + blockIdx.y;
-    const Plan<NT> plan(J);
+    const Plan<NT, kKeys> plan(J);
     const Seq s = plan.sequence(b);
     const bool some = group < s.groups && s.tiles > 0;
     if (some && warp == 0) {
@@ -527,7 +555,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
         sum_units(plan, b, total, before);
         if (lane == 0) {
             const uint32_t units = segment_units(plan, s), u0 = before + uint32_t(g * s.groups + group) * units;
-            const uint32_t ctas = share_count(total, J.ctas), c0 = share_of(total, u0 + Plan<NT>::kPieceUnits, ctas);
+            const uint32_t ctas = share_count(total, J.ctas), c0 = share_of(total, u0 + Plan<NT, kKeys>::kPieceUnits, ctas);
             range[0] = int(c0);
             range[1] = int(share_of(total, u0 + units - 1, ctas));
             range[2] = 2 * int(c0) + (share_begin(total, c0, ctas) < u0 ? 1 : 0);   // a piece of another segment before it
@@ -674,9 +702,9 @@ void carve(Carver& c, const slimkv_tree_attention_args* a, Job& J) {
     J.part_lse = c.take<float>(rows);
 }
 
-template <int G, int NT, bool kHalf>
+template <int G, int NT, bool kHalf, bool kExact>
 int launch(const CUtensorMap& km, const CUtensorMap& vm, const Job& J, cudaStream_t stream) {
-    auto kernel = cache4_attention_kernel<G, NT, kHalf>;
+    auto kernel = cache4_attention_kernel<G, NT, kHalf, kExact>;
     const uint32_t bytes = smem_bytes<G, NT>(J.k_pitch, J.v_pitch);
     static bool configured[64] = {};
     const int dev = device_info().device;
@@ -697,7 +725,7 @@ int launch(const CUtensorMap& km, const CUtensorMap& vm, const Job& J, cudaStrea
     cfg.attrs = &dependent;
     cfg.numAttrs = 1;
     cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, combine_kernel<NT, kHalf>, J);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, combine_kernel<NT, Shape<G, NT>::kKeys, kHalf>, J);
     return e == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "4-bit attention launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -733,7 +761,8 @@ extern "C" int slimkv_cache4_attention(const slimkv_tree_attention_args* a, void
     if (!workspace || !c.fits() || !aligned16(workspace))
         return fail(SLIMKV_ERR_WORKSPACE, "4-bit attention: %zu bytes of 16-byte aligned workspace needed", c.used);
     // A box of TMA rows stays inside a page.
-    J.box = paged && cache.rows % kSlab ? 8 : kSlab;
+    const int slab = with_shape(a, [](auto g, auto nt) { return Shape<decltype(g)::value, decltype(nt)::value>::kSlab; });
+    J.box = paged ? std::min(slab, cache.rows & -cache.rows) : slab;
     J.shared_cache = !paged && cache.k_stride[0] == 0 && cache.v_stride[0] == 0;
     if (a->batch > 1 && !paged && !J.shared_cache && (cache.k_stride[0] == 0 || cache.v_stride[0] == 0))
         return fail(SLIMKV_ERR_INVALID_ARGUMENT, "4-bit attention: K and V are both shared by the batch or neither");
@@ -762,7 +791,7 @@ extern "C" int slimkv_cache4_attention(const slimkv_tree_attention_args* a, void
     J.paged = paged;
     J.cache = cache_view(cache);
     J.capacity = cache_capacity(J.cache);
-    if (double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / kKeys + 1 + Plan<1>::kPieceUnits) >= 2147483648.0)
+    if (double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / (slab * kWarps) + 1 + Plan<1, 64>::kPieceUnits) >= 2147483648.0)
         return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "4-bit attention: too many rows in one call");
     J.lengths = a->lengths;
     J.nodes_len = a->nodes_len;
@@ -781,6 +810,7 @@ extern "C" int slimkv_cache4_attention(const slimkv_tree_attention_args* a, void
     const bool half = a->type == SLIMKV_FP16;
     return with_shape(a, [&](auto g, auto nt) {
         constexpr int kG = decltype(g)::value, kNt = decltype(nt)::value;
-        return half ? launch<kG, kNt, true>(km, vm, J, st) : launch<kG, kNt, false>(km, vm, J, st);
+        if (J.kg == kG && J.vg == kG) return half ? launch<kG, kNt, true, true>(km, vm, J, st) : launch<kG, kNt, false, true>(km, vm, J, st);
+        return half ? launch<kG, kNt, true, false>(km, vm, J, st) : launch<kG, kNt, false, false>(km, vm, J, st);
     });
 }

@@ -82,17 +82,21 @@ struct Bars {
 };
 template <int G>
 uint32_t smem_bytes(int k_pitch) {
-    return 128 + uint32_t(kWarps * kStages<G> * kSlab * k_pitch) + 512 + uint32_t(kTiles) * G * 512 + uint32_t(sizeof(Bars<G>)) + 128;
+    return uint32_t(kWarps * kStages<G> * kSlab * k_pitch) + 512 + uint32_t(kTiles) * G * 512 + uint32_t(sizeof(Bars<G>));
 }
 
-template <int G, bool kHalf>
+template <int G, bool kHalf, bool kExact>
 __global__ void __launch_bounds__(kThreads, kBlocks<G>)
 cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ Job J) {
     constexpr int kRing = kStages<G>;
-    extern __shared__ __align__(128) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 127) {                  // (TMA writes at multiples of 128 bytes)
+        report(J.status, SLIMKV_DEVICE_MISALIGNED);
+        return;
+    }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t stage_bytes = uint32_t(kSlab * J.k_pitch), area = uint32_t(kWarps * kRing) * stage_bytes + 512u;
+    const RowShape<G, kExact> shape{J.kg};
+    const uint32_t pitch = uint32_t(shape.pitch()), stage_bytes = kSlab * pitch, area = uint32_t(kWarps * kRing) * stage_bytes + 512u;
     uint8_t* ring = smem + uint32_t(warp * kRing) * stage_bytes;
     uint4* q_shared = reinterpret_cast<uint4*>(smem + area);
     Bars<G>* bs = reinterpret_cast<Bars<G>*>(smem + area + uint32_t(kTiles) * G * 512u);
@@ -111,6 +115,7 @@ cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     __syncthreads();
     if (int(blockIdx.x) >= bs->share.ctas) return;
 
+    const typename Pair<kHalf>::Constants constants;
     const int boxes = kSlab / J.box;
     int stage = 0;                               // of the next slab to be used
     uint32_t lap = 0;
@@ -134,7 +139,7 @@ cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             uint64_t* bar = &bs->full[warp][st];
             if (lane == 0) mbar_expect_tx(bar, stage_bytes);
             __syncwarp();
-            if (lane < boxes) tma_load_4d(ring + uint32_t(st) * stage_bytes + lane * J.box * J.k_pitch, &kmap, bar, 0, w.g, row, page);
+            if (lane < boxes) tma_load_4d(ring + uint32_t(st) * stage_bytes + uint32_t(lane * J.box) * pitch, &kmap, bar, 0, w.g, row, page);
             pending |= 1u << st;
         };
         float* mass = J.mass + w.b * J.m_sb + w.g * J.m_sh;
@@ -164,7 +169,7 @@ cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 int node, h;
                 source(row0 + i / G * 8 + g, some, node, h);
                 uint4 x = make_uint4(0, 0, 0, 0);
-                if (some && d < J.kg * kGroupDims)
+                if (some && shape.has(d))
                     x = __ldg(reinterpret_cast<const uint4*>(J.q + w.b * J.q_sb + node * J.q_st + h * J.q_sh + d));
                 q_shared[i * 32 + lane] = x;
             }
@@ -187,7 +192,7 @@ cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 const float old = !live ? 0.f : row0 ? mass[n] : n < w.s.len ? J.decay * mass[n] : 0.f;
                 if (!(ok = warp_wait(&bs->full[warp][stage], lap, bs, J))) break;
                 pending &= ~(1u << stage);
-                const uint8_t* k0 = ring + uint32_t(stage) * stage_bytes + g * J.k_pitch;
+                const uint8_t* k0 = ring + uint32_t(stage) * stage_bytes + uint32_t(g) * pitch;
                 // First of the block's rows that see the keys g and g + 8: all see an old key, an
                 // accepted one its own row and those behind it.
                 const int first0 = key0 + g < w.s.len ? 0 : (key0 + g - w.s.len) * J.group - row0;
@@ -198,7 +203,7 @@ cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     float s[NT][4];
 #pragma unroll
                     for (int m = 0; m < NT; ++m) s[m][0] = s[m][1] = s[m][2] = s[m][3] = 0.f;
-                    key_products<G, NT, kHalf>(s, k0, k0 + 8 * J.k_pitch, J.kg, t, [&](int m, int j) { return q_shared[(m * G + j) * 32 + lane]; });
+                    key_products<G, NT, kHalf>(s, k0, shape, t, constants, [&](int m, int j) { return q_shared[(m * G + j) * 32 + lane]; });
 #pragma unroll
                     for (int m = 0; m < NT; ++m) {
                         const int r = 8 * m + 2 * t;
@@ -234,9 +239,9 @@ cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             }
 }
 
-template <int G, bool kHalf>
+template <int G, bool kHalf, bool kExact>
 int launch(const CUtensorMap& km, const Job& J, cudaStream_t stream) {
-    auto kernel = cache4_mass_kernel<G, kHalf>;
+    auto kernel = cache4_mass_kernel<G, kHalf, kExact>;
     static bool configured[64] = {};
     const int dev = device_info().device;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
@@ -312,7 +317,8 @@ extern "C" int slimkv_cache4_key_mass(const slimkv_key_mass_args* a, void* strea
     auto run = [&](auto groups) {
         constexpr int G = decltype(groups)::value;
         J.ctas = device_info().sm_count * kBlocks<G>;
-        return half ? launch<G, true>(km, J, st) : launch<G, false>(km, J, st);
+        if (J.kg == G) return half ? launch<G, true, true>(km, J, st) : launch<G, false, true>(km, J, st);
+        return half ? launch<G, true, false>(km, J, st) : launch<G, false, false>(km, J, st);
     };
     using std::integral_constant;
     switch (J.kg) {
