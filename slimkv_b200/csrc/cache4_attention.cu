@@ -40,7 +40,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kRingKeys = 64;                    // keys of a warp's ring
 constexpr float kLazyLog2 = 8.f;                 // O is rescaled when a score passes the row's maximum by 2^8
 // P = 2^(s - m), m this far below the maximum: of fp16's exponents P uses those up to 2^15.
 template <bool kHalf>
@@ -50,6 +49,7 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 struct Job {
     int batch, nodes, heads, kv_heads, group;
+    FastDiv group_div, page_div;    // by the query heads of a KV head, by the rows of a page
     int rows, row_groups;       // query rows of a KV head, and groups of 8 NT of them
     int kg, vg;                 // groups of 32 dims of a K and a V row
     int k_pitch, v_pitch;       // bytes of a row
@@ -117,26 +117,40 @@ struct Shape {
     static constexpr int kWordsV = ValueWords<G>::kWords;
     // Blocks of 16 keys in a warp's step: two where their scores have room in registers.
     static constexpr int kHalves = NT * G > 10 ? 1 : 2;
-    static constexpr int kSlab = 16 * kHalves, kKeys = kSlab * kWarps, kStages = kRingKeys / kSlab;
+    static constexpr int kSlab = 16 * kHalves, kKeys = kSlab * kWarps;
+    // Slabs of a warp's ring: what leaves shared memory to kBlocks blocks.
+    static constexpr int kStages = G <= 6 ? 64 / kSlab : kHalves == 2 ? 2 : 3;
     // Q operands in registers where there is room for them, else in shared memory.
     static constexpr bool kQShared = NT * G > 10;
     static constexpr int kBlocks = G <= 4 ? (NT == 1 ? 4 : 3) : G <= 6 && NT == 1 ? 3 : 2;
     // What the four warps' O takes when they are added up (over the rings).
     static constexpr uint32_t kMerge = uint32_t(kWordsV) * 2 * NT * kWarps * 32 * 32;
     static constexpr uint32_t kQBytes = kQShared ? uint32_t(NT) * G * 512 : 0;
+    static constexpr uint32_t kRing = uint32_t(kWarps) * kStages * kSlab * 2 * row4_bytes(kGroupDims * G) + 512;
+    static_assert(kBlocks * ((kRing > kMerge ? kRing : kMerge) + kQBytes + 2048) <= 228 * 1024, "shared memory of the blocks of an SM");
 };
 
-template <int kRows, int kStages>
+// A CTA's part of a segment.
+struct Piece {
+    int more;                   // 0: there is none
+    int b, g, group;
+    int t0, t1;                 // its key tiles
+    Seq s;
+    int slot;                   // of its partial rows, -1: a whole segment
+};
+template <class Work, int kRows, int kStages>
 struct Bars {
     uint64_t full[kWarps][kStages];
     int abort;
     Share share;
+    Walk<Work> walk;            // thread 0's
+    Piece piece[2];             // this one and the next
     float top[kWarps][kRows], sum[kWarps][kRows];
 };
 template <int G, int NT>
 uint32_t smem_bytes(int k_pitch, int v_pitch) {
-    const uint32_t ring = uint32_t(kWarps * kRingKeys) * uint32_t(k_pitch + v_pitch) + 512;    // 512: words behind a short row
-    return std::max(ring, Shape<G, NT>::kMerge) + Shape<G, NT>::kQBytes + uint32_t(sizeof(Bars<8 * NT, Shape<G, NT>::kStages>));
+    const uint32_t ring = uint32_t(kWarps * Shape<G, NT>::kStages * Shape<G, NT>::kSlab) * uint32_t(k_pitch + v_pitch) + 512;    // 512: words behind a short row
+    return std::max(ring, Shape<G, NT>::kMerge) + Shape<G, NT>::kQBytes + uint32_t(sizeof(Bars<Plan<NT, Shape<G, NT>::kKeys>, 8 * NT, Shape<G, NT>::kStages>));
 }
 
 template <bool kHalf>
@@ -169,7 +183,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     const uint32_t area = max(uint32_t(kWarps * kStages) * stage_bytes + 512u, S::kMerge);
     uint8_t* ring = smem + uint32_t(warp * kStages) * stage_bytes;
     uint4* q_shared = reinterpret_cast<uint4*>(smem + area);
-    auto* bs = reinterpret_cast<Bars<kRows, kStages>*>(smem + area + S::kQBytes);
+    auto* bs = reinterpret_cast<Bars<Work, kRows, kStages>*>(smem + area + S::kQBytes);
 
     if (tid < kWarps * kStages) mbar_init(&bs->full[tid / kStages][tid % kStages], 1);
     if (tid == 0) bs->abort = 0;
@@ -180,40 +194,64 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     }
     grid_launch_dependents();
     const Work plan(J);
-    if (warp == 0) find_share(plan, &bs->share);
+    // One thread goes through the share's pieces; the others find each in shared memory.
+    auto next_piece = [&](Piece& p) {
+        Walk<Work>& w = bs->walk;
+        p.more = w.next(plan);
+        p.b = w.b; p.g = w.g; p.group = w.group;
+        p.t0 = w.t0; p.t1 = w.t1;
+        p.s = w.s;
+        p.slot = w.whole() ? -1 : 2 * int(blockIdx.x) + (w.piece > 0);
+    };
+    if (warp == 0) {
+        find_share(plan, &bs->share);
+        __syncwarp();
+        if (lane == 0 && int(blockIdx.x) < bs->share.ctas) {
+            bs->walk.start(plan, &bs->share);
+            next_piece(bs->piece[0]);
+        }
+    }
     __syncthreads();
     if (int(blockIdx.x) >= bs->share.ctas) return;
 
-    const int boxes = kSlab / J.box;
+    const int boxes = kSlab / J.box, box_shift = 31 - __clz(boxes);
     const typename P::Constants constants;
     const float unscale = 1.f / J.scale_log2;
     int stage = 0;                               // of the next slab to be used
     uint32_t lap = 0;
     uint32_t pending = 0;                        // stages with a load under way
     bool ok = true;
-    Walk<Work> w;
-    w.start(plan, &bs->share);
-    while (w.next(plan)) {
+    for (int turn = 0;; turn ^= 1) {
+        const Piece w = bs->piece[turn];
+        if (!w.more) break;
         // The piece's slabs of this warp, a quarter of each tile; the last may lie behind the keys.
         const int first_key = w.t0 * kKeys + warp * kSlab;
         const int slabs = max(0, min(w.t1 - w.t0, (w.s.end - first_key + kKeys - 1) / kKeys));
-        // Where a slab's box of this lane lies: its page (dense: its sequence) and row.  Boxes
-        // past the last used row repeat that row's (they are masked).
-        auto locate = [&](int slab, int& row) {
-            row = first_key + slab * kKeys + lane * J.box;
+        // Where box lane % boxes of slab `first` + lane / boxes lies: its page (dense: its sequence)
+        // and row.  Boxes past the last used row repeat that row's (they are masked).
+        auto locate = [&](int first, int& row) {
+            const int slab = first + (lane >> box_shift);
+            row = first_key + slab * kKeys + (lane & (boxes - 1)) * J.box;
             if (!J.paged) return J.shared_cache ? 0 : w.b;
-            int64_t page = 0;
-            if (lane < boxes && slab < slabs) {
-                if (!cache_row(J.cache, w.b, min(row, (w.s.end - 1) / J.box * J.box), page, row)) report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+            int page = 0;
+            if (slab < min(slabs, first + kStages)) {
+                const int n = min(row, (w.s.end - 1) & -J.box), i = int(J.page_div.div(uint32_t(n)));
+                page = __ldg(J.cache.table + w.b * J.cache.table_stride + i);
+                row = n - i * J.cache.rows;
+                if (page < 0 || page >= J.cache.num_pages) {
+                    report(J.status, SLIMKV_DEVICE_BAD_LENGTH);
+                    page = min(max(page, 0), J.cache.num_pages - 1);
+                }
             }
-            return int(page);
+            return page;
         };
-        auto issue = [&](int st, int page, int row) {
+        // Loads a slab that the lanes from `from` on have located.
+        auto issue = [&](int st, int page, int row, int from) {
             uint64_t* bar = &bs->full[warp][st];
             uint8_t* at = ring + uint32_t(st) * stage_bytes;
             // One elected thread has the copies: their operands are uniform registers.
             for (int box = 0; box < boxes; ++box) {
-                const int p = __shfl_sync(0xffffffffu, page, box), r = __shfl_sync(0xffffffffu, row, box);
+                const int p = __shfl_sync(0xffffffffu, page, from + box), r = __shfl_sync(0xffffffffu, row, from + box);
                 if (elect_one()) {
                     if (box == 0) mbar_expect_tx(bar, stage_bytes);
                     tma_load_4d(at + uint32_t(box * J.box) * k_pitch, &kmap, bar, 0, w.g, r, p);
@@ -223,12 +261,12 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             pending |= 1u << st;
         };
         if (ok) {
-            int page[kStages], row[kStages];
-#pragma unroll
-            for (int s = 0; s < kStages; ++s) page[s] = locate(s, row[s]);
-#pragma unroll
-            for (int s = 0; s < kStages; ++s)
-                if (s < slabs) issue((stage + s) % kStages, page[s], row[s]);
+            int row;
+            const int page = locate(0, row);
+            for (int s = 0, st = stage; s < min(slabs, kStages); ++s) {
+                issue(st, page, row, s << box_shift);
+                if (++st == kStages) st = 0;
+            }
         }
 
         // ---- Q: row g of each row tile, the dims of lane column t ----
@@ -237,7 +275,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         auto load_q = [&](int n, int i) {
             const int r = row0 + 8 * n + g, d = KeyWords<G>::dim(i, t);
             if (r >= J.rows || !kshape.has(d)) return make_uint4(0, 0, 0, 0);
-            const int node = r / J.group, h = w.g * J.group + r - node * J.group;
+            const int node = int(J.group_div.div(uint32_t(r))), h = w.g * J.group + r - node * J.group;
             return __ldg(reinterpret_cast<const uint4*>(J.q + w.b * J.q_sb + node * J.q_st + h * J.q_sh + d));
         };
         if constexpr (S::kQShared) {
@@ -290,7 +328,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
             // ---- what the rows see of the slab's keys (16 b + g and 16 b + g + 8 here) ----
             auto seen_of = [&](int r) {
-                const int node = r / J.group;
+                const int node = int(J.group_div.div(uint32_t(r)));
                 if (node >= w.s.nodes) return 0u;
                 if (J.context_only) return low_bits(w.s.end - key0);
                 const int32_t* words = J.mask ? J.mask + w.b * J.mask_stride + int64_t(node) * J.words : nullptr;
@@ -434,7 +472,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             if (key0 + kSlab <= w.s.len) step(std::true_type());
             else step(std::false_type());
             __syncwarp();
-            if (i + kStages < slabs) issue(stage, next_page, next_row);
+            if (i + kStages < slabs) issue(stage, next_page, next_row, 0);
             if (++stage == kStages) { stage = 0; lap ^= 1; }
         }
 
@@ -470,7 +508,8 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             for (int e = 0; e < 2; ++e) {
                 float m;
                 const float l = row_total(8 * n + 2 * t + e, m);
-                const float f = l == 0.f ? 0.f : top[n][e] == -INFINITY ? 0.f / l : sfu_exp2(top[n][e] - m) / l;
+                // (a NaN sum stays)
+                const float f = l == 0.f ? 0.f : (top[n][e] == -INFINITY ? 0.f : sfu_exp2(top[n][e] - m)) * __fdividef(1.f, l);
 #pragma unroll
                 for (int k = 0; k < kWordsV; ++k)
 #pragma unroll
@@ -479,9 +518,10 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                             make_float4(o[4 * k + 2 * half][n][e] * f, o[4 * k + 2 * half][n][2 + e] * f,
                                         o[4 * k + 2 * half + 1][n][e] * f, o[4 * k + 2 * half + 1][n][2 + e] * f);
             }
+        if (tid == 0) next_piece(bs->piece[turn ^ 1]);
         __syncthreads();
-        const bool whole = w.whole();
-        const int slot = 2 * blockIdx.x + (w.piece > 0);
+        const bool whole = w.slot < 0;
+        const int slot = w.slot;
         if (ok) {
             for (int u = warp; u < kWordsV * NT * 2; u += kWarps) {
                 const int k = u / (2 * NT), n = u / 2 % NT, e = u & 1, r = row0 + 8 * n + 2 * t + e;
@@ -500,7 +540,7 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                     }
                 }
                 if (r >= J.rows || d >= vshape.groups() * kGroupDims) continue;
-                const int node = r / J.group, h = w.g * J.group + r - node * J.group;
+                const int node = int(J.group_div.div(uint32_t(r))), h = w.g * J.group + r - node * J.group;
                 if (whole) {
                     uint4 y = make_uint4(0, 0, 0, 0);
                     if (node < w.s.nodes)
@@ -780,6 +820,8 @@ extern "C" int slimkv_cache4_attention(const slimkv_tree_attention_args* a, void
     J.heads = a->heads;
     J.kv_heads = a->kv_heads;
     J.group = a->heads / a->kv_heads;
+    J.group_div = FastDiv(uint32_t(J.group));
+    J.page_div = FastDiv(uint32_t(cache.rows));
     J.rows = a->nodes * J.group;
     const int nt = row_tiles(a);
     J.row_groups = (J.rows + 8 * nt - 1) / (8 * nt);
