@@ -8,10 +8,9 @@
 // two shuffles, and every lane writes the four bytes of its codes.
 //
 // Bound: HBM (2.625 bytes a value either way); the codes cost about ten
-// operations each, so what is exact is bought cheaply: the nearest code comes from
-// a product with 1 / scale, whose error shows in the exact remainder
-// x - low - code * scale (one fused operation); a remainder of half a scale or more
-// sends the lane's codes through the exact rule.
+// operations each, so what is exact is bought cheaply: the quotient is a product
+// with 1 / scale, put right by its exact remainder (Markstein's division).
+#include <algorithm>
 #include <type_traits>
 
 #include "cache4.cuh"
@@ -21,20 +20,25 @@
 namespace slimkv {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kUnits = 4;               // units of eight dims a thread has under way
+constexpr int kThreads = 256;           // at most
+constexpr int kAhead = 4;               // rows that a thread has under way
+constexpr int kMaxTurns = 8;            // rows of a thread
+constexpr int kMaxRows = kThreads / 4 * kMaxTurns;
 
-struct Job4 {
-    int rows, dim, units, upr;          // units of eight dims of a sequence (rows x heads x upr), and of a row
-    FastDiv per_row, per_head;          // by heads * upr and by upr
-    const uint16_t* dense;              // 16-bit rows: read by write, written by read
-    uint16_t* out;
+// Columns are the eight-dim units of a row's heads; a block has up to 256 of them and as many
+// rows side by side as it has threads for, so a thread keeps its column.
+struct Part4 {
+    int dim, cols, block_cols, side;    // columns in all and of a block, rows side by side
+    FastDiv per_block, per_head;        // by block_cols and by a head's columns
+    uint16_t* dense;                    // 16-bit rows: read by write, written by read
     int64_t stride[3];
     uint8_t* cache;
     int64_t c_stride[3];                // bytes
 };
 struct Args4 {
-    Job4 part[2];                       // K and V
+    Part4 part[2];                      // K and V
+    int rows, turns;                    // rows of a thread
+    FastDiv page;
     CacheView view;
     int64_t capacity;
     const int32_t *starts, *counts;
@@ -44,131 +48,135 @@ struct Args4 {
 
 // A sequence's rows: cache rows [start, start + count), without what the cache cannot hold
 // (behind a negative start: none).
-__device__ __forceinline__ bool span_of(const Args4& a, int b, int rows, int& start, int& count) {
-    const int s = a.starts ? __ldg(a.starts + b) : 0, c = a.counts ? __ldg(a.counts + b) : rows;
+__device__ __forceinline__ bool span_of(const Args4& a, int b, int& start, int& count) {
+    const int s = a.starts ? __ldg(a.starts + b) : 0, c = a.counts ? __ldg(a.counts + b) : a.rows;
     start = max(s, 0);
-    count = s < 0 ? 0 : min(max(c, 0), rows);
-    const bool fits = s >= 0 && c >= 0 && c <= rows && int64_t(start) + count <= a.capacity;
+    count = s < 0 ? 0 : min(max(c, 0), a.rows);
+    const bool fits = s >= 0 && c >= 0 && c <= a.rows && int64_t(start) + count <= a.capacity;
     count = int(max(min(int64_t(count), a.capacity - start), int64_t(0)));
     return fits;
 }
 
-// The place of a unit: its row, head, and the byte address of the cache row.
-__device__ __forceinline__ bool place_of(const Args4& a, const Job4& p, int b, uint32_t unit, int start, int& row, int& head, int& u,
-                                         int64_t& at) {
-    row = int(p.per_row.div(unit));
-    const uint32_t in_row = unit - uint32_t(row) * p.per_row.d;
-    head = int(p.per_head.div(in_row));
-    u = int(in_row) - head * p.upr;
-    int64_t page;
-    int r;
-    const bool ok = cache_row(a.view, b, start + row, page, r);
-    at = page * p.c_stride[0] + r * p.c_stride[1] + head * p.c_stride[2];
-    return ok;
+// A thread's column, and the places of its block's cache rows (in shared memory).
+struct Place {
+    int start, count;           // the sequence's
+    int first, rows;            // the block's rows
+    int row, head, unit;        // the thread's first row of the block; its column
+    bool some;                  // it has a column
+};
+__device__ __forceinline__ Place place_of(const Args4& a, const Part4& p, int chunk, int64_t* at, bool for_write) {
+    Place w;
+    const int b = blockIdx.y, tid = threadIdx.x;
+    if (!span_of(a, b, w.start, w.count) && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
+    w.first = blockIdx.x * (p.side * a.turns);
+    w.rows = min(p.side * a.turns, w.count - w.first);
+    for (int i = tid; i < w.rows; i += blockDim.x) {
+        int page = b, r = w.start + w.first + i;
+        bool ok = true;
+        if (a.view.table) {
+            const int n = r, k = int(a.page.div(uint32_t(n)));
+            page = __ldg(a.view.table + b * a.view.table_stride + k);
+            r = n - k * a.view.rows;
+            ok = page >= 0 && page < a.view.num_pages;
+            if (!ok) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
+            page = min(max(page, 0), a.view.num_pages - 1);
+        }
+        at[i] = ok || !for_write ? page * p.c_stride[0] + r * p.c_stride[1] : -1;
+    }
+    w.row = int(p.per_block.div(uint32_t(tid)));
+    const int col = chunk * p.block_cols + tid - w.row * p.block_cols;
+    w.head = int(p.per_head.div(uint32_t(col)));
+    w.unit = col - w.head * (p.dim / 8);
+    w.some = w.row < p.side && col < p.cols;
+    __syncthreads();
+    return w;
 }
 
-// Code of a value whose quick code (of remainder r, with the sign of value minus what the code
-// stands for) is at most one off: the nearest, an even one at a tie.
-__device__ __noinline__ float exact_code(float c, float r, float scale) {
-    const float half = 0.5f * scale;
-    if (r > half || (r == half && (int(c) & 1))) c += 1.f;
-    else if (r < -half || (r == -half && (int(c) & 1))) c -= 1.f;
-    return fminf(fmaxf(c, 0.f), 15.f);
+// The pair and the eight codes of a unit (four lanes: a group).
+template <bool kHalf>
+__device__ __forceinline__ void quantise(const uint4& raw, uint32_t& word, uint32_t& pair) {
+    using P = Pair<kHalf>;
+    using T2 = typename P::T2;
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    T2 lo = P::as(w[0]), hi = lo;
+#pragma unroll
+    for (int e = 1; e < 4; ++e) { lo = __hmin2_nan(lo, P::as(w[e])); hi = __hmax2_nan(hi, P::as(w[e])); }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = __hmin2_nan(lo, P::as(__shfl_xor_sync(0xffffffffu, P::bits(lo), o)));
+        hi = __hmax2_nan(hi, P::as(__shfl_xor_sync(0xffffffffu, P::bits(hi), o)));
+    }
+    auto lo1 = __hmin_nan(lo.x, lo.y), hi1 = __hmax_nan(hi.x, hi.y);
+    const float low = float(lo1), high = float(hi1);
+    // In halves: the difference of two large values has to stay finite.
+    decltype(lo1) scale_t;
+    if constexpr (kHalf) scale_t = __float2half_rn((0.5f * high - 0.5f * low) / 7.5f);
+    else scale_t = __float2bfloat16_rn((0.5f * high - 0.5f * low) / 7.5f);
+    float scale = float(scale_t);
+    constexpr float kLargest = kHalf ? 65504.f : 3.3895313892515355e38f;
+    // What code 15 stands for must not pass the type's largest value: a scale rounded up that far goes one step down.
+    if (scale <= kLargest && fmaf(15.f, scale, low) > kLargest) {
+        if constexpr (kHalf) scale_t = __ushort_as_half(__half_as_ushort(scale_t) - 1);
+        else scale_t = __ushort_as_bfloat16(__bfloat16_as_ushort(scale_t) - 1);
+        scale = float(scale_t);
+    }
+    const bool finite = scale <= kLargest;                  // (of infinities and NaN the scale is one)
+    if (scale < 1.17549435e-38f) scale = 0.f;
+    // Distances and steps in halves too (those of tiny scales times 2^60, out of the subnormals).
+    const float f = scale > 0.f && scale < 0x1p-60f ? 0x1p59f : 0.5f, low2 = -f * low, s2 = f * scale;
+    const float inv = scale > 0.f ? __fdividef(1.f, s2) : 0.f;
+    // Nearest whole number: added to 1.5 2^23, whose last bit is 1.
+    constexpr float kMagic = 12582912.f;
+    word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float x;
+        if constexpr (kHalf) x = e & 1 ? __high2float(P::as(w[e / 2])) : __low2float(P::as(w[e / 2]));
+        else x = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        const float d = fmaf(x, f, low2);                   // the distance, rounded once
+        // The quotient, put right by its exact remainder: a half stays a half (in bf16 two of three
+        // warps have one), and nothing else becomes one.
+        float q = d * inv;
+        q = fmaf(fmaf(-q, s2, d), inv, q);
+        float t = q + kMagic;
+        // (bf16: the scale's rounding takes a quotient to 15.06 at most, and it has no small scales of few bits.)
+        if constexpr (kHalf) t = fminf(t, kMagic + 15.f);
+        word += __float_as_uint(t) << (16 * (e & 1) + 4 * (e / 2));
+    }
+    constexpr uint32_t kBits = 0x4b400000u;                 // kMagic's, as they were added up
+    word -= (kBits + (kBits << 4) + (kBits << 8) + (kBits << 12)) + ((kBits << 16) + (kBits << 20) + (kBits << 24) + (kBits << 28));
+    // scale, low; a group with an infinity or a NaN is NaN throughout.
+    if constexpr (kHalf) pair = uint32_t(__half_as_ushort(__float2half_rn(scale))) | uint32_t(__half_as_ushort(lo1)) << 16;
+    else pair = uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(scale))) | uint32_t(__bfloat16_as_ushort(lo1)) << 16;
+    if (!finite) { word = 0; pair = 0x7fff7fffu; }
 }
 
 template <bool kHalf>
 __global__ void __launch_bounds__(kThreads) cache4_write_kernel(const __grid_constant__ Args4 a) {
-    using P = Pair<kHalf>;
-    using T2 = typename P::T2;
-    const Job4& p = a.part[blockIdx.z];
-    const int b = blockIdx.y, lane = threadIdx.x & 31;
-    int start, count;
-    if (!span_of(a, b, p.rows, start, count) && blockIdx.x == 0 && threadIdx.x == 0) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
-    const uint32_t units = uint32_t(count) * p.per_row.d, first = blockIdx.x * (kThreads * kUnits) + threadIdx.x;
-    if (first - threadIdx.x >= units) return;
-    uint4 raw[kUnits];
-    int64_t at[kUnits];
-    int u[kUnits];
-    // Whole groups of four lanes have work or none (a row's units are a multiple of four).
+    __shared__ int64_t at[kMaxRows];
+    const Part4& p = a.part[blockIdx.z & 1];
+    const Place w = place_of(a, p, blockIdx.z >> 1, at, true);
+    const uint16_t* src = p.dense + blockIdx.y * p.stride[0] + (w.first + w.row) * p.stride[1] + w.head * p.stride[2] + 8 * w.unit;
+    const int64_t step = p.side * p.stride[1];
+    uint8_t* dst = p.cache + w.head * p.c_stride[2] + 4 * w.unit;
+    const int pair_at = codes_bytes(p.dim) - 3 * w.unit;    // of the first lane of a group: D / 2 + unit, seen from its codes
+    for (int i0 = 0; i0 * p.side < w.rows; i0 += kAhead) {
+        uint4 raw[kAhead];
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-        raw[k] = make_uint4(0, 0, 0, 0);
-        u[k] = -1;
-        const uint32_t unit = first + k * kThreads;
-        if (unit >= units) continue;
-        int row, head;
-        const bool ok = place_of(a, p, b, unit, start, row, head, u[k], at[k]);
-        raw[k] = __ldcs(reinterpret_cast<const uint4*>(p.dense + b * p.stride[0] + row * p.stride[1] + head * p.stride[2]) + u[k]);
-        if (!ok) {
-            report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
-            u[k] = -1;
+        for (int k = 0; k < kAhead; ++k) {
+            raw[k] = make_uint4(0, 0, 0, 0);
+            if (w.some && w.row + (i0 + k) * p.side < w.rows) raw[k] = __ldcs(reinterpret_cast<const uint4*>(src + (i0 + k) * step));
         }
-    }
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-        if (first + k * kThreads - lane >= units) break;        // the whole warp
-        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-        T2 lo = P::as(w[0]), hi = lo;
-#pragma unroll
-        for (int e = 1; e < 4; ++e) { lo = __hmin2_nan(lo, P::as(w[e])); hi = __hmax2_nan(hi, P::as(w[e])); }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            lo = __hmin2_nan(lo, P::as(__shfl_xor_sync(0xffffffffu, P::bits(lo), o)));
-            hi = __hmax2_nan(hi, P::as(__shfl_xor_sync(0xffffffffu, P::bits(hi), o)));
-        }
-        auto lo1 = __hmin_nan(lo.x, lo.y), hi1 = __hmax_nan(hi.x, hi.y);
-        const float low = float(lo1), high = float(hi1);
-        // In halves: the difference of two large values has to stay finite.
-        decltype(lo1) scale_t;
-        if constexpr (kHalf) scale_t = __float2half_rn((0.5f * high - 0.5f * low) / 7.5f);
-        else scale_t = __float2bfloat16_rn((0.5f * high - 0.5f * low) / 7.5f);
-        float scale = float(scale_t);
-        constexpr float kLargest = kHalf ? 65504.f : 3.3895313892515355e38f;
-        // What code 15 stands for must not pass the type's largest value: a scale rounded up that far goes one step down.
-        if (scale <= kLargest && fmaf(15.f, scale, low) > kLargest) {
-            if constexpr (kHalf) scale_t = __ushort_as_half(__half_as_ushort(scale_t) - 1);
-            else scale_t = __ushort_as_bfloat16(__bfloat16_as_ushort(scale_t) - 1);
-            scale = float(scale_t);
-        }
-        const bool finite = scale <= kLargest;                  // (of infinities and NaN the scale is one)
-        if (scale < 1.17549435e-38f) scale = 0.f;
-        const float s2 = 0.5f * scale, inv = scale > 0.f ? 1.f / s2 : 0.f, half = scale > 0.f ? 0.5f * s2 : INFINITY;
-        // Nearest whole number: added to 1.5 2^23, whose last bit is 1.
-        constexpr float kMagic = 12582912.f;
-        float c[8], r[8];
-        uint32_t word = 0;
-        bool off = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float2 x = [&] {
-                if constexpr (kHalf) return __half22float2(P::as(w[e / 2]));
-                else return __bfloat1622float2(P::as(w[e / 2]));
-            }();
-            const float d = fmaf(e & 1 ? x.y : x.x, 0.5f, -0.5f * low);     // half the distance, rounded once
-            const float t = fminf(fmaf(d, inv, kMagic), kMagic + 15.f);
-            c[e] = t - kMagic;
-            r[e] = fmaf(-c[e], s2, d);                          // exact where it matters
-            off |= fabsf(r[e]) >= half;
-            word += __float_as_uint(t) << (16 * (e & 1) + 4 * (e / 2));
-        }
-        constexpr uint32_t kBits = 0x4b400000u;                 // kMagic's, as they were added up
-        word -= (kBits + (kBits << 4) + (kBits << 8) + (kBits << 12)) + ((kBits << 16) + (kBits << 20) + (kBits << 24) + (kBits << 28));
-        if (off && finite && u[k] >= 0) {
-            word = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) word |= uint32_t(exact_code(c[e], r[e], s2)) << (16 * (e & 1) + 4 * (e / 2));
-        }
-        if (u[k] < 0) continue;
-        uint8_t* row = p.cache + at[k];
-        reinterpret_cast<uint32_t*>(row)[u[k]] = finite ? word : 0u;
-        if ((lane & 3) == 0) {
-            // scale, low; a group with an infinity or a NaN is NaN throughout.
-            uint32_t pair = 0x7fff7fffu;
-            if (finite) {
-                if constexpr (kHalf) pair = uint32_t(__half_as_ushort(__float2half_rn(scale))) | uint32_t(__half_as_ushort(lo1)) << 16;
-                else pair = uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(scale))) | uint32_t(__bfloat16_as_ushort(lo1)) << 16;
-            }
-            *reinterpret_cast<uint32_t*>(row + codes_bytes(p.dim) + u[k]) = pair;
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = w.row + (i0 + k) * p.side;
+            if (!__any_sync(0xffffffffu, w.some && i < w.rows)) continue;
+            uint32_t word, pair;
+            quantise<kHalf>(raw[k], word, pair);
+            if (!w.some || i >= w.rows || at[i] < 0) continue;
+            uint8_t* row = dst + at[i];
+            *reinterpret_cast<uint32_t*>(row) = word;
+            if ((w.unit & 3) == 0) *reinterpret_cast<uint32_t*>(row + pair_at) = pair;
         }
     }
 }
@@ -176,38 +184,36 @@ __global__ void __launch_bounds__(kThreads) cache4_write_kernel(const __grid_con
 template <bool kHalf>
 __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const __grid_constant__ Args4 a) {
     using P = Pair<kHalf>;
-    const Job4& p = a.part[blockIdx.z];
-    const int b = blockIdx.y;
-    int start, count;
-    if (!span_of(a, b, p.rows, start, count) && blockIdx.x == 0 && threadIdx.x == 0) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
-    const uint32_t units = uint32_t(a.zero_rest ? p.rows : count) * p.per_row.d, first = blockIdx.x * (kThreads * kUnits) + threadIdx.x;
-    uint32_t code[kUnits], pair[kUnits];
-    uint4* dst[kUnits];
+    __shared__ int64_t at[kMaxRows];
+    const Part4& p = a.part[blockIdx.z & 1];
+    const Place w = place_of(a, p, blockIdx.z >> 1, at, false);
+    if (!w.some) return;
+    const uint8_t* src = p.cache + w.head * p.c_stride[2] + 4 * w.unit;
+    const int pair_at = codes_bytes(p.dim) + (w.unit & ~3) - 4 * w.unit;
+    uint16_t* dst = p.dense + blockIdx.y * p.stride[0] + (w.first + w.row) * p.stride[1] + w.head * p.stride[2] + 8 * w.unit;
+    const int64_t step = p.side * p.stride[1];
+    const int rows = a.zero_rest ? min(p.side * a.turns, a.rows - w.first) : w.rows;
+    const typename P::Constants constants;
+    for (int i0 = 0; i0 * p.side < rows; i0 += kAhead) {
+        uint32_t code[kAhead], pair[kAhead];
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-        dst[k] = nullptr;
-        code[k] = pair[k] = 0;
-        const uint32_t unit = first + k * kThreads;
-        if (unit >= units) continue;
-        const int row = int(p.per_row.div(unit));
-        const uint32_t in_row = unit - uint32_t(row) * p.per_row.d;
-        const int head = int(p.per_head.div(in_row)), u = int(in_row) - head * p.upr;
-        dst[k] = reinterpret_cast<uint4*>(p.out + b * p.stride[0] + row * p.stride[1] + head * p.stride[2]) + u;
-        if (row >= count) continue;                             // zeros: scale and low of 0
-        int64_t page;
-        int r;
-        if (!cache_row(a.view, b, start + row, page, r)) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
-        const uint8_t* from = p.cache + page * p.c_stride[0] + r * p.c_stride[1] + head * p.c_stride[2];
-        code[k] = __ldcs(reinterpret_cast<const uint32_t*>(from) + u);
-        pair[k] = __ldcs(reinterpret_cast<const uint32_t*>(from + codes_bytes(p.dim) + (u & ~3)));
-    }
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = w.row + (i0 + k) * p.side;
+            code[k] = pair[k] = 0;                          // zeros: scale and low of 0
+            if (i < w.rows) {
+                const uint8_t* row = src + at[i];
+                code[k] = __ldcs(reinterpret_cast<const uint32_t*>(row));
+                pair[k] = __ldcs(reinterpret_cast<const uint32_t*>(row + pair_at));
+            }
+        }
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-        if (!dst[k]) continue;
-        const typename P::Constants constants;
-        const auto scale = P::as(low_twice(pair[k])), low = P::as(high_twice(pair[k]));
-        __stcs(dst[k], make_uint4(P::template values<0>(constants, code[k], scale, low), P::template values<1>(constants, code[k], scale, low),
-                                  P::template values<2>(constants, code[k], scale, low), P::template values<3>(constants, code[k], scale, low)));
+        for (int k = 0; k < kAhead; ++k) {
+            if (w.row + (i0 + k) * p.side >= rows) break;
+            const auto scale = P::as(low_twice(pair[k])), low = P::as(high_twice(pair[k]));
+            __stcs(reinterpret_cast<uint4*>(dst + (i0 + k) * step),
+                   make_uint4(P::template values<0>(constants, code[k], scale, low), P::template values<1>(constants, code[k], scale, low),
+                              P::template values<2>(constants, code[k], scale, low), P::template values<3>(constants, code[k], scale, low)));
+        }
     }
 }
 
@@ -220,8 +226,8 @@ int check_rows4(const slimkv_cache4_rows_args* a, const char* what) {
     for (int dim : {a->dim_qk, a->dim_v})
         if (dim < kGroupDims || dim > kMaxDims4 || dim % kGroupDims)
             return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "%s: dims must be multiples of 32 up to 320", what);
-    if (double(a->rows) * a->kv_heads * (a->dim_qk > a->dim_v ? a->dim_qk : a->dim_v) / 8 >= 2147483648.0 - kThreads * kUnits)
-        return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "%s: too many rows in one call", what);
+    if (a->rows > (1 << 28) || a->kv_heads > 4096)
+        return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "%s: at most 2^28 rows of 4096 heads in one call", what);
     if (int rc = check_cache(a->cache, a->batch, row4_bytes(a->dim_qk), row4_bytes(a->dim_v), 1, true, what)) return rc;
     if (!aligned16(a->k) || !aligned16(a->v)) return fail(SLIMKV_ERR_ALIGNMENT, "%s: 16-byte aligned rows", what);
     for (int i = 0; i < 3; ++i)
@@ -248,21 +254,22 @@ bool own_places(const Rows& r) {
 Args4 args_of(const slimkv_cache4_rows_args* a) {
     Args4 k{};
     for (int i = 0; i < 2; ++i) {
-        Job4& p = k.part[i];
-        p.rows = a->rows;
+        Part4& p = k.part[i];
         p.dim = i ? a->dim_v : a->dim_qk;
-        p.upr = p.dim / 8;
-        p.units = a->rows * a->kv_heads * p.upr;
-        p.per_row = FastDiv(uint32_t(a->kv_heads * p.upr));
-        p.per_head = FastDiv(uint32_t(p.upr));
-        p.out = static_cast<uint16_t*>(const_cast<void*>(i ? a->v : a->k));
-        p.dense = p.out;
+        p.cols = a->kv_heads * p.dim / 8;
+        p.block_cols = p.cols < kThreads ? p.cols : kThreads;
+        p.side = kThreads / p.block_cols;
+        p.per_block = FastDiv(uint32_t(p.block_cols));
+        p.per_head = FastDiv(uint32_t(p.dim / 8));
+        p.dense = static_cast<uint16_t*>(const_cast<void*>(i ? a->v : a->k));
         p.cache = static_cast<uint8_t*>(const_cast<void*>(i ? a->cache.v : a->cache.k));
         for (int s = 0; s < 3; ++s) {
             p.stride[s] = (i ? a->v_stride : a->k_stride)[s];
             p.c_stride[s] = (i ? a->cache.v_stride : a->cache.k_stride)[s];
         }
     }
+    k.rows = a->rows;
+    k.page = FastDiv(uint32_t(a->cache.rows));
     k.view = cache_view(a->cache);
     k.capacity = cache_capacity(k.view);
     k.starts = a->starts;
@@ -273,9 +280,19 @@ Args4 args_of(const slimkv_cache4_rows_args* a) {
 }
 
 template <class Kernel>
-int launch_rows4(Kernel kernel, const Args4& k, int batch, const char* what, void* stream) {
-    const int units = k.part[0].units > k.part[1].units ? k.part[0].units : k.part[1].units;
-    kernel<<<dim3((units - 1) / (kThreads * kUnits) + 1, batch, 2), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(k);
+int launch_rows4(Kernel kernel, Args4 k, int batch, const char* what, void* stream) {
+    // K and V by turns; where their rows differ, the blocks that the longer one needs.
+    int chunks = 0, row_blocks = 0, threads = 0;
+    for (const Part4& p : k.part) {
+        chunks = std::max(chunks, (p.cols + p.block_cols - 1) / p.block_cols);
+        row_blocks = std::max(row_blocks, (k.rows - 1) / p.side + 1);
+        threads = std::max(threads, (p.block_cols * p.side + 31) / 32 * 32);
+    }
+    // Few rows: a row to a thread, as long as that fills the GPU; many: several, for one look at their places.
+    const int64_t fill = int64_t(row_blocks) * batch * 2 * chunks / (8 * device_info().sm_count);
+    k.turns = int(std::max<int64_t>(1, std::min<int64_t>(kMaxTurns, fill)));
+    row_blocks = (row_blocks - 1) / k.turns + 1;
+    kernel<<<dim3(row_blocks, batch, 2 * chunks), threads, 0, static_cast<cudaStream_t>(stream)>>>(k);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? SLIMKV_OK : fail(SLIMKV_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
 }
