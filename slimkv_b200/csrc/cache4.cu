@@ -289,7 +289,7 @@ int launch_rows4(Kernel kernel, Args4 k, int batch, const char* what, void* stre
         threads = std::max(threads, (p.block_cols * p.side + 31) / 32 * 32);
     }
     // Few rows: a row to a thread, as long as that fills the GPU; many: several, for one look at their places.
-    const int64_t fill = int64_t(row_blocks) * batch * 2 * chunks / (8 * device_info().sm_count);
+    const int64_t fill = int64_t(row_blocks) * batch * 2 * chunks / (2 * device_info().sm_count);
     k.turns = int(std::max<int64_t>(1, std::min<int64_t>(kMaxTurns, fill)));
     row_blocks = (row_blocks - 1) / k.turns + 1;
     kernel<<<dim3(row_blocks, batch, 2 * chunks), threads, 0, static_cast<cudaStream_t>(stream)>>>(k);
