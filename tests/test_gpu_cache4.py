@@ -293,54 +293,60 @@ def test_latents(rank, T, lengths, page):
     run(*make(3, T, 32, 1, rank, lengths, context_only=True, page=page), context_only=True)
 
 
+# Dims of 128 and of 256, whose rows (20 and more) the two kernels take.
+@pytest.mark.parametrize('D', [128, 256])
 @pytest.mark.parametrize('T', [5, 40])
-def test_ragged_trees(T):
+def test_ragged_trees(T, D):
     """Sequences with fewer nodes (or none): the rows past them are empty."""
-    q, k4, v4, lens, _ = make(4, T, 8, 2, 128, [0, 140, 256, 0])
+    q, k4, v4, lens, _ = make(4, T, 8, 2, D, [0, 140, 256, 0])
     run(q, k4, v4, lens, seen=trees(4, T, 1), nodes=i32([T, T - 3, 0, 1]))
 
 
-def test_empty_rows():
+@pytest.mark.parametrize('D', [128, 256])
+def test_empty_rows(D):
     """Mask rows without a bit: over an empty context nothing is seen."""
-    q, k4, v4, lens, _ = make(2, 6, 8, 2, 128, [0, 40])
+    q, k4, v4, lens, _ = make(2, 6, 8, 2, D, [0, 40])
     seen = trees(2, 6, 2)
     seen[:, 3] = False
     got = run(q, k4, v4, lens, seen=seen)
     assert (got[0][0, 3] == 0).all() and (got[1][0, 3] == -math.inf).all() and got[1][1, 3].isfinite().all()
 
 
+@pytest.mark.parametrize('D', [128, 256])
 @pytest.mark.parametrize('T,page', [(6, 0), (40, 0), (6, 16)])
-def test_unseen_nans_do_not_spread(T, page):
+def test_unseen_nans_do_not_spread(T, page, D):
     """A node's non-finite key or value reaches the rows that see it and no other."""
-    q, k4, v4, lens, tables = make(2, T, 8, 2, 128, [100, 133], page=page)
+    q, k4, v4, lens, tables = make(2, T, 8, 2, D, [100, 133], page=page)
     seen = trees(2, T, 4)
     for b, n in enumerate([100, 133]):
         for node, x4, group in ((2, v4, 0), (3, v4, 3), (4, k4, 1), (1, v4, 2)):
             seen[b, :, node] = torch.arange(T) == node           # only the node itself sees it
-            place(x4, tables, b, n + node)[1, 64 + 4 * group:64 + 4 * group + 4] = 0xFF
+            place(x4, tables, b, n + node)[1, D // 2 + 4 * group:D // 2 + 4 * group + 4] = 0xFF
     got = run(q, k4, v4, lens, tables, seen=seen)
     assert got[0][:, 0].isfinite().all() and got[0][:, 5:].isfinite().all() and got[0][:, 1:5].isnan().any()
 
 
+@pytest.mark.parametrize('T,D', [(3, 128), (7, 256), (9, 320)])
 @pytest.mark.parametrize('scale', [2.0, 0.5])
 @pytest.mark.parametrize('dtype', [BF16, FP16])
-def test_peaked_scores(scale, dtype):
+def test_peaked_scores(scale, dtype, T, D):
     """Scores up to the hundreds: maxima that keep growing along the keys."""
-    q, k4, v4, lens, _ = make(1, 3, 8, 2, 128, [700], dtype=dtype)
-    k = torch.randn(1, 703, 2, 128, device='cuda') * torch.linspace(0.1, 3, 703, device='cuda')[None, :, None, None]
+    q, k4, v4, lens, _ = make(1, T, 8, 2, D, [700], dtype=dtype)
+    k = torch.randn(1, 700 + T, 2, D, device='cuda') * torch.linspace(0.1, 3, 700 + T, device='cuda')[None, :, None, None]
     cache4.write(k.to(dtype), k.to(dtype), k4, v4)
     run(q, k4, v4, lens, scale=scale)
 
 
-def test_small_probabilities_count_in_fp16():
+@pytest.mark.parametrize('H,D', [(1, 32), (17, 224)])
+def test_small_probabilities_count_in_fp16(H, D):
     """One key far above 20,000 others: their share of the weight stays."""
     n = 20000
-    k4, v4 = cache4.empty(1, n + 1, 1, 32)
-    k = torch.zeros(1, n + 1, 1, 32, device='cuda', dtype=FP16)
+    k4, v4 = cache4.empty(1, n + 1, 1, D)
+    k = torch.zeros(1, n + 1, 1, D, device='cuda', dtype=FP16)
     v = torch.ones_like(k)
     k[0, 5, 0, 0], v[0, 5] = 15.0, 0.0
     cache4.write(k, v, k4, v4)
-    q = torch.zeros(1, 1, 1, 32, device='cuda', dtype=FP16)
+    q = torch.zeros(1, 1, H, D, device='cuda', dtype=FP16)
     q[..., 0] = 1.0
     run(q, k4, v4, i32([n]), scale=1.0)
 
@@ -364,12 +370,14 @@ def test_strided_queries():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
-@pytest.mark.parametrize('B,H,G,lengths', [(40, 32, 8, [(7 * b) % 30 for b in range(40)]), (1, 4, 1, [70000]), (3, 8, 4, [20000, 3, 9000])])
-def test_many_and_long_segments(B, H, G, lengths):
+@pytest.mark.parametrize('B,H,G,D,lengths', [
+    (40, 32, 8, 64, [(7 * b) % 30 for b in range(40)]), (1, 4, 1, 64, [70000]), (3, 8, 4, 64, [20000, 3, 9000]),
+    (40, 40, 2, 224, [(11 * b) % 300 for b in range(40)]), (1, 40, 1, 320, [40000]), (3, 68, 2, 256, [9000, 3, 129])])
+def test_many_and_long_segments(B, H, G, D, lengths):
     """Shares of many short segments, and segments over many shares; twice the same bits."""
-    args = make(B, 1, H, G, 64, lengths)
+    args = make(B, 1, H, G, D, lengths)
     got = run(*args)
-    again = cache4.attention(*args[:3], args[3], 0.5 * 64 ** -0.5)
+    again = cache4.attention(*args[:3], args[3], 0.5 * D ** -0.5)
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
@@ -387,8 +395,9 @@ def test_offsets_past_32_bits():
     assert rows4.same(back.cpu(), rows4.values(*codes))
 
 
-def test_another_stream_and_two_graphs():
-    q, k4, v4, lens, _ = make(2, 8, 8, 2, 128, [300, 10])
+@pytest.mark.parametrize('D', [128, 256])
+def test_another_stream_and_two_graphs(D):
+    q, k4, v4, lens, _ = make(2, 8, 8, 2, D, [300, 10])
     mask = oracle.words_of(trees(2, 8, 7)).cuda()
     want = cache4.attention(q, k4, v4, lens, 0.09, mask=mask)
     torch.cuda.synchronize()
@@ -421,8 +430,9 @@ def test_attention_is_that_over_the_rows_read_back():
     assert (got[1] - want[1]).abs().max() <= 2e-5
 
 
-def test_lengths_past_the_cache_are_reported():
-    q, k4, v4, _, _ = make(1, 2, 8, 2, 128, [60], spare=0)
+@pytest.mark.parametrize('H,D', [(8, 128), (40, 320)])
+def test_lengths_past_the_cache_are_reported(H, D):
+    q, k4, v4, _, _ = make(1, 2, H, 2, D, [60], spare=0)
     _lib.device_status(clear=True)
     cache4.attention(q, k4, v4, i32([61]), 0.1)
     assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH
@@ -430,22 +440,26 @@ def test_lengths_past_the_cache_are_reported():
     assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH
 
 
-def test_pages_outside_the_pool_are_reported():
-    q, k4, v4, lens, tables = make(1, 2, 8, 2, 128, [60], page=16)
+@pytest.mark.parametrize('H,D', [(8, 128), (40, 320)])
+def test_pages_outside_the_pool_are_reported(H, D):
+    q, k4, v4, lens, tables = make(1, 2, H, 2, D, [60], page=16)
     _lib.device_status(clear=True)
     tables[0, 2] = k4.shape[0]
     cache4.attention(q, k4, v4, lens, 0.1, block_tables=tables)
     assert _lib.device_status(clear=True) == _lib.DEVICE_BAD_LENGTH
 
 
-def test_a_wait_that_runs_out_is_reported():
-    q, k4, v4, lens, _ = make(1, 2, 8, 2, 128, [9000])
-    _lib.device_status(clear=True)
-    cache4.attention(q, k4, v4, lens, 0.1, wait_limit_ns=1)
-    assert _lib.device_status(clear=True) in (0, _lib.DEVICE_TIMEOUT)
-    mass = torch.zeros(1, 2, 9010, device='cuda')
-    cache4.key_mass(q, k4, torch.zeros(1, 2, 8, device='cuda'), mass, lens, 0.1, wait_limit_ns=1)
-    assert _lib.device_status(clear=True) in (0, _lib.DEVICE_TIMEOUT)
+@pytest.mark.parametrize('H,D,n', [(8, 128, 9000), (8, 64, 40), (40, 320, 9000), (40, 256, 300)])
+def test_a_wait_that_runs_out_is_reported(H, D, n):
+    """Every wait ends at its limit, the call returns, and the next one is right."""
+    q, k4, v4, lens, _ = make(3, 2, H, 2, D, [n, n // 2, n])
+    lse = torch.zeros(3, 2, H, device='cuda')
+    for limit in (1, 1000):
+        _lib.device_status(clear=True)
+        cache4.attention(q, k4, v4, lens, 0.1, wait_limit_ns=limit)
+        assert _lib.device_status(clear=True) in (0, _lib.DEVICE_TIMEOUT)
+        cache4.key_mass(q, k4, lse, torch.zeros(3, 2, n + 10, device='cuda'), lens, 0.1, wait_limit_ns=limit)
+        assert _lib.device_status(clear=True) in (0, _lib.DEVICE_TIMEOUT)
     run(q, k4, v4, lens)
 
 
