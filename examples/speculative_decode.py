@@ -15,9 +15,10 @@ A small decoder with random weights, batched.  Each step:
 
 While nothing has been evicted the tokens are those of one-token-at-a-time
 greedy decoding.  Keys are cached rotated, so the rows that stay need no
-change.
+change.  With ``--four-bit`` the caches hold 4-bit rows (``cache4``): written,
+attended over and weighed by its calls, committed and evicted by the same ones.
 
-    python examples/speculative_decode.py [--steps 64] [--budget 192]
+    python examples/speculative_decode.py [--steps 64] [--budget 192] [--four-bit]
 """
 import argparse
 import os
@@ -27,7 +28,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from slimkv_b200 import eviction, kernels, tree  # noqa: E402
+from slimkv_b200 import cache4, eviction, kernels, tree  # noqa: E402
 from slimkv_b200.rope import rope_tables  # noqa: E402
 
 
@@ -57,9 +58,11 @@ class Model:
 class Cache:
     """K, V and masses of all layers; a second set of buffers takes what an eviction keeps."""
 
-    def __init__(self, model, batch, capacity):
-        shape = (model.layers, batch, capacity, model.kv_heads, model.head_dim)
-        self.k, self.v, self.k2, self.v2 = (torch.zeros(shape, dtype=torch.bfloat16, device='cuda') for _ in range(4))
+    def __init__(self, model, batch, capacity, four_bit=False):
+        self.four_bit = four_bit
+        width, dtype = (cache4.row_bytes(model.head_dim), torch.uint8) if four_bit else (model.head_dim, torch.bfloat16)
+        shape = (model.layers, batch, capacity, model.kv_heads, width)
+        self.k, self.v, self.k2, self.v2 = (torch.zeros(shape, dtype=dtype, device='cuda') for _ in range(4))
         self.mass, self.mass2 = (torch.zeros((model.layers, batch, model.kv_heads, capacity), device='cuda')
                                  for _ in range(2))
         # Where each kept row stood in the sequence.
@@ -87,9 +90,15 @@ def forward(model, cache, tokens, positions, mask=None):
     for l in range(model.layers):
         qkv = (kernels.rms_norm(x, model.norm, model.eps) @ model.qkv[l].T).view(batch, t, heads + 2 * kv_heads, dim)
         q = kernels.rope_rows(qkv[:, :, :heads], positions, model.cos, model.sin)
-        cache.k[l, sequences, rows] = kernels.rope_rows(qkv[:, :, heads:heads + kv_heads], positions, model.cos, model.sin)
-        cache.v[l, sequences, rows] = qkv[:, :, heads + kv_heads:]
-        out, lse = tree.tree_attention(q, cache.k[l], cache.v[l], cache.lengths, dim ** -0.5, mask=mask)
+        k = kernels.rope_rows(qkv[:, :, heads:heads + kv_heads], positions, model.cos, model.sin)
+        v = qkv[:, :, heads + kv_heads:]
+        if cache.four_bit:
+            cache4.write(k, v, cache.k[l], cache.v[l], cache.lengths)
+            out, lse = cache4.attention(q, cache.k[l], cache.v[l], cache.lengths, dim ** -0.5, mask=mask)
+        else:
+            cache.k[l, sequences, rows] = k
+            cache.v[l, sequences, rows] = v
+            out, lse = tree.tree_attention(q, cache.k[l], cache.v[l], cache.lengths, dim ** -0.5, mask=mask)
         seen.append((q, lse))
         x = x + out.view(batch, t, heads * dim) @ model.o[l].T
         gate_up = kernels.rms_norm(x, model.norm, model.eps).view(batch * t, -1) @ model.gate_up[l].T
@@ -98,9 +107,10 @@ def forward(model, cache, tokens, positions, mask=None):
 
 
 def add_masses(model, cache, seen, lengths, rows=None, counts=None, decay=1.0):
+    key_mass = cache4.key_mass if cache.four_bit else eviction.key_mass
     for l, (q, lse) in enumerate(seen):
-        eviction.key_mass(q, cache.k[l], lse, cache.mass[l], lengths, model.head_dim ** -0.5, rows=rows, counts=counts,
-                          decay=decay)
+        key_mass(q, cache.k[l], lse, cache.mass[l], lengths, model.head_dim ** -0.5, rows=rows, counts=counts,
+                 decay=decay)
 
 
 def prefill(model, cache, prompt, chunk=64):
@@ -133,14 +143,15 @@ def draft(history, branches, depth):
     return tokens, parents
 
 
-def generate(model, prompt, steps, budget=None, slack=32, sinks=4, recent=64, branches=3, depth=4, decay=1.0):
+def generate(model, prompt, steps, budget=None, slack=32, sinks=4, recent=64, branches=3, depth=4, decay=1.0,
+             four_bit=False):
     """``steps`` speculative steps behind ``prompt [B, n]``; returns each
     sequence's new tokens, and the cache."""
     batch, n = prompt.shape
     nodes = 1 + branches * depth
     # A step adds up to depth + 1 rows and needs room for the nodes' rows behind the context.
     most = n + steps * (depth + 1) if budget is None else max(n, budget + slack) + depth + 1
-    cache = Cache(model, batch, most + nodes)
+    cache = Cache(model, batch, most + nodes, four_bit)
     first = prefill(model, cache, prompt)
     history = [p + [t] for p, t in zip(prompt.tolist(), first.tolist())]
     length = n
@@ -179,11 +190,12 @@ def main():
     parser.add_argument('--prompt', type=int, default=160)
     parser.add_argument('--steps', type=int, default=64)
     parser.add_argument('--budget', type=int, default=192)
+    parser.add_argument('--four-bit', action='store_true')
     args = parser.parse_args()
     model = Model()
     gen = torch.Generator(device='cuda').manual_seed(1)
     prompt = torch.randint(0, model.vocab, (args.batch, args.prompt), generator=gen, device='cuda')
-    tokens, cache = generate(model, prompt, args.steps, budget=args.budget)
+    tokens, cache = generate(model, prompt, args.steps, budget=args.budget, four_bit=args.four_bit)
     made = sum(map(len, tokens))
     print(f'{made} tokens in {args.steps} steps of {args.batch} sequences '
           f'({made / args.steps / args.batch:.2f} per sequence and step); cache rows {cache.lengths.tolist()}')
