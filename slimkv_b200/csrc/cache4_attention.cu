@@ -646,7 +646,8 @@ extern "C" int slimkv_cache4_attention(const slimkv_tree_attention_args* a, void
     J.v = static_cast<const uint8_t*>(cache.v);
     J.cache = cache_view(cache);
     J.capacity = cache_capacity(J.cache);
-    if (double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / tile + 1 + Plan<4, kWideKeys>::kPieceUnits) >= 2147483648.0)
+    if (J.capacity > 0x7fffffffLL - 4096 ||
+        double(J.batch) * J.kv_heads * J.row_groups * double(J.capacity / tile + 1 + Plan<4, kWideKeys>::kPieceUnits) >= 2147483648.0)
         return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "4-bit attention: too many rows in one call");
     J.lengths = a->lengths;
     J.nodes_len = a->nodes_len;

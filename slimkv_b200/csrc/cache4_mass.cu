@@ -322,7 +322,8 @@ extern "C" int slimkv_cache4_key_mass(const slimkv_key_mass_args* a, void* strea
     J.paged = paged;
     J.cache = cache_view(cache);
     J.capacity = std::min<int64_t>(cache_capacity(J.cache), a->mass_rows);
-    if (double(J.batch) * J.kv_heads * (double(J.capacity / kKeys + 1) * (kMaxRows / 32 + 1) + Plan::kPieceUnits) >= 2147483648.0)
+    if (J.capacity > 0x7fffffffLL - 4096 ||
+        double(J.batch) * J.kv_heads * (double(J.capacity / kKeys + 1) * (kMaxRows / 32 + 1) + Plan::kPieceUnits) >= 2147483648.0)
         return fail(SLIMKV_ERR_UNSUPPORTED_SHAPE, "%s: too many rows in one call", what);
     J.q = static_cast<const uint16_t*>(a->q);
     J.q_sb = a->q_stride[0]; J.q_st = a->q_stride[1]; J.q_sh = a->q_stride[2];
