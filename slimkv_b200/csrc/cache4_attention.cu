@@ -19,12 +19,26 @@
 // keys; P goes from the layout of S to that of the second product by two
 // transpositions of 8 x 8 blocks in registers.
 //
-// Work: equal shares of all segments' 64-key tiles (key_shares.cuh), a segment
-// being the keys of one (sequence, KV head, 8 or 16 query rows); in a CTA's
+// Work: equal shares of all segments' tiles of 64 or 128 keys (key_shares.cuh), a
+// segment being the keys of one (sequence, KV head, 8 or 16 query rows); in a CTA's
 // piece of a segment each of its four warps takes a quarter of every tile, with
 // its own ring of TMA loads and its own running softmax, and the warps meet only
 // at the piece's end.  Pieces that are not a whole segment leave normalised
 // partial rows, which a dependent launch merges.  Lengths are read on the device.
+//
+// Bound: instructions.  A word of codes (8 values) takes 15 of them, 7 of the
+// logic unit and 8 on pairs of 16-bit values, and either kind issues every other
+// cycle; over a long context the kernel goes through the keys at 5.5 TB/s, from
+// HBM and from L2 alike.  Around that a call spends 5 us before the first keys,
+// 2 on its merge and 6 on CTAs that end before others.  Measured in a graph (bf16,
+// 32 / 8 heads of 128 dims): 16 sequences of 8k rows, one token 47 us = 3.6 TB/s
+// (the same rows in 16 bits: 107 us), four nodes 64, one sequence of 131072 rows in
+// 16-row pages 51, one token over 517 rows 8.4.  What that took, for the first:
+// 67.5 us; constant row lengths, plain shared-memory loads 61; and + or of the
+// codes in one instruction 55; 32 keys to a warp's step 49; masks only in a
+// sequence's last steps 47.  More CTAs than fit (each pays the start): 54 to 63; five
+// of 16 keys a step on an SM instead of four of 32: 56; contiguous copies in place of
+// the TMA's boxes: 48.
 #include <algorithm>
 #include <type_traits>
 

@@ -2,10 +2,9 @@
 // than 192 dims: the heads of a token over the latents (C ABI
 // slimkv_cache4_attention).
 //
-// The warp-level products of cache4_attention.cu run at 256 multiply-adds a clock
-// and SM, which 32 rows of 320 dims would keep busy for four times as long as HBM
-// takes for the keys.  Here tcgen05 has the products, keys on its M side, the rows
-// on N:
+// A warp of cache4_attention.cu has registers for 16 rows of 320 dims, so 32 rows
+// would turn every code into an operand twice.  Here tcgen05 has the products, keys
+// on its M side, the rows on N:
 //   S^T [128 keys x N rows] = K . Q^T,    O^T [128 dims x N rows] (up to 3) += V^T . P^T.
 // The codes become 16-bit operands once for 32 rows.  A K row belongs to one
 // thread, which writes it to tensor memory (the A operand of S); V^T needs its keys
@@ -19,7 +18,8 @@
 // exponentials it would be 29, without the loads too 24: 5 us to the first tile,
 // 3 of a piece's end, 5 of the merge, and about 1.4 us a tile of barriers between
 // the roles.  (K's codes in eight warps of their own: the same.  Sixteen warps for
-// all codes: 43.)
+// all codes: 43.  64 rows to a pass: 156 against 170 us for 256 rows, slower for
+// fewer than 128.)
 //
 // Warps: 0 and 3 load the 4-bit K and V rows (TMA; 3 finds the CTA's share), 1
 // issues the products, 2 owns tensor memory, 4-11 turn K's codes into operands and
@@ -103,12 +103,6 @@ __device__ __forceinline__ int ordered(float x) {
     return i ^ (i >> 31 & 0x7fffffff);
 }
 __device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ (i >> 31 & 0x7fffffff)); }
-
-template <int NC>
-__device__ __forceinline__ void tmem_st_cols(uint32_t at, const float* v) {
-#pragma unroll
-    for (int c = 0; c < NC; c += 16) tmem_st16(at + c, v + c);
-}
 
 template <int G, int N, bool kHalf>
 __global__ void __launch_bounds__(kThreads, 1)
