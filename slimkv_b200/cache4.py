@@ -141,8 +141,10 @@ def attention(q, k4, v4, lengths, scale, mask=None, nodes=None, block_tables=Non
     """``tree.tree_attention`` over a 4-bit cache (``slimkv_cache4_attention``):
     the same arguments and results, ``k4`` / ``v4`` the caches that
     :func:`write` filled from rows of q's type.  The query rows of a KV head are
-    taken 8 or 16 at a time, each time over all keys: made for single tokens and
-    small trees (many rows: :func:`read`, then ``tree.tree_attention``)."""
+    taken 8, 16 or (of wide rows) 32 at a time, each time over all keys: made for
+    single tokens and small trees.  For many (over long caches from about 17
+    nodes of 4 heads, over latents from 4 of 32) :func:`read`, then
+    ``tree.tree_attention`` is faster."""
     dim, dim_v = _caches(k4, v4)
     if q.dim() != 4 or q.shape[3] != dim:
         _refuse('q must be [B, T, H, D] with caches of row_bytes(D) bytes a row')
@@ -156,7 +158,8 @@ def attention(q, k4, v4, lengths, scale, mask=None, nodes=None, block_tables=Non
 def key_mass(q, k4, lse, mass, lengths, scale, rows=None, counts=None, decay=1.0, block_tables=None,
              context_only=False, wait_limit_ns=0):
     """``eviction.key_mass`` over the keys of a 4-bit cache
-    (``slimkv_cache4_key_mass``): the same arguments and results."""
+    (``slimkv_cache4_key_mass``): the same arguments and results.  Over latents
+    with many accepted rows, ``read`` and ``eviction.key_mass`` are faster."""
     if not (k4.is_cuda and k4.dim() == 4 and q.dim() == 4 and q.shape[3] == _dim_of(k4, 'k4')):
         _refuse('q must be [B, T, H, D], k4 a CUDA cache of row_bytes(D) bytes a row')
     a = mass_args(q, k4, lse, mass, lengths, scale, rows, counts, decay, block_tables, context_only, wait_limit_ns,

@@ -7,15 +7,15 @@
 // dims (one 16-byte load) each; the least and largest value go between them by
 // two shuffles, and every lane writes the four bytes of its codes.
 //
-// Bound: HBM (2.625 bytes a value either way) and, close behind, instructions,
-// most of which issue every other cycle.  So a thread keeps its column and a block
-// looks its rows' places up once (with two divisions and a table look-up for every
-// eight values reading 16 x 8k latents took 62 us), and what is exact is bought
-// cheaply: the quotient is a product with 1 / scale, put right by its exact remainder
-// (Markstein's division), which leaves a half a half; a separate rule for ties
-// cost 13 us of 47, two of three warps having one in bf16.  Measured in a graph:
-// a prompt chunk of 18k rows of 8 heads of 128 dims written and read back 47 us
-// (27 of them the write: 3.7 TB/s), 16 x 8k latents of 320 dims read 38 us = 5.4 TB/s.
+// Bound: reading, HBM (2.625 bytes a value either way); writing, instructions.  So
+// a thread keeps its column and a block looks its rows' places up once (with two
+// divisions and a table look-up for every eight values reading 16 x 8k latents took
+// 62 us), and the quotient is a product with 1 / scale, put right by its exact
+// remainder (Markstein's division), which leaves a half a half: a rule of its own
+// for ties made the chunk below 56 us in place of 47.  Measured in a graph (bf16): 4
+// sequences of 4608 rows of 8 heads of 128 dims, write 31 us = 3.2 TB/s, read 19 us
+// = 5.2 TB/s; 4 of 4097 to 5120 rows written and read back 47 us; 16 x 8k latents of
+// 320 dims out of pages read 38 us = 5.4 TB/s.
 #include <algorithm>
 #include <type_traits>
 

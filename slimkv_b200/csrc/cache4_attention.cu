@@ -26,11 +26,12 @@
 // at the piece's end.  Pieces that are not a whole segment leave normalised
 // partial rows, which a dependent launch merges.  Lengths are read on the device.
 //
-// Bound: instructions.  A word of codes (8 values) takes 15 of them, 7 of the
+// Bound: instructions and their latency (61 % of the cycles issue, the logic unit
+// is busy for 50 %).  A word of bf16 codes (8 values) takes 15 of them, 7 of the
 // logic unit and 8 on pairs of 16-bit values, and either kind issues every other
-// cycle; over a long context the kernel goes through the keys at 5.5 TB/s, from
-// HBM and from L2 alike.  Around that a call spends 5 us before the first keys,
-// 2 on its merge and 6 on CTAs that end before others.  Measured in a graph (bf16,
+// cycle; in its steady state the kernel goes through the keys at 5.5 TB/s, from HBM
+// and from L2 alike.  Around that, of 44 us, the first keys come after 5.6, and the CTAs
+// end between 28 and 44 (37 in the mean).  Measured in a graph (bf16,
 // 32 / 8 heads of 128 dims): 16 sequences of 8k rows, one token 47 us = 3.6 TB/s
 // (the same rows in 16 bits: 107 us), four nodes 64, one sequence of 131072 rows in
 // 16-row pages 51, one token over 517 rows 8.4.  What that took, for the first:

@@ -19,7 +19,7 @@
 // 3 of a piece's end, 5 of the merge, and about 1.4 us a tile of barriers between
 // the roles.  (K's codes in eight warps of their own: the same.  Sixteen warps for
 // all codes: 43.  64 rows to a pass: 156 against 170 us for 256 rows, slower for
-// fewer than 128.)
+// 32 to 96.)
 //
 // Warps: 0 and 3 load the 4-bit K and V rows (TMA; 3 finds the CTA's share), 1
 // issues the products, 2 owns tensor memory, 4-11 turn K's codes into operands and

@@ -11,11 +11,12 @@
 // Work: the 64-key tiles of all (sequence, KV head) segments in equal shares
 // (key_shares.cuh), a quarter of each tile to a warp with its own ring of TMA
 // loads.  More than 64 rows are taken block by block over the piece's tiles.
-// Bound: instructions (codes, and products of few rows that the warps wait for);
-// with many rows the products.  Measured in a graph: 1 to 5 accepted rows of 32
-// heads for 16 sequences of 8k keys (8 KV heads of 128 dims) 48 us = 1.9 TB/s, one
-// row over 1028 keys 5.5 us, 1 to 8 rows over 16 x 8k latents of 320 dims 105 us
-// (the 16-bit keys' kernel, on tcgen05, 29).
+// Bound: instructions and their latency (57 % of the cycles issue, at a third of
+// HBM's rate).  Measured in a graph (bf16): 1 to 5 accepted rows of 32 heads for 16
+// sequences of 8k keys (8 KV heads of 128 dims) 48 us = 1.9 TB/s, one row over 1028
+// keys 5.6 us.  Against the 16-bit keys' kernel (tcgen05), every row accepted: 5
+// rows of that shape 54 us and 53; 8 rows (256 queries of a KV head) over 16 x 8k
+// latents of 320 dims 137 us and 31: it saves memory, and time only for few rows.
 #include <algorithm>
 #include <type_traits>
 
