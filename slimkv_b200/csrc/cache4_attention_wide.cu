@@ -495,7 +495,10 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         tmem_wait_ld();
                         if (d >= dims) continue;        // (the whole warp)
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) v[c] *= bs->inv[cb + c0 + c];
+                        for (int c = 0; c < 16; ++c) {
+                            const float f = bs->inv[cb + c0 + c];
+                            v[c] = f == 0.f ? 0.f : v[c] * f;       // (a row of no node may hold NaN)
+                        }
                         if (bad) {
 #pragma unroll 1
                             for (int c = 0; c < 16; ++c)

@@ -302,6 +302,26 @@ def test_ragged_trees(T, D):
     run(q, k4, v4, lens, seen=trees(4, T, 1), nodes=i32([T, T - 3, 0, 1]))
 
 
+# One tile of keys (a segment written by one block) and several (merged).
+@pytest.mark.parametrize('lengths', [[0, 20, 100, 90], [0, 140, 2000, 700]])
+@pytest.mark.parametrize('D', [128, 256, 320])
+@pytest.mark.parametrize('context_only', [False, True])
+def test_rows_past_the_nodes_are_empty_whatever_they_hold(lengths, D, context_only):
+    """Queries of a padded batch hold anything, and a value of the context may be NaN."""
+    T, nodes = 9, [9, 6, 0, 1]
+    q, k4, v4, lens, _ = make(4, T, 8, 2, D, lengths, context_only=context_only)
+    for b, (n, fill) in enumerate(zip(nodes, (0.0, math.nan, math.inf, -math.inf))):
+        q[b, n:] = fill
+    v4[3, 5, 1, D // 2:D // 2 + 4] = 0xFF                # a value of the context, in all rows of sequence 3
+    out, lse = cache4.attention(q, k4, v4, lens, 0.5 * D ** -0.5, nodes=i32(nodes), context_only=context_only)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    for b, n in enumerate(nodes):
+        assert (out[b, n:] == 0).all() and (lse[b, n:] == -math.inf).all()
+    assert lse[0, :].isfinite().all() == (not context_only) and out[1, :6].isfinite().all() and lse[1, :6].isfinite().all()
+    assert out[3, 0, 4:, :32].isnan().all() and out[3, 0, :4].isfinite().all() and out[3, 0, 4:, 32:].isfinite().all()
+
+
 @pytest.mark.parametrize('D', [128, 256])
 def test_empty_rows(D):
     """Mask rows without a bit: over an empty context nothing is seen."""
