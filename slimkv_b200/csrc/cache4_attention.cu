@@ -34,7 +34,7 @@
 // end between 28 and 44 (37 in the mean).  Measured in a graph (bf16,
 // 32 / 8 heads of 128 dims): 16 sequences of 8k rows, one token 47 us = 3.6 TB/s
 // (the same rows in 16 bits: 107 us), four nodes 64, one sequence of 131072 rows in
-// 16-row pages 51, one token over 517 rows 8.4.  What that took, for the first:
+// 16-row pages 51 or 56 (two GPUs), one token over 517 rows 8.4.  What that took, for the first:
 // 67.5 us; constant row lengths, plain shared-memory loads 61; and + or of the
 // codes in one instruction 55; 32 keys to a warp's step 49; masks only in a
 // sequence's last steps 47.  More CTAs than fit (each pays the start): 54 to 63; five
