@@ -65,9 +65,12 @@ struct Layout {
 template <int N, class Work>
 struct Bars {
     uint64_t kraw_full[6], kraw_empty[6], vraw_full[6], vraw_empty[6];
+    // pempty: P . V of the tile in the buffer is over, so O has it.  One for each buffer: a softmax warp
+    // waits for every phase of it in order, before the tile that starts the next, and so never takes
+    // the phase before last, which has the same parity, for the one that it waits for.
     uint64_t kfull[2], kempty[2], sfull[2], sempty[2], pfull[2], pempty[2];
     uint64_t vfull[4], vempty[4];                // half V tiles
-    uint64_t qfull, odone, oempty, final_mma;
+    uint64_t qfull, oempty, final_mma;
     uint32_t tmem_base;
     int abort;
     int bad_values[4];                           // 1 + a piece whose nodes' values hold NaN, by piece % 4
@@ -131,7 +134,6 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         bs->bad_values[i] = bs->bad_values[2 + i] = 0;
     } else if (tid == 10) {
         mbar_init(&bs->qfull, kSoftWarps);
-        mbar_init(&bs->odone, 1);
         mbar_init(&bs->oempty, kSoftWarps);
         mbar_init(&bs->final_mma, 1);
         bs->abort = 0;
@@ -218,10 +220,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                             umma_bf16(uint32_t(b * N), v_desc + ((vb * L::kV + 2 * b * kChunk + h * (kChunk / 2) + k * 2048) >> 4),
                                       p_desc + ((pb * L::kP + h * (kChunk / 2) + k * 2048) >> 4), idesc_o, !first || h || k);
                     umma_commit(&bs->vempty[2 * vb + h]);
-                    if (h) {
-                        umma_commit(&bs->pempty[pb]);
-                        umma_commit(&bs->odone);
-                    }
+                    if (h) umma_commit(&bs->pempty[pb]);
                 }
                 __syncwarp();
             }
@@ -407,7 +406,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 #pragma unroll
                     for (int c = 0; c < NC; ++c) sum[c] *= bs->alpha[cb + c];
                     if (tile > w.t0) {
-                        ok = ok && warp_wait(&bs->odone, (o - 1) & 1, bs, J);
+                        ok = ok && warp_wait(&bs->pempty[(o - 1) % L::kPBufs], ((o - 1) / L::kPBufs) & 1, bs, J);
                         if (ok) {
                             tc_fence_after();
 #pragma unroll 1
@@ -479,7 +478,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 }
             }
             named_bar(1 + a, 128);
-            ok = ok && warp_wait(&bs->odone, (o - 1) & 1, bs, J);
+            ok = ok && warp_wait(&bs->pempty[(o - 1) % L::kPBufs], ((o - 1) / L::kPBufs) & 1, bs, J);
             if (ok) {
                 tc_fence_after();
                 const bool bad = *const_cast<volatile int*>(&bs->bad_values[piece & 3]) == int(piece) + 1, whole = w.whole();

@@ -401,6 +401,28 @@ def test_many_and_long_segments(B, H, G, D, lengths):
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
 
+# More than 16 query rows of 224 or 256 dims: two tiles' probabilities may be under way at a piece's end.
+@pytest.mark.parametrize('H,D,Dv,dtype', [(24, 256, 256, BF16), (40, 224, 256, FP16), (40, 256, 64, BF16), (24, 64, 224, FP16)])
+def test_pieces_end_with_all_their_products(H, D, Dv, dtype):
+    """Pieces of 1 to 12 tiles, over and over beside other traffic: the exact result, and the same bits each time."""
+    B = 150
+    lengths = [128 * (1 + b % 12) - b % 7 for b in range(B)]
+    q, k4, v4, lens, _ = make(B, 1, H, 1, D, lengths, Dv=Dv, dtype=dtype, layout='shared', context_only=True)
+    want = run(q, k4, v4, lens, context_only=True)
+    side, a = torch.cuda.Stream(), torch.zeros(1 << 28, dtype=torch.uint8, device='cuda')
+    b = torch.empty_like(a)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                b.copy_(a)
+        for _ in range(10):
+            got = cache4.attention(q, k4, v4, lens, 0.5 * D ** -0.5, context_only=True)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
 def test_offsets_past_32_bits():
     """Sequence strides of more than 2^32 bytes."""
     big = torch.empty(2, (1 << 32) + (1 << 12), dtype=torch.uint8, device='cuda')
