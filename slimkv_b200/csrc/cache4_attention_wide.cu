@@ -26,7 +26,10 @@
 // have the softmax (4-7 every other group of 32 dims and the first half of the
 // rows, 8-11 the others), 12-19 turn V's codes into operands.  K of a tile is made
 // ready before the softmax of the tile before it, which hides S.  Every wait is
-// bounded; after one that ran out all threads still meet at every barrier.
+// bounded; after one that ran out a warp still meets the others at every barrier
+// of threads, but arrives at no mbarrier any more: a ring slot that is called empty
+// while its copy is under way would get another copy, on a barrier whose phase has
+// had its one arrival, and the CTA could end with copies under way.
 #include <algorithm>
 #include <type_traits>
 
@@ -304,7 +307,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             }
             fence_async_shared();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bs->qfull);
+            if (ok && lane == 0) mbar_arrive(&bs->qfull);
             if (gt < NC) {
                 bs->top[cb + gt] = -INFINITY;
                 bs->shift[cb + gt] = 3e38f;
@@ -345,7 +348,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) {
+                if (ok && lane == 0) {
                     mbar_arrive(&bs->kraw_empty[slot]);
                     mbar_arrive(&bs->kfull[kb]);
                 }
@@ -361,7 +364,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 tmem_wait_ld();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bs->sempty[sb]);
+                if (ok && lane == 0) mbar_arrive(&bs->sempty[sb]);
                 if ((tile + 1) * kKeys > w.s.len) {
                     // Which rows see the key: all the context, a node's those that have it among their ancestors.
                     const int node = n - w.s.len;
@@ -448,7 +451,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bs->pfull[pb]);
+                if (ok && lane == 0) mbar_arrive(&bs->pfull[pb]);
                 ++o;
             };
             for (int tile = w.t0; tile < w.t1; ++tile) {
@@ -521,7 +524,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 tc_fence_before();
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bs->oempty);
+            if (ok && lane == 0) mbar_arrive(&bs->oempty);
             ++piece;
         }
     } else if (any && warp >= 4 + kSoftWarps) {
@@ -573,7 +576,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     fence_async_shared();
                 }
                 __syncwarp();
-                if (lane == 0) {
+                if (ok && lane == 0) {
                     mbar_arrive(&bs->vraw_empty[slot]);
                     mbar_arrive(&bs->vfull[buf]);
                 }

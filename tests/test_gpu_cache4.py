@@ -505,6 +505,20 @@ def test_a_wait_that_runs_out_is_reported(H, D, n):
     run(q, k4, v4, lens)
 
 
+@pytest.mark.parametrize('B,H,G,D', [(3, 40, 2, 320), (3, 40, 2, 256), (20, 24, 1, 224)])
+def test_waits_that_run_out_end_the_wide_pipeline(B, H, G, D):
+    """With a limit of 1 ns the first products' waits run out while copies are under way (they take a microsecond):
+    the call reports it and ends with nothing under way, again and again, and the next one is right."""
+    q, k4, v4, lens, _ = make(B, 1, H, G, D, [9000 - 400 * b for b in range(B)])
+    for _ in range(3):
+        _lib.device_status(clear=True)
+        cache4.attention(q, k4, v4, lens, 0.1, wait_limit_ns=1)
+        assert _lib.device_status(clear=True) == _lib.DEVICE_TIMEOUT
+    if B > 3:
+        q, k4, v4, lens = q[:2], k4[:2], v4[:2], lens[:2]
+    run(q, k4, v4, lens)
+
+
 # ------------------------------------------------------------------- mass --
 def run_mass(q, k4, lens, tables=None, rows=None, counts=None, decay=1.0, context_only=False, scale=None, cap=None):
     B, T, H, D = q.shape
