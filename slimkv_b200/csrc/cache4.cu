@@ -74,7 +74,8 @@ __device__ __forceinline__ Place place_of(const Args4& a, const Part4& p, int ch
     Place w;
     const int b = blockIdx.y, tid = threadIdx.x;
     if (!span_of(a, b, w.start, w.count) && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) report(a.status, SLIMKV_DEVICE_BAD_LENGTH);
-    w.first = blockIdx.x * (p.side * a.turns);
+    // (The grid is the longer row's: of the shorter one's blocks some lie behind all rows, up to 2^32.)
+    w.first = int(min(int64_t(blockIdx.x) * (p.side * a.turns), int64_t(a.rows)));
     w.rows = min(p.side * a.turns, w.count - w.first);
     for (int i = tid; i < w.rows; i += blockDim.x) {
         int page = b, r = w.start + w.first + i;

@@ -158,6 +158,22 @@ def test_read_into_buffers_leaves_the_rest():
     assert (wide[..., 64:] == 7).all()
 
 
+def test_rows_of_very_different_lengths_in_a_large_call():
+    """2^28 rows of 32 and 320 dims in one call: of blocks cut for the longer rows, those of the shorter lie past 2^31."""
+    n = 1 << 28
+    k, v = make_rows((1, 4, 1, 32), BF16), make_rows((1, 4, 1, 320), BF16, 1)
+    guarded = [torch.full((1, 4096, 1, cache4.row_bytes(d)), 0xA5, dtype=torch.uint8, device='cuda') for d in (32, 320)]
+    k4, v4 = (x[:, 2040:2050] for x in guarded)
+    cache4.write(k[:, :1].expand(1, n, 1, 32), v[:, :1].expand(1, n, 1, 320), k4, v4, i32([2]), i32([3]))
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    got = cache4.read(k4, v4, i32([3]), BF16, rows=3, starts=i32([2]))
+    for x, x4, back in ((k, guarded[0], got[0]), (v, guarded[1], got[1])):
+        assert rows4.same(back.cpu(), rows4.values(*rows4.quantise(x[:, :1].expand(1, 3, 1, -1).cpu())))
+        touched = (x4 != 0xA5).any(-1).nonzero()[:, 1].tolist()
+        assert touched == [2042, 2043, 2044]
+
+
 def test_sequences_that_share_pages_and_caches_read_the_same_rows():
     k = make_rows((1, 40, 2, 128), FP16)
     k4, v4, tables = caches(1, 40, 2, 128, 128, 8)
