@@ -83,12 +83,15 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 // Merges the pieces of a segment's rows (a block each), and writes the rows
 // that see nothing.  The four warps take the pieces by turns, a lane four dims.
+// Pieces whose weight underflows to 0 stay out of the sums (what overflowed in
+// them must not count); only NaN of theirs is looked for afterwards, since 0 x NaN
+// is NaN, as it is within a piece.
 template <int NT, int kKeys, bool kHalf>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Job J) {
     constexpr int kRows = 8 * NT;
     __shared__ int range[3];                // first and last CTA of the segment's pieces, slot of the first
     __shared__ float4 acc[4][kMaxDims4 / 4];
-    __shared__ float tops[4], sums[4];
+    __shared__ float tops[4], sums[4], lows[4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int at = blockIdx.x;
     const int group = at % J.row_groups;
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
     }
     // In one pass, the largest exponent so far taken out: a piece's lse and rows are one latency.
     constexpr int kAhead = 4, kSpan = (kMaxDims4 + 127) / 128;
-    float m = -INFINITY, sum = 0.f;
+    float m = -INFINITY, sum = 0.f, low = INFINITY;     // low: of the pieces that saw anything
     float4 x[kSpan];
 #pragma unroll
     for (int k = 0; k < kSpan; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -146,7 +149,10 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
         }
         const float before = m;
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) m = fmaxf(m, w[a]);
+        for (int a = 0; a < kAhead; ++a) {
+            m = fmaxf(m, w[a]);
+            if (w[a] != -INFINITY) low = fminf(low, w[a]);
+        }
         const float shift = m == -INFINITY ? 0.f : m, old = before == -INFINITY ? 0.f : sfu_exp2(before - shift);
         if (before != -INFINITY) {
             sum *= old;
@@ -157,7 +163,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
         for (int a = 0; a < kAhead; ++a) {
             const float f = sfu_exp2(w[a] - shift);
             sum += f;
-            if (f == 0.f) continue;             // (a piece without weight: its rows stay out)
+            if (f == 0.f) continue;
 #pragma unroll
             for (int k = 0; k < kSpan; ++k)
                 if (4 * lane + 128 * k < dims) {
@@ -169,7 +175,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
 #pragma unroll
     for (int k = 0; k < kSpan; ++k)
         if (4 * lane + 128 * k < dims) acc[warp][lane + 32 * k] = x[k];
-    if (lane == 0) { tops[warp] = m; sums[warp] = sum; }
+    if (lane == 0) { tops[warp] = m; sums[warp] = sum; lows[warp] = low; }
     __syncthreads();
     const float all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), shift = all == -INFINITY ? 0.f : all;
     float f[4], l = 0.f;
@@ -179,6 +185,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
         l += tops[k] == -INFINITY ? sums[k] : f[k] * sums[k];
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
+    const bool light = fminf(fminf(lows[0], lows[1]), fminf(lows[2], lows[3])) < all - 120.f;      // (of some the weight may be 0)
     for (int d = 8 * tid; d < dims; d += 8 * 128) {
         float4 y[2];
 #pragma unroll
@@ -190,6 +197,18 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Jo
                 const float4 z = acc[k][d / 4 + half];
                 y[half].x = fmaf(f[k], z.x, y[half].x); y[half].y = fmaf(f[k], z.y, y[half].y);
                 y[half].z = fmaf(f[k], z.z, y[half].z); y[half].w = fmaf(f[k], z.w, y[half].w);
+            }
+        }
+        for (int c = c0; light && c <= c1; ++c) {
+            const int64_t row = int64_t(c == c0 ? slot0 : 2 * c) * kRows + blockIdx.y;
+            if (__ldcg(J.part_lse + row) == -INFINITY) continue;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float4 z = __ldcg(reinterpret_cast<const float4*>(J.part_o + row * dims + d) + half);
+                if (z.x != z.x) y[half].x = z.x;
+                if (z.y != z.y) y[half].y = z.y;
+                if (z.z != z.z) y[half].z = z.z;
+                if (z.w != z.w) y[half].w = z.w;
             }
         }
         *reinterpret_cast<uint4*>(out + d) =

@@ -387,6 +387,25 @@ def test_small_probabilities_count_in_fp16(H, D):
     run(q, k4, v4, i32([n]), scale=1.0)
 
 
+@pytest.mark.parametrize('H,D,dtype', [(4, 128, BF16), (12, 64, FP16), (40, 320, BF16), (20, 256, FP16)])
+@pytest.mark.parametrize('n', [40, 20000])
+def test_values_without_weight_that_are_nan(H, D, dtype, n):
+    """A context's NaN value makes its group NaN whatever its weight (the formula's 0 x NaN), in one piece and in many."""
+    k4, v4 = cache4.empty(1, n + 1, 1, D)
+    k, v = torch.zeros(1, n + 1, 1, D, device='cuda', dtype=dtype), make_rows((1, n + 1, 1, D), dtype)
+    k[..., 0] = -16.0                                       # e^-512 of the last row's weight
+    k[:, n] = 0.0
+    k[:, n, :, 0] = 16.0
+    cache4.write(k, v, k4, v4)
+    for row in (7, n // 2):
+        v4[0, row, 0, D // 2 + 4:D // 2 + 8] = 0xFF
+        q = torch.zeros(1, 1, H, D, device='cuda', dtype=dtype)
+        q[..., 0] = 16.0
+        got = run(q, k4, v4, i32([n]), scale=1.0)
+        assert got[0][..., 32:64].isnan().all() and got[0][..., :32].isfinite().all() and got[0][..., 64:].isfinite().all()
+        cache4.write(k, v, k4, v4)
+
+
 def test_shared_cache_and_strided_outputs():
     q, k4, v4, lens, _ = make(3, 4, 8, 2, 128, [50, 60, 170], layout='shared')
     run(q, k4, v4, lens, seen=trees(3, 4, 5))
