@@ -540,6 +540,19 @@ def test_a_wait_that_runs_out_is_reported(H, D, n):
     run(q, k4, v4, lens)
 
 
+@pytest.mark.parametrize('B,H,G,D,dtype', [(3, 8, 2, 128, BF16), (16, 4, 1, 64, FP16), (4, 12, 1, 192, BF16)])
+def test_waits_that_run_out_end_the_narrow_pipeline(B, H, G, D, dtype):
+    """With a limit of 1 ns a wait for the first keys runs out, since no warp has anything to do meanwhile and a copy
+    takes a microsecond: reported each time, and the next call is right.  (12 rows of 192 dims have their Q in shared
+    memory: the block loads it and meets at a barrier first, by which time the keys may have come.)"""
+    q, k4, v4, lens, _ = make(B, 1, H, G, D, [9000 - 300 * b for b in range(B)], dtype=dtype)
+    for _ in range(3):
+        _lib.device_status(clear=True)
+        cache4.attention(q, k4, v4, lens, 0.1, wait_limit_ns=1)
+        assert _lib.device_status(clear=True) in ((0, _lib.DEVICE_TIMEOUT) if D == 192 else (_lib.DEVICE_TIMEOUT,))
+    run(q[:2], k4[:2], v4[:2], lens[:2])
+
+
 @pytest.mark.parametrize('B,H,G,D', [(3, 40, 2, 320), (3, 40, 2, 256), (20, 24, 1, 224)])
 def test_waits_that_run_out_end_the_wide_pipeline(B, H, G, D):
     """With a limit of 1 ns the first products' waits run out while copies are under way (they take a microsecond):
