@@ -47,32 +47,36 @@ constexpr int kThreads = 32 * (4 + kSoftWarps + kValueWarps);
 constexpr uint32_t kChunk = kKeys * 128;         // [128 keys x 64] 16-bit elements
 constexpr uint32_t kTileArea = 223 * 1024;
 
-// Shared memory: V tiles | P tiles | Q | ring of 4-bit K rows | ring of 4-bit V rows.
+// Shared memory: V tile | P tiles | Q | ring of 4-bit K rows | ring of 4-bit V rows.
 template <int G, int N>
 struct Layout {
-    static constexpr int kChunks = (G + 1) / 2;                  // 64-dim chunks of a row
+    static_assert(G % 2 == 0, "whole chunks");
+    static constexpr int kChunks = G / 2;                        // 64-dim chunks of a row
     static constexpr uint32_t kV = uint32_t(kChunks) * kChunk, kP = kChunk, kQ = uint32_t(kChunks) * N * 128;
     static constexpr uint32_t kSlot = kHalfKeys * uint32_t(row4_bytes(kGroupDims * G));
-    static constexpr int kVBufs = 2 * kV + 2 * kP + kQ + 12 * kSlot <= kTileArea ? 2 : 1;
-    static constexpr int kPBufs = kVBufs * kV + 2 * kP + kQ + 8 * kSlot <= kTileArea ? 2 : 1;
-    static constexpr uint32_t kOffP = kVBufs * kV, kOffQ = kOffP + kPBufs * kP, kOffRing = kOffQ + kQ;
+    static constexpr int kPBufs = kV + 2 * kP + kQ + 8 * kSlot <= kTileArea ? 2 : 1;
+    static constexpr uint32_t kOffP = kV, kOffQ = kOffP + kPBufs * kP, kOffRing = kOffQ + kQ;
     static constexpr int kRing = (kTileArea - kOffRing) / (2 * kSlot) < 6 ? int((kTileArea - kOffRing) / (2 * kSlot)) : 6;
     static_assert(kRing >= 3, "a tile and a half under way");
     // Tensor memory: O^T blocks of 128 dims, two S^T, K.
     static constexpr int kBlocks = (kChunks + 1) / 2;
     static constexpr int kColS = kBlocks * N, kColK = kColS + 2 * N;
-    static constexpr int kKBufs = kColK + 32 * G <= 512 ? 2 : 1;
+    static constexpr int kKBufs = 2;
     static_assert(kColK + 16 * G * kKBufs <= 512, "tensor memory");
+    // A K slot is half a tile and belongs to the warps of its keys.  Of an odd ring they skip every
+    // other phase of a slot's barrier; that one is over, since the other half's warps have been through
+    // its tile, kKBufs or more tiles back, when kempty lets them go on.
+    static_assert(kRing % 2 == 0 || kRing > 2 * kKBufs, "phases of the K slots");
 };
 
-template <int N, class Work>
+template <int N>
 struct Bars {
     uint64_t kraw_full[6], kraw_empty[6], vraw_full[6], vraw_empty[6];
     // pempty: P . V of the tile in the buffer is over, so O has it.  One for each buffer: a softmax warp
     // waits for every phase of it in order, before the tile that starts the next, and so never takes
     // the phase before last, which has the same parity, for the one that it waits for.
     uint64_t kfull[2], kempty[2], sfull[2], sempty[2], pfull[2], pempty[2];
-    uint64_t vfull[4], vempty[4];                // half V tiles
+    uint64_t vfull[2], vempty[2];                // half V tiles
     uint64_t qfull, oempty, final_mma;
     uint32_t tmem_base;
     int abort;
@@ -83,7 +87,7 @@ struct Bars {
     float column[kSoftWarps][N / 2];             // a warp's maxima, then sums, of its columns
 };
 template <int G, int N>
-constexpr uint32_t kSmemBytes = 1024 + kTileArea + uint32_t(sizeof(Bars<N, Plan<N / 8, kKeys>>));
+constexpr uint32_t kSmemBytes = 1024 + kTileArea + uint32_t(sizeof(Bars<N>));
 
 // A from tensor memory (two 16-bit K elements to a column), B from shared memory.
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -119,7 +123,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     constexpr int NC = N / 2;                    // columns (rows of the segment) of a softmax thread
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    auto* bs = reinterpret_cast<Bars<N, Work>*>(smem + kTileArea);
+    auto* bs = reinterpret_cast<Bars<N>*>(smem + kTileArea);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t slot_k = uint32_t(kHalfKeys * J.k_pitch), slot_v = uint32_t(kHalfKeys * J.v_pitch);
     uint8_t* const ring_k = smem + L::kOffRing;
@@ -133,7 +137,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         mbar_init(&bs->kfull[i], kSoftWarps); mbar_init(&bs->kempty[i], 1);
         mbar_init(&bs->sfull[i], 1); mbar_init(&bs->sempty[i], kSoftWarps);
         mbar_init(&bs->pfull[i], kSoftWarps); mbar_init(&bs->pempty[i], 1);
-        for (int h = 0; h < 2; ++h) { mbar_init(&bs->vfull[2 * i + h], kValueWarps); mbar_init(&bs->vempty[2 * i + h], 1); }
+        mbar_init(&bs->vfull[i], kValueWarps); mbar_init(&bs->vempty[i], 1);
         bs->bad_values[i] = bs->bad_values[2 + i] = 0;
     } else if (tid == 10) {
         mbar_init(&bs->qfull, kSoftWarps);
@@ -207,12 +211,12 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         uint32_t o = 0;                          // tiles whose P . V has been
         uint32_t piece = 0;
         auto issue_o = [&](bool first) {
-            const uint32_t pb = o % L::kPBufs, vb = o % L::kVBufs;
+            const uint32_t pb = o % L::kPBufs;
             ok = ok && wait_bar(&bs->pfull[pb], (o / L::kPBufs) & 1, bs, J);
             if (first && piece > 0) ok = ok && wait_bar(&bs->oempty, (piece - 1) & 1, bs, J);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                ok = ok && wait_bar(&bs->vfull[2 * vb + h], (o / L::kVBufs) & 1, bs, J);
+                ok = ok && wait_bar(&bs->vfull[h], o & 1, bs, J);
                 if (!all_lanes(ok)) return;
                 tc_fence_after();
                 if (elect_one()) {
@@ -220,9 +224,9 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     for (int b = 0; b < L::kBlocks; ++b)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            umma_bf16(uint32_t(b * N), v_desc + ((vb * L::kV + 2 * b * kChunk + h * (kChunk / 2) + k * 2048) >> 4),
+                            umma_bf16(uint32_t(b * N), v_desc + ((2 * b * kChunk + h * (kChunk / 2) + k * 2048) >> 4),
                                       p_desc + ((pb * L::kP + h * (kChunk / 2) + k * 2048) >> 4), idesc_o, !first || h || k);
-                    umma_commit(&bs->vempty[2 * vb + h]);
+                    umma_commit(&bs->vempty[h]);
                     if (h) umma_commit(&bs->pempty[pb]);
                 }
                 __syncwarp();
@@ -325,9 +329,8 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     tc_fence_after();
                     const uint8_t* row = ring_k + slot * L::kSlot + (key & (kHalfKeys - 1)) * J.k_pitch;
 #pragma unroll
-                    for (int g2 = 0; g2 < (G + 1) / 2; ++g2) {
+                    for (int g2 = 0; g2 < G / 2; ++g2) {
                         const int grp = 2 * g2 + a;
-                        if (G % 2 && grp >= G) break;
                         float x[16];
                         uint32_t word[4] = {0, 0, 0, 0}, pair = 0;      // (dims behind the row: zeros)
                         if (grp < J.kg) {
@@ -544,12 +547,12 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         w.start(plan, &bs->share);
         while (w.next(plan)) {
             for (int half = 2 * w.t0; half < 2 * w.t1; ++half, ++i) {
-                const uint32_t slot = i % L::kRing, buf = i % (2 * L::kVBufs);
-                if (i >= uint32_t(2 * L::kVBufs)) ok = ok && warp_wait(&bs->vempty[buf], (i / (2 * L::kVBufs) - 1) & 1, bs, J);
+                const uint32_t slot = i % L::kRing, buf = i & 1;
+                if (i >= 2) ok = ok && warp_wait(&bs->vempty[buf], (i / 2 - 1) & 1, bs, J);
                 ok = ok && warp_wait(&bs->vraw_full[slot], (i / L::kRing) & 1, bs, J);
                 if (ok) {
                     const uint8_t* row = from + slot * L::kSlot;
-                    uint8_t* tile = to + (buf >> 1) * L::kV + (buf & 1) * (kChunk / 2);
+                    uint8_t* tile = to + buf * (kChunk / 2);
                     const bool context = (half + 1) * kHalfKeys <= w.s.len;
                     const int n = half * kHalfKeys + key;
                     bool bad = false;
@@ -571,7 +574,7 @@ cache4_wide_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                                 make_uint4(P::template values<0>(constants, word[e], sc, lo), P::template values<1>(constants, word[e], sc, lo),
                                            P::template values<2>(constants, word[e], sc, lo), P::template values<3>(constants, word[e], sc, lo));
                     }
-                    // (V is two tiles ahead of the products at most, so four pieces' flags are enough.)
+                    // (V is one tile ahead of the products at most, so four pieces' flags are more than enough.)
                     if (bad) *const_cast<volatile int*>(&bs->bad_values[piece & 3]) = int(piece) + 1;
                     fence_async_shared();
                 }
