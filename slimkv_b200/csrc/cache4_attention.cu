@@ -29,12 +29,12 @@
 // Bound: instructions and their latency (61 % of the cycles issue, the logic unit
 // is busy for 50 %).  A word of bf16 codes (8 values) takes 15 of them, 7 of the
 // logic unit and 8 on pairs of 16-bit values, and either kind issues every other
-// cycle; in its steady state the kernel goes through the keys at 5.5 TB/s, from HBM
-// and from L2 alike.  Around that, of 44 us, the first keys come after 5.6, and the CTAs
-// end between 28 and 44 (37 in the mean).  Measured in a graph (bf16,
-// 32 / 8 heads of 128 dims): 16 sequences of 8k rows, one token 47 us = 3.6 TB/s
-// (the same rows in 16 bits: 107 us), four nodes 64, one sequence of 131072 rows in
-// 16-row pages 51 or 56 (two GPUs), one token over 517 rows 8.4.  What that took, for the first:
+// cycle; once started the CTAs go through the keys at 5.7 TB/s together.  Around that,
+// by time stamps of each, the first keys come after 6.0 us and the CTAs end between 30
+// and 44 (38 in the mean).  Measured in a graph (bf16, 32 / 8 heads of 128 dims): 16
+// sequences of 8k rows, one token 47 us = 3.6 TB/s (the same rows in 16 bits: 107 us),
+// four nodes 64, one sequence of 131072 rows in 16-row pages 51 or 56 (two GPUs), one
+// token over 517 rows 8.5.  What that took, for the first:
 // 67.5 us; constant row lengths, plain shared-memory loads 61; and + or of the
 // codes in one instruction 55; 32 keys to a warp's step 49; masks only in a
 // sequence's last steps 47.  More CTAs than fit (each pays the start): 54 to 63; five
@@ -523,9 +523,10 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
 // ------------------------------------------------------------------- host --
 // The wide kernel or this file's.  In a graph, 8 sequences of one KV head, wide against not:
-// 32 rows over 8192 keys of 320 dims 27.8 and 32.4 us, 128 rows 57.5 and 76.3, of 256 dims 24.7 and
-// 28.0, 52.3 and 64.1, of 192 dims 26.1 and 24.3, 61.2 and 56.4, 20 rows of 128 dims (8 KV heads)
-// 69.7 and 62.9; over 600 keys of 256 or 320 dims 15.0 and 13.4, 16.6 and 15.4, 22.3 and 22.3.
+// 32 rows over 8192 keys of 320 dims 28.0 and 32.2 us, 128 rows 58.6 and 76.2, of 256 dims 24.8 and
+// 26.4, 52.9 and 63.6, 32 rows of 224 dims 24.4 and 26.4, of 192 dims 27.0 and 23.2, 128 rows 62.6
+// and 56.3, 20 rows of 128 dims (8 KV heads) 83.9 and 63.2.  Short caches lose by the rule: 600 keys,
+// 32 rows of 256 dims 15.4 and 13.4, of 320 16.0 and 14.7, 128 rows 22.5 and 21.9.
 bool is_wide(const slimkv_tree_attention_args* a) {
     return a->nodes * (a->heads / a->kv_heads) > 16 && std::max(a->dim_qk, a->dim_v) > 192;
 }

@@ -13,13 +13,13 @@
 // each row's sum are its own; a row's maximum is kept until a score passes it by
 // 2^8, so only then do threads exchange maxima.
 //
-// Bound: what surrounds the work.  16 sequences of 8k latents of 320 dims, 32 rows
-// (7 tiles to a CTA), in a graph 38 us; without K's and V's codes, products and
-// exponentials it would be 29, without the loads too 24: 5 us to the first tile,
-// 3 of a piece's end, 5 of the merge, and about 1.4 us a tile of barriers between
-// the roles.  (K's codes in eight warps of their own: the same.  Sixteen warps for
-// all codes: 43.  64 rows to a pass: 156 against 170 us for 256 rows, slower for
-// 32 to 96.)
+// Bound: a tile's steps, which follow one another through one V tile and (320 dims)
+// one P tile, and what surrounds them.  16 sequences of 8k latents of 320 dims, 32 rows
+// (7 tiles to a CTA), in a graph 39 us: by time stamps of each CTA the first tile's K
+// is ready after 6.8 us, a tile takes 2.7, from the last P to the rows written it takes
+// 4.9, the last CTA ends after 35.8, and the merge comes behind.  (K's codes in eight
+// warps of their own: the same.  Sixteen warps for all codes: 43.  64 rows to a pass:
+// 156 against 170 us for 256 rows, slower for 32 to 96.)
 //
 // Warps: 0 and 3 load the 4-bit K and V rows (TMA; 3 finds the CTA's share), 1
 // issues the products, 2 owns tensor memory, 4-11 turn K's codes into operands and

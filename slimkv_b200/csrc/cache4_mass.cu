@@ -14,7 +14,7 @@
 // Bound: instructions and their latency (57 % of the cycles issue, at a third of
 // HBM's rate).  Measured in a graph (bf16): 1 to 5 accepted rows of 32 heads for 16
 // sequences of 8k keys (8 KV heads of 128 dims) 48 us = 1.9 TB/s, one row over 1028
-// keys 5.6 us.  Against the 16-bit keys' kernel (tcgen05), every row accepted: 5
+// keys 6 us.  Against the 16-bit keys' kernel (tcgen05), every row accepted: 5
 // rows of that shape 54 us and 53; 8 rows (256 queries of a KV head) over 16 x 8k
 // latents of 320 dims 137 us and 31: it saves memory, and time only for few rows.
 #include <algorithm>
@@ -203,7 +203,7 @@ cache4_mass_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             __syncthreads();
 
             // Lane column 0 has the key g of a slab, column 1 the key g + 8; their old masses are on
-            // their way a slab ahead (16 sequences of 8k keys 55.5 -> 47.2 us).
+            // their way a slab ahead (16 sequences of 8k keys took 55.5 us without, 48 with it).
             auto old_mass = [&](int i) {
                 const int n = first_key + i * kKeys + g + 8 * t;
                 if (t > 1 || i >= slabs || n >= w.s.end) return 0.f;
