@@ -78,10 +78,11 @@ struct Bars {
     uint64_t kfull[2], kempty[2], sfull[2], sempty[2], pfull[2], pempty[2];
     uint64_t vfull[2], vempty[2];                // half V tiles
     uint64_t qfull, oempty, final_mma;
+    // (Not at a multiple of 16 bytes, where its loads become one: 16 x 8k latents took 38.7 us then, 37.3 so.)
+    Share share;
     uint32_t tmem_base;
     int abort;
     int bad_values[4];                           // 1 + a piece whose nodes' values hold NaN, by piece % 4
-    Share share;
     alignas(16) float top[N], shift[N], alpha[N], inv[N];
     int64_t out_at[N];                           // of each row
     float column[kSoftWarps][N / 2];             // a warp's maxima, then sums, of its columns
