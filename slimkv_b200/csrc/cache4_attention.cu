@@ -523,10 +523,10 @@ cache4_attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 
 // ------------------------------------------------------------------- host --
 // The wide kernel or this file's.  In a graph, 8 sequences of one KV head, wide against not:
-// 32 rows over 8192 keys of 320 dims 28.0 and 32.2 us, 128 rows 58.6 and 76.2, of 256 dims 24.8 and
-// 26.4, 52.9 and 63.6, 32 rows of 224 dims 24.4 and 26.4, of 192 dims 27.0 and 23.2, 128 rows 62.6
-// and 56.3, 20 rows of 128 dims (8 KV heads) 83.9 and 63.2.  Short caches lose by the rule: 600 keys,
-// 32 rows of 256 dims 15.4 and 13.4, of 320 16.0 and 14.7, 128 rows 22.5 and 21.9.
+// 32 rows over 8192 keys of 320 dims 27.1 and 32.2 us, 128 rows 56.9 and 76.2, of 256 dims 24.3 and
+// 26.8, 52.4 and 63.6, 32 rows of 224 dims 24.3 and 26.3, of 192 dims 27.0 and 23.4, 128 rows 62.3
+// and 56.2, 20 rows of 128 dims (8 KV heads) 83.4 and 63.2.  Short caches lose by the rule: 600 keys,
+// 32 rows of 256 dims 15.4 and 13.4, of 320 16.0 and 14.7, 128 rows 22.3 and 21.9.
 bool is_wide(const slimkv_tree_attention_args* a) {
     return a->nodes * (a->heads / a->kv_heads) > 16 && std::max(a->dim_qk, a->dim_v) > 192;
 }

@@ -15,9 +15,9 @@
 //
 // Bound: a tile's steps, which follow one another through one V tile and (320 dims)
 // one P tile, and what surrounds them.  16 sequences of 8k latents of 320 dims, 32 rows
-// (7 tiles to a CTA), in a graph 39 us: by time stamps of each CTA the first tile's K
-// is ready after 6.8 us, a tile takes 2.7, from the last P to the rows written it takes
-// 4.9, the last CTA ends after 35.8, and the merge comes behind.  (K's codes in eight
+// (7 tiles to a CTA), in a graph 37 us: by time stamps of each CTA the first tile's K
+// is ready after 6.0 us, a tile takes 2.7, from the last P to the rows written it takes
+// 4.9, the last CTA ends after 34.0, and the merge comes behind.  (K's codes in eight
 // warps of their own: the same.  Sixteen warps for all codes: 43.  64 rows to a pass:
 // 156 against 170 us for 256 rows, slower for 32 to 96.)
 //
